@@ -9,6 +9,11 @@ void kr_fail(ml_status st, const char *what, hipError_t e);
 // records a launch error, if any
 void kr_check_launch(const char *what);
 
+// The fault words: kernels that take tables, lengths or rows from device memory
+// store to them (kr_paged.h) where one is out of range; krh_sync reports
+// them. Pinned host memory, so that reading them costs no copy.
+int *kr_fault_word(void);
+
 // devices whose static scratch addresses the library keeps
 constexpr int KR_MAX_DEVICES = 16;
 // kr_attn.hip: takes this device's address of the attention scratch array

@@ -1,0 +1,493 @@
+// Several sequences over one paged cache: the rows of new tokens into their
+// pages (per-head norm and rotation on the way), attention of one token of each
+// sequence, and eviction by accumulated attention weight.
+#include "kr_internal.h"
+#include "kr_numerics.h"
+#include "kr_paged.h"
+
+namespace {
+
+constexpr int PG_T = 256;
+
+enum { PG_F32 = ML_F32, PG_Q8 = ML_Q8_0, PG_F16 = ML_F16 };
+
+// a pool and the view of its sequences
+struct PgView {
+    void *k, *v;
+    float *kd, *vd;
+    const int *table;
+    int ld, n_seq, n_pages, shift, n_kv, hd;
+};
+
+__device__ __forceinline__ int pg_page(const PgView &p, int seq, int row, int &bad) {
+    return kr_page_of(p.table + (size_t)seq * p.ld, p.ld, row, p.shift, p.n_pages, bad);
+}
+
+// ---- rows into and out of pages ----
+// An item is one head's vector of one token; 2^LPS >= hd / 4 lanes share it,
+// four values each (whole 16-byte accesses), so a wave holds one to eight
+// items and its loads are contiguous. Bound by HBM: 8 bytes a query value, 4 +
+// the cache's width a key or value.
+
+// over the 2^lps lanes of an item
+__device__ __forceinline__ double pg_sum(double v, int n) {
+    for (int o = n >> 1; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ float pg_max(float v, int n) {
+    for (int o = n >> 1; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+
+struct QkvArgs {
+    float *qo;
+    const float *q, *k, *v, *qw, *kw, *cs, *sn;
+    const int *seq, *row, *pos;
+    size_t ldqo, ldq, ldk, ldv;
+    float eps;
+    int ntok, nh, n_pos;
+};
+
+// row `at` (in rows of the pool) of K or V from four values a lane, l < hd / 4;
+// the conversions of krh_store_kv
+template <int KT> __device__ __forceinline__ void pg_store(void *dst, float *d, size_t at, int hd, float4 x, int l, bool live, int n) {
+    const size_t e = at * hd + 4 * l;
+    if (KT == PG_F32) {
+        if (live) *(float4 *)((float *)dst + e) = x;
+    } else if (KT == PG_F16) {
+        const ushort4 h = make_ushort4(kr_f2h(x.x), kr_f2h(x.y), kr_f2h(x.z), kr_f2h(x.w));
+        if (live) *(ushort4 *)((uint16_t *)dst + e) = h;
+    } else {
+        float m = live ? fmaxf(fmaxf(fmaxf(fmaxf(0.0f, fabsf(x.x)), fabsf(x.y)), fabsf(x.z)), fabsf(x.w)) : 0.0f;
+        m = pg_max(m, n);
+        const bool zero = m < KR_QUANT_TINY;
+        const float id = zero ? 0.0f : kr_fdiv(127.0f, m);
+        char4 c = make_char4(0, 0, 0, 0);
+        if (!zero)
+            c = make_char4((signed char)kr_q8_elem(x.x, id), (signed char)kr_q8_elem(x.y, id),
+                           (signed char)kr_q8_elem(x.z, id), (signed char)kr_q8_elem(x.w, id));
+        if (live) *(char4 *)((int8_t *)dst + e) = c;
+        if (l == 0) d[at] = zero ? 0.0f : kr_fdiv(m, 127.0f);
+    }
+}
+
+template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_qkv(const PgView p, const QkvArgs a, int lps, int *fault) {
+    const int n = 1 << lps, l = (int)threadIdx.x & (n - 1), per = a.nh + 2 * p.n_kv;
+    const size_t item = ((size_t)blockIdx.x * PG_T + threadIdx.x) >> lps;
+    if (item >= (size_t)a.ntok * per) return;   // whole items: the lanes that shuffle leave together
+    const int t = (int)(item / per), h = (int)(item % per), hd = p.hd;
+    const bool live = 4 * l < hd, isq = h < a.nh, isk = !isq && h < a.nh + p.n_kv;
+    const int kvh = h - a.nh - (isk || isq ? 0 : p.n_kv);
+    const float *src = isq ? a.q + (size_t)t * a.ldq + (size_t)h * hd
+                           : (isk ? a.k + (size_t)t * a.ldk : a.v + (size_t)t * a.ldv) + (size_t)kvh * hd;
+    float4 x = live ? *(const float4 *)(src + 4 * l) : make_float4(0, 0, 0, 0);
+    int bad = 0, seq = 0, row = 0, page = 0;
+    if (!isq) {
+        seq = kr_page_in(a.seq[t], p.n_seq, KR_BAD_SEQ, bad);
+        row = kr_page_in(a.row[t], INT_MAX, KR_BAD_PAGE, bad);
+        page = pg_page(p, seq, row, bad);
+    }
+    const bool keep = bad == 0;
+    if (isq || isk) {
+        const float *w = isq ? a.qw : a.kw;
+        if (w) {
+            const double s = pg_sum((double)x.x * x.x + (double)x.y * x.y + ((double)x.z * x.z + (double)x.w * x.w), n);
+            const float inv = (float)(1.0 / sqrt(s / hd + (double)a.eps));
+            if (live) {
+                const float4 g = *(const float4 *)(w + 4 * l);
+                x = make_float4(kr_fmul(kr_fmul(x.x, inv), g.x), kr_fmul(kr_fmul(x.y, inv), g.y),
+                                kr_fmul(kr_fmul(x.z, inv), g.z), kr_fmul(kr_fmul(x.w, inv), g.w));
+            }
+        }
+        if (a.cs) {
+            const int pos = kr_page_in(a.pos[t], a.n_pos, KR_BAD_POS, bad);
+            if (live) {
+                const float2 c = *(const float2 *)(a.cs + (size_t)pos * (hd >> 1) + 2 * l);
+                const float2 s = *(const float2 *)(a.sn + (size_t)pos * (hd >> 1) + 2 * l);
+                x = make_float4(kr_fsub(kr_fmul(x.x, c.x), kr_fmul(x.y, s.x)), kr_fadd(kr_fmul(x.x, s.x), kr_fmul(x.y, c.x)),
+                                kr_fsub(kr_fmul(x.z, c.y), kr_fmul(x.w, s.y)), kr_fadd(kr_fmul(x.z, s.y), kr_fmul(x.w, c.y)));
+            }
+        }
+    }
+    if (l == 0) kr_report(fault, bad);
+    if (isq) {
+        if (live) *(float4 *)(a.qo + (size_t)t * a.ldqo + (size_t)h * hd + 4 * l) = x;
+        return;
+    }
+    if (!keep) return;
+    pg_store<KT>(isk ? p.k : p.v, isk ? p.kd : p.vd, kr_page_row(page, p.n_kv, kvh, p.shift, row), hd, x, l, live, n);
+}
+
+template <int KT> __device__ __forceinline__ float4 pg_load4(const void *src, const float *d, size_t at, int hd, int l) {
+    const size_t e = at * hd + 4 * l;
+    if (KT == PG_F32) return *(const float4 *)((const float *)src + e);
+    if (KT == PG_F16) {
+        const ushort4 h = *(const ushort4 *)((const uint16_t *)src + e);
+        return make_float4(kr_h2f(h.x), kr_h2f(h.y), kr_h2f(h.z), kr_h2f(h.w));
+    }
+    const char4 c = *(const char4 *)((const int8_t *)src + e);
+    const float s = d[at];
+    return make_float4(kr_fmul((float)c.x, s), kr_fmul((float)c.y, s), kr_fmul((float)c.z, s), kr_fmul((float)c.w, s));
+}
+
+template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_load(const PgView p, float *k, size_t ldk, float *v, size_t ldv,
+                                                                       int n_rows, const int *seqs, const int *rows, int lps, int *fault) {
+    const int n = 1 << lps, l = (int)threadIdx.x & (n - 1), per = 2 * p.n_kv;
+    const size_t item = ((size_t)blockIdx.x * PG_T + threadIdx.x) >> lps;
+    if (item >= (size_t)n_rows * per || 4 * l >= p.hd) return;
+    const int i = (int)(item / per), h = (int)(item % per), kvh = h < p.n_kv ? h : h - p.n_kv;
+    int bad = 0;
+    const int seq = kr_page_in(seqs[i], p.n_seq, KR_BAD_SEQ, bad), row = kr_page_in(rows[i], INT_MAX, KR_BAD_PAGE, bad);
+    const size_t at = kr_page_row(pg_page(p, seq, row, bad), p.n_kv, kvh, p.shift, row);
+    const bool isk = h < p.n_kv;
+    float4 x = make_float4(0, 0, 0, 0);
+    if (!bad) x = pg_load4<KT>(isk ? p.k : p.v, isk ? p.kd : p.vd, at, p.hd, l);
+    if (l == 0) kr_report(fault, bad);
+    *(float4 *)((isk ? k + (size_t)i * ldk : v + (size_t)i * ldv) + (size_t)kvh * p.hd + 4 * l) = x;
+}
+
+// ---- attention ----
+
+struct AttArgs {
+    float *o;
+    const float *q;
+    const int *len;
+    float *mass;
+    size_t mass_ld;
+    float *ws;
+    int nh, max_len, window;
+    float scale, cap;
+};
+
+// one workgroup a (sequence, KV head), a query head at a time: scores to the
+// workspace, their maximum and sum, then a lane a dim over the rows
+template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_attn(const PgView p, const AttArgs a, int *fault) {
+    __shared__ float red[PG_T / 64];
+    __shared__ float qs[KR_PAGE_HD_MAX];
+    const int s = blockIdx.y, kvh = blockIdx.x, tid = threadIdx.x, hd = p.hd, group = a.nh / p.n_kv;
+    int bad = 0;
+    const int len = kr_page_len(a.len[s], a.max_len, bad);
+    const int first = a.window > 0 && len > a.window ? len - a.window : 0;
+    for (int g = 0; g < group; g++) {
+        const int h = kvh * group + g;
+        const size_t qat = ((size_t)s * a.nh + h) * hd;
+        float *z = a.ws + ((size_t)s * a.nh + h) * a.max_len;
+        for (int d = tid; d < hd; d += PG_T) qs[d] = a.q[qat + d];
+        __syncthreads();
+        float m = -INFINITY;
+        for (int r = first + tid; r < len; r += PG_T) {
+            const size_t at = kr_page_row(pg_page(p, s, r, bad), p.n_kv, kvh, p.shift, r);
+            float acc = 0.0f;
+            for (int l = 0; 4 * l < hd; l++) {
+                const float4 x = pg_load4<KT>(p.k, p.kd, at, hd, l);
+                acc += qs[4 * l] * x.x + qs[4 * l + 1] * x.y + qs[4 * l + 2] * x.z + qs[4 * l + 3] * x.w;
+            }
+            acc *= a.scale;
+            if (a.cap > 0.0f) acc = a.cap * kr_tanhf(acc / a.cap);
+            z[r] = acc;
+            m = fmaxf(m, acc);
+        }
+        m = pg_max(m, 64);
+        if ((tid & 63) == 0) red[tid >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        __syncthreads();
+        float sum = 0.0f;
+        for (int r = first + tid; r < len; r += PG_T) {
+            z[r] = kr_expf(z[r] - m);
+            sum += z[r];
+        }
+        for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+        if ((tid & 63) == 0) red[tid >> 6] = sum;
+        __threadfence_block();
+        __syncthreads();
+        const float inv = 1.0f / (red[0] + red[1] + red[2] + red[3]);
+        for (int d = tid; d < hd; d += PG_T) {
+            float acc = 0.0f;
+            for (int r = first; r < len; r++) {
+                const size_t at = kr_page_row(pg_page(p, s, r, bad), p.n_kv, kvh, p.shift, r);
+                const float4 x = pg_load4<KT>(p.v, p.vd, at, hd, d >> 2);
+                acc += z[r] * ((d & 2) ? ((d & 1) ? x.w : x.z) : ((d & 1) ? x.y : x.x));
+            }
+            a.o[qat + d] = len > 0 ? acc * inv : 0.0f;
+        }
+        if (a.mass)
+            for (int r = first + tid; r < len; r += PG_T) a.mass[((size_t)s * p.n_kv + kvh) * a.mass_ld + r] += z[r] * inv;
+        __syncthreads();
+    }
+    kr_report(fault, bad);
+}
+
+// ---- eviction ----
+
+// Weights in an order of unsigned integers: larger is heavier, NaN the
+// heaviest, -0 as +0
+__device__ __forceinline__ unsigned ev_key(float w) {
+    const unsigned u = __float_as_uint(w == 0.0f ? 0.0f : w);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+    return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+constexpr int EV_T = 1024, EV_W = EV_T / 64;
+
+struct EvArgs {
+    const int *len;
+    const float *mass;
+    size_t mass_ld;
+    int max_len, keep, recent;
+    const int *out_table;
+    int out_ld;
+    int *out_len;
+    float *out_mass;
+    size_t out_mass_ld;
+    int *idx;   // [n_seq][n_kv][keep]: the rows kept, in order
+    int *cnt;   // [n_seq]: how many
+};
+
+// One workgroup a (sequence, KV head): the weight of the last row kept by a
+// radix select (8 bits a pass), then the kept rows' numbers in order, equal
+// weights from the lowest row on.
+__global__ void __launch_bounds__(EV_T) k_evict_select(const EvArgs a, int *fault) {
+    __shared__ int hist[256];
+    __shared__ int wsum[2][EV_W];
+    __shared__ unsigned s_prefix;
+    __shared__ int s_need;
+    const int kvh = blockIdx.x, s = blockIdx.y, n_kv = gridDim.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int bad = 0;
+    const int len = kr_page_len(a.len[s], a.max_len, bad);
+    if (tid == 0) kr_report(fault, bad);
+    const size_t sh = (size_t)s * n_kv + kvh;
+    const float *mass = a.mass + sh * a.mass_ld;
+    float *om = a.out_mass + sh * a.out_mass_ld;
+    int *idx = a.idx + sh * a.keep;
+    const int kept = min(len, a.keep);
+    if (kvh == 0 && tid == 0) a.cnt[s] = kept;
+    // past the kept rows nothing is left, for rows that come later
+    const int end = (int)min(a.out_mass_ld, (size_t)max(a.keep, a.max_len));
+    if (len <= a.keep) {
+        for (int r = tid; r < end; r += EV_T) {
+            if (r < len) idx[r] = r;
+            om[r] = r < len ? mass[r] : 0.0f;
+        }
+        return;
+    }
+    const int old = len - a.recent, want = a.keep - a.recent;   // 0 <= want < old
+    unsigned prefix = 0;
+    int need = want;
+    if (want > 0)
+        for (int b = 24; b >= 0; b -= 8) {
+            for (int i = tid; i < 256; i += EV_T) hist[i] = 0;
+            __syncthreads();
+            for (int r = tid; r < old; r += EV_T) {
+                const unsigned u = ev_key(mass[r]);
+                if (b == 24 || (u >> (b + 8)) == (prefix >> (b + 8))) atomicAdd(&hist[u >> b & 255], 1);
+            }
+            __syncthreads();
+            if (tid == 0) {
+                int d = 255, left = need;
+                while (hist[d] < left) left -= hist[d--];   // need <= the counts' sum: ends at d >= 0
+                s_prefix = prefix | (unsigned)d << b;
+                s_need = left;
+            }
+            __syncthreads();
+            prefix = s_prefix;
+            need = s_need;
+            __syncthreads();
+        }
+    // rows above `prefix`, and the first `need` of those at it
+    int base = 0, ties = 0;
+    for (int r0 = 0; r0 < len; r0 += EV_T) {
+        const int r = r0 + tid;
+        const float w = r < len ? mass[r] : 0.0f;
+        const unsigned u = ev_key(w);
+        const bool tail = r >= old && r < len, tie = want > 0 && r < old && u == prefix;
+        const unsigned long long bt = __ballot(tie), below = ((unsigned long long)1 << lane) - 1;
+        if (lane == 0) wsum[0][wave] = __popcll(bt);
+        __syncthreads();
+        int before = ties;
+        for (int i = 0; i < EV_W; i++) {
+            if (i < wave) before += wsum[0][i];
+            ties += wsum[0][i];
+        }
+        const bool take = tail || (want > 0 && r < old && u > prefix) || (tie && before + __popcll(bt & below) < need);
+        const unsigned long long bk = __ballot(take);
+        if (lane == 0) wsum[1][wave] = __popcll(bk);
+        __syncthreads();
+        int at = base;
+        for (int i = 0; i < EV_W; i++) {
+            if (i < wave) at += wsum[1][i];
+            base += wsum[1][i];
+        }
+        if (take) {
+            at += __popcll(bk & below);
+            idx[at] = r;
+            om[at] = w;   // at <= r: in place, no weight of a later chunk is lost
+        }
+        __syncthreads();
+    }
+    for (int r = a.keep + tid; r < end; r += EV_T) om[r] = 0.0f;
+}
+
+// rows into the new pages, in units of U bytes; a unit a thread and step
+template <class U> __global__ void __launch_bounds__(PG_T) k_evict_move(const PgView p, const EvArgs a, int rb, int *fault) {
+    const int s = blockIdx.z, kvh = blockIdx.y, per = rb / (int)sizeof(U), kept = a.cnt[s];
+    const size_t sh = (size_t)s * p.n_kv + kvh;
+    const int *idx = a.idx + sh * a.keep, *ot = a.out_table + (size_t)s * a.out_ld;
+    if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0) a.out_len[s] = kept;
+    int bad = 0;
+    for (size_t e = (size_t)blockIdx.x * PG_T + threadIdx.x; e < (size_t)kept * per; e += (size_t)gridDim.x * PG_T) {
+        const int j = (int)(e / per), u = (int)(e % per), r = idx[j];
+        int b = 0;
+        const size_t from = kr_page_row(pg_page(p, s, r, b), p.n_kv, kvh, p.shift, r);
+        const size_t to = kr_page_row(kr_page_of(ot, a.out_ld, j, p.shift, p.n_pages, b), p.n_kv, kvh, p.shift, j);
+        bad |= b;
+        if (b) continue;
+        ((U *)p.k)[to * per + u] = ((const U *)p.k)[from * per + u];
+        ((U *)p.v)[to * per + u] = ((const U *)p.v)[from * per + u];
+        if (u == 0 && p.kd) {
+            p.kd[to] = p.kd[from];
+            p.vd[to] = p.vd[from];
+        }
+    }
+    kr_report(fault, bad);
+}
+
+int log2_of(int v) {
+    int l = 0;
+    while ((1 << l) < v) l++;
+    return l;
+}
+
+bool pages_ok(const krh_pages *kv) {
+    return kv && kv->k && kv->v && !(((uintptr_t)kv->k | (uintptr_t)kv->v) & 15) && kv->n_pages > 0 &&
+           kv->page_size >= KR_PAGE_MIN && kv->page_size <= KR_PAGE_MAX && !(kv->page_size & (kv->page_size - 1)) &&
+           kv->n_kv_heads > 0 && kv->n_kv_heads <= KRH_ROWS_MAX && kv->head_dim >= 8 && kv->head_dim <= KR_PAGE_HD_MAX &&
+           kv->head_dim % 8 == 0 &&
+           (kv->kv_type == ML_F32 || kv->kv_type == ML_F16 || (kv->kv_type == ML_Q8_0 && kv->kd && kv->vd));
+}
+
+bool aligned16(const void *p) { return !((uintptr_t)p & 15); }
+
+PgView view_of(const krh_pages *kv, const int *table, int ld, int n_seq) {
+    const bool q8 = kv->kv_type == ML_Q8_0;
+    return { kv->k, kv->v, q8 ? kv->kd : nullptr, q8 ? kv->vd : nullptr, table, ld, n_seq, kv->n_pages, log2_of(kv->page_size),
+             kv->n_kv_heads, kv->head_dim };
+}
+
+bool refuse(bool ok, const char *what) {
+    if (!ok) kr_fail(ML_E_SHAPE, what, hipSuccess);
+    return !ok;
+}
+
+// workgroups for `items` items of 2^lps lanes; 0: more than a launch holds
+unsigned item_blocks(size_t items, int lps) {
+    const size_t b = ((items << lps) + PG_T - 1) / PG_T;
+    return b <= 0x7fffffff / PG_T ? (unsigned)b : 0;
+}
+
+}  // namespace
+
+extern "C" void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const int *table, int table_ld, int n_seq,
+                              const float *q, size_t ldq, const float *k, size_t ldk, const float *v, size_t ldv,
+                              int ntok, int n_heads, const int *seq, const int *row, const int *pos,
+                              const float *q_norm, const float *k_norm, float eps, const float *cos_t,
+                              const float *sin_t, int n_pos) {
+    if (refuse(pages_ok(kv), "paged_qkv: the pages") ||
+        refuse(ntok >= 0 && n_heads >= 0 && n_heads <= KRH_ROWS_MAX && n_seq > 0 && table_ld > 0, "paged_qkv sizes"))
+        return;
+    if (ntok == 0) return;
+    const size_t kvd = (size_t)kv->n_kv_heads * kv->head_dim, qd = (size_t)n_heads * kv->head_dim;
+    if (refuse(table && k && v && seq && row && (n_heads == 0 || (q && qo)) && (!cos_t) == (!sin_t) &&
+                   (!cos_t || (pos && n_pos > 0)) && (n_heads == 0 || (!q_norm) == (!k_norm)), "paged_qkv: a missing array") ||
+        refuse(ldk >= kvd && ldv >= kvd && ldk % 4 == 0 && ldv % 4 == 0 && aligned16(k) && aligned16(v) && aligned16(k_norm) &&
+                   aligned16(cos_t) && aligned16(sin_t) &&
+                   (n_heads == 0 || (ldq >= qd && ldqo >= qd && ldq % 4 == 0 && ldqo % 4 == 0 && aligned16(q) &&
+                                     aligned16(qo) && aligned16(q_norm))), "paged_qkv: row strides or alignment"))
+        return;
+    const int lps = log2_of(kv->head_dim / 4);
+    const unsigned grid = item_blocks((size_t)ntok * (n_heads + 2 * (size_t)kv->n_kv_heads), lps);
+    if (refuse(grid > 0, "paged_qkv: too many tokens")) return;
+    const PgView p = view_of(kv, table, table_ld, n_seq);
+    const QkvArgs a = { qo, q, k, v, q_norm, k_norm, cos_t, sin_t, seq, row, pos, ldqo, ldq, ldk, ldv, eps, ntok, n_heads, n_pos };
+    const auto f = kv->kv_type == ML_F32 ? k_paged_qkv<PG_F32> : kv->kv_type == ML_F16 ? k_paged_qkv<PG_F16> : k_paged_qkv<PG_Q8>;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(PG_T), 0, kr_stream(), p, a, lps, kr_fault_word());
+    kr_check_launch("paged_qkv");
+}
+
+extern "C" void krh_paged_load(float *k, size_t ldk, float *v, size_t ldv, const krh_pages *kv, const int *table,
+                               int table_ld, int n_seq, int n, const int *seq, const int *row) {
+    if (refuse(pages_ok(kv), "paged_load: the pages") || refuse(n >= 0 && n_seq > 0 && table_ld > 0, "paged_load sizes")) return;
+    if (n == 0) return;
+    const size_t kvd = (size_t)kv->n_kv_heads * kv->head_dim;
+    if (refuse(table && k && v && seq && row, "paged_load: a missing array") ||
+        refuse(ldk >= kvd && ldv >= kvd && ldk % 4 == 0 && ldv % 4 == 0 && aligned16(k) && aligned16(v),
+               "paged_load: row strides or alignment"))
+        return;
+    const int lps = log2_of(kv->head_dim / 4);
+    const unsigned grid = item_blocks((size_t)n * 2 * kv->n_kv_heads, lps);
+    if (refuse(grid > 0, "paged_load: too many rows")) return;
+    const auto f = kv->kv_type == ML_F32 ? k_paged_load<PG_F32> : kv->kv_type == ML_F16 ? k_paged_load<PG_F16> : k_paged_load<PG_Q8>;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(PG_T), 0, kr_stream(), view_of(kv, table, table_ld, n_seq), k, ldk, v, ldv, n, seq, row,
+                       lps, kr_fault_word());
+    kr_check_launch("paged_load");
+}
+
+static bool attention_sizes(const krh_pages *kv, int n_seq, int n_heads, int max_len) {
+    return pages_ok(kv) && n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && n_heads > 0 && n_heads % kv->n_kv_heads == 0 &&
+           n_heads / kv->n_kv_heads <= KR_PAGE_GROUP_MAX;
+}
+
+extern "C" size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int max_len, int mass) {
+    if (!attention_sizes(kv, n_seq, n_heads, max_len)) return 0;
+    return sizeof(float) * (size_t)n_seq * n_heads * max_len;
+}
+
+extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len,
+                                    int n_seq, const float *q, int n_heads, int max_len, int window, float scale,
+                                    float softcap, float *mass, size_t mass_ld, void *ws) {
+    if (n_seq == 0) return;
+    if (refuse(attention_sizes(kv, n_seq, n_heads, max_len), "paged_attention sizes") ||
+        refuse(o && table && table_ld > 0 && len && q && ws && aligned16(o) && aligned16(q) && aligned16(ws),
+               "paged_attention: a missing or unaligned array") ||
+        refuse(window >= 0 && softcap >= 0.0f && (!mass || mass_ld >= (size_t)max_len), "paged_attention: window, soft-cap or mass rows"))
+        return;
+    const AttArgs a = { o, q, len, mass, mass_ld, (float *)ws, n_heads, max_len, window, scale, softcap };
+    const auto f = kv->kv_type == ML_F32 ? k_paged_attn<PG_F32> : kv->kv_type == ML_F16 ? k_paged_attn<PG_F16> : k_paged_attn<PG_Q8>;
+    hipLaunchKernelGGL(f, dim3(kv->n_kv_heads, n_seq), dim3(PG_T), 0, kr_stream(), view_of(kv, table, table_ld, n_seq), a,
+                       kr_fault_word());
+    kr_check_launch("paged_attention");
+}
+
+extern "C" size_t krh_paged_evict_ws(int n_seq, int n_kv_heads, int keep) {
+    if (n_seq <= 0 || n_kv_heads <= 0 || keep <= 0) return 0;
+    return sizeof(int) * ((size_t)n_seq * n_kv_heads * keep + n_seq);
+}
+
+extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table_ld, const int *len, const float *mass,
+                                size_t mass_ld, int n_seq, int max_len, int keep, int recent, const int *out_table,
+                                int out_table_ld, int *out_len, float *out_mass, size_t out_ld, void *ws) {
+    if (n_seq == 0) return;
+    if (refuse(pages_ok(kv), "paged_evict: the pages") ||
+        refuse(n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && keep > 0 && recent >= 0 && recent <= keep && table_ld > 0 &&
+                   out_table_ld > 0, "paged_evict sizes") ||
+        refuse(table && len && mass && out_table && out_len && out_mass && ws && !((uintptr_t)ws & 3) && out_table != table,
+               "paged_evict: a missing array, or the pages onto themselves") ||
+        refuse(mass_ld >= (size_t)max_len && out_ld >= (size_t)keep && (out_mass != mass || out_ld == mass_ld),
+               "paged_evict: mass rows") ||
+        refuse((size_t)out_table_ld * kv->page_size >= (size_t)(keep < max_len ? keep : max_len), "paged_evict: out_table's pages"))
+        return;
+    int *w = (int *)ws;
+    const EvArgs a = { len, mass, mass_ld, max_len, keep, recent, out_table, out_table_ld, out_len, out_mass, out_ld, w + n_seq, w };
+    hipLaunchKernelGGL(k_evict_select, dim3(kv->n_kv_heads, n_seq), dim3(EV_T), 0, kr_stream(), a, kr_fault_word());
+    kr_check_launch("paged_evict");
+    const int rb = kv->head_dim * (kv->kv_type == ML_F32 ? 4 : kv->kv_type == ML_F16 ? 2 : 1);
+    const PgView p = view_of(kv, table, table_ld, n_seq);
+    const int rows = keep < max_len ? keep : max_len;
+    const size_t units = (size_t)rows * (rb % 16 ? rb / 8 : rb / 16), want = (units + 4 * PG_T - 1) / (4 * PG_T);
+    const dim3 grid((unsigned)(want < 1024 ? want : 1024), kv->n_kv_heads, n_seq);
+    if (rb % 16)
+        hipLaunchKernelGGL(k_evict_move<uint2>, grid, dim3(PG_T), 0, kr_stream(), p, a, rb, kr_fault_word());
+    else
+        hipLaunchKernelGGL(k_evict_move<uint4>, grid, dim3(PG_T), 0, kr_stream(), p, a, rb, kr_fault_word());
+    kr_check_launch("paged_evict");
+}

@@ -4,6 +4,7 @@
 #include <stdio.h>
 #include <string.h>
 #include "kr_internal.h"
+#include "kr_paged.h"
 
 static int g_ready = 0;
 static hipStream_t g_stream = nullptr;
@@ -11,8 +12,10 @@ static char g_arch[64] = "";
 static int g_cus = 0;
 static ml_status g_status = ML_OK;
 static char g_msg[512] = "";
+static int *g_fault = nullptr;   // KR_FAULT_WORDS ints
 
 hipStream_t kr_stream(void) { return g_stream; }
+int *kr_fault_word(void) { return g_fault; }
 
 void kr_fail(ml_status st, const char *what, hipError_t e) {
     if (g_status != ML_OK) return;
@@ -47,6 +50,12 @@ extern "C" ml_status krh_init(void) {
         snprintf(g_msg, sizeof g_msg, "cannot take the address of the attention scratch array");
         return ML_E_ISA;
     }
+    void *f = nullptr;
+    if (!g_fault && hipHostMalloc(&f, KR_FAULT_WORDS * sizeof(int), hipHostMallocDefault) != hipSuccess) {
+        snprintf(g_msg, sizeof g_msg, "cannot allocate the fault words");
+        return ML_E_ISA;
+    }
+    if (f) g_fault = (int *)memset(f, 0, KR_FAULT_WORDS * sizeof(int));
     if (hipStreamCreateWithFlags(&g_stream, hipStreamNonBlocking) != hipSuccess) {
         snprintf(g_msg, sizeof g_msg, "cannot create a stream");
         return ML_E_ISA;
@@ -60,6 +69,20 @@ extern "C" int krh_device_cus(void) { return g_cus; }
 extern "C" ml_status krh_status(void) { return g_status; }
 extern "C" const char *krh_last_error(void) { return g_msg; }
 extern "C" void krh_clear_error(void) { g_status = ML_OK; g_msg[0] = 0; }
+
+// what the kernels since the last look reported (the stream is idle)
+static void take_faults(void) {
+    static const char *const what[KR_FAULT_WORDS] = {
+        "a page id or row outside the page table or the pool", "a length or count outside its range",
+        "a sequence outside the page table", "a position outside the RoPE tables"
+    };
+    volatile int *f = g_fault;
+    for (int i = 0; f && i < KR_FAULT_WORDS; i++)
+        if (f[i]) {
+            f[i] = 0;
+            kr_fail(ML_E_SHAPE, what[i], hipSuccess);
+        }
+}
 
 extern "C" void *krh_alloc(size_t bytes) {
     void *p = nullptr;
@@ -91,6 +114,7 @@ extern "C" void krh_copy_d2d_async(void *dst, const void *src, size_t bytes) {
 extern "C" ml_status krh_sync(void) {
     const hipError_t e = hipStreamSynchronize(g_stream);
     if (e != hipSuccess) kr_fail(ML_E_IO, "device fault", e);
+    else take_faults();
     return g_status;
 }
 

@@ -53,6 +53,17 @@ class KrhMat(C.Structure):
                 ("d16", C.c_int)]
 
 
+class KrhPages(C.Structure):
+    """krh_pages: one layer's pool of cache pages, device pointers"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("kd", C.c_void_p), ("vd", C.c_void_p), ("kv_type", C.c_int),
+                ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
+
+
+class LogitRule(C.Structure):
+    """krh_logit_rule: one row's penalties and token mask"""
+    _fields_ = [("repeat", C.c_float), ("presence", C.c_float), ("frequency", C.c_float), ("mask", C.c_int)]
+
+
 class GenSpec(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("dim", "n_layers", "n_heads", "n_kv_heads", "hidden_dim", "vocab",
                                        "max_seq")] + [
@@ -174,6 +185,18 @@ for name, res, args in [
     ("krh_softcap_att", None, [_P, C.c_int, C.c_int, C.c_int, _P, C.c_int, C.c_float]),
     ("krh_attention_kv_softcap", None, [_P, _P, _P, C.POINTER(MlKvLayer), C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _P, C.c_int,
                                         C.c_int, C.c_float]),
+    ("krh_paged_qkv", None, [_P, C.c_size_t, C.POINTER(KrhPages), _P, C.c_int, C.c_int, _P, C.c_size_t, _P, C.c_size_t,
+                             _P, C.c_size_t, C.c_int, C.c_int, _P, _P, _P, _P, _P, C.c_float, _P, _P, C.c_int]),
+    ("krh_paged_load", None, [_P, C.c_size_t, _P, C.c_size_t, C.POINTER(KrhPages), _P, C.c_int, C.c_int, C.c_int, _P,
+                              _P]),
+    ("krh_paged_attention_ws", C.c_size_t, [C.POINTER(KrhPages), C.c_int, C.c_int, C.c_int, C.c_int]),
+    ("krh_paged_attention", None, [_P, C.POINTER(KrhPages), _P, C.c_int, _P, C.c_int, _P, C.c_int, C.c_int, C.c_int,
+                                   C.c_float, C.c_float, _P, C.c_size_t, _P]),
+    ("krh_paged_evict_ws", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    ("krh_paged_evict", None, [C.POINTER(KrhPages), _P, C.c_int, _P, _P, C.c_size_t, C.c_int, C.c_int, C.c_int,
+                               C.c_int, _P, C.c_int, _P, _P, C.c_size_t, _P]),
+    ("krh_logit_rules", None, [_P, C.c_size_t, _P, C.c_size_t, C.c_int, C.c_int, _P, _P, C.c_size_t, _P, _P, _P,
+                               C.c_size_t, _P, _P, C.c_int]),
     ("krh_tanhf_range", None, [_P, C.c_uint32, C.c_size_t]),
     ("krh_rmsnorm_q8_t", None, [_P, _P, C.c_int, _P, _P, _P, C.c_int, C.c_float, C.c_int]),
     ("krh_quantize_q8_t", None, [_P, _P, C.c_int, _P, C.c_int, C.c_int]),
