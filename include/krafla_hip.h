@@ -351,7 +351,7 @@ uint64_t krh_sampler_rng(const krh_sampler *s);
  * stream, graphs among them, may share it. */
 typedef struct {
     void *k, *v;        /* ML_F32 floats, ML_F16 halves or ML_Q8_0 int8; 16-byte aligned */
-    float *kd, *vd;     /* ML_Q8_0: a scale a row, [n_pages][n_kv_heads][page_size]; else unused */
+    float *kd, *vd;     /* ML_Q8_0: a scale a row, [n_pages][n_kv_heads][page_size], 16-byte aligned; else unused */
     int kv_type;
     int n_pages;
     int page_size;      /* a power of two, 16 to 1024 */
@@ -364,7 +364,9 @@ typedef struct {
  * the n_pos-row tables when cos_t is non-NULL (krh_heads_norm_rope; head_dim /
  * 2 floats a row); keys and values are converted as krh_store_kv does (F32 as they are). The
  * same bits as those calls, but that the norm's sum of squares is formed in 64
- * bits instead of in index order in 32. n_heads 0: no queries (q, qo unused); qo may be q. q, qo,
+ * bits instead of in index order in 32, and a Q8 row's factor as 127 times the
+ * reciprocal of its maximum instead of their quotient (an element next to a border
+ * may round to its other side). n_heads 0: no queries (q, qo unused); qo may be q. q, qo,
  * k, v, the norms and tables 16-byte aligned, row strides multiples of 4; the rows
  * of a call are distinct. pos may be NULL without tables. */
 void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const int *table, int table_ld, int n_seq,

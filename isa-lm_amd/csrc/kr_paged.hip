@@ -4,24 +4,11 @@
 #include "kr_internal.h"
 #include "kr_numerics.h"
 #include "kr_paged.h"
+#include "kr_paged_dev.h"
 
 namespace {
 
 constexpr int PG_T = 256;
-
-enum { PG_F32 = ML_F32, PG_Q8 = ML_Q8_0, PG_F16 = ML_F16 };
-
-// a pool and the view of its sequences
-struct PgView {
-    void *k, *v;
-    float *kd, *vd;
-    const int *table;
-    int ld, n_seq, n_pages, shift, n_kv, hd;
-};
-
-__device__ __forceinline__ int pg_page(const PgView &p, int seq, int row, int &bad) {
-    return kr_page_of(p.table + (size_t)seq * p.ld, p.ld, row, p.shift, p.n_pages, bad);
-}
 
 // ---- rows into and out of pages ----
 // An item is one head's vector of one token; 2^LPS >= hd / 4 lanes share it,
@@ -49,7 +36,9 @@ struct QkvArgs {
 };
 
 // row `at` (in rows of the pool) of K or V from four values a lane, l < hd / 4;
-// the conversions of krh_store_kv
+// the conversions of krh_store_kv, but that an 8-bit row's factor is 127 times
+// the rounded reciprocal of its maximum, as tensor libraries form 127 / max (a
+// step of the factor at most: an element next to a border may fall on its other side)
 template <int KT> __device__ __forceinline__ void pg_store(void *dst, float *d, size_t at, int hd, float4 x, int l, bool live, int n) {
     const size_t e = at * hd + 4 * l;
     if (KT == PG_F32) {
@@ -61,7 +50,7 @@ template <int KT> __device__ __forceinline__ void pg_store(void *dst, float *d, 
         float m = live ? fmaxf(fmaxf(fmaxf(fmaxf(0.0f, fabsf(x.x)), fabsf(x.y)), fabsf(x.z)), fabsf(x.w)) : 0.0f;
         m = pg_max(m, n);
         const bool zero = m < KR_QUANT_TINY;
-        const float id = zero ? 0.0f : kr_fdiv(127.0f, m);
+        const float id = zero ? 0.0f : kr_fmul(127.0f, kr_fdiv(1.0f, m));
         char4 c = make_char4(0, 0, 0, 0);
         if (!zero)
             c = make_char4((signed char)kr_q8_elem(x.x, id), (signed char)kr_q8_elem(x.y, id),
@@ -144,78 +133,6 @@ template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_load(const PgV
     if (!bad) x = pg_load4<KT>(isk ? p.k : p.v, isk ? p.kd : p.vd, at, p.hd, l);
     if (l == 0) kr_report(fault, bad);
     *(float4 *)((isk ? k + (size_t)i * ldk : v + (size_t)i * ldv) + (size_t)kvh * p.hd + 4 * l) = x;
-}
-
-// ---- attention ----
-
-struct AttArgs {
-    float *o;
-    const float *q;
-    const int *len;
-    float *mass;
-    size_t mass_ld;
-    float *ws;
-    int nh, max_len, window;
-    float scale, cap;
-};
-
-// one workgroup a (sequence, KV head), a query head at a time: scores to the
-// workspace, their maximum and sum, then a lane a dim over the rows
-template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_attn(const PgView p, const AttArgs a, int *fault) {
-    __shared__ float red[PG_T / 64];
-    __shared__ float qs[KR_PAGE_HD_MAX];
-    const int s = blockIdx.y, kvh = blockIdx.x, tid = threadIdx.x, hd = p.hd, group = a.nh / p.n_kv;
-    int bad = 0;
-    const int len = kr_page_len(a.len[s], a.max_len, bad);
-    const int first = a.window > 0 && len > a.window ? len - a.window : 0;
-    for (int g = 0; g < group; g++) {
-        const int h = kvh * group + g;
-        const size_t qat = ((size_t)s * a.nh + h) * hd;
-        float *z = a.ws + ((size_t)s * a.nh + h) * a.max_len;
-        for (int d = tid; d < hd; d += PG_T) qs[d] = a.q[qat + d];
-        __syncthreads();
-        float m = -INFINITY;
-        for (int r = first + tid; r < len; r += PG_T) {
-            const size_t at = kr_page_row(pg_page(p, s, r, bad), p.n_kv, kvh, p.shift, r);
-            float acc = 0.0f;
-            for (int l = 0; 4 * l < hd; l++) {
-                const float4 x = pg_load4<KT>(p.k, p.kd, at, hd, l);
-                acc += qs[4 * l] * x.x + qs[4 * l + 1] * x.y + qs[4 * l + 2] * x.z + qs[4 * l + 3] * x.w;
-            }
-            acc *= a.scale;
-            if (a.cap > 0.0f) acc = a.cap * kr_tanhf(acc / a.cap);
-            z[r] = acc;
-            m = fmaxf(m, acc);
-        }
-        m = pg_max(m, 64);
-        if ((tid & 63) == 0) red[tid >> 6] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        __syncthreads();
-        float sum = 0.0f;
-        for (int r = first + tid; r < len; r += PG_T) {
-            z[r] = kr_expf(z[r] - m);
-            sum += z[r];
-        }
-        for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
-        if ((tid & 63) == 0) red[tid >> 6] = sum;
-        __threadfence_block();
-        __syncthreads();
-        const float inv = 1.0f / (red[0] + red[1] + red[2] + red[3]);
-        for (int d = tid; d < hd; d += PG_T) {
-            float acc = 0.0f;
-            for (int r = first; r < len; r++) {
-                const size_t at = kr_page_row(pg_page(p, s, r, bad), p.n_kv, kvh, p.shift, r);
-                const float4 x = pg_load4<KT>(p.v, p.vd, at, hd, d >> 2);
-                acc += z[r] * ((d & 2) ? ((d & 1) ? x.w : x.z) : ((d & 1) ? x.y : x.x));
-            }
-            a.o[qat + d] = len > 0 ? acc * inv : 0.0f;
-        }
-        if (a.mass)
-            for (int r = first + tid; r < len; r += PG_T) a.mass[((size_t)s * p.n_kv + kvh) * a.mass_ld + r] += z[r] * inv;
-        __syncthreads();
-    }
-    kr_report(fault, bad);
 }
 
 // ---- eviction ----
@@ -352,33 +269,6 @@ template <class U> __global__ void __launch_bounds__(PG_T) k_evict_move(const Pg
     kr_report(fault, bad);
 }
 
-int log2_of(int v) {
-    int l = 0;
-    while ((1 << l) < v) l++;
-    return l;
-}
-
-bool pages_ok(const krh_pages *kv) {
-    return kv && kv->k && kv->v && !(((uintptr_t)kv->k | (uintptr_t)kv->v) & 15) && kv->n_pages > 0 &&
-           kv->page_size >= KR_PAGE_MIN && kv->page_size <= KR_PAGE_MAX && !(kv->page_size & (kv->page_size - 1)) &&
-           kv->n_kv_heads > 0 && kv->n_kv_heads <= KRH_ROWS_MAX && kv->head_dim >= 8 && kv->head_dim <= KR_PAGE_HD_MAX &&
-           kv->head_dim % 8 == 0 &&
-           (kv->kv_type == ML_F32 || kv->kv_type == ML_F16 || (kv->kv_type == ML_Q8_0 && kv->kd && kv->vd));
-}
-
-bool aligned16(const void *p) { return !((uintptr_t)p & 15); }
-
-PgView view_of(const krh_pages *kv, const int *table, int ld, int n_seq) {
-    const bool q8 = kv->kv_type == ML_Q8_0;
-    return { kv->k, kv->v, q8 ? kv->kd : nullptr, q8 ? kv->vd : nullptr, table, ld, n_seq, kv->n_pages, log2_of(kv->page_size),
-             kv->n_kv_heads, kv->head_dim };
-}
-
-bool refuse(bool ok, const char *what) {
-    if (!ok) kr_fail(ML_E_SHAPE, what, hipSuccess);
-    return !ok;
-}
-
 // workgroups for `items` items of 2^lps lanes; 0: more than a launch holds
 unsigned item_blocks(size_t items, int lps) {
     const size_t b = ((items << lps) + PG_T - 1) / PG_T;
@@ -392,22 +282,22 @@ extern "C" void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const
                               int ntok, int n_heads, const int *seq, const int *row, const int *pos,
                               const float *q_norm, const float *k_norm, float eps, const float *cos_t,
                               const float *sin_t, int n_pos) {
-    if (refuse(pages_ok(kv), "paged_qkv: the pages") ||
-        refuse(ntok >= 0 && n_heads >= 0 && n_heads <= KRH_ROWS_MAX && n_seq > 0 && table_ld > 0, "paged_qkv sizes"))
+    if (pg_refuse(pg_pages_ok(kv), "paged_qkv: the pages") ||
+        pg_refuse(ntok >= 0 && n_heads >= 0 && n_heads <= KRH_ROWS_MAX && n_seq > 0 && table_ld > 0, "paged_qkv sizes"))
         return;
     if (ntok == 0) return;
     const size_t kvd = (size_t)kv->n_kv_heads * kv->head_dim, qd = (size_t)n_heads * kv->head_dim;
-    if (refuse(table && k && v && seq && row && (n_heads == 0 || (q && qo)) && (!cos_t) == (!sin_t) &&
+    if (pg_refuse(table && k && v && seq && row && (n_heads == 0 || (q && qo)) && (!cos_t) == (!sin_t) &&
                    (!cos_t || (pos && n_pos > 0)) && (n_heads == 0 || (!q_norm) == (!k_norm)), "paged_qkv: a missing array") ||
-        refuse(ldk >= kvd && ldv >= kvd && ldk % 4 == 0 && ldv % 4 == 0 && aligned16(k) && aligned16(v) && aligned16(k_norm) &&
-                   aligned16(cos_t) && aligned16(sin_t) &&
-                   (n_heads == 0 || (ldq >= qd && ldqo >= qd && ldq % 4 == 0 && ldqo % 4 == 0 && aligned16(q) &&
-                                     aligned16(qo) && aligned16(q_norm))), "paged_qkv: row strides or alignment"))
+        pg_refuse(ldk >= kvd && ldv >= kvd && ldk % 4 == 0 && ldv % 4 == 0 && pg_aligned(k) && pg_aligned(v) && pg_aligned(k_norm) &&
+                   pg_aligned(cos_t) && pg_aligned(sin_t) &&
+                   (n_heads == 0 || (ldq >= qd && ldqo >= qd && ldq % 4 == 0 && ldqo % 4 == 0 && pg_aligned(q) &&
+                                     pg_aligned(qo) && pg_aligned(q_norm))), "paged_qkv: row strides or alignment"))
         return;
-    const int lps = log2_of(kv->head_dim / 4);
+    const int lps = pg_log2(kv->head_dim / 4);
     const unsigned grid = item_blocks((size_t)ntok * (n_heads + 2 * (size_t)kv->n_kv_heads), lps);
-    if (refuse(grid > 0, "paged_qkv: too many tokens")) return;
-    const PgView p = view_of(kv, table, table_ld, n_seq);
+    if (pg_refuse(grid > 0, "paged_qkv: too many tokens")) return;
+    const PgView p = pg_view(kv, table, table_ld, n_seq);
     const QkvArgs a = { qo, q, k, v, q_norm, k_norm, cos_t, sin_t, seq, row, pos, ldqo, ldq, ldk, ldv, eps, ntok, n_heads, n_pos };
     const auto f = kv->kv_type == ML_F32 ? k_paged_qkv<PG_F32> : kv->kv_type == ML_F16 ? k_paged_qkv<PG_F16> : k_paged_qkv<PG_Q8>;
     hipLaunchKernelGGL(f, dim3(grid), dim3(PG_T), 0, kr_stream(), p, a, lps, kr_fault_word());
@@ -416,46 +306,20 @@ extern "C" void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const
 
 extern "C" void krh_paged_load(float *k, size_t ldk, float *v, size_t ldv, const krh_pages *kv, const int *table,
                                int table_ld, int n_seq, int n, const int *seq, const int *row) {
-    if (refuse(pages_ok(kv), "paged_load: the pages") || refuse(n >= 0 && n_seq > 0 && table_ld > 0, "paged_load sizes")) return;
+    if (pg_refuse(pg_pages_ok(kv), "paged_load: the pages") || pg_refuse(n >= 0 && n_seq > 0 && table_ld > 0, "paged_load sizes")) return;
     if (n == 0) return;
     const size_t kvd = (size_t)kv->n_kv_heads * kv->head_dim;
-    if (refuse(table && k && v && seq && row, "paged_load: a missing array") ||
-        refuse(ldk >= kvd && ldv >= kvd && ldk % 4 == 0 && ldv % 4 == 0 && aligned16(k) && aligned16(v),
+    if (pg_refuse(table && k && v && seq && row, "paged_load: a missing array") ||
+        pg_refuse(ldk >= kvd && ldv >= kvd && ldk % 4 == 0 && ldv % 4 == 0 && pg_aligned(k) && pg_aligned(v),
                "paged_load: row strides or alignment"))
         return;
-    const int lps = log2_of(kv->head_dim / 4);
+    const int lps = pg_log2(kv->head_dim / 4);
     const unsigned grid = item_blocks((size_t)n * 2 * kv->n_kv_heads, lps);
-    if (refuse(grid > 0, "paged_load: too many rows")) return;
+    if (pg_refuse(grid > 0, "paged_load: too many rows")) return;
     const auto f = kv->kv_type == ML_F32 ? k_paged_load<PG_F32> : kv->kv_type == ML_F16 ? k_paged_load<PG_F16> : k_paged_load<PG_Q8>;
-    hipLaunchKernelGGL(f, dim3(grid), dim3(PG_T), 0, kr_stream(), view_of(kv, table, table_ld, n_seq), k, ldk, v, ldv, n, seq, row,
+    hipLaunchKernelGGL(f, dim3(grid), dim3(PG_T), 0, kr_stream(), pg_view(kv, table, table_ld, n_seq), k, ldk, v, ldv, n, seq, row,
                        lps, kr_fault_word());
     kr_check_launch("paged_load");
-}
-
-static bool attention_sizes(const krh_pages *kv, int n_seq, int n_heads, int max_len) {
-    return pages_ok(kv) && n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && n_heads > 0 && n_heads % kv->n_kv_heads == 0 &&
-           n_heads / kv->n_kv_heads <= KR_PAGE_GROUP_MAX;
-}
-
-extern "C" size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int max_len, int mass) {
-    if (!attention_sizes(kv, n_seq, n_heads, max_len)) return 0;
-    return sizeof(float) * (size_t)n_seq * n_heads * max_len;
-}
-
-extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len,
-                                    int n_seq, const float *q, int n_heads, int max_len, int window, float scale,
-                                    float softcap, float *mass, size_t mass_ld, void *ws) {
-    if (n_seq == 0) return;
-    if (refuse(attention_sizes(kv, n_seq, n_heads, max_len), "paged_attention sizes") ||
-        refuse(o && table && table_ld > 0 && len && q && ws && aligned16(o) && aligned16(q) && aligned16(ws),
-               "paged_attention: a missing or unaligned array") ||
-        refuse(window >= 0 && softcap >= 0.0f && (!mass || mass_ld >= (size_t)max_len), "paged_attention: window, soft-cap or mass rows"))
-        return;
-    const AttArgs a = { o, q, len, mass, mass_ld, (float *)ws, n_heads, max_len, window, scale, softcap };
-    const auto f = kv->kv_type == ML_F32 ? k_paged_attn<PG_F32> : kv->kv_type == ML_F16 ? k_paged_attn<PG_F16> : k_paged_attn<PG_Q8>;
-    hipLaunchKernelGGL(f, dim3(kv->n_kv_heads, n_seq), dim3(PG_T), 0, kr_stream(), view_of(kv, table, table_ld, n_seq), a,
-                       kr_fault_word());
-    kr_check_launch("paged_attention");
 }
 
 extern "C" size_t krh_paged_evict_ws(int n_seq, int n_kv_heads, int keep) {
@@ -467,21 +331,21 @@ extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table
                                 size_t mass_ld, int n_seq, int max_len, int keep, int recent, const int *out_table,
                                 int out_table_ld, int *out_len, float *out_mass, size_t out_ld, void *ws) {
     if (n_seq == 0) return;
-    if (refuse(pages_ok(kv), "paged_evict: the pages") ||
-        refuse(n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && keep > 0 && recent >= 0 && recent <= keep && table_ld > 0 &&
+    if (pg_refuse(pg_pages_ok(kv), "paged_evict: the pages") ||
+        pg_refuse(n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && keep > 0 && recent >= 0 && recent <= keep && table_ld > 0 &&
                    out_table_ld > 0, "paged_evict sizes") ||
-        refuse(table && len && mass && out_table && out_len && out_mass && ws && !((uintptr_t)ws & 3) && out_table != table,
+        pg_refuse(table && len && mass && out_table && out_len && out_mass && ws && !((uintptr_t)ws & 3) && out_table != table,
                "paged_evict: a missing array, or the pages onto themselves") ||
-        refuse(mass_ld >= (size_t)max_len && out_ld >= (size_t)keep && (out_mass != mass || out_ld == mass_ld),
+        pg_refuse(mass_ld >= (size_t)max_len && out_ld >= (size_t)keep && (out_mass != mass || out_ld == mass_ld),
                "paged_evict: mass rows") ||
-        refuse((size_t)out_table_ld * kv->page_size >= (size_t)(keep < max_len ? keep : max_len), "paged_evict: out_table's pages"))
+        pg_refuse((size_t)out_table_ld * kv->page_size >= (size_t)(keep < max_len ? keep : max_len), "paged_evict: out_table's pages"))
         return;
     int *w = (int *)ws;
     const EvArgs a = { len, mass, mass_ld, max_len, keep, recent, out_table, out_table_ld, out_len, out_mass, out_ld, w + n_seq, w };
     hipLaunchKernelGGL(k_evict_select, dim3(kv->n_kv_heads, n_seq), dim3(EV_T), 0, kr_stream(), a, kr_fault_word());
     kr_check_launch("paged_evict");
     const int rb = kv->head_dim * (kv->kv_type == ML_F32 ? 4 : kv->kv_type == ML_F16 ? 2 : 1);
-    const PgView p = view_of(kv, table, table_ld, n_seq);
+    const PgView p = pg_view(kv, table, table_ld, n_seq);
     const int rows = keep < max_len ? keep : max_len;
     const size_t units = (size_t)rows * (rb % 16 ? rb / 8 : rb / 16), want = (units + 4 * PG_T - 1) / (4 * PG_T);
     const dim3 grid((unsigned)(want < 1024 ? want : 1024), kv->n_kv_heads, n_seq);
