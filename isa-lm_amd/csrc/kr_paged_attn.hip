@@ -1,9 +1,11 @@
 // Attention of one token of each sequence over a paged cache (krh_paged_attention).
 //
-// A workgroup takes a chunk of one sequence's rows for one KV head, its four waves
-// every fourth tile of 32 rows; each wave passes over its rows once with the running
-// maximum and sum of the softmax. The waves' parts are joined in LDS, a
-// sequence's chunks by a second launch.
+// The rows of all sequences, in tiles of 32, are cut into equal shares, one a
+// wave and KV head (pa_share): the lengths decide on the device, so a batch of all
+// lengths loads the chip as one long sequence does. A wave passes over each
+// sequence's part of its share once with the running maximum and sum of the
+// softmax; a sequence within one share is done, the others' parts are joined by a second
+// launch (k_paged_join), which finds them by the same arithmetic.
 //
 // Both products run on the matrix cores, transposed so that nothing passes
 // through LDS: S^T = K Q^T has rows as the tile's rows and query heads as its
@@ -25,8 +27,9 @@
 
 namespace {
 
-constexpr int PA_T = 256, PA_W = PA_T / 64, PA_TILE = 32, PA_STEP = PA_W * PA_TILE;
-constexpr float PA_UP = 0x1p14f;   // the weights' scale (halves end at 2^16)
+constexpr int PA_TILE = 32;
+constexpr int PA_SHARE = 4;        // tiles that a share is worth at least
+constexpr float PA_UP = 14.0f;     // the weights' scale (log2; halves end at 2^16)
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -41,34 +44,84 @@ struct PaArgs {
     const int *len;
     float *mass;
     size_t mass_ld;
-    float *part;    // [n_seq][nh][n_split][hd]: a chunk's sums
-    float *pml;     // [n_seq][nh][n_split][2]: their maximum (log2) and weight
-    float *fin;     // [n_seq][nh][2]: the whole row's, for the mass
+    float *part;    // [n_kv][n_seq + shares][group][hd]: a share's sums of a sequence, at their numbers' sum
+    float *pml;     // [n_kv][n_seq + shares][group][2]: their maximum (log2) and weight
     float *z;       // [n_seq][nh][z_ld]: the scores (log2), for the mass
     size_t z_ld;
-    int nh, max_len, window, chunk, n_split;
-    float scale, cap;
+    int nh, max_len, window, shares;
+    float scale, cap, z_up;   // z_up: log2 of the weights' scale in the sums
 };
 
-// rows [first, len) of a sequence in chunks from the tile that holds `first`
+// rows [first, len) of a sequence, in tiles from the one that holds `first`; a
+// sequence of no rows has one tile, whose output is zeros
 struct PaSpan {
-    int len, first, begin, parts;
+    int len, first, begin, tiles;
 };
-__device__ __forceinline__ PaSpan pa_span(const PaArgs &a, int s, int &bad) {
+__device__ __forceinline__ PaSpan pa_span(const PaArgs &a, int len, int &bad) {
     PaSpan r;
-    r.len = kr_page_len(a.len[s], a.max_len, bad);
+    r.len = kr_page_len(len, a.max_len, bad);
     r.first = a.window > 0 && r.len > a.window ? r.len - a.window : 0;
     r.begin = r.first & ~(PA_TILE - 1);
-    r.parts = (r.len - r.begin + a.chunk - 1) / a.chunk;
+    r.tiles = max(1, (r.len - r.begin + PA_TILE - 1) / PA_TILE);
     return r;
+}
+
+// Inclusive sums over the wave's lanes
+__device__ __forceinline__ int pa_scan(int v) {
+    for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(v, o);
+        if ((int)(threadIdx.x & 63) >= o) v += t;
+    }
+    return v;
+}
+
+// All sequences' tiles, and how many shares they make: share u has tiles
+// [u T / n, (u + 1) T / n)
+struct PaAll {
+    int tiles, shares;
+};
+__device__ __forceinline__ PaAll pa_all(const PgView &p, const PaArgs &a, int &bad) {
+    const int lane = threadIdx.x & 63;
+    int t = 0;
+    for (int i = lane; i < p.n_seq; i += 64) t += pa_span(a, a.len[i], bad).tiles;
+    for (int o = 32; o >= 1; o >>= 1) t += __shfl_xor(t, o);
+    t = __builtin_amdgcn_readfirstlane(t);
+    return { t, max(1, min(a.shares, (t + PA_SHARE - 1) / PA_SHARE)) };
+}
+// the sequence that holds tile t of all, and the tile's number in it
+__device__ __forceinline__ int pa_find(const PgView &p, const PaArgs &a, int &t, int &bad) {
+    const int lane = threadIdx.x & 63;
+    for (int i0 = 0;; i0 += 64) {
+        const int i = i0 + lane, own = i < p.n_seq ? pa_span(a, a.len[i], bad).tiles : 0, sum = pa_scan(own);
+        const int n = __popcll(__ballot(i < p.n_seq && sum <= t));
+        if (n < 64 || i0 + 64 >= p.n_seq) {
+            t -= n ? __builtin_amdgcn_readlane(sum, n - 1) : 0;
+            return i0 + n;
+        }
+        t -= __builtin_amdgcn_readlane(sum, 63);
+    }
+}
+__device__ __forceinline__ int pa_bound(const PaAll &all, int u) { return (int)((long long)all.tiles * u / all.shares); }
+// the share that holds tile t
+__device__ __forceinline__ int pa_share(const PaAll &all, int t) {
+    return (int)((((long long)t + 1) * all.shares - 1) / all.tiles);
 }
 
 __device__ __forceinline__ float pa_swap8(float x) {   // the lane 8 away in its row of 16
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
 }
-__device__ __forceinline__ float pa_max_g(float v) {   // over the 4 lanes of a column
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+// over the 4 lanes of a column: both halves, then both rows of each, swapped in registers
+__device__ __forceinline__ float pa_max_g(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float pa_sum_g(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 // halves of 4 int8 (xor 0x80: 0..255) as 1024 + u - 1152, exact
@@ -85,6 +138,7 @@ template <int KT, int CL> struct PaRaw {
     static constexpr int KB = KT == PG_F32 ? 4 : KT == PG_F16 ? 4 : 2; // words a load
     static constexpr int VB = KT == PG_F32 ? W : KT == PG_F16 ? W / 2 : W / 4;
     unsigned k[2][KS][KB], v[8][VB];
+    float kd[KT == PG_Q8 ? 8 : 1], vd[KT == PG_Q8 ? 8 : 1];
 };
 
 template <int N> __device__ __forceinline__ void pa_load(unsigned (&x)[N], const void *p) {
@@ -107,94 +161,104 @@ template <int N> __device__ __forceinline__ void pa_load(unsigned (&x)[N], const
     }
 }
 
-template <int KT, int CL, int NB, bool FULL>
-__global__ void __launch_bounds__(PA_T, KT == PG_F32 ? 1 : 2) k_paged_split(const PgView p, const PaArgs a, int *fault) {
+// Whether two tiles' rows fit in registers: the next tile's are read while one
+// is worked on; where they do not, its K rows are, once this tile's are used.
+constexpr bool pa_two(int kt, int cl) { return cl <= (kt == PG_F32 ? 64 : 128); }
+constexpr int pa_waves(int kt, int cl) { return pa_two(kt, cl) || kt == PG_Q8 ? 2 : 1; }   // a SIMD
+
+template <int KT, int CL, int NB, bool FULL> struct PaWave {
     using Raw = PaRaw<KT, CL>;
-    constexpr int W = Raw::W, KS = Raw::KS, EB = KT == PG_F32 ? 4 : KT == PG_F16 ? 2 : 1;
-    constexpr int KD = KT == PG_F32 ? 4 : 8;   // dims a K load
-    constexpr bool HALF = KT != PG_F32;
-    __shared__ float s_o[PA_W - 1][W * 4][64];
-    __shared__ float s_m[PA_W][16], s_l[PA_W][16];
+    static constexpr int W = Raw::W, KS = Raw::KS, EB = KT == PG_F32 ? 4 : KT == PG_F16 ? 2 : 1;
+    static constexpr int KD = KT == PG_F32 ? 4 : 8;   // dims a K load
+    static constexpr bool HALF = KT != PG_F32;
 
-    const int s = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = lane & 15, g = lane >> 4, hd = FULL ? CL : p.hd, group = a.nh / p.n_kv;
-    int bad = 0;
-    const PaSpan sp = pa_span(a, s, bad);
-    if (split >= (sp.parts > 1 ? sp.parts : 1)) return;
-
-    const int col = NB == 1 && HALF ? n & 7 : n;
-    const bool live = col < group, is_lo = NB == 1 && HALF && n >= 8;
-    const size_t head = (size_t)s * a.nh + kvh * group + (live ? col : 0);
-
-    // the queries as operands
-    const float *q = a.q + head * hd;
+    const PgView &p;
+    const PaArgs &a;
+    const int lane, n, g, kvh, hd, group, col;
+    const bool live, is_lo;
+    int seq, t_ids, bad;
+    PaSpan sp;
+    int ids;   // the pages of 64 half tiles from t_ids on, one a lane
     float qf[HALF ? 1 : KS][4];
     half8 qh[HALF ? KS : 1][NB];
-    int e = 0;
-    if (HALF) {
-        float x[KS][8], m = 0.0f;
-#pragma unroll
-        for (int j = 0; j < KS; j++) {
-            const int d = j * 32 + g * 8;
-            const bool in = live && (FULL || d < hd);
-#pragma unroll
-            for (int i = 0; i < 8; i += 4) {
-                const float4v t = in ? *(const float4v *)(q + d + i) : float4v{ 0, 0, 0, 0 };
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    x[j][i + c] = t[c];
-                    m = fmaxf(m, fabsf(t[c]));
-                }
-            }
-        }
-        m = pa_max_g(m);
-        if (m > 0.0f && m < INFINITY) e = 13 - ilogbf(m);
-#pragma unroll
-        for (int j = 0; j < KS; j++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float y = ldexpf(x[j][i], e);
-                const _Float16 hi = (_Float16)y;
-                const _Float16 lo = (_Float16)(y - (float)hi);
-                if (NB == 1) {
-                    qh[j][0][i] = is_lo ? lo : hi;
-                } else {
-                    qh[j][0][i] = hi;
-                    qh[j][NB - 1][i] = lo;
-                }
-            }
-    } else {
-#pragma unroll
-        for (int j = 0; j < KS; j++) {
-            const int d = j * 16 + g * 4;
-            const float4v t = live && (FULL || d < hd) ? *(const float4v *)(q + d) : float4v{ 0, 0, 0, 0 };
-#pragma unroll
-            for (int c = 0; c < 4; c++) qf[j][c] = t[c];
-        }
+    float cs, m_run, l_run;
+    int ev;    // Q8: the weights carry the V scales over 2^ev
+    float4v o[W];
+
+    __device__ __forceinline__ PaWave(const PgView &p_, const PaArgs &a_, int kvh_)
+        : p(p_), a(a_), lane(threadIdx.x & 63), n(lane & 15), g(lane >> 4), kvh(kvh_), hd(FULL ? CL : p_.hd),
+          group(a_.nh / p_.n_kv), col(NB == 1 && HALF ? n & 7 : n), live(col < group), is_lo(NB == 1 && HALF && n >= 8),
+          bad(0) {}
+
+    __device__ __forceinline__ size_t head() const { return (size_t)seq * a.nh + kvh * group + (live ? col : 0); }
+
+    // the pages of the half tiles from row t0 on that have rows attended; 0 elsewhere
+    __device__ __forceinline__ void find(int t0) {
+        t_ids = t0;
+        const int r = t0 + 16 * lane;
+        ids = r + 16 > sp.first && r < sp.len ? pg_page(p, seq, r, bad) : -1;
+    }
+    // pool rows of the halves of the tile at t0; a half without rows attended takes the other's
+    __device__ __forceinline__ void rows_of(int t0, size_t &lo, size_t &hi) {
+        const int i = (t0 - t_ids) >> 4;
+        const int pl = __builtin_amdgcn_readlane(ids, i), ph = __builtin_amdgcn_readlane(ids, i + 1);
+        lo = kr_page_row(pl >= 0 ? pl : ph, p.n_kv, kvh, p.shift, t0);
+        hi = kr_page_row(ph >= 0 ? ph : pl, p.n_kv, kvh, p.shift, t0 + 16);
     }
 
-    float m_run = -INFINITY, l_run = 0.0f;
-    int ev = -120;   // Q8: the weights carry the V scales over 2^ev
-    float4v o[W];
+    // the queries as operands
+    __device__ __forceinline__ void queries() {
+        const float *q = a.q + head() * hd;
+        int e = 0;
+        if constexpr (HALF) {
+            float x[KS][8], m = 0.0f;
 #pragma unroll
-    for (int c = 0; c < W; c++) o[c] = float4v{ 0, 0, 0, 0 };
+            for (int j = 0; j < KS; j++) {
+                const int d = j * 32 + g * 8;
+                const bool in = live && (FULL || d < hd);
+#pragma unroll
+                for (int i = 0; i < 8; i += 4) {
+                    const float4v t = in ? *(const float4v *)(q + d + i) : float4v{ 0, 0, 0, 0 };
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        x[j][i + c] = t[c];
+                        m = fmaxf(m, fabsf(t[c]));
+                    }
+                }
+            }
+            m = pa_max_g(m);
+            if (m > 0.0f && m < INFINITY) e = 13 - ilogbf(m);
+#pragma unroll
+            for (int j = 0; j < KS; j++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float y = ldexpf(x[j][i], e);
+                    const _Float16 hi = (_Float16)y;
+                    const _Float16 lo = (_Float16)(y - (float)hi);
+                    if (NB == 1) {
+                        qh[j][0][i] = is_lo ? lo : hi;
+                    } else {
+                        qh[j][0][i] = hi;
+                        qh[j][NB - 1][i] = lo;
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                const int d = j * 16 + g * 4;
+                const float4v t = live && (FULL || d < hd) ? *(const float4v *)(q + d) : float4v{ 0, 0, 0, 0 };
+#pragma unroll
+                for (int c = 0; c < 4; c++) qf[j][c] = t[c];
+            }
+        }
+        // a product's factor: the scale, in log2 unless the cap comes first
+        cs = ldexpf(a.cap > 0.0f ? a.scale : a.scale * 1.4426950408889634f, -e);
+    }
 
-    const int c0 = sp.begin + split * a.chunk, c1 = min(sp.len, c0 + a.chunk);
-    Raw raw;
-    float kd[8], vd[8];
-    size_t row_lo = 0, row_hi = 0;   // pool rows of the tile's two halves
-    // a half's page, looked up where the half has rows that are attended
-    auto find = [&](int t0) {
-        const int pl = t0 + 16 > sp.first ? pg_page(p, s, t0, bad) : -1;
-        const int ph = t0 + 16 < sp.len ? pg_page(p, s, t0 + 16, bad) : -1;
-        const int lo = __builtin_amdgcn_readfirstlane(pl >= 0 ? pl : ph), hi = __builtin_amdgcn_readfirstlane(ph >= 0 ? ph : pl);
-        row_lo = kr_page_row(lo, p.n_kv, kvh, p.shift, t0);
-        row_hi = kr_page_row(hi, p.n_kv, kvh, p.shift, t0 + 16);
-    };
-    const int kr0 = 8 * (n >> 2) + (n & 3);   // this lane's K rows of the tile: kr0, kr0 + 4
-    auto load_k = [&]() {
-        const size_t r = (kr0 < 16 ? row_lo + kr0 : row_hi + (kr0 - 16));
+    // this lane's K rows of a tile are 8 (n / 4) + n % 4 and 4 after it
+    __device__ __forceinline__ void load_k(Raw &raw, size_t lo, size_t hi) const {
+        const int r0 = 8 * (n >> 2) + (n & 3);
+        const size_t r = r0 < 16 ? lo + r0 : hi + (r0 - 16);
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             const char *at = (const char *)p.k + (r + 4 * b) * hd * EB;
@@ -208,25 +272,26 @@ __global__ void __launch_bounds__(PA_T, KT == PG_F32 ? 1 : 2) k_paged_split(cons
                     for (int i = 0; i < Raw::KB; i++) raw.k[b][j][i] = in ? raw.k[b][j][i] : 0u;
             }
         }
-    };
-    const int vr0 = 8 * g;   // its V rows: vr0 .. vr0 + 7
-    auto load_v = [&]() {
-        const size_t r = vr0 < 16 ? row_lo + vr0 : row_hi + (vr0 - 16);
-        if (KT == PG_Q8) {
+    }
+    // its V rows 8 g .. 8 g + 7, dims n W ..
+    __device__ __forceinline__ void load_v(Raw &raw, size_t lo, size_t hi) const {
+        const int r0 = 8 * g;
+        const size_t r = r0 < 16 ? lo + r0 : hi + (r0 - 16);
+        if constexpr (KT == PG_Q8) {
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
                 const float4v x = *(const float4v *)(p.kd + r + i), y = *(const float4v *)(p.vd + r + i);
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    kd[i + c] = x[c];
-                    vd[i + c] = y[c];
+                    raw.kd[i + c] = x[c];
+                    raw.vd[i + c] = y[c];
                 }
             }
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const char *at = (const char *)p.v + (r + i) * hd * EB;
-            if (FULL) {
+            if constexpr (FULL) {
                 pa_load(raw.v[i], at + n * W * EB);
             } else {
                 // 4 dims at a time where a lane has them, else 8 (head_dim is a multiple of 8)
@@ -241,17 +306,10 @@ __global__ void __launch_bounds__(PA_T, KT == PG_F32 ? 1 : 2) k_paged_split(cons
                 }
             }
         }
-    };
-
-    int t0 = c0 + wave * PA_TILE;
-    if (t0 < c1) {
-        find(t0);
-        load_k();
     }
-    for (; t0 < c1; t0 += PA_STEP) {
-        load_v();
-        // scores: rows t0 + 8 g + i of head `col`, i < 8
-        float sc[8];
+
+    // products of the tile's rows 8 g + i with the queries of head `col`
+    __device__ __forceinline__ void scores(const Raw &raw, float (&sc)[8]) const {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             float4v acc = { 0, 0, 0, 0 };
@@ -277,49 +335,50 @@ __global__ void __launch_bounds__(PA_T, KT == PG_F32 ? 1 : 2) k_paged_split(cons
 #pragma unroll
             for (int i = 0; i < 4; i++) sc[4 * b + i] = acc[i];
         }
-        // the next tile's K while the rest runs
-        if (t0 + PA_STEP < c1) {
-            find(t0 + PA_STEP);
-            load_k();
-        }
+    }
+
+    // the softmax's step over the tile at t0, then its V rows by their weights
+    __device__ __forceinline__ void rest(Raw &raw, float (&sc)[8], int t0) {
         const bool whole = t0 >= sp.first && t0 + PA_TILE <= sp.len;
         const int r0 = t0 + 8 * g;
         float m_tile = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             float x = sc[i];
-            if (HALF) {
-                if (NB == 1) x += pa_swap8(x);
-                x = ldexpf(x, -e);
-            }
-            x *= a.scale;
-            if (KT == PG_Q8) x *= kd[i];
-            sc[i] = x;
+            if (NB == 1 && HALF) x += pa_swap8(x);
+            sc[i] = x * (KT == PG_Q8 ? cs * raw.kd[i] : cs);
         }
         if (a.cap > 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) sc[i] = a.cap * kr_tanhf(sc[i] / a.cap);
+            for (int i = 0; i < 8; i++) sc[i] = a.cap * kr_tanhf(sc[i] / a.cap) * 1.4426950408889634f;
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const bool in = r0 + i >= sp.first && r0 + i < sp.len;
+                sc[i] = in ? sc[i] : -INFINITY;
+                // rows that are not attended may hold anything
+                if constexpr (KT == PG_Q8) {
+                    raw.vd[i] = in ? raw.vd[i] : 0.0f;
+                } else {
+#pragma unroll
+                    for (int w = 0; w < Raw::VB; w++) raw.v[i][w] = in ? raw.v[i][w] : 0u;
+                }
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            sc[i] *= 1.4426950408889634f;
-            if (!whole && (r0 + i < sp.first || r0 + i >= sp.len)) sc[i] = -INFINITY;
-            m_tile = fmaxf(m_tile, sc[i]);
-        }
+        for (int i = 0; i < 8; i++) m_tile = fmaxf(m_tile, sc[i]);
         if (a.z && live && !is_lo) {
-            float *z = a.z + head * a.z_ld + r0;
+            float *z = a.z + head() * a.z_ld + r0;
             *(float4v *)z = float4v{ sc[0], sc[1], sc[2], sc[3] };
             *(float4v *)(z + 4) = float4v{ sc[4], sc[5], sc[6], sc[7] };
         }
         m_tile = pa_max_g(m_tile);
         int ev_new = ev;
-        if (KT == PG_Q8) {
+        if constexpr (KT == PG_Q8) {
             float vm = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if (!whole && (r0 + i < sp.first || r0 + i >= sp.len)) vd[i] = 0.0f;
-                vm = fmaxf(vm, fabsf(vd[i]));
-            }
+            for (int i = 0; i < 8; i++) vm = fmaxf(vm, fabsf(raw.vd[i]));
             vm = pa_max_g(vm);
             ev_new = max(ev, min((int)(__float_as_uint(vm) >> 23) - 126, 120));
         }
@@ -333,36 +392,36 @@ __global__ void __launch_bounds__(PA_T, KT == PG_F32 ? 1 : 2) k_paged_split(cons
 #pragma unroll
             for (int c = 0; c < W; c++) o[c] *= fo;
         }
-        const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+        // weights of no finite maximum: 0 for -inf, NaN for NaN
+        const float base = (m_run == -INFINITY ? 0.0f : m_run) - (HALF ? PA_UP : 0.0f);
         const float vs = KT == PG_Q8 ? ldexpf(1.0f, -ev) : 1.0f;
-        half8 ph[NB];
+        half8 ph[NB], pl;
         float pf[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            float x = __builtin_amdgcn_exp2f(sc[i] - m_use);
-            if (HALF) x *= PA_UP;
+            float x = __builtin_amdgcn_exp2f(sc[i] - base);
             l_run += x;
-            if (KT == PG_Q8) x *= vd[i] * vs;
-            if (HALF) {
+            if constexpr (KT == PG_Q8) {
+                // a rounded product: left to itself the compiler rounds it to a
+                // half twice, once from the exact product, and at a tie the hi
+                // that is multiplied is not the one taken off for lo
+                x *= raw.vd[i] * vs;
+                asm("" : "+v"(x));
+            }
+            if constexpr (HALF) {
                 const _Float16 hi = (_Float16)x;
-                const float rest = x - (float)hi;
-                if (NB == 1) {
-                    ph[0][i] = is_lo ? (_Float16)rest : hi;
-                } else {
-                    ph[0][i] = hi;
-                    ph[NB - 1][i] = (_Float16)rest;
-                }
+                ph[0][i] = hi;
+                pl[i] = (_Float16)(x - (float)hi);
             } else {
                 pf[i] = x;
             }
         }
-        // rows that are not attended may hold anything
-        if (KT != PG_Q8 && !whole) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const bool in = r0 + i >= sp.first && r0 + i < sp.len;
-#pragma unroll
-                for (int w = 0; w < Raw::VB; w++) raw.v[i][w] = in ? raw.v[i][w] : 0u;
+        if constexpr (HALF) {
+            if constexpr (NB == 1) {
+                const uint4v x = __builtin_bit_cast(uint4v, ph[0]), y = __builtin_bit_cast(uint4v, pl);
+                ph[0] = __builtin_bit_cast(half8, is_lo ? y : x);
+            } else {
+                ph[1] = pl;
             }
         }
         if constexpr (KT == PG_F32) {
@@ -405,167 +464,222 @@ __global__ void __launch_bounds__(PA_T, KT == PG_F32 ? 1 : 2) k_paged_split(cons
             }
         }
     }
-    if (lane == 0) kr_report(fault, bad);
 
-    // the waves' parts
-    if (NB == 1 && HALF) {
-#pragma unroll
-        for (int c = 0; c < W; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[c][i] += pa_swap8(o[c][i]);
+    __device__ __forceinline__ void load(Raw &raw, int t0) {
+        size_t lo, hi;
+        rows_of(t0, lo, hi);
+        load_k(raw, lo, hi);
+        load_v(raw, lo, hi);
     }
-    l_run += __shfl_xor(l_run, 16);
-    l_run += __shfl_xor(l_run, 32);
-    if (g == 0) {
-        s_m[wave][n] = m_run;
-        s_l[wave][n] = l_run;
-    }
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < PA_W; w++) m = fmaxf(m, s_m[w][n]);
-#pragma unroll
-    for (int w = 0; w < PA_W; w++) l += s_m[w][n] == -INFINITY ? s_l[w][n] : s_l[w][n] * __builtin_amdgcn_exp2f(s_m[w][n] - m);
-    // a part of no finite score holds nothing, or NaN
-    float f = m_run == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m);
-    if (KT == PG_Q8) f = ldexpf(f, ev);
-#pragma unroll
-    for (int c = 0; c < W; c++) o[c] *= f;
-    if (wave > 0) {
-#pragma unroll
-        for (int c = 0; c < W; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) s_o[wave - 1][4 * c + i][lane] = o[c][i];
-    }
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int w = 0; w < PA_W - 1; w++)
-#pragma unroll
-        for (int c = 0; c < W; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[c][i] += s_o[w][4 * c + i][lane];
-    if (!live || is_lo) return;
-    const bool alone = sp.parts <= 1;
-    float *out;
-    if (alone) {
-        out = a.o + head * hd;
-        const float inv = 1.0f / l;
-#pragma unroll
-        for (int c = 0; c < W; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[c][i] = sp.len > 0 ? o[c][i] * inv : 0.0f;
-    } else {
-        out = a.part + (head * a.n_split + split) * hd;
-    }
-    if (g == 0) {
-        if (!alone) {
-            a.pml[(head * a.n_split + split) * 2] = m;
-            a.pml[(head * a.n_split + split) * 2 + 1] = l;
-        } else if (a.fin) {
-            a.fin[head * 2] = m;
-            a.fin[head * 2 + 1] = l;
+
+    // rows [t0, t1) of the sequence, whole tiles but at its end: at most 32, whose pages are in ids
+    __device__ __forceinline__ void pass(int t0, int t1) {
+        float sc[8];
+        if constexpr (pa_two(KT, CL)) {
+            Raw x, y;
+            load(x, t0);
+            for (;; t0 += 2 * PA_TILE) {
+                const bool more = t0 + PA_TILE < t1;
+                if (more) load(y, t0 + PA_TILE);
+                scores(x, sc);
+                rest(x, sc, t0);
+                if (!more) break;
+                const bool again = t0 + 2 * PA_TILE < t1;
+                if (again) load(x, t0 + 2 * PA_TILE);
+                scores(y, sc);
+                rest(y, sc, t0 + PA_TILE);
+                if (!again) break;
+            }
+        } else {
+            Raw x;
+            size_t lo, hi;
+            rows_of(t0, lo, hi);
+            load_k(x, lo, hi);
+            for (;; t0 += PA_TILE) {
+                load_v(x, lo, hi);
+                scores(x, sc);
+                const bool more = t0 + PA_TILE < t1;
+                if (more) {
+                    rows_of(t0 + PA_TILE, lo, hi);
+                    load_k(x, lo, hi);
+                }
+                rest(x, sc, t0);
+                if (!more) break;
+            }
         }
     }
+
+    // tiles [t, end) of sequence `seq`, then its output or this share's part of it
+    __device__ __forceinline__ void part(int t, int end, size_t slot) {
+        m_run = -INFINITY;
+        l_run = 0.0f;
+        ev = -120;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int d0 = (4 * g + i) * W;
+        for (int c = 0; c < W; c++) o[c] = float4v{ 0, 0, 0, 0 };
+        const bool alone = t == 0 && end == sp.tiles;
+        if (sp.len > 0) {
+            const int r1 = min(sp.len, sp.begin + end * PA_TILE);
+            find(sp.begin + t * PA_TILE);
+            queries();
+            for (int r = sp.begin + t * PA_TILE; r < r1; r += 32 * PA_TILE) {
+                if (r != t_ids) find(r);
+                pass(r, min(r1, r + 32 * PA_TILE));
+            }
+        }
+        if (NB == 1 && HALF) {
 #pragma unroll
-        for (int c = 0; c < W; c += 4)
-            if (FULL || d0 + c < hd) *(float4v *)(out + d0 + c) = float4v{ o[c][i], o[c + 1][i], o[c + 2][i], o[c + 3][i] };
-    }
-}
-
-// A head's chunks: 2^dl lanes hold its dims four at a time, the workgroup's other
-// factor the chunks side by side.
-constexpr int PJ_T = 512;
-__global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArgs a, int dl) {
-    __shared__ float4v s_o[PJ_T];
-    __shared__ float s_l[PJ_T / 64];
-    const int s = blockIdx.y, tid = threadIdx.x;
-    int bad = 0;   // reported by the chunks
-    const PaSpan sp = pa_span(a, s, bad);
-    if (sp.parts <= 1) return;
-    const size_t head = (size_t)s * a.nh + blockIdx.x;
-    const float *ml = a.pml + head * a.n_split * 2, *part = a.part + head * a.n_split * p.hd;
-    float m = -INFINITY;
-    for (int i = tid & 63; i < sp.parts; i += 64) m = fmaxf(m, ml[2 * i]);
-    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    const int l = tid & ((1 << dl) - 1), lanes = PJ_T >> dl;
-    float4v acc = { 0, 0, 0, 0 };
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int i = tid >> dl; i < sp.parts; i += lanes) {
-        const float f = __builtin_amdgcn_exp2f(ml[2 * i] - m);
-        sum += ml[2 * i + 1] * f;
-        if (4 * l < p.hd) acc += *(const float4v *)(part + (size_t)i * p.hd + 4 * l) * f;
-    }
-    // the lanes of one group have the same sum: one of each counts
-    float ls = l == 0 ? sum : 0.0f;
-    for (int o = 32; o >= 1; o >>= 1) ls += __shfl_xor(ls, o);
-    if ((tid & 63) == 0) s_l[tid >> 6] = ls;
-    s_o[tid] = acc;
-    __syncthreads();
-    float all = 0.0f;
+            for (int c = 0; c < W; c++)
 #pragma unroll
-    for (int i = 0; i < PJ_T / 64; i++) all += s_l[i];
-    if (tid >> dl) return;
-    for (int i = 1; i < lanes; i++) acc += s_o[(i << dl) + l];
-    const float inv = 1.0f / all;
-    if (4 * l < p.hd) *(float4v *)(a.o + head * p.hd + 4 * l) = acc * inv;
-    if (a.fin && l == 0) {
-        a.fin[head * 2] = m;
-        a.fin[head * 2 + 1] = all;
+                for (int i = 0; i < 4; i++) o[c][i] += pa_swap8(o[c][i]);
+        }
+        const float l = pa_sum_g(l_run);
+        if (!live || is_lo) return;
+        float f = alone ? 1.0f / l : 1.0f;
+        if (KT == PG_Q8) f = ldexpf(f, ev);
+        if (sp.len == 0) f = 0.0f;
+        if (g == 0 && (!alone || a.z)) {
+            a.pml[(slot * group + col) * 2] = m_run;
+            a.pml[(slot * group + col) * 2 + 1] = l;
+        }
+        float *out = alone ? a.o + head() * hd : a.part + (slot * group + col) * hd;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d0 = (4 * g + i) * W;
+#pragma unroll
+            for (int c = 0; c < W; c += 4)
+                if (FULL || d0 + c < hd)
+                    *(float4v *)(out + d0 + c) = float4v{ o[c][i] * f, o[c + 1][i] * f, o[c + 2][i] * f, o[c + 3][i] * f };
+        }
     }
-}
-
-// mass[r] += the row's weights over the KV head's query heads, in head order
-__global__ void __launch_bounds__(PA_T) k_paged_mass(const PgView p, const PaArgs a, float up) {
-    const int s = blockIdx.z, kvh = blockIdx.y, group = a.nh / p.n_kv;
-    int bad = 0;
-    const PaSpan sp = pa_span(a, s, bad);
-    const int r = sp.first + (int)(blockIdx.x * PA_T + threadIdx.x);
-    if (r >= sp.len) return;
-    float sum = 0.0f;
-    for (int h = 0; h < group; h++) {
-        const size_t head = (size_t)s * a.nh + kvh * group + h;
-        sum += __builtin_amdgcn_exp2f(a.z[head * a.z_ld + r] - a.fin[2 * head]) * (up / a.fin[2 * head + 1]);
-    }
-    a.mass[((size_t)s * p.n_kv + kvh) * a.mass_ld + r] += sum;
-}
-
-// Rows a chunk, a multiple of a workgroup's step: about PA_PARTS chunks in all
-// within [PA_LEAST, PA_MOST] rows.
-constexpr int PA_PARTS = 2048, PA_LEAST = 128, PA_MOST = 512;
-int pa_chunk(int n_seq, int n_kv, int rows) {
-    const long long c = (long long)n_seq * n_kv * rows / PA_PARTS;
-    return (int)((c < PA_LEAST ? PA_LEAST : c > PA_MOST ? PA_MOST : c) + PA_STEP - 1) / PA_STEP * PA_STEP;
-}
-// the most chunks that any number of rows up to `rows` is cut into: those of the
-// largest chunk, or one more than PA_PARTS over the heads
-int pa_most_parts(int n_seq, int n_kv, int rows) {
-    const long long heads = (long long)n_seq * n_kv, big = (rows + PA_MOST - 1) / PA_MOST, even = PA_PARTS / heads + 1;
-    const long long least = (rows + PA_LEAST - 1) / PA_LEAST, n = big > even ? big : even;
-    return (int)(n < least ? n : least);
-}
-
-// the workspace's pieces, in floats, for n_split chunks
-struct PaSizes {
-    size_t part, pml, fin, z_ld, z;
 };
-PaSizes pa_sizes(const krh_pages *kv, int n_seq, int nh, int max_len, int n_split, bool mass) {
+
+template <int KT, int CL, int NB, bool FULL>
+__global__ void __launch_bounds__(64, pa_waves(KT, CL)) k_paged_shares(const PgView p, const PaArgs a, int *fault) {
+    const int u = blockIdx.x, kvh = blockIdx.y;
+    PaWave<KT, CL, NB, FULL> w(p, a, kvh);
+    const PaAll all = pa_all(p, a, w.bad);
+    if (u < all.shares) {
+        int left = pa_bound(all, u + 1) - pa_bound(all, u), t = pa_bound(all, u);
+        for (w.seq = pa_find(p, a, t, w.bad); left > 0; w.seq++, t = 0) {
+            w.sp = pa_span(a, a.len[w.seq], w.bad);
+            const int end = min(w.sp.tiles, t + left);
+            w.part(t, end, (size_t)kvh * (p.n_seq + a.shares) + w.seq + u);
+            left -= end - t;
+        }
+    }
+    kr_report(fault, w.bad);
+}
+
+// The shares of a sequence: their first slot and number, by the arithmetic that made them.
+struct PaParts {
+    size_t slot;
+    int n;
+};
+__device__ __forceinline__ PaParts pa_parts(const PgView &p, const PaArgs &a, int s, int kvh) {
+    int bad = 0, before = 0;   // reported by the shares
+    const PaAll all = pa_all(p, a, bad);
+    for (int i = threadIdx.x & 63; i < s; i += 64) before += pa_span(a, a.len[i], bad).tiles;
+    for (int o = 32; o >= 1; o >>= 1) before += __shfl_xor(before, o);
+    before = __builtin_amdgcn_readfirstlane(before);
+    const int u0 = pa_share(all, before), u1 = pa_share(all, before + pa_span(a, a.len[s], bad).tiles - 1);
+    return { (size_t)kvh * (p.n_seq + a.shares) + s + u0, u1 - u0 + 1 };
+}
+
+// A head's maximum and 1 / its sum, by one wave
+__device__ __forceinline__ void pa_stats(const float *ml, int group, int n, float &m, float &inv) {
+    float l = 0.0f;
+    m = -INFINITY;
+    for (int i = threadIdx.x & 63; i < n; i += 64) m = fmaxf(m, ml[(size_t)i * group * 2]);
+    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    for (int i = threadIdx.x & 63; i < n; i += 64) l += ml[(size_t)i * group * 2 + 1] * __builtin_amdgcn_exp2f(ml[(size_t)i * group * 2] - m);
+    for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
+    inv = 1.0f / l;
+}
+
+// Workgroups x < nh: head x's parts (2^dl lanes hold its dims four at a time, the
+// workgroup's other factor the parts side by side). The others, with a mass:
+// PJ_ROWS rows of one KV head each, mass[r] += its weights over the query heads.
+constexpr int PJ_T = 256, PJ_ROWS = 1024;
+__global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArgs a, int dl, int blocks) {
+    __shared__ float4v s_o[PJ_T];
+    __shared__ float s_m[KR_PAGE_GROUP_MAX], s_i[KR_PAGE_GROUP_MAX];
+    const int s = blockIdx.y, x = blockIdx.x, tid = threadIdx.x, group = a.nh / p.n_kv;
+    if (x < a.nh) {
+        const int kvh = x / group, col = x % group;
+        const PaParts r = pa_parts(p, a, s, kvh);
+        if (r.n <= 1) return;
+        const float *ml = a.pml + (r.slot * group + col) * 2, *part = a.part + (r.slot * group + col) * p.hd;
+        float m, inv;
+        pa_stats(ml, group, r.n, m, inv);
+        const int l = tid & ((1 << dl) - 1), lanes = PJ_T >> dl;
+        float4v acc = { 0, 0, 0, 0 };
+        if (4 * l < p.hd) {
+#pragma unroll 4
+            for (int i = tid >> dl; i < r.n; i += lanes)
+                acc += *(const float4v *)(part + (size_t)i * group * p.hd + 4 * l) * __builtin_amdgcn_exp2f(ml[(size_t)i * group * 2] - m);
+        }
+        s_o[tid] = acc;
+        for (int h = lanes >> 1; h >= 1; h >>= 1) {
+            __syncthreads();
+            if ((tid >> dl) < h) s_o[tid] = acc = acc + s_o[tid + (h << dl)];
+        }
+        if (tid >> dl == 0 && 4 * l < p.hd) *(float4v *)(a.o + ((size_t)s * a.nh + x) * p.hd + 4 * l) = acc * inv;
+        return;
+    }
+    const int kvh = (x - a.nh) / blocks, block = (x - a.nh) % blocks;
+    int bad = 0;
+    const PaSpan sp = pa_span(a, a.len[s], bad);
+    const int r0 = sp.first + block * PJ_ROWS;
+    if (r0 >= sp.len) return;
+    const PaParts r = pa_parts(p, a, s, kvh);
+    for (int h = tid >> 6; h < group; h += PJ_T / 64) {
+        float m, inv;
+        pa_stats(a.pml + (r.slot * group + h) * 2, group, r.n, m, inv);
+        if ((tid & 63) == 0) {
+            s_m[h] = m;
+            s_i[h] = inv;
+        }
+    }
+    __syncthreads();
+    const float up = a.z_up;
+    const float *z = a.z + ((size_t)s * a.nh + kvh * group) * a.z_ld;
+    float *mass = a.mass + ((size_t)s * p.n_kv + kvh) * a.mass_ld;
+#pragma unroll
+    for (int k = 0; k < PJ_ROWS / PJ_T; k++) {
+        const int i = r0 + k * PJ_T + tid;
+        if (i >= sp.len) break;
+        float sum = 0.0f;
+        for (int h = 0; h < group; h++) sum += __builtin_amdgcn_exp2f(z[h * a.z_ld + i] - s_m[h] + up) * s_i[h];
+        mass[i] += sum;
+    }
+}
+
+// Shares in all, of every KV head: about PA_WAVES waves, fewer where the rows
+// are few. The lengths are the device's, so this is what they may be at most.
+constexpr int PA_WAVES = 2048;
+int pa_shares(int n_seq, int n_kv, int rows) {
+    const long long tiles = (long long)n_seq * ((rows + PA_TILE - 1) / PA_TILE), most = (tiles + PA_SHARE - 1) / PA_SHARE;
+    const long long want = PA_WAVES / n_kv > 1 ? PA_WAVES / n_kv : 1;
+    return (int)(want < most ? want : most);
+}
+
+// the workspace's pieces, in floats
+struct PaSizes {
+    size_t part, pml, z_ld, z;
+};
+PaSizes pa_sizes(const krh_pages *kv, int n_seq, int nh, int max_len, int shares, bool mass) {
     PaSizes r;
-    const size_t heads = (size_t)n_seq * nh;
-    r.part = n_split > 1 ? heads * n_split * kv->head_dim : 0;
-    r.pml = n_split > 1 ? (heads * n_split * 2 + 3) & ~(size_t)3 : 0;
-    r.fin = mass ? (heads * 2 + 3) & ~(size_t)3 : 0;
+    const size_t slots = (size_t)kv->n_kv_heads * (n_seq + shares) * (nh / kv->n_kv_heads);
+    r.part = shares > 1 ? slots * kv->head_dim : 0;
+    r.pml = shares > 1 || mass ? (slots * 2 + 3) & ~(size_t)3 : 0;
     r.z_ld = mass ? ((size_t)max_len + PA_TILE - 1) / PA_TILE * PA_TILE : 0;
-    r.z = heads * r.z_ld;
+    r.z = (size_t)n_seq * nh * r.z_ld;
     return r;
 }
 
 bool pa_args_ok(const krh_pages *kv, int n_seq, int n_heads, int max_len) {
-    return pg_pages_ok(kv) && n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && max_len <= INT32_MAX / 2 && n_heads > 0 &&
+    return pg_pages_ok(kv) && n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && max_len <= INT32_MAX / 2 &&
+           (long long)n_seq * (max_len / PA_TILE + 1) <= INT32_MAX / 2 && n_heads > 0 &&
            n_heads % kv->n_kv_heads == 0 && n_heads / kv->n_kv_heads <= KR_PAGE_GROUP_MAX;
 }
 
@@ -573,10 +687,10 @@ using PaKernel = void (*)(const PgView, const PaArgs, int *);
 
 template <int KT, int CL> PaKernel pa_kernel(int group, int hd) {
     if constexpr (KT == PG_F32) {
-        return hd == CL ? k_paged_split<KT, CL, 1, true> : k_paged_split<KT, CL, 1, false>;
+        return hd == CL ? k_paged_shares<KT, CL, 1, true> : k_paged_shares<KT, CL, 1, false>;
     } else {
-        if (hd != CL) return k_paged_split<KT, CL, 2, false>;
-        return group <= 8 ? k_paged_split<KT, CL, 1, true> : k_paged_split<KT, CL, 2, true>;
+        if (hd != CL) return k_paged_shares<KT, CL, 2, false>;
+        return group <= 8 ? k_paged_shares<KT, CL, 1, true> : k_paged_shares<KT, CL, 2, true>;
     }
 }
 template <int KT> PaKernel pa_kernel(int group, int hd) {
@@ -587,8 +701,8 @@ template <int KT> PaKernel pa_kernel(int group, int hd) {
 
 extern "C" size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int max_len, int mass) {
     if (!pa_args_ok(kv, n_seq, n_heads, max_len)) return 0;
-    const PaSizes r = pa_sizes(kv, n_seq, n_heads, max_len, pa_most_parts(n_seq, kv->n_kv_heads, max_len), mass != 0);
-    return sizeof(float) * (r.part + r.pml + r.fin + r.z + 4);
+    const PaSizes r = pa_sizes(kv, n_seq, n_heads, max_len, pa_shares(n_seq, kv->n_kv_heads, max_len), mass != 0);
+    return sizeof(float) * (r.part + r.pml + r.z + 4);
 }
 
 extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len,
@@ -603,28 +717,24 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
         return;
     // a window's rows, and those before them in its first tile
     const int rows = window > 0 && window < max_len - PA_TILE ? window + PA_TILE - 1 : max_len;
-    const int chunk = pa_chunk(n_seq, kv->n_kv_heads, rows), n_split = (rows + chunk - 1) / chunk;
-    const PaSizes r = pa_sizes(kv, n_seq, n_heads, max_len, n_split, mass != nullptr);
+    const int shares = pa_shares(n_seq, kv->n_kv_heads, rows);
+    const PaSizes r = pa_sizes(kv, n_seq, n_heads, max_len, shares, mass != nullptr);
     float *w = (float *)ws;
     PaArgs a = {};
     a.o = o, a.q = q, a.len = len, a.mass = mass, a.mass_ld = mass_ld;
-    a.part = w, a.pml = w + r.part, a.fin = mass ? w + r.part + r.pml : nullptr;
-    a.z = mass ? w + r.part + r.pml + r.fin : nullptr, a.z_ld = r.z_ld;
-    a.nh = n_heads, a.max_len = max_len, a.window = window, a.chunk = chunk, a.n_split = n_split;
-    a.scale = scale, a.cap = softcap;
+    a.part = w, a.pml = w + r.part, a.z = mass ? w + r.part + r.pml : nullptr, a.z_ld = r.z_ld;
+    a.nh = n_heads, a.max_len = max_len, a.window = window, a.shares = shares;
+    a.scale = scale, a.cap = softcap, a.z_up = kv->kv_type == ML_F32 ? 0.0f : PA_UP;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
     const int group = n_heads / kv->n_kv_heads, hd = kv->head_dim;
     const PaKernel f = kv->kv_type == ML_F32 ? pa_kernel<PG_F32>(group, hd) : kv->kv_type == ML_F16 ? pa_kernel<PG_F16>(group, hd)
                                                                                                     : pa_kernel<PG_Q8>(group, hd);
-    hipLaunchKernelGGL(f, dim3(n_split, kv->n_kv_heads, n_seq), dim3(PA_T), 0, kr_stream(), p, a, kr_fault_word());
+    hipLaunchKernelGGL(f, dim3(shares, kv->n_kv_heads), dim3(64), 0, kr_stream(), p, a, kr_fault_word());
     kr_check_launch("paged_attention");
-    if (n_split > 1) {
-        hipLaunchKernelGGL(k_paged_join, dim3(n_heads, n_seq), dim3(PJ_T), 0, kr_stream(), p, a, pg_log2(hd / 4));
-        kr_check_launch("paged_attention");
-    }
-    if (mass) {
-        hipLaunchKernelGGL(k_paged_mass, dim3((rows + PA_T - 1) / PA_T, kv->n_kv_heads, n_seq), dim3(PA_T), 0, kr_stream(), p, a,
-                           kv->kv_type == ML_F32 ? 1.0f : PA_UP);
+    if (shares > 1 || mass) {
+        const int blocks = mass ? (rows + PJ_ROWS - 1) / PJ_ROWS : 0;
+        hipLaunchKernelGGL(k_paged_join, dim3(n_heads + kv->n_kv_heads * blocks, n_seq), dim3(PJ_T), 0, kr_stream(), p, a,
+                           pg_log2(hd / 4), blocks);
         kr_check_launch("paged_attention");
     }
 }
