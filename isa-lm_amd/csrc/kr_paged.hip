@@ -61,10 +61,9 @@ template <int KT> __device__ __forceinline__ void pg_store(void *dst, float *d, 
 }
 
 template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_qkv(const PgView p, const QkvArgs a, int lps, int *fault) {
-    const int n = 1 << lps, l = (int)threadIdx.x & (n - 1), per = a.nh + 2 * p.n_kv;
-    const size_t item = ((size_t)blockIdx.x * PG_T + threadIdx.x) >> lps;
-    if (item >= (size_t)a.ntok * per) return;   // whole items: the lanes that shuffle leave together
-    const int t = (int)(item / per), h = (int)(item % per), hd = p.hd;
+    const unsigned n = 1u << lps, per = a.nh + 2 * p.n_kv, item = (blockIdx.x * PG_T + threadIdx.x) >> lps;
+    if (item >= a.ntok * per) return;   // whole items: the lanes that shuffle leave together
+    const int l = (int)(threadIdx.x & (n - 1)), t = (int)(item / per), h = (int)(item % per), hd = p.hd;
     const bool live = 4 * l < hd, isq = h < a.nh, isk = !isq && h < a.nh + p.n_kv;
     const int kvh = h - a.nh - (isk || isq ? 0 : p.n_kv);
     const float *src = isq ? a.q + (size_t)t * a.ldq + (size_t)h * hd
@@ -121,9 +120,9 @@ template <int KT> __device__ __forceinline__ float4 pg_load4(const void *src, co
 
 template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_load(const PgView p, float *k, size_t ldk, float *v, size_t ldv,
                                                                        int n_rows, const int *seqs, const int *rows, int lps, int *fault) {
-    const int n = 1 << lps, l = (int)threadIdx.x & (n - 1), per = 2 * p.n_kv;
-    const size_t item = ((size_t)blockIdx.x * PG_T + threadIdx.x) >> lps;
-    if (item >= (size_t)n_rows * per || 4 * l >= p.hd) return;
+    const unsigned n = 1u << lps, per = 2 * p.n_kv, item = (blockIdx.x * PG_T + threadIdx.x) >> lps;
+    const int l = (int)(threadIdx.x & (n - 1));
+    if (item >= n_rows * per || 4 * l >= p.hd) return;
     const int i = (int)(item / per), h = (int)(item % per), kvh = h < p.n_kv ? h : h - p.n_kv;
     int bad = 0;
     const int seq = kr_page_in(seqs[i], p.n_seq, KR_BAD_SEQ, bad), row = kr_page_in(rows[i], INT_MAX, KR_BAD_PAGE, bad);
@@ -145,7 +144,8 @@ __device__ __forceinline__ unsigned ev_key(float w) {
     return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
-constexpr int EV_T = 1024, EV_W = EV_T / 64;
+constexpr int EV_T = 1024, EV_W = EV_T / 64, EV_D = 11, EV_B = 1 << EV_D;   // radix digits of 11, 11 and 10 bits
+constexpr int EV_U = 8;   // rows a lane reads ahead
 
 struct EvArgs {
     const int *len;
@@ -157,103 +157,153 @@ struct EvArgs {
     int *out_len;
     float *out_mass;
     size_t out_mass_ld;
-    int *idx;   // [n_seq][n_kv][keep]: the rows kept, in order
-    int *cnt;   // [n_seq]: how many
+    int *cnt;   // [n_seq]: rows kept
+    int *idx;   // [n_seq][n_kv][keep]: which, in order
+    float *w;   // [n_seq][n_kv][keep]: their weights
 };
 
+// Inclusive sums over the wave's lanes
+__device__ __forceinline__ int ev_scan(int v) {
+    for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(v, o);
+        if ((int)(threadIdx.x & 63) >= o) v += t;
+    }
+    return v;
+}
+
+// EV_U rows of 64 from r0 on for each lane, none past r1
+template <class F> __device__ __forceinline__ void ev_rows(const float *mass, int r0, int r1, F f) {
+    const int lane = threadIdx.x & 63;
+    for (int r = r0 + lane; r - lane < r1; r += 64 * EV_U) {
+        float w[EV_U];
+#pragma unroll
+        for (int k = 0; k < EV_U; k++) w[k] = mass[min(r + 64 * k, r1 - 1)];
+#pragma unroll
+        for (int k = 0; k < EV_U; k++)
+            if (r - lane + 64 * k < r1) f(r + 64 * k, r + 64 * k < r1, w[k]);
+    }
+}
+
 // One workgroup a (sequence, KV head): the weight of the last row kept by a
-// radix select (8 bits a pass), then the kept rows' numbers in order, equal
-// weights from the lowest row on.
+// radix select, then the kept rows' numbers in order, equal weights from the
+// lowest row on. Each wave has an even part of the rows. Bound by the passes'
+// latencies: the rows come from L2 after the first (32,001 rows, 8 workgroups:
+// 102 us with one lane looking through the digits' counts and barriers every 1024 rows).
 __global__ void __launch_bounds__(EV_T) k_evict_select(const EvArgs a, int *fault) {
-    __shared__ int hist[256];
-    __shared__ int wsum[2][EV_W];
+    __shared__ int hist[EV_B];
+    __shared__ int s_sum[EV_W], s_tie[EV_W], s_take[EV_W];
     __shared__ unsigned s_prefix;
     __shared__ int s_need;
-    const int kvh = blockIdx.x, s = blockIdx.y, n_kv = gridDim.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int kvh = blockIdx.x, s = blockIdx.y, n_kv = gridDim.x, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int bad = 0;
     const int len = kr_page_len(a.len[s], a.max_len, bad);
     if (tid == 0) kr_report(fault, bad);
     const size_t sh = (size_t)s * n_kv + kvh;
     const float *mass = a.mass + sh * a.mass_ld;
-    float *om = a.out_mass + sh * a.out_mass_ld;
     int *idx = a.idx + sh * a.keep;
+    float *ow = a.w + sh * a.keep;
     const int kept = min(len, a.keep);
     if (kvh == 0 && tid == 0) a.cnt[s] = kept;
-    // past the kept rows nothing is left, for rows that come later
-    const int end = (int)min(a.out_mass_ld, (size_t)max(a.keep, a.max_len));
     if (len <= a.keep) {
-        for (int r = tid; r < end; r += EV_T) {
-            if (r < len) idx[r] = r;
-            om[r] = r < len ? mass[r] : 0.0f;
+        for (int r = tid; r < len; r += EV_T) {
+            idx[r] = r;
+            ow[r] = mass[r];
         }
         return;
     }
     const int old = len - a.recent, want = a.keep - a.recent;   // 0 <= want < old
+    const int part = (old + EV_W - 1) / EV_W, r0 = min(old, wave * part), r1 = min(old, r0 + part);
     unsigned prefix = 0;
     int need = want;
     if (want > 0)
-        for (int b = 24; b >= 0; b -= 8) {
-            for (int i = tid; i < 256; i += EV_T) hist[i] = 0;
+        for (int b = 32 - EV_D; ; b = max(0, b - EV_D)) {
+            const int top = b == 32 - EV_D ? 32 : b ? 32 - EV_D : 32 - 2 * EV_D;   // bits from here up are known
+            for (int i = tid; i < EV_B; i += EV_T) hist[i] = 0;
             __syncthreads();
-            for (int r = tid; r < old; r += EV_T) {
-                const unsigned u = ev_key(mass[r]);
-                if (b == 24 || (u >> (b + 8)) == (prefix >> (b + 8))) atomicAdd(&hist[u >> b & 255], 1);
-            }
+            ev_rows(mass, r0, r1, [&](int, bool in, float w) {
+                const unsigned u = ev_key(w), d = (u >> b) & ((1u << (top - b)) - 1);
+                in = in && (top == 32 || (u >> top) == (prefix >> top));
+                // the digit of the first lane, often that of many (zeros), counts once
+                const unsigned long long any = __ballot(in);
+                if (!any) return;
+                const unsigned d0 = (unsigned)__builtin_amdgcn_readlane((int)d, __builtin_ctzll(any));
+                const unsigned long long same = __ballot(in && d == d0);
+                if (lane == __builtin_ctzll(any)) atomicAdd(&hist[d0], (int)__popcll(same));
+                else if (in && d != d0) atomicAdd(&hist[d], 1);
+            });
             __syncthreads();
-            if (tid == 0) {
-                int d = 255, left = need;
-                while (hist[d] < left) left -= hist[d--];   // need <= the counts' sum: ends at d >= 0
-                s_prefix = prefix | (unsigned)d << b;
-                s_need = left;
+            // from the heaviest digit down: where the counts' sum reaches `need`
+            const int hi = EV_B - 1 - 2 * tid, c0 = hist[hi], c1 = hist[hi - 1], sum = ev_scan(c0 + c1);
+            if (lane == 63) s_sum[wave] = sum;
+            __syncthreads();
+            int before = sum - c0 - c1;
+            for (int i = 0; i < wave; i++) before += s_sum[i];
+            if (before < need && before + c0 + c1 >= need) {
+                const bool second = before + c0 < need;
+                s_prefix = prefix | (unsigned)(second ? hi - 1 : hi) << b;
+                s_need = need - before - (second ? c0 : 0);
             }
             __syncthreads();
             prefix = s_prefix;
             need = s_need;
             __syncthreads();
+            if (b == 0) break;
         }
     // rows above `prefix`, and the first `need` of those at it
-    int base = 0, ties = 0;
-    for (int r0 = 0; r0 < len; r0 += EV_T) {
-        const int r = r0 + tid;
-        const float w = r < len ? mass[r] : 0.0f;
-        const unsigned u = ev_key(w);
-        const bool tail = r >= old && r < len, tie = want > 0 && r < old && u == prefix;
-        const unsigned long long bt = __ballot(tie), below = ((unsigned long long)1 << lane) - 1;
-        if (lane == 0) wsum[0][wave] = __popcll(bt);
-        __syncthreads();
-        int before = ties;
-        for (int i = 0; i < EV_W; i++) {
-            if (i < wave) before += wsum[0][i];
-            ties += wsum[0][i];
-        }
-        const bool take = tail || (want > 0 && r < old && u > prefix) || (tie && before + __popcll(bt & below) < need);
-        const unsigned long long bk = __ballot(take);
-        if (lane == 0) wsum[1][wave] = __popcll(bk);
-        __syncthreads();
-        int at = base;
-        for (int i = 0; i < EV_W; i++) {
-            if (i < wave) at += wsum[1][i];
-            base += wsum[1][i];
-        }
-        if (take) {
-            at += __popcll(bk & below);
-            idx[at] = r;
-            om[at] = w;   // at <= r: in place, no weight of a later chunk is lost
-        }
-        __syncthreads();
+    int ties = 0, take = 0;
+    if (want > 0)
+        ev_rows(mass, r0, r1, [&](int, bool in, float w) {
+            const unsigned u = ev_key(w);
+            ties += __popcll(__ballot(in && u == prefix));
+            take += __popcll(__ballot(in && u > prefix));
+        });
+    if (lane == 0) {
+        s_tie[wave] = ties;
+        s_take[wave] = take;
     }
-    for (int r = a.keep + tid; r < end; r += EV_T) om[r] = 0.0f;
+    __syncthreads();
+    int at = 0;
+    ties = 0;
+    for (int i = 0; i < wave; i++) {
+        ties += s_tie[i];
+        at += s_take[i];
+    }
+    at += min(ties, need);
+    if (want > 0)
+        ev_rows(mass, r0, r1, [&](int r, bool in, float w) {
+            const unsigned u = ev_key(w);
+            const unsigned long long bt = __ballot(in && u == prefix), below = ((unsigned long long)1 << lane) - 1;
+            const bool take = in && (u > prefix || (u == prefix && ties + __popcll(bt & below) < need));
+            const unsigned long long bk = __ballot(take);
+            if (take) {
+                const int j = at + __popcll(bk & below);
+                idx[j] = r;
+                ow[j] = w;
+            }
+            ties += __popcll(bt);
+            at += __popcll(bk);
+        });
+    for (int r = tid; r < a.recent; r += EV_T) {
+        idx[want + r] = old + r;
+        ow[want + r] = mass[old + r];
+    }
 }
 
-// rows into the new pages, in units of U bytes; a unit a thread and step
+// Rows into the new pages, in units of U bytes, EM_ROWS a workgroup and KV
+// head; their weights, and zeros past them. Bound by HBM: each row read once
+// and written once (16 sequences of up to 4096 rows, 8B shape, half kept: 4.7
+// TB/s).
+constexpr int EM_ROWS = 64;
 template <class U> __global__ void __launch_bounds__(PG_T) k_evict_move(const PgView p, const EvArgs a, int rb, int *fault) {
-    const int s = blockIdx.z, kvh = blockIdx.y, per = rb / (int)sizeof(U), kept = a.cnt[s];
+    const int s = blockIdx.z, kvh = blockIdx.y, per = rb / (int)sizeof(U), kept = a.cnt[s], tid = threadIdx.x;
     const size_t sh = (size_t)s * p.n_kv + kvh;
     const int *idx = a.idx + sh * a.keep, *ot = a.out_table + (size_t)s * a.out_ld;
-    if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0) a.out_len[s] = kept;
+    if (blockIdx.x == 0 && kvh == 0 && tid == 0) a.out_len[s] = kept;
     int bad = 0;
-    for (size_t e = (size_t)blockIdx.x * PG_T + threadIdx.x; e < (size_t)kept * per; e += (size_t)gridDim.x * PG_T) {
-        const int j = (int)(e / per), u = (int)(e % per), r = idx[j];
+    const int j0 = blockIdx.x * EM_ROWS, n = min(kept - j0, EM_ROWS) * per;
+    for (int e = tid; e < n; e += PG_T) {
+        const int j = j0 + e / per, u = e % per, r = idx[j];
         int b = 0;
         const size_t from = kr_page_row(pg_page(p, s, r, b), p.n_kv, kvh, p.shift, r);
         const size_t to = kr_page_row(kr_page_of(ot, a.out_ld, j, p.shift, p.n_pages, b), p.n_kv, kvh, p.shift, j);
@@ -266,13 +316,16 @@ template <class U> __global__ void __launch_bounds__(PG_T) k_evict_move(const Pg
             p.vd[to] = p.vd[from];
         }
     }
+    float *om = a.out_mass + sh * a.out_mass_ld;
+    const int end = (int)min(a.out_mass_ld, (size_t)max(a.keep, a.max_len)), blocks = gridDim.x;
+    for (int j = blockIdx.x * PG_T + tid; j < end; j += blocks * PG_T) om[j] = j < kept ? a.w[sh * a.keep + j] : 0.0f;
     kr_report(fault, bad);
 }
 
 // workgroups for `items` items of 2^lps lanes; 0: more than a launch holds
 unsigned item_blocks(size_t items, int lps) {
     const size_t b = ((items << lps) + PG_T - 1) / PG_T;
-    return b <= 0x7fffffff / PG_T ? (unsigned)b : 0;
+    return b <= 0x7fffffff / PG_T ? (unsigned)b : 0;   // lanes stay within 31 bits
 }
 
 }  // namespace
@@ -324,7 +377,7 @@ extern "C" void krh_paged_load(float *k, size_t ldk, float *v, size_t ldv, const
 
 extern "C" size_t krh_paged_evict_ws(int n_seq, int n_kv_heads, int keep) {
     if (n_seq <= 0 || n_kv_heads <= 0 || keep <= 0) return 0;
-    return sizeof(int) * ((size_t)n_seq * n_kv_heads * keep + n_seq);
+    return sizeof(int) * (2 * (size_t)n_seq * n_kv_heads * keep + n_seq);
 }
 
 extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table_ld, const int *len, const float *mass,
@@ -341,17 +394,15 @@ extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table
         pg_refuse((size_t)out_table_ld * kv->page_size >= (size_t)(keep < max_len ? keep : max_len), "paged_evict: out_table's pages"))
         return;
     int *w = (int *)ws;
-    const EvArgs a = { len, mass, mass_ld, max_len, keep, recent, out_table, out_table_ld, out_len, out_mass, out_ld, w + n_seq, w };
+    const size_t rows = (size_t)n_seq * kv->n_kv_heads * keep;
+    const EvArgs a = { len, mass, mass_ld, max_len, keep, recent, out_table, out_table_ld, out_len, out_mass, out_ld,
+                       w + 2 * rows, w, (float *)(w + rows) };
     hipLaunchKernelGGL(k_evict_select, dim3(kv->n_kv_heads, n_seq), dim3(EV_T), 0, kr_stream(), a, kr_fault_word());
     kr_check_launch("paged_evict");
-    const int rb = kv->head_dim * (kv->kv_type == ML_F32 ? 4 : kv->kv_type == ML_F16 ? 2 : 1);
+    const int rb = kv->head_dim * (kv->kv_type == ML_F32 ? 4 : kv->kv_type == ML_F16 ? 2 : 1), most = keep < max_len ? keep : max_len;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
-    const int rows = keep < max_len ? keep : max_len;
-    const size_t units = (size_t)rows * (rb % 16 ? rb / 8 : rb / 16), want = (units + 4 * PG_T - 1) / (4 * PG_T);
-    const dim3 grid((unsigned)(want < 1024 ? want : 1024), kv->n_kv_heads, n_seq);
-    if (rb % 16)
-        hipLaunchKernelGGL(k_evict_move<uint2>, grid, dim3(PG_T), 0, kr_stream(), p, a, rb, kr_fault_word());
-    else
-        hipLaunchKernelGGL(k_evict_move<uint4>, grid, dim3(PG_T), 0, kr_stream(), p, a, rb, kr_fault_word());
+    hipLaunchKernelGGL(rb % 16 ? k_evict_move<uint2> : k_evict_move<uint4>,
+                       dim3((most + EM_ROWS - 1) / EM_ROWS, kv->n_kv_heads, n_seq), dim3(PG_T), 0, kr_stream(), p, a, rb,
+                       kr_fault_word());
     kr_check_launch("paged_evict");
 }

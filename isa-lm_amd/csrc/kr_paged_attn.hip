@@ -1,6 +1,6 @@
 // Attention of one token of each sequence over a paged cache (krh_paged_attention).
 //
-// The rows of all sequences, in tiles of 32, are cut into equal shares, one a
+// The rows of all sequences, in tiles of 32 (16), are cut into equal shares, one a
 // wave and KV head (pa_share): the lengths decide on the device, so a batch of all
 // lengths loads the chip as one long sequence does. A wave passes over each
 // sequence's part of its share once with the running maximum and sum of the
@@ -9,7 +9,7 @@
 //
 // Both products run on the matrix cores, transposed so that nothing passes
 // through LDS: S^T = K Q^T has rows as the tile's rows and query heads as its
-// columns, and the lane that holds a head's scores of 8 consecutive rows holds
+// columns, and the lane that holds a head's scores of 8 (4) consecutive rows holds
 // them as the operand P^T of O^T = V^T P^T. K's rows are read straight into
 // operand registers (the order of the contraction is free, so a lane reads 8
 // dims at a time); V's are transposed 2 by 2 in registers by byte permutes
@@ -27,11 +27,12 @@
 
 namespace {
 
-constexpr int PA_TILE = 32;
-constexpr int PA_SHARE = 4;        // tiles that a share is worth at least
+// Rows of a tile: 32, and 16 for heads past 128 dims, whose rows fill the registers
+constexpr int pa_tile(int hd) { return hd > 128 ? 16 : 32; }
 constexpr float PA_UP = 14.0f;     // the weights' scale (log2; halves end at 2^16)
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
@@ -48,7 +49,7 @@ struct PaArgs {
     float *pml;     // [n_kv][n_seq + shares][group][2]: their maximum (log2) and weight
     float *z;       // [n_seq][nh][z_ld]: the scores (log2), for the mass
     size_t z_ld;
-    int nh, max_len, window, shares;
+    int nh, max_len, window, shares, tl, least;   // tl: log2 of a tile's rows; least: tiles a share is worth
     float scale, cap, z_up;   // z_up: log2 of the weights' scale in the sums
 };
 
@@ -57,49 +58,73 @@ struct PaArgs {
 struct PaSpan {
     int len, first, begin, tiles;
 };
-__device__ __forceinline__ PaSpan pa_span(const PaArgs &a, int len, int &bad) {
+__device__ __forceinline__ PaSpan pa_span(const PaArgs &a, int len) {   // len within [0, max_len]
     PaSpan r;
-    r.len = kr_page_len(len, a.max_len, bad);
+    r.len = len;
     r.first = a.window > 0 && r.len > a.window ? r.len - a.window : 0;
-    r.begin = r.first & ~(PA_TILE - 1);
-    r.tiles = max(1, (r.len - r.begin + PA_TILE - 1) / PA_TILE);
+    r.begin = r.first & -(1 << a.tl);
+    r.tiles = max(1, (r.len - r.begin + (1 << a.tl) - 1) >> a.tl);
     return r;
 }
 
-// Inclusive sums over the wave's lanes
+// Inclusive sums over the wave's lanes, in registers
+template <int CTRL, int ROWS> __device__ __forceinline__ int pa_add_dpp(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
 __device__ __forceinline__ int pa_scan(int v) {
-    for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(v, o);
-        if ((int)(threadIdx.x & 63) >= o) v += t;
-    }
-    return v;
+    v = pa_add_dpp<0x111, 0xf>(v);   // from 1, 2, 4 and 8 lanes below in the row of 16
+    v = pa_add_dpp<0x112, 0xf>(v);
+    v = pa_add_dpp<0x114, 0xf>(v);
+    v = pa_add_dpp<0x118, 0xf>(v);
+    v = pa_add_dpp<0x142, 0xa>(v);   // the sums of rows 0 and 2 to rows 1 and 3
+    return pa_add_dpp<0x143, 0xc>(v);   // of the lower half to the upper
 }
 
 // All sequences' tiles, and how many shares they make: share u has tiles
-// [u T / n, (u + 1) T / n)
+// [u T / n, (u + 1) T / n). With it the spans of 64 sequences, one a lane.
 struct PaAll {
     int tiles, shares;
+    int base, len, sum;   // the lanes' sequences from `base` on: lengths, inclusive sums of tiles
+    int before;           // tiles of the sequences before `base`
 };
-__device__ __forceinline__ PaAll pa_all(const PgView &p, const PaArgs &a, int &bad) {
-    const int lane = threadIdx.x & 63;
-    int t = 0;
-    for (int i = lane; i < p.n_seq; i += 64) t += pa_span(a, a.len[i], bad).tiles;
-    for (int o = 32; o >= 1; o >>= 1) t += __shfl_xor(t, o);
-    t = __builtin_amdgcn_readfirstlane(t);
-    return { t, max(1, min(a.shares, (t + PA_SHARE - 1) / PA_SHARE)) };
+__device__ __forceinline__ void pa_fetch(const PgView &p, const PaArgs &a, PaAll &r, int base, int &bad) {
+    const int i = base + (int)(threadIdx.x & 63);
+    r.base = base;
+    r.len = i < p.n_seq ? kr_page_len(a.len[i], a.max_len, bad) : 0;
+    r.sum = pa_scan(i < p.n_seq ? pa_span(a, r.len).tiles : 0);
 }
-// the sequence that holds tile t of all, and the tile's number in it
-__device__ __forceinline__ int pa_find(const PgView &p, const PaArgs &a, int &t, int &bad) {
-    const int lane = threadIdx.x & 63;
-    for (int i0 = 0;; i0 += 64) {
-        const int i = i0 + lane, own = i < p.n_seq ? pa_span(a, a.len[i], bad).tiles : 0, sum = pa_scan(own);
-        const int n = __popcll(__ballot(i < p.n_seq && sum <= t));
-        if (n < 64 || i0 + 64 >= p.n_seq) {
-            t -= n ? __builtin_amdgcn_readlane(sum, n - 1) : 0;
-            return i0 + n;
-        }
-        t -= __builtin_amdgcn_readlane(sum, 63);
+__device__ __forceinline__ PaAll pa_all(const PgView &p, const PaArgs &a, int &bad) {
+    PaAll r;
+    int t = 0;
+    for (int i0 = 0; i0 < p.n_seq; i0 += 64) {
+        r.before = t;
+        pa_fetch(p, a, r, i0, bad);
+        t += __builtin_amdgcn_readlane(r.sum, 63);
     }
+    r.tiles = t;
+    r.shares = max(1, min(a.shares, (t + a.least - 1) / a.least));
+    return r;
+}
+__device__ __forceinline__ int pa_len(const PgView &p, const PaArgs &a, PaAll &r, int s, int &bad) {
+    if (s - r.base >= 64 || s < r.base) pa_fetch(p, a, r, s & ~63, bad);
+    return __builtin_amdgcn_readlane(r.len, s - r.base);
+}
+// the sequence that holds tile t of all; t becomes the tile's number in it
+__device__ __forceinline__ int pa_find(const PgView &p, const PaArgs &a, PaAll &r, int &t, int &bad) {
+    if (t >= r.before) {
+        t -= r.before;
+    } else {
+        pa_fetch(p, a, r, 0, bad);
+    }
+    for (;;) {
+        const int all = __builtin_amdgcn_readlane(r.sum, 63);
+        if (t < all) break;
+        t -= all;
+        pa_fetch(p, a, r, r.base + 64, bad);
+    }
+    const int n = __popcll(__ballot(r.sum <= t));
+    if (n) t -= __builtin_amdgcn_readlane(r.sum, n - 1);
+    return r.base + n;
 }
 __device__ __forceinline__ int pa_bound(const PaAll &all, int u) { return (int)((long long)all.tiles * u / all.shares); }
 // the share that holds tile t
@@ -124,6 +149,9 @@ __device__ __forceinline__ float pa_sum_g(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+__device__ __forceinline__ float4v pa_weigh(half8 v, half8 p, float4v o) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, o, 0, 0, 0); }
+__device__ __forceinline__ float4v pa_weigh(half4 v, half4 p, float4v o) { return __builtin_amdgcn_mfma_f32_16x16x16f16(v, p, o, 0, 0, 0); }
+
 // halves of 4 int8 (xor 0x80: 0..255) as 1024 + u - 1152, exact
 __device__ __forceinline__ unsigned pa_h2(unsigned u, unsigned sel) {
     const half2v h = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, sel));
@@ -131,21 +159,22 @@ __device__ __forceinline__ unsigned pa_h2(unsigned u, unsigned sel) {
 }
 
 // what a lane holds of a tile, as it lies in memory. K: per product step its
-// rows r and r + 4; V: W dims of each of its 8 rows.
+// NT rows 4 apart; V: W dims of each of its 4 NT rows.
 template <int KT, int CL> struct PaRaw {
     static constexpr int W = CL / 16;                                  // dims a lane has of a V row
     static constexpr int KS = KT == PG_F32 ? CL / 16 : CL / 32;        // loads a K row
     static constexpr int KB = KT == PG_F32 ? 4 : KT == PG_F16 ? 4 : 2; // words a load
     static constexpr int VB = KT == PG_F32 ? W : KT == PG_F16 ? W / 2 : W / 4;
-    unsigned k[2][KS][KB], v[8][VB];
-    float kd[KT == PG_Q8 ? 8 : 1], vd[KT == PG_Q8 ? 8 : 1];
+    static constexpr int NT = pa_tile(CL) / 16, R = 4 * NT;            // products a tile, V rows a lane
+    unsigned k[NT][KS][KB], v[R][VB];
+    float kd[KT == PG_Q8 ? R : 1], vd[KT == PG_Q8 ? R : 1];
 };
 
 template <int N> __device__ __forceinline__ void pa_load(unsigned (&x)[N], const void *p) {
     static_assert(N == 1 || N == 2 || N % 4 == 0, "whole loads");
-    if (N == 1) {
+    if constexpr (N == 1) {
         x[0] = *(const unsigned *)p;
-    } else if (N == 2) {
+    } else if constexpr (N == 2) {
         const uint2v t = *(const uint2v *)p;
         x[0] = t.x;
         x[1] = t.y;
@@ -163,12 +192,12 @@ template <int N> __device__ __forceinline__ void pa_load(unsigned (&x)[N], const
 
 // Whether two tiles' rows fit in registers: the next tile's are read while one
 // is worked on; where they do not, its K rows are, once this tile's are used.
-constexpr bool pa_two(int kt, int cl) { return cl <= (kt == PG_F32 ? 64 : 128); }
-constexpr int pa_waves(int kt, int cl) { return pa_two(kt, cl) || kt == PG_Q8 ? 2 : 1; }   // a SIMD
+constexpr bool pa_two(int kt, int cl) { return cl <= (kt == PG_F32 ? 64 : 128) || kt == PG_Q8; }
+constexpr int pa_waves(int kt, int cl) { return cl > (kt == PG_Q8 ? 128 : 64) ? 1 : 2; }   // a SIMD
 
 template <int KT, int CL, int NB, bool FULL> struct PaWave {
     using Raw = PaRaw<KT, CL>;
-    static constexpr int W = Raw::W, KS = Raw::KS, EB = KT == PG_F32 ? 4 : KT == PG_F16 ? 2 : 1;
+    static constexpr int W = Raw::W, KS = Raw::KS, NT = Raw::NT, R = Raw::R, TILE = 16 * NT, EB = KT == PG_F32 ? 4 : KT == PG_F16 ? 2 : 1;
     static constexpr int KD = KT == PG_F32 ? 4 : 8;   // dims a K load
     static constexpr bool HALF = KT != PG_F32;
 
@@ -179,8 +208,7 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
     int seq, t_ids, bad;
     PaSpan sp;
     int ids;   // the pages of 64 half tiles from t_ids on, one a lane
-    float qf[HALF ? 1 : KS][4];
-    half8 qh[HALF ? KS : 1][NB];
+    std::conditional_t<HALF, half8, float4v> qf[KS][NB];   // the queries as operands
     float cs, m_run, l_run;
     int ev;    // Q8: the weights carry the V scales over 2^ev
     float4v o[W];
@@ -200,10 +228,14 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
     }
     // pool rows of the halves of the tile at t0; a half without rows attended takes the other's
     __device__ __forceinline__ void rows_of(int t0, size_t &lo, size_t &hi) {
-        const int i = (t0 - t_ids) >> 4;
-        const int pl = __builtin_amdgcn_readlane(ids, i), ph = __builtin_amdgcn_readlane(ids, i + 1);
-        lo = kr_page_row(pl >= 0 ? pl : ph, p.n_kv, kvh, p.shift, t0);
-        hi = kr_page_row(ph >= 0 ? ph : pl, p.n_kv, kvh, p.shift, t0 + 16);
+        const int i = (t0 - t_ids) >> 4, pl = __builtin_amdgcn_readlane(ids, i);
+        if constexpr (NT == 1) {
+            lo = hi = kr_page_row(pl, p.n_kv, kvh, p.shift, t0);
+        } else {
+            const int ph = __builtin_amdgcn_readlane(ids, i + 1);
+            lo = kr_page_row(pl >= 0 ? pl : ph, p.n_kv, kvh, p.shift, t0);
+            hi = kr_page_row(ph >= 0 ? ph : pl, p.n_kv, kvh, p.shift, t0 + 16);
+        }
     }
 
     // the queries as operands
@@ -229,38 +261,39 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             m = pa_max_g(m);
             if (m > 0.0f && m < INFINITY) e = 13 - ilogbf(m);
 #pragma unroll
-            for (int j = 0; j < KS; j++)
+            for (int j = 0; j < KS; j++) {
+                half8 h, l;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const float y = ldexpf(x[j][i], e);
-                    const _Float16 hi = (_Float16)y;
-                    const _Float16 lo = (_Float16)(y - (float)hi);
-                    if (NB == 1) {
-                        qh[j][0][i] = is_lo ? lo : hi;
-                    } else {
-                        qh[j][0][i] = hi;
-                        qh[j][NB - 1][i] = lo;
-                    }
+                    h[i] = (_Float16)y;
+                    l[i] = (_Float16)(y - (float)h[i]);
                 }
+                if constexpr (NB == 1) {
+                    qf[j][0] = is_lo ? l : h;
+                } else {
+                    qf[j][0] = h;
+                    qf[j][1] = l;
+                }
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < KS; j++) {
                 const int d = j * 16 + g * 4;
                 const float4v t = live && (FULL || d < hd) ? *(const float4v *)(q + d) : float4v{ 0, 0, 0, 0 };
-#pragma unroll
-                for (int c = 0; c < 4; c++) qf[j][c] = t[c];
+                qf[j][0] = t;
             }
         }
         // a product's factor: the scale, in log2 unless the cap comes first
         cs = ldexpf(a.cap > 0.0f ? a.scale : a.scale * 1.4426950408889634f, -e);
     }
 
-    // this lane's K rows of a tile are 8 (n / 4) + n % 4 and 4 after it
+    // this lane's K rows of a tile are R (n / 4) + n % 4 and 4 after it
     __device__ __forceinline__ void load_k(Raw &raw, size_t lo, size_t hi) const {
-        const int r0 = 8 * (n >> 2) + (n & 3);
-        const size_t r = r0 < 16 ? lo + r0 : hi + (r0 - 16);
+        const int r0 = R * (n >> 2) + (n & 3);
+        const size_t r = NT == 1 || r0 < 16 ? lo + r0 : hi + (r0 - 16);
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
+        for (int b = 0; b < NT; b++) {
             const char *at = (const char *)p.k + (r + 4 * b) * hd * EB;
 #pragma unroll
             for (int j = 0; j < KS; j++) {
@@ -273,13 +306,13 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             }
         }
     }
-    // its V rows 8 g .. 8 g + 7, dims n W ..
+    // its V rows R g .. R g + R - 1, dims n W ..
     __device__ __forceinline__ void load_v(Raw &raw, size_t lo, size_t hi) const {
-        const int r0 = 8 * g;
-        const size_t r = r0 < 16 ? lo + r0 : hi + (r0 - 16);
+        const int r0 = R * g;
+        const size_t r = NT == 1 || r0 < 16 ? lo + r0 : hi + (r0 - 16);
         if constexpr (KT == PG_Q8) {
 #pragma unroll
-            for (int i = 0; i < 8; i += 4) {
+            for (int i = 0; i < R; i += 4) {
                 const float4v x = *(const float4v *)(p.kd + r + i), y = *(const float4v *)(p.vd + r + i);
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
@@ -289,7 +322,7 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < R; i++) {
             const char *at = (const char *)p.v + (r + i) * hd * EB;
             if constexpr (FULL) {
                 pa_load(raw.v[i], at + n * W * EB);
@@ -308,10 +341,10 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
         }
     }
 
-    // products of the tile's rows 8 g + i with the queries of head `col`
-    __device__ __forceinline__ void scores(const Raw &raw, float (&sc)[8]) const {
+    // products of the tile's rows R g + i with the queries of head `col`
+    __device__ __forceinline__ void scores(const Raw &raw, float (&sc)[R]) const {
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
+        for (int b = 0; b < NT; b++) {
             float4v acc = { 0, 0, 0, 0 };
 #pragma unroll
             for (int j = 0; j < KS; j++) {
@@ -323,13 +356,13 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
                         const unsigned x = raw.k[b][j][0] ^ 0x80808080u, y = raw.k[b][j][1] ^ 0x80808080u;
                         w = uint4v{ pa_h2(x, 0x04010400), pa_h2(x, 0x04030402), pa_h2(y, 0x04010400), pa_h2(y, 0x04030402) };
                     }
-                    const half8 kf = __builtin_bit_cast(half8, w);
 #pragma unroll
-                    for (int x = 0; x < NB; x++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[j][x], acc, 0, 0, 0);
+                    for (int x = 0; x < NB; x++)
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), qf[j][x], acc, 0, 0, 0);
                 } else {
 #pragma unroll
                     for (int c = 0; c < 4; c++)
-                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(raw.k[b][j][c]), qf[j][c], acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(raw.k[b][j][c]), qf[j][0][c], acc, 0, 0, 0);
                 }
             }
 #pragma unroll
@@ -338,23 +371,23 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
     }
 
     // the softmax's step over the tile at t0, then its V rows by their weights
-    __device__ __forceinline__ void rest(Raw &raw, float (&sc)[8], int t0) {
-        const bool whole = t0 >= sp.first && t0 + PA_TILE <= sp.len;
-        const int r0 = t0 + 8 * g;
+    __device__ __forceinline__ void rest(Raw &raw, float (&sc)[R], int t0) {
+        const bool whole = t0 >= sp.first && t0 + TILE <= sp.len;
+        const int r0 = t0 + R * g;
         float m_tile = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < R; i++) {
             float x = sc[i];
             if (NB == 1 && HALF) x += pa_swap8(x);
             sc[i] = x * (KT == PG_Q8 ? cs * raw.kd[i] : cs);
         }
         if (a.cap > 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) sc[i] = a.cap * kr_tanhf(sc[i] / a.cap) * 1.4426950408889634f;
+            for (int i = 0; i < R; i++) sc[i] = a.cap * kr_tanhf(sc[i] / a.cap) * 1.4426950408889634f;
         }
         if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < R; i++) {
                 const bool in = r0 + i >= sp.first && r0 + i < sp.len;
                 sc[i] = in ? sc[i] : -INFINITY;
                 // rows that are not attended may hold anything
@@ -367,18 +400,18 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) m_tile = fmaxf(m_tile, sc[i]);
+        for (int i = 0; i < R; i++) m_tile = fmaxf(m_tile, sc[i]);
         if (a.z && live && !is_lo) {
             float *z = a.z + head() * a.z_ld + r0;
-            *(float4v *)z = float4v{ sc[0], sc[1], sc[2], sc[3] };
-            *(float4v *)(z + 4) = float4v{ sc[4], sc[5], sc[6], sc[7] };
+#pragma unroll
+            for (int i = 0; i < R; i += 4) *(float4v *)(z + i) = float4v{ sc[i], sc[i + 1], sc[i + 2], sc[i + 3] };
         }
         m_tile = pa_max_g(m_tile);
         int ev_new = ev;
         if constexpr (KT == PG_Q8) {
             float vm = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) vm = fmaxf(vm, fabsf(raw.vd[i]));
+            for (int i = 0; i < R; i++) vm = fmaxf(vm, fabsf(raw.vd[i]));
             vm = pa_max_g(vm);
             ev_new = max(ev, min((int)(__float_as_uint(vm) >> 23) - 126, 120));
         }
@@ -395,10 +428,13 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
         // weights of no finite maximum: 0 for -inf, NaN for NaN
         const float base = (m_run == -INFINITY ? 0.0f : m_run) - (HALF ? PA_UP : 0.0f);
         const float vs = KT == PG_Q8 ? ldexpf(1.0f, -ev) : 1.0f;
-        half8 ph[NB], pl;
-        float pf[8];
+        // the weights as operands: R halves, or floats
+        typedef _Float16 halfr __attribute__((ext_vector_type(R)));
+        typedef unsigned uintr __attribute__((ext_vector_type(R / 2)));
+        halfr ph[NB], pl;
+        float pf[R];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < R; i++) {
             float x = __builtin_amdgcn_exp2f(sc[i] - base);
             l_run += x;
             if constexpr (KT == PG_Q8) {
@@ -418,35 +454,34 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
         }
         if constexpr (HALF) {
             if constexpr (NB == 1) {
-                const uint4v x = __builtin_bit_cast(uint4v, ph[0]), y = __builtin_bit_cast(uint4v, pl);
-                ph[0] = __builtin_bit_cast(half8, is_lo ? y : x);
+                const uintr x = __builtin_bit_cast(uintr, ph[0]), y = __builtin_bit_cast(uintr, pl);
+                ph[0] = __builtin_bit_cast(halfr, is_lo ? y : x);
             } else {
                 ph[1] = pl;
             }
         }
         if constexpr (KT == PG_F32) {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int i = 0; i < R; i++)
 #pragma unroll
                 for (int c = 0; c < W; c++)
                     o[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(raw.v[i][c]), pf[i], o[c], 0, 0, 0);
         } else if constexpr (KT == PG_F16) {
 #pragma unroll
             for (int c = 0; c < W; c++) {
-                uint4v w;
+                uintr w;
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < R / 2; i++)
                     w[i] = __builtin_amdgcn_perm(raw.v[2 * i + 1][c / 2], raw.v[2 * i][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
-                const half8 vf = __builtin_bit_cast(half8, w);
 #pragma unroll
-                for (int x = 0; x < NB; x++) o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[x], o[c], 0, 0, 0);
+                for (int x = 0; x < NB; x++) o[c] = pa_weigh(__builtin_bit_cast(halfr, w), ph[x], o[c]);
             }
         } else {
 #pragma unroll
             for (int c4 = 0; c4 < W; c4 += 4) {
-                uint4v w[4];
+                uintr w[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < R / 2; i++) {
                     const unsigned x = raw.v[2 * i][c4 / 4] ^ 0x80808080u, y = raw.v[2 * i + 1][c4 / 4] ^ 0x80808080u;
                     const unsigned u = __builtin_amdgcn_perm(y, x, 0x05010400u), v = __builtin_amdgcn_perm(y, x, 0x07030602u);
                     w[0][i] = pa_h2(u, 0x04010400);
@@ -456,10 +491,8 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
                 }
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    const half8 vf = __builtin_bit_cast(half8, w[c]);
 #pragma unroll
-                    for (int x = 0; x < NB; x++)
-                        o[c4 + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[x], o[c4 + c], 0, 0, 0);
+                    for (int x = 0; x < NB; x++) o[c4 + c] = pa_weigh(__builtin_bit_cast(halfr, w[c]), ph[x], o[c4 + c]);
                 }
             }
         }
@@ -472,22 +505,24 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
         load_v(raw, lo, hi);
     }
 
-    // rows [t0, t1) of the sequence, whole tiles but at its end: at most 32, whose pages are in ids
-    __device__ __forceinline__ void pass(int t0, int t1) {
-        float sc[8];
+    // rows [t0, t1) of the sequence, whole tiles but at its end: at most 64 half tiles, whose
+    // pages are in ids. The first rows are asked for before the queries are.
+    __device__ __forceinline__ void pass(int t0, int t1, bool begin) {
+        float sc[R];
         if constexpr (pa_two(KT, CL)) {
             Raw x, y;
             load(x, t0);
-            for (;; t0 += 2 * PA_TILE) {
-                const bool more = t0 + PA_TILE < t1;
-                if (more) load(y, t0 + PA_TILE);
+            if (begin) queries();
+            for (;; t0 += 2 * TILE) {
+                const bool more = t0 + TILE < t1;
+                if (more) load(y, t0 + TILE);
                 scores(x, sc);
                 rest(x, sc, t0);
                 if (!more) break;
-                const bool again = t0 + 2 * PA_TILE < t1;
-                if (again) load(x, t0 + 2 * PA_TILE);
+                const bool again = t0 + 2 * TILE < t1;
+                if (again) load(x, t0 + 2 * TILE);
                 scores(y, sc);
-                rest(y, sc, t0 + PA_TILE);
+                rest(y, sc, t0 + TILE);
                 if (!again) break;
             }
         } else {
@@ -495,12 +530,13 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             size_t lo, hi;
             rows_of(t0, lo, hi);
             load_k(x, lo, hi);
-            for (;; t0 += PA_TILE) {
+            if (begin) queries();
+            for (;; t0 += TILE) {
                 load_v(x, lo, hi);
                 scores(x, sc);
-                const bool more = t0 + PA_TILE < t1;
+                const bool more = t0 + TILE < t1;
                 if (more) {
-                    rows_of(t0 + PA_TILE, lo, hi);
+                    rows_of(t0 + TILE, lo, hi);
                     load_k(x, lo, hi);
                 }
                 rest(x, sc, t0);
@@ -518,12 +554,11 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
         for (int c = 0; c < W; c++) o[c] = float4v{ 0, 0, 0, 0 };
         const bool alone = t == 0 && end == sp.tiles;
         if (sp.len > 0) {
-            const int r1 = min(sp.len, sp.begin + end * PA_TILE);
-            find(sp.begin + t * PA_TILE);
-            queries();
-            for (int r = sp.begin + t * PA_TILE; r < r1; r += 32 * PA_TILE) {
-                if (r != t_ids) find(r);
-                pass(r, min(r1, r + 32 * PA_TILE));
+            const int r1 = min(sp.len, sp.begin + end * TILE);
+            const int r0 = sp.begin + t * TILE;
+            for (int r = r0; r < r1; r += (64 / NT) * TILE) {
+                find(r);
+                pass(r, min(r1, r + (64 / NT) * TILE), r == r0);
             }
         }
         if (NB == 1 && HALF) {
@@ -533,13 +568,11 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
                 for (int i = 0; i < 4; i++) o[c][i] += pa_swap8(o[c][i]);
         }
         const float l = pa_sum_g(l_run);
-        if (!live || is_lo) return;
         float f = alone ? 1.0f / l : 1.0f;
         if (KT == PG_Q8) f = ldexpf(f, ev);
         if (sp.len == 0) f = 0.0f;
-        if (g == 0 && (!alone || a.z)) {
-            a.pml[(slot * group + col) * 2] = m_run;
-            a.pml[(slot * group + col) * 2 + 1] = l;
+        if (g == 0 && live && !is_lo && (!alone || a.z)) {
+            *(float2v *)(a.pml + (slot * group + col) * 2) = float2v{ m_run, l };
         }
         float *out = alone ? a.o + head() * hd : a.part + (slot * group + col) * hd;
 #pragma unroll
@@ -547,7 +580,7 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             const int d0 = (4 * g + i) * W;
 #pragma unroll
             for (int c = 0; c < W; c += 4)
-                if (FULL || d0 + c < hd)
+                if (live && !is_lo && (FULL || d0 + c < hd))
                     *(float4v *)(out + d0 + c) = float4v{ o[c][i] * f, o[c + 1][i] * f, o[c + 2][i] * f, o[c + 3][i] * f };
         }
     }
@@ -557,11 +590,11 @@ template <int KT, int CL, int NB, bool FULL>
 __global__ void __launch_bounds__(64, pa_waves(KT, CL)) k_paged_shares(const PgView p, const PaArgs a, int *fault) {
     const int u = blockIdx.x, kvh = blockIdx.y;
     PaWave<KT, CL, NB, FULL> w(p, a, kvh);
-    const PaAll all = pa_all(p, a, w.bad);
+    PaAll all = pa_all(p, a, w.bad);
     if (u < all.shares) {
         int left = pa_bound(all, u + 1) - pa_bound(all, u), t = pa_bound(all, u);
-        for (w.seq = pa_find(p, a, t, w.bad); left > 0; w.seq++, t = 0) {
-            w.sp = pa_span(a, a.len[w.seq], w.bad);
+        for (w.seq = pa_find(p, a, all, t, w.bad); left > 0; w.seq++, t = 0) {
+            w.sp = pa_span(a, pa_len(p, a, all, w.seq, w.bad));
             const int end = min(w.sp.tiles, t + left);
             w.part(t, end, (size_t)kvh * (p.n_seq + a.shares) + w.seq + u);
             left -= end - t;
@@ -575,23 +608,31 @@ struct PaParts {
     size_t slot;
     int n;
 };
-__device__ __forceinline__ PaParts pa_parts(const PgView &p, const PaArgs &a, int s, int kvh) {
-    int bad = 0, before = 0;   // reported by the shares
-    const PaAll all = pa_all(p, a, bad);
-    for (int i = threadIdx.x & 63; i < s; i += 64) before += pa_span(a, a.len[i], bad).tiles;
+__device__ __forceinline__ PaParts pa_parts(const PgView &p, const PaArgs &a, int s, int kvh, PaSpan &sp) {
+    int bad = 0;   // reported by the shares
+    PaAll all = pa_all(p, a, bad);
+    int before = 0;
+    for (int i = threadIdx.x & 63; i < (s & ~63); i += 64) before += pa_span(a, kr_page_len(a.len[i], a.max_len, bad)).tiles;
     for (int o = 32; o >= 1; o >>= 1) before += __shfl_xor(before, o);
-    before = __builtin_amdgcn_readfirstlane(before);
-    const int u0 = pa_share(all, before), u1 = pa_share(all, before + pa_span(a, a.len[s], bad).tiles - 1);
+    sp = pa_span(a, pa_len(p, a, all, s, bad));
+    const int end = __builtin_amdgcn_readfirstlane(before) + __builtin_amdgcn_readlane(all.sum, s - all.base);
+    const int u0 = pa_share(all, end - sp.tiles), u1 = pa_share(all, end - 1);
     return { (size_t)kvh * (p.n_seq + a.shares) + s + u0, u1 - u0 + 1 };
 }
 
 // A head's maximum and 1 / its sum, by one wave
 __device__ __forceinline__ void pa_stats(const float *ml, int group, int n, float &m, float &inv) {
-    float l = 0.0f;
-    m = -INFINITY;
-    for (int i = threadIdx.x & 63; i < n; i += 64) m = fmaxf(m, ml[(size_t)i * group * 2]);
+    const int lane = threadIdx.x & 63;
+    auto get = [&](int i) { return i < n ? *(const float2v *)(ml + (size_t)i * group * 2) : float2v{ -INFINITY, 0.0f }; };
+    const float2v own = get(lane);   // up to 64 parts are read once
+    m = own.x;
+    for (int i = lane + 64; i < n; i += 64) m = fmaxf(m, get(i).x);
     for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    for (int i = threadIdx.x & 63; i < n; i += 64) l += ml[(size_t)i * group * 2 + 1] * __builtin_amdgcn_exp2f(ml[(size_t)i * group * 2] - m);
+    float l = lane < n ? own.y * __builtin_amdgcn_exp2f(own.x - m) : 0.0f;
+    for (int i = lane + 64; i < n; i += 64) {
+        const float2v x = get(i);
+        l += x.y * __builtin_amdgcn_exp2f(x.x - m);
+    }
     for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
     inv = 1.0f / l;
 }
@@ -599,39 +640,55 @@ __device__ __forceinline__ void pa_stats(const float *ml, int group, int n, floa
 // Workgroups x < nh: head x's parts (2^dl lanes hold its dims four at a time, the
 // workgroup's other factor the parts side by side). The others, with a mass:
 // PJ_ROWS rows of one KV head each, mass[r] += its weights over the query heads.
-constexpr int PJ_T = 256, PJ_ROWS = 1024;
+constexpr int PJ_T = 256, PJ_ROWS = 1024, PJ_U = 4;
 __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArgs a, int dl, int blocks) {
     __shared__ float4v s_o[PJ_T];
     __shared__ float s_m[KR_PAGE_GROUP_MAX], s_i[KR_PAGE_GROUP_MAX];
     const int s = blockIdx.y, x = blockIdx.x, tid = threadIdx.x, group = a.nh / p.n_kv;
+    PaSpan sp;
     if (x < a.nh) {
         const int kvh = x / group, col = x % group;
-        const PaParts r = pa_parts(p, a, s, kvh);
+        const PaParts r = pa_parts(p, a, s, kvh, sp);
         if (r.n <= 1) return;
         const float *ml = a.pml + (r.slot * group + col) * 2, *part = a.part + (r.slot * group + col) * p.hd;
+        const int l = tid & ((1 << dl) - 1), lanes = PJ_T >> dl, d = 4 * l < p.hd ? 4 * l : 0, i0 = tid >> dl;
+        // the first parts are under way while their weights are found
+        float4v v[PJ_U];
+        float w[PJ_U];
+#pragma unroll
+        for (int k = 0; k < PJ_U; k++) {
+            const int i = min(i0 + k * lanes, r.n - 1);
+            v[k] = *(const float4v *)(part + (size_t)i * group * p.hd + d);
+            w[k] = ml[(size_t)i * group * 2];
+        }
         float m, inv;
         pa_stats(ml, group, r.n, m, inv);
-        const int l = tid & ((1 << dl) - 1), lanes = PJ_T >> dl;
         float4v acc = { 0, 0, 0, 0 };
-        if (4 * l < p.hd) {
-#pragma unroll 4
-            for (int i = tid >> dl; i < r.n; i += lanes)
-                acc += *(const float4v *)(part + (size_t)i * group * p.hd + 4 * l) * __builtin_amdgcn_exp2f(ml[(size_t)i * group * 2] - m);
+        for (int k0 = 0;;) {
+#pragma unroll
+            for (int k = 0; k < PJ_U; k++)
+                if (i0 + (k0 + k) * lanes < r.n) acc += v[k] * __builtin_amdgcn_exp2f(w[k] - m);
+            k0 += PJ_U;
+            if (i0 + k0 * lanes >= r.n) break;
+#pragma unroll
+            for (int k = 0; k < PJ_U; k++) {
+                const int i = min(i0 + (k0 + k) * lanes, r.n - 1);
+                v[k] = *(const float4v *)(part + (size_t)i * group * p.hd + d);
+                w[k] = ml[(size_t)i * group * 2];
+            }
         }
         s_o[tid] = acc;
         for (int h = lanes >> 1; h >= 1; h >>= 1) {
             __syncthreads();
             if ((tid >> dl) < h) s_o[tid] = acc = acc + s_o[tid + (h << dl)];
         }
-        if (tid >> dl == 0 && 4 * l < p.hd) *(float4v *)(a.o + ((size_t)s * a.nh + x) * p.hd + 4 * l) = acc * inv;
+        if (tid >> dl == 0 && 4 * l < p.hd) *(float4v *)(a.o + ((size_t)s * a.nh + x) * p.hd + d) = acc * inv;
         return;
     }
     const int kvh = (x - a.nh) / blocks, block = (x - a.nh) % blocks;
-    int bad = 0;
-    const PaSpan sp = pa_span(a, a.len[s], bad);
+    const PaParts r = pa_parts(p, a, s, kvh, sp);
     const int r0 = sp.first + block * PJ_ROWS;
     if (r0 >= sp.len) return;
-    const PaParts r = pa_parts(p, a, s, kvh);
     for (int h = tid >> 6; h < group; h += PJ_T / 64) {
         float m, inv;
         pa_stats(a.pml + (r.slot * group + h) * 2, group, r.n, m, inv);
@@ -641,26 +698,43 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
         }
     }
     __syncthreads();
-    const float up = a.z_up;
     const float *z = a.z + ((size_t)s * a.nh + kvh * group) * a.z_ld;
     float *mass = a.mass + ((size_t)s * p.n_kv + kvh) * a.mass_ld;
+    float sum[PJ_ROWS / PJ_T], old[PJ_ROWS / PJ_T];
+#pragma unroll
+    for (int k = 0; k < PJ_ROWS / PJ_T; k++) {
+        sum[k] = 0.0f;
+        old[k] = mass[min(r0 + k * PJ_T + tid, sp.len - 1)];
+    }
+    for (int h = 0; h < group; h++) {
+        const float m = s_m[h] - a.z_up, inv = s_i[h];
+#pragma unroll
+        for (int k = 0; k < PJ_ROWS / PJ_T; k++)
+            sum[k] += __builtin_amdgcn_exp2f(z[h * a.z_ld + min(r0 + k * PJ_T + tid, sp.len - 1)] - m) * inv;
+    }
 #pragma unroll
     for (int k = 0; k < PJ_ROWS / PJ_T; k++) {
         const int i = r0 + k * PJ_T + tid;
-        if (i >= sp.len) break;
-        float sum = 0.0f;
-        for (int h = 0; h < group; h++) sum += __builtin_amdgcn_exp2f(z[h * a.z_ld + i] - s_m[h] + up) * s_i[h];
-        mass[i] += sum;
+        if (i < sp.len) mass[i] = old[k] + sum[k];
     }
 }
 
-// Shares in all, of every KV head: about PA_WAVES waves, fewer where the rows
-// are few. The lengths are the device's, so this is what they may be at most.
-constexpr int PA_WAVES = 2048;
-int pa_shares(int n_seq, int n_kv, int rows) {
-    const long long tiles = (long long)n_seq * ((rows + PA_TILE - 1) / PA_TILE), most = (tiles + PA_SHARE - 1) / PA_SHARE;
-    const long long want = PA_WAVES / n_kv > 1 ? PA_WAVES / n_kv : 1;
-    return (int)(want < most ? want : most);
+// Shares in all, of every KV head, so that each SIMD has a wave (8-bit caches:
+// two, their waves work more and read less), fewer where the rows are few: a
+// share is worth PA_BYTES of K and V at least. The lengths are the device's, so
+// this is what they may be at most.
+// Measured (us, 1024 / 2048 waves): 8B shape, 16 sequences 30.2 / 32.7, one of
+// 120,001 rows 98 / 105; 8-bit heads of 64 31.9 / 27.8. With 16, 32 and 64 KB:
+// one sequence of 4000 rows 15.5, 13.7, 13.7; 64 of up to 300 23.5, 23.0, 25.4.
+constexpr int PA_WAVES = 1024, PA_BYTES = 32 * 1024;
+int pa_least(const krh_pages *kv) {
+    const int tile = 2 * pa_tile(kv->head_dim) * kv->head_dim * (kv->kv_type == ML_F32 ? 4 : kv->kv_type == ML_F16 ? 2 : 1);
+    return tile < PA_BYTES ? PA_BYTES / tile : 1;
+}
+int pa_shares(const krh_pages *kv, int n_seq, int rows) {
+    const long long tile = pa_tile(kv->head_dim), tiles = n_seq * ((rows + tile - 1) / tile), least = pa_least(kv);
+    const long long most = (tiles + least - 1) / least, want = (kv->kv_type == ML_Q8_0 ? 2 * PA_WAVES : PA_WAVES) / kv->n_kv_heads;
+    return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
 // the workspace's pieces, in floats
@@ -672,14 +746,14 @@ PaSizes pa_sizes(const krh_pages *kv, int n_seq, int nh, int max_len, int shares
     const size_t slots = (size_t)kv->n_kv_heads * (n_seq + shares) * (nh / kv->n_kv_heads);
     r.part = shares > 1 ? slots * kv->head_dim : 0;
     r.pml = shares > 1 || mass ? (slots * 2 + 3) & ~(size_t)3 : 0;
-    r.z_ld = mass ? ((size_t)max_len + PA_TILE - 1) / PA_TILE * PA_TILE : 0;
+    r.z_ld = mass ? ((size_t)max_len + 31) / 32 * 32 : 0;
     r.z = (size_t)n_seq * nh * r.z_ld;
     return r;
 }
 
 bool pa_args_ok(const krh_pages *kv, int n_seq, int n_heads, int max_len) {
     return pg_pages_ok(kv) && n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && max_len <= INT32_MAX / 2 &&
-           (long long)n_seq * (max_len / PA_TILE + 1) <= INT32_MAX / 2 && n_heads > 0 &&
+           (long long)n_seq * (max_len / 16 + 1) <= INT32_MAX / 2 && n_heads > 0 &&
            n_heads % kv->n_kv_heads == 0 && n_heads / kv->n_kv_heads <= KR_PAGE_GROUP_MAX;
 }
 
@@ -701,7 +775,7 @@ template <int KT> PaKernel pa_kernel(int group, int hd) {
 
 extern "C" size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int max_len, int mass) {
     if (!pa_args_ok(kv, n_seq, n_heads, max_len)) return 0;
-    const PaSizes r = pa_sizes(kv, n_seq, n_heads, max_len, pa_shares(n_seq, kv->n_kv_heads, max_len), mass != 0);
+    const PaSizes r = pa_sizes(kv, n_seq, n_heads, max_len, pa_shares(kv, n_seq, max_len), mass != 0);
     return sizeof(float) * (r.part + r.pml + r.z + 4);
 }
 
@@ -716,14 +790,14 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
                   "paged_attention: window, soft-cap or mass rows"))
         return;
     // a window's rows, and those before them in its first tile
-    const int rows = window > 0 && window < max_len - PA_TILE ? window + PA_TILE - 1 : max_len;
-    const int shares = pa_shares(n_seq, kv->n_kv_heads, rows);
+    const int rows = window > 0 && window < max_len - 32 ? window + 31 : max_len;
+    const int shares = pa_shares(kv, n_seq, rows);
     const PaSizes r = pa_sizes(kv, n_seq, n_heads, max_len, shares, mass != nullptr);
     float *w = (float *)ws;
     PaArgs a = {};
     a.o = o, a.q = q, a.len = len, a.mass = mass, a.mass_ld = mass_ld;
     a.part = w, a.pml = w + r.part, a.z = mass ? w + r.part + r.pml : nullptr, a.z_ld = r.z_ld;
-    a.nh = n_heads, a.max_len = max_len, a.window = window, a.shares = shares;
+    a.nh = n_heads, a.max_len = max_len, a.window = window, a.shares = shares, a.least = pa_least(kv), a.tl = pg_log2(pa_tile(kv->head_dim));
     a.scale = scale, a.cap = softcap, a.z_up = kv->kv_type == ML_F32 ? 0.0f : PA_UP;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
     const int group = n_heads / kv->n_kv_heads, hd = kv->head_dim;

@@ -1,10 +1,10 @@
 // Rules on a batch of logit rows before the draw: penalties for the ids a
 // sequence has seen, per-id biases and token masks, in one pass.
 //
-// A workgroup takes RL_N ids of one row: it counts the row's seen ids that
-// fall among them in LDS (integer atomics: the order does not matter) and
-// finds the last bias pair of each (a maximum of pair numbers), then passes
-// over the logits once. Bound by HBM: 8 bytes a logit, when the seen ids are few.
+// A workgroup takes RL_N ids of one row: their logits are under way while it
+// counts the row's seen ids that fall among them in LDS (integer atomics: the order
+// does not matter) and finds the last bias pair of each (a maximum of pair
+// numbers). Bound by HBM, 8 bytes a logit, when the seen ids are few.
 #include "kr_internal.h"
 #include "kr_numerics.h"
 #include "kr_paged.h"
@@ -25,50 +25,92 @@ struct RlArgs {
     int n, n_masks;
 };
 
-__global__ void __launch_bounds__(RL_T) k_logit_rules(const RlArgs a, int *fault) {
-    __shared__ int cnt[RL_N];
-    __shared__ int last[RL_N];
+struct RlRow {
+    krh_logit_rule p;
+    const float *bias;
+};
+
+// one logit after its penalties, bias and mask bit
+__device__ __forceinline__ float rl_apply(const RlRow &r, float x, int c, int b, bool allowed) {
+    if (c > 0) {
+        x = x > 0.0f ? kr_fdiv(x, r.p.repeat) : kr_fmul(x, r.p.repeat);
+        x = kr_fsub(kr_fsub(x, kr_fmul(r.p.frequency, (float)c)), r.p.presence);
+    }
+    if (b >= 0) x = kr_fadd(x, r.bias[b]);
+    return allowed ? x : -INFINITY;
+}
+
+// VEC: rows of the logits and the output 16-byte aligned, four ids a lane and step
+template <bool VEC> __global__ void __launch_bounds__(RL_T) k_logit_rules(const RlArgs a, int *fault) {
+    constexpr int V = VEC ? 4 : 1, STEPS = RL_N / (RL_T * V);
+    __shared__ __align__(16) int cnt[RL_N];
+    __shared__ __align__(16) int last[RL_N];
     const int tid = threadIdx.x, i0 = blockIdx.x * RL_N, n = min(RL_N, a.n - i0);
     const size_t r = blockIdx.y;
-    const krh_logit_rule p = a.rule[r];
+    const float *in = a.logits + r * a.ld + i0;
+    float *out = a.out + r * a.ldo + i0;
+    float x[STEPS][V];
+#pragma unroll
+    for (int k = 0; k < STEPS; k++) {
+        const int i = (k * RL_T + tid) * V;
+        if constexpr (VEC) {
+            if (i + 4 <= n) {
+                const float4 t = *(const float4 *)(in + i);
+                x[k][0] = t.x, x[k][1] = t.y, x[k][2] = t.z, x[k][3] = t.w;
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; c++) x[k][c] = i + c < n ? in[i + c] : 0.0f;
+            }
+        } else {
+            x[k][0] = i < n ? in[i] : 0.0f;
+        }
+    }
+    const RlRow row = { a.rule[r], a.bias + r * a.bias_ld };
     int bad = 0;
-    for (int i = tid; i < n; i += RL_T) {
-        cnt[i] = 0;
-        last[i] = -1;
-    }
-    __syncthreads();
-    if (a.seen) {
-        const int m = kr_page_len(a.n_seen[r], (int)a.seen_ld, bad);
-        for (int j = tid; j < m; j += RL_T) {
-            const int t = a.seen[r * a.seen_ld + j] - i0;
-            if (t >= 0 && t < n) atomicAdd(&cnt[t], 1);
-        }
-    }
-    if (a.bias_id) {
-        const int m = kr_page_len(a.n_bias[r], (int)a.bias_ld, bad);
-        for (int j = tid; j < m; j += RL_T) {
-            const int t = a.bias_id[r * a.bias_ld + j] - i0;
-            if (t >= 0 && t < n) atomicMax(&last[t], j);
-        }
-    }
-    int mask = p.mask;
+    const int ns = a.seen ? kr_page_len(a.n_seen[r], (int)a.seen_ld, bad) : 0;
+    const int nb = a.bias_id ? kr_page_len(a.n_bias[r], (int)a.bias_ld, bad) : 0;
+    int mask = row.p.mask;
     if (mask < -1 || mask >= a.n_masks) {
         bad |= KR_BAD_LEN;
         mask = -1;
     }
     if (tid == 0) kr_report(fault, bad);
-    __syncthreads();
-    const unsigned *bits = mask >= 0 ? a.masks + (size_t)mask * (((size_t)a.n + 31) / 32) : nullptr;
-    for (int i = tid; i < n; i += RL_T) {
-        float x = a.logits[r * a.ld + i0 + i];
-        const int c = cnt[i], b = last[i];
-        if (c > 0) {
-            x = x > 0.0f ? kr_fdiv(x, p.repeat) : kr_fmul(x, p.repeat);
-            x = kr_fsub(kr_fsub(x, kr_fmul(p.frequency, (float)c)), p.presence);
+    if (ns > 0 || nb > 0) {
+        for (int i = tid; i < RL_N / 4; i += RL_T) {
+            if (ns > 0) ((int4 *)cnt)[i] = make_int4(0, 0, 0, 0);
+            if (nb > 0) ((int4 *)last)[i] = make_int4(-1, -1, -1, -1);
         }
-        if (b >= 0) x = kr_fadd(x, a.bias[r * a.bias_ld + b]);
-        if (bits && !(bits[(i0 + i) >> 5] >> ((i0 + i) & 31) & 1)) x = -INFINITY;
-        a.out[r * a.ldo + i0 + i] = x;
+        __syncthreads();
+        const int *seen = a.seen + r * a.seen_ld, *ids = a.bias_id + r * a.bias_ld;
+#pragma unroll 4
+        for (int j = tid; j < ns; j += RL_T) {
+            const int t = seen[j] - i0;
+            if (t >= 0 && t < n) atomicAdd(&cnt[t], 1);
+        }
+        for (int j = tid; j < nb; j += RL_T) {
+            const int t = ids[j] - i0;
+            if (t >= 0 && t < n) atomicMax(&last[t], j);
+        }
+        __syncthreads();
+    }
+    const unsigned *bits = a.masks + (mask >= 0 ? (size_t)mask * (((size_t)a.n + 31) / 32) : 0);
+#pragma unroll
+    for (int k = 0; k < STEPS; k++) {
+        const int i = (k * RL_T + tid) * V;
+        if (i >= n) break;
+        const unsigned word = mask >= 0 ? bits[(i0 + i) >> 5] >> ((i0 + i) & 31) : ~0u;
+#pragma unroll
+        for (int c = 0; c < V; c++)
+            x[k][c] = rl_apply(row, x[k][c], ns > 0 ? cnt[i + c] : 0, nb > 0 ? last[i + c] : -1, word >> c & 1);
+        if constexpr (VEC) {
+            if (i + 4 <= n) {
+                *(float4 *)(out + i) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
+                continue;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < V; c++)
+            if (i + c < n) out[i + c] = x[k][c];
     }
 }
 
@@ -90,6 +132,7 @@ extern "C" void krh_logit_rules(float *out, size_t ldo, const float *logits, siz
         return;
     }
     const RlArgs a = { out, logits, ldo, ld, rule, seen, n_seen, bias_id, n_bias, bias, seen_ld, bias_ld, masks, n, n_masks };
-    hipLaunchKernelGGL(k_logit_rules, dim3((n + RL_N - 1) / RL_N, rows), dim3(RL_T), 0, kr_stream(), a, kr_fault_word());
+    const bool vec = !(((uintptr_t)out | (uintptr_t)logits) & 15) && ldo % 4 == 0 && ld % 4 == 0;
+    hipLaunchKernelGGL(vec ? k_logit_rules<true> : k_logit_rules<false>, dim3((n + RL_N - 1) / RL_N, rows), dim3(RL_T), 0, kr_stream(), a, kr_fault_word());
     kr_check_launch("logit_rules");
 }
