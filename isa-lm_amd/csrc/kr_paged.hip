@@ -11,19 +11,53 @@ namespace {
 constexpr int PG_T = 256;
 
 // ---- rows into and out of pages ----
-// An item is one head's vector of one token; 2^LPS >= hd / 4 lanes share it,
-// four values each (whole 16-byte accesses), so a wave holds one to eight
-// items and its loads are contiguous. Bound by HBM: 8 bytes a query value, 4 +
-// the cache's width a key or value.
+// An item is one head's vector of one token; 2^lps >= hd / 8 lanes share it,
+// eight values each, so a wave holds two to eight items of the usual heads and
+// its accesses are contiguous. Bound by HBM (8 bytes a query value, 4 + the cache's
+// width a key or value) without a norm, 8-bit rows and norms by the instructions
+// an item takes: with four values a lane 2047 tokens of the 1B shape took 14.7 us
+// normalized into 8 bits, 11 into halves as they are.
 
-// over the 2^lps lanes of an item
-__device__ __forceinline__ double pg_sum(double v, int n) {
-    for (int o = n >> 1; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+// Sums and maxima over the n lanes of an item (n a power of two), in registers:
+// pairs, fours, then the mirrors of 8 and 16 lanes, whose parts agree by then,
+// and the rows and halves swapped.
+template <int CTRL> __device__ __forceinline__ unsigned pg_dpp(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <class T, class F> __device__ __forceinline__ T pg_reduce(T v, int n, F f) {
+    constexpr int W = sizeof(T) / 4;
+    struct Words { unsigned w[W]; };
+    auto other = [&](auto move) {
+        Words x = __builtin_bit_cast(Words, v);
+#pragma unroll
+        for (int i = 0; i < W; i++) x.w[i] = move(x.w[i]);
+        return __builtin_bit_cast(T, x);
+    };
+    if (n > 1) v = f(v, other([](unsigned x) { return pg_dpp<0xb1>(x); }));
+    if (n > 2) v = f(v, other([](unsigned x) { return pg_dpp<0x4e>(x); }));
+    if (n > 4) v = f(v, other([](unsigned x) { return pg_dpp<0x141>(x); }));
+    if (n > 8) v = f(v, other([](unsigned x) { return pg_dpp<0x140>(x); }));
+    const bool row = threadIdx.x & 16, half = threadIdx.x & 32;
+    if (n > 16) v = f(v, other([&](unsigned x) { const auto s = __builtin_amdgcn_permlane16_swap(x, x, false, false); return row ? s[0] : s[1]; }));
+    if (n > 32) v = f(v, other([&](unsigned x) { const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false); return half ? s[0] : s[1]; }));
     return v;
 }
+__device__ __forceinline__ double pg_sum(double v, int n) {
+    return pg_reduce(v, n, [](double a, double b) { return a + b; });
+}
 __device__ __forceinline__ float pg_max(float v, int n) {
-    for (int o = n >> 1; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    return pg_reduce(v, n, [](float a, float b) { return fmaxf(a, b); });
+}
+
+// 1 / sqrt(x) to a last bit or two of 64 by two steps from the instruction's
+// estimate (the library's quotient and root took more of the kernel's time than
+// its memory)
+__device__ __forceinline__ double pg_rsqrt(double x) {
+    if (!(x > 0.0 && x < (double)INFINITY)) return 1.0 / sqrt(x);
+    double r = __builtin_amdgcn_rsq(x);
+#pragma unroll
+    for (int i = 0; i < 2; i++) r = __builtin_fma(r * 0.5, __builtin_fma(-x * r, r, 1.0), r);
+    return r;
 }
 
 struct QkvArgs {
@@ -32,30 +66,47 @@ struct QkvArgs {
     const int *seq, *row, *pos;
     size_t ldqo, ldq, ldk, ldv;
     float eps;
+    double inv_hd;
     int ntok, nh, n_pos;
 };
 
-// row `at` (in rows of the pool) of K or V from four values a lane, l < hd / 4;
+struct Pg8 {
+    float v[8];
+};
+__device__ __forceinline__ Pg8 pg_get(const float *p) {
+    const float4 x = *(const float4 *)p, y = *(const float4 *)(p + 4);
+    return { { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w } };
+}
+__device__ __forceinline__ void pg_put(float *p, const Pg8 &x) {
+    *(float4 *)p = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
+    *(float4 *)(p + 4) = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
+}
+
+// row `at` (in rows of the pool) of K or V from eight values a lane, l < hd / 8;
 // the conversions of krh_store_kv, but that an 8-bit row's factor is 127 times
 // the rounded reciprocal of its maximum, as tensor libraries form 127 / max (a
 // step of the factor at most: an element next to a border may fall on its other side)
-template <int KT> __device__ __forceinline__ void pg_store(void *dst, float *d, size_t at, int hd, float4 x, int l, bool live, int n) {
-    const size_t e = at * hd + 4 * l;
-    if (KT == PG_F32) {
-        if (live) *(float4 *)((float *)dst + e) = x;
-    } else if (KT == PG_F16) {
-        const ushort4 h = make_ushort4(kr_f2h(x.x), kr_f2h(x.y), kr_f2h(x.z), kr_f2h(x.w));
-        if (live) *(ushort4 *)((uint16_t *)dst + e) = h;
+template <int KT> __device__ __forceinline__ void pg_store(void *dst, float *d, size_t at, int hd, const Pg8 &x, int l, bool live, int n) {
+    const size_t e = at * hd + 8 * l;
+    if constexpr (KT == PG_F32) {
+        if (live) pg_put((float *)dst + e, x);
+    } else if constexpr (KT == PG_F16) {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = (unsigned)kr_f2h(x.v[2 * i]) | (unsigned)kr_f2h(x.v[2 * i + 1]) << 16;
+        if (live) *(uint4 *)((uint16_t *)dst + e) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-        float m = live ? fmaxf(fmaxf(fmaxf(fmaxf(0.0f, fabsf(x.x)), fabsf(x.y)), fabsf(x.z)), fabsf(x.w)) : 0.0f;
-        m = pg_max(m, n);
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x.v[i]));
+        m = pg_max(live ? m : 0.0f, n);
         const bool zero = m < KR_QUANT_TINY;
         const float id = zero ? 0.0f : kr_fmul(127.0f, kr_fdiv(1.0f, m));
-        char4 c = make_char4(0, 0, 0, 0);
-        if (!zero)
-            c = make_char4((signed char)kr_q8_elem(x.x, id), (signed char)kr_q8_elem(x.y, id),
-                           (signed char)kr_q8_elem(x.z, id), (signed char)kr_q8_elem(x.w, id));
-        if (live) *(char4 *)((int8_t *)dst + e) = c;
+        unsigned w[2] = { 0, 0 };
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (!zero) w[i / 4] |= ((unsigned)kr_q8_elem(x.v[i], id) & 255u) << (8 * (i % 4));
+        if (live) *(uint2 *)((int8_t *)dst + e) = make_uint2(w[0], w[1]);
         if (l == 0) d[at] = zero ? 0.0f : kr_fdiv(m, 127.0f);
     }
 }
@@ -64,14 +115,14 @@ template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_qkv(const PgVi
     const unsigned n = 1u << lps, per = a.nh + 2 * p.n_kv, item = (blockIdx.x * PG_T + threadIdx.x) >> lps;
     if (item >= a.ntok * per) return;   // whole items: the lanes that shuffle leave together
     const int l = (int)(threadIdx.x & (n - 1)), t = (int)(item / per), h = (int)(item % per), hd = p.hd;
-    const bool live = 4 * l < hd, isq = h < a.nh, isk = !isq && h < a.nh + p.n_kv;
-    const int kvh = h - a.nh - (isk || isq ? 0 : p.n_kv);
+    const bool live = 8 * l < hd, isq = h < a.nh, isk = !isq && h < a.nh + p.n_kv;
+    const int kvh = h - a.nh - (isk || isq ? 0 : p.n_kv), d = live ? 8 * l : 0;
     const float *src = isq ? a.q + (size_t)t * a.ldq + (size_t)h * hd
                            : (isk ? a.k + (size_t)t * a.ldk : a.v + (size_t)t * a.ldv) + (size_t)kvh * hd;
-    float4 x = live ? *(const float4 *)(src + 4 * l) : make_float4(0, 0, 0, 0);
-    int bad = 0, seq = 0, row = 0, page = 0;
+    Pg8 x = pg_get(src + d);
+    int bad = 0, row = 0, page = 0;
     if (!isq) {
-        seq = kr_page_in(a.seq[t], p.n_seq, KR_BAD_SEQ, bad);
+        const int seq = kr_page_in(a.seq[t], p.n_seq, KR_BAD_SEQ, bad);
         row = kr_page_in(a.row[t], INT_MAX, KR_BAD_PAGE, bad);
         page = pg_page(p, seq, row, bad);
     }
@@ -79,59 +130,72 @@ template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_qkv(const PgVi
     if (isq || isk) {
         const float *w = isq ? a.qw : a.kw;
         if (w) {
-            const double s = pg_sum((double)x.x * x.x + (double)x.y * x.y + ((double)x.z * x.z + (double)x.w * x.w), n);
-            const float inv = (float)(1.0 / sqrt(s / hd + (double)a.eps));
-            if (live) {
-                const float4 g = *(const float4 *)(w + 4 * l);
-                x = make_float4(kr_fmul(kr_fmul(x.x, inv), g.x), kr_fmul(kr_fmul(x.y, inv), g.y),
-                                kr_fmul(kr_fmul(x.z, inv), g.z), kr_fmul(kr_fmul(x.w, inv), g.w));
-            }
+            double s = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) s = __builtin_fma((double)x.v[i], (double)x.v[i], s);
+            s = pg_sum(live ? s : 0.0, n);
+            const float inv = (float)pg_rsqrt(__builtin_fma(s, a.inv_hd, (double)a.eps));
+            const Pg8 g = pg_get(w + d);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x.v[i] = kr_fmul(kr_fmul(x.v[i], inv), g.v[i]);
         }
         if (a.cs) {
-            const int pos = kr_page_in(a.pos[t], a.n_pos, KR_BAD_POS, bad);
-            if (live) {
-                const float2 c = *(const float2 *)(a.cs + (size_t)pos * (hd >> 1) + 2 * l);
-                const float2 s = *(const float2 *)(a.sn + (size_t)pos * (hd >> 1) + 2 * l);
-                x = make_float4(kr_fsub(kr_fmul(x.x, c.x), kr_fmul(x.y, s.x)), kr_fadd(kr_fmul(x.x, s.x), kr_fmul(x.y, c.x)),
-                                kr_fsub(kr_fmul(x.z, c.y), kr_fmul(x.w, s.y)), kr_fadd(kr_fmul(x.z, s.y), kr_fmul(x.w, c.y)));
+            const size_t at = (size_t)kr_page_in(a.pos[t], a.n_pos, KR_BAD_POS, bad) * (hd >> 1) + d / 2;
+            const float4 c4 = *(const float4 *)(a.cs + at), s4 = *(const float4 *)(a.sn + at);
+            const float c[4] = { c4.x, c4.y, c4.z, c4.w }, s[4] = { s4.x, s4.y, s4.z, s4.w };
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float u = x.v[2 * i], v = x.v[2 * i + 1];
+                x.v[2 * i] = kr_fsub(kr_fmul(u, c[i]), kr_fmul(v, s[i]));
+                x.v[2 * i + 1] = kr_fadd(kr_fmul(u, s[i]), kr_fmul(v, c[i]));
             }
         }
     }
     if (l == 0) kr_report(fault, bad);
     if (isq) {
-        if (live) *(float4 *)(a.qo + (size_t)t * a.ldqo + (size_t)h * hd + 4 * l) = x;
+        if (live) pg_put(a.qo + (size_t)t * a.ldqo + (size_t)h * hd + d, x);
         return;
     }
     if (!keep) return;
     pg_store<KT>(isk ? p.k : p.v, isk ? p.kd : p.vd, kr_page_row(page, p.n_kv, kvh, p.shift, row), hd, x, l, live, n);
 }
 
-template <int KT> __device__ __forceinline__ float4 pg_load4(const void *src, const float *d, size_t at, int hd, int l) {
-    const size_t e = at * hd + 4 * l;
-    if (KT == PG_F32) return *(const float4 *)((const float *)src + e);
-    if (KT == PG_F16) {
-        const ushort4 h = *(const ushort4 *)((const uint16_t *)src + e);
-        return make_float4(kr_h2f(h.x), kr_h2f(h.y), kr_h2f(h.z), kr_h2f(h.w));
+template <int KT> __device__ __forceinline__ Pg8 pg_load8(const void *src, const float *d, size_t at, int hd, int l) {
+    const size_t e = at * hd + 8 * l;
+    if constexpr (KT == PG_F32) {
+        return pg_get((const float *)src + e);
+    } else if constexpr (KT == PG_F16) {
+        const uint4 h = *(const uint4 *)((const uint16_t *)src + e);
+        const unsigned w[4] = { h.x, h.y, h.z, h.w };
+        Pg8 x;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x.v[i] = kr_h2f((uint16_t)(w[i / 2] >> (16 * (i % 2))));
+        return x;
+    } else {
+        const uint2 c = *(const uint2 *)((const int8_t *)src + e);
+        const unsigned w[2] = { c.x, c.y };
+        const float s = d[at];
+        Pg8 x;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x.v[i] = kr_fmul((float)(int8_t)(w[i / 4] >> (8 * (i % 4))), s);
+        return x;
     }
-    const char4 c = *(const char4 *)((const int8_t *)src + e);
-    const float s = d[at];
-    return make_float4(kr_fmul((float)c.x, s), kr_fmul((float)c.y, s), kr_fmul((float)c.z, s), kr_fmul((float)c.w, s));
 }
 
 template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_load(const PgView p, float *k, size_t ldk, float *v, size_t ldv,
                                                                        int n_rows, const int *seqs, const int *rows, int lps, int *fault) {
     const unsigned n = 1u << lps, per = 2 * p.n_kv, item = (blockIdx.x * PG_T + threadIdx.x) >> lps;
     const int l = (int)(threadIdx.x & (n - 1));
-    if (item >= n_rows * per || 4 * l >= p.hd) return;
+    if (item >= n_rows * per || 8 * l >= p.hd) return;
     const int i = (int)(item / per), h = (int)(item % per), kvh = h < p.n_kv ? h : h - p.n_kv;
     int bad = 0;
     const int seq = kr_page_in(seqs[i], p.n_seq, KR_BAD_SEQ, bad), row = kr_page_in(rows[i], INT_MAX, KR_BAD_PAGE, bad);
     const size_t at = kr_page_row(pg_page(p, seq, row, bad), p.n_kv, kvh, p.shift, row);
     const bool isk = h < p.n_kv;
-    float4 x = make_float4(0, 0, 0, 0);
-    if (!bad) x = pg_load4<KT>(isk ? p.k : p.v, isk ? p.kd : p.vd, at, p.hd, l);
+    Pg8 x = {};
+    if (!bad) x = pg_load8<KT>(isk ? p.k : p.v, isk ? p.kd : p.vd, at, p.hd, l);
     if (l == 0) kr_report(fault, bad);
-    *(float4 *)((isk ? k + (size_t)i * ldk : v + (size_t)i * ldv) + (size_t)kvh * p.hd + 4 * l) = x;
+    pg_put((isk ? k + (size_t)i * ldk : v + (size_t)i * ldv) + (size_t)kvh * p.hd + 8 * l, x);
 }
 
 // ---- eviction ----
@@ -139,9 +203,8 @@ template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_load(const PgV
 // Weights in an order of unsigned integers: larger is heavier, NaN the
 // heaviest, -0 as +0
 __device__ __forceinline__ unsigned ev_key(float w) {
-    const unsigned u = __float_as_uint(w == 0.0f ? 0.0f : w);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
-    return (u >> 31) ? ~u : u | 0x80000000u;
+    const unsigned u = __float_as_uint(w + 0.0f);   // -0 + 0 = +0
+    return w != w ? 0xffffffffu : u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
 
 constexpr int EV_T = 1024, EV_W = EV_T / 64, EV_D = 11, EV_B = 1 << EV_D;   // radix digits of 11, 11 and 10 bits
@@ -162,38 +225,67 @@ struct EvArgs {
     float *w;   // [n_seq][n_kv][keep]: their weights
 };
 
-// Inclusive sums over the wave's lanes
-__device__ __forceinline__ int ev_scan(int v) {
-    for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(v, o);
-        if ((int)(threadIdx.x & 63) >= o) v += t;
-    }
-    return v;
+// Sums of a count over the waves before this one; all of them read at once
+__device__ __forceinline__ int ev_before(const int *s, int wave) {
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < EV_W; i++) sum += i < wave ? s[i] : 0;
+    return sum;
 }
 
-// EV_U rows of 64 from r0 on for each lane, none past r1
+// Rows r0 .. r1 - 1, EV_U x 64 at a time, a lane's reads side by side
 template <class F> __device__ __forceinline__ void ev_rows(const float *mass, int r0, int r1, F f) {
     const int lane = threadIdx.x & 63;
-    for (int r = r0 + lane; r - lane < r1; r += 64 * EV_U) {
+    int r = r0;
+    for (; r + 64 * EV_U <= r1; r += 64 * EV_U) {
         float w[EV_U];
+        const float *at = mass + r + lane;
 #pragma unroll
-        for (int k = 0; k < EV_U; k++) w[k] = mass[min(r + 64 * k, r1 - 1)];
+        for (int k = 0; k < EV_U; k++) w[k] = at[64 * k];
 #pragma unroll
-        for (int k = 0; k < EV_U; k++)
-            if (r - lane + 64 * k < r1) f(r + 64 * k, r + 64 * k < r1, w[k]);
+        for (int k = 0; k < EV_U; k++) f(r + lane + 64 * k, true, w[k]);
     }
+    if (r >= r1) return;
+    float w[EV_U];
+#pragma unroll
+    for (int k = 0; k < EV_U; k++) w[k] = mass[min(r + lane + 64 * k, r1 - 1)];
+#pragma unroll
+    for (int k = 0; k < EV_U; k++)
+        if (r + 64 * k < r1) f(r + lane + 64 * k, r + lane + 64 * k < r1, w[k]);
+}
+
+// From the heaviest digit down: the one where the counts' sum reaches `need`,
+// and how many of it are wanted. The whole workgroup; leaves the counts at zero.
+__device__ __forceinline__ void ev_digit(int *hist, int *s_sum, int *s_res, int &digit, int &need) {
+    const int tid = threadIdx.x, wave = tid >> 6;
+    __syncthreads();
+    const int hi = EV_B - 1 - 2 * tid, c0 = hist[hi], c1 = hist[hi - 1], sum = pg_scan(c0 + c1);
+    if ((tid & 63) == 63) s_sum[wave] = sum;
+    __syncthreads();
+    const int before = sum - c0 - c1 + ev_before(s_sum, wave);
+    if (before < need && before + c0 + c1 >= need) {
+        const bool second = before + c0 < need;
+        s_res[0] = second ? hi - 1 : hi;
+        s_res[1] = need - before - (second ? c0 : 0);
+    }
+    hist[hi] = hist[hi - 1] = 0;
+    __syncthreads();
+    digit = s_res[0];
+    need = s_res[1];
 }
 
 // One workgroup a (sequence, KV head): the weight of the last row kept by a
 // radix select, then the kept rows' numbers in order, equal weights from the
-// lowest row on. Each wave has an even part of the rows. Bound by the passes'
-// latencies: the rows come from L2 after the first (32,001 rows, 8 workgroups:
-// 102 us with one lane looking through the digits' counts and barriers every 1024 rows).
+// lowest row on. Each wave has an even part of the rows. The rows with the
+// first digit's bits go to LDS, where they are few (each wave up to EV_C), and the
+// other digits look at those. Bound by the one CU's instructions, three passes over
+// the rows: 32,001 rows, 8 workgroups, 102 us with one lane looking through the
+// counts and barriers every 1024 rows; 45 with five passes over all rows.
+constexpr int EV_C = 512;
 __global__ void __launch_bounds__(EV_T) k_evict_select(const EvArgs a, int *fault) {
     __shared__ int hist[EV_B];
-    __shared__ int s_sum[EV_W], s_tie[EV_W], s_take[EV_W];
-    __shared__ unsigned s_prefix;
-    __shared__ int s_need;
+    __shared__ unsigned s_key[EV_W][EV_C];
+    __shared__ int s_sum[EV_W], s_res[2], s_above[EV_W], s_cand[EV_W], s_take[EV_W], s_tie[EV_W];
     const int kvh = blockIdx.x, s = blockIdx.y, n_kv = gridDim.x, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int bad = 0;
@@ -213,81 +305,95 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(const EvArgs a, int *faul
         return;
     }
     const int old = len - a.recent, want = a.keep - a.recent;   // 0 <= want < old
-    const int part = (old + EV_W - 1) / EV_W, r0 = min(old, wave * part), r1 = min(old, r0 + part);
-    unsigned prefix = 0;
-    int need = want;
-    if (want > 0)
-        for (int b = 32 - EV_D; ; b = max(0, b - EV_D)) {
-            const int top = b == 32 - EV_D ? 32 : b ? 32 - EV_D : 32 - 2 * EV_D;   // bits from here up are known
-            for (int i = tid; i < EV_B; i += EV_T) hist[i] = 0;
-            __syncthreads();
-            ev_rows(mass, r0, r1, [&](int, bool in, float w) {
-                const unsigned u = ev_key(w), d = (u >> b) & ((1u << (top - b)) - 1);
-                in = in && (top == 32 || (u >> top) == (prefix >> top));
-                // the digit of the first lane, often that of many (zeros), counts once
-                const unsigned long long any = __ballot(in);
-                if (!any) return;
-                const unsigned d0 = (unsigned)__builtin_amdgcn_readlane((int)d, __builtin_ctzll(any));
-                const unsigned long long same = __ballot(in && d == d0);
-                if (lane == __builtin_ctzll(any)) atomicAdd(&hist[d0], (int)__popcll(same));
-                else if (in && d != d0) atomicAdd(&hist[d], 1);
-            });
-            __syncthreads();
-            // from the heaviest digit down: where the counts' sum reaches `need`
-            const int hi = EV_B - 1 - 2 * tid, c0 = hist[hi], c1 = hist[hi - 1], sum = ev_scan(c0 + c1);
-            if (lane == 63) s_sum[wave] = sum;
-            __syncthreads();
-            int before = sum - c0 - c1;
-            for (int i = 0; i < wave; i++) before += s_sum[i];
-            if (before < need && before + c0 + c1 >= need) {
-                const bool second = before + c0 < need;
-                s_prefix = prefix | (unsigned)(second ? hi - 1 : hi) << b;
-                s_need = need - before - (second ? c0 : 0);
-            }
-            __syncthreads();
-            prefix = s_prefix;
-            need = s_need;
-            __syncthreads();
-            if (b == 0) break;
-        }
-    // rows above `prefix`, and the first `need` of those at it
-    int ties = 0, take = 0;
-    if (want > 0)
-        ev_rows(mass, r0, r1, [&](int, bool in, float w) {
-            const unsigned u = ev_key(w);
-            ties += __popcll(__ballot(in && u == prefix));
-            take += __popcll(__ballot(in && u > prefix));
-        });
-    if (lane == 0) {
-        s_tie[wave] = ties;
-        s_take[wave] = take;
-    }
-    __syncthreads();
-    int at = 0;
-    ties = 0;
-    for (int i = 0; i < wave; i++) {
-        ties += s_tie[i];
-        at += s_take[i];
-    }
-    at += min(ties, need);
-    if (want > 0)
-        ev_rows(mass, r0, r1, [&](int r, bool in, float w) {
-            const unsigned u = ev_key(w);
-            const unsigned long long bt = __ballot(in && u == prefix), below = ((unsigned long long)1 << lane) - 1;
-            const bool take = in && (u > prefix || (u == prefix && ties + __popcll(bt & below) < need));
-            const unsigned long long bk = __ballot(take);
-            if (take) {
-                const int j = at + __popcll(bk & below);
-                idx[j] = r;
-                ow[j] = w;
-            }
-            ties += __popcll(bt);
-            at += __popcll(bk);
-        });
     for (int r = tid; r < a.recent; r += EV_T) {
         idx[want + r] = old + r;
         ow[want + r] = mass[old + r];
     }
+    if (want == 0) return;
+    const int part = (old + EV_W - 1) / EV_W, r0 = min(old, wave * part), r1 = min(old, r0 + part);
+    const unsigned long long below = ((unsigned long long)1 << lane) - 1;
+    int need = want, digit;
+    for (int i = tid; i < EV_B; i += EV_T) hist[i] = 0;
+    __syncthreads();
+    // zeros, which rows that no head looks at all have, count together
+    int zeros = 0;
+    ev_rows(mass, r0, r1, [&](int, bool in, float w) {
+        zeros += __popcll(__ballot(in && w == 0.0f));
+        if (in && w != 0.0f) atomicAdd(&hist[ev_key(w) >> (32 - EV_D)], 1);
+    });
+    if (lane == 0 && zeros) atomicAdd(&hist[0x80000000u >> (32 - EV_D)], zeros);
+    ev_digit(hist, s_sum, s_res, digit, need);
+    // each wave's rows above that digit, and the keys of those at it
+    const unsigned d1 = digit;
+    int above = 0, cand = 0;
+    ev_rows(mass, r0, r1, [&](int, bool in, float w) {
+        const unsigned u = ev_key(w), d = u >> (32 - EV_D);
+        above += __popcll(__ballot(in && d > d1));
+        const unsigned long long b = __ballot(in && d == d1);
+        const int j = cand + __popcll(b & below);
+        if (in && d == d1 && j < EV_C) s_key[wave][j] = u;
+        cand += __popcll(b);
+    });
+    if (lane == 0) {
+        s_above[wave] = above;
+        s_cand[wave] = cand;
+    }
+    __syncthreads();
+    int most = 0;
+#pragma unroll
+    for (int i = 0; i < EV_W; i++) most = max(most, s_cand[i]);
+    const bool few = most <= EV_C;
+    // the keys at the first digit, from LDS or from the rows again
+    auto keys = [&](auto f) {
+        if (few) {
+            for (int j = lane; j < cand; j += 64) f(s_key[wave][j]);
+        } else {
+            ev_rows(mass, r0, r1, [&](int, bool in, float w) {
+                const unsigned u = ev_key(w);
+                if (in && u >> (32 - EV_D) == d1) f(u);
+            });
+        }
+    };
+    unsigned prefix = d1 << (32 - EV_D);
+    for (int b = 32 - 2 * EV_D;; b = 0) {   // bits 10 to 20, then 0 to 9
+        const int top = b ? 32 - EV_D : 32 - 2 * EV_D;
+        keys([&](unsigned u) {
+            if (u >> top == prefix >> top) atomicAdd(&hist[u >> b & ((1u << (top - b)) - 1)], 1);
+        });
+        ev_digit(hist, s_sum, s_res, digit, need);
+        prefix |= (unsigned)digit << b;
+        if (b == 0) break;
+    }
+    // rows above `prefix`, and the first `need` of those at it
+    int take = 0, ties = 0;
+    keys([&](unsigned u) {
+        take += u > prefix;
+        ties += u == prefix;
+    });
+    for (int o = 32; o >= 1; o >>= 1) {
+        take += __shfl_xor(take, o);
+        ties += __shfl_xor(ties, o);
+    }
+    if (lane == 0) {
+        s_take[wave] = above + take;
+        s_tie[wave] = ties;
+    }
+    __syncthreads();
+    ties = ev_before(s_tie, wave);
+    int at = ev_before(s_take, wave) + min(ties, need);
+    ev_rows(mass, r0, r1, [&](int r, bool in, float w) {
+        const unsigned u = ev_key(w);
+        const unsigned long long bt = __ballot(in && u == prefix);
+        const bool got = in && (u > prefix || (u == prefix && ties + __popcll(bt & below) < need));
+        const unsigned long long bk = __ballot(got);
+        if (got) {
+            const int j = at + __popcll(bk & below);
+            idx[j] = r;
+            ow[j] = w;
+        }
+        ties += __popcll(bt);
+        at += __popcll(bk);
+    });
 }
 
 // Rows into the new pages, in units of U bytes, EM_ROWS a workgroup and KV
@@ -347,11 +453,12 @@ extern "C" void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const
                    (n_heads == 0 || (ldq >= qd && ldqo >= qd && ldq % 4 == 0 && ldqo % 4 == 0 && pg_aligned(q) &&
                                      pg_aligned(qo) && pg_aligned(q_norm))), "paged_qkv: row strides or alignment"))
         return;
-    const int lps = pg_log2(kv->head_dim / 4);
+    const int lps = pg_log2(kv->head_dim / 8);
     const unsigned grid = item_blocks((size_t)ntok * (n_heads + 2 * (size_t)kv->n_kv_heads), lps);
     if (pg_refuse(grid > 0, "paged_qkv: too many tokens")) return;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
-    const QkvArgs a = { qo, q, k, v, q_norm, k_norm, cos_t, sin_t, seq, row, pos, ldqo, ldq, ldk, ldv, eps, ntok, n_heads, n_pos };
+    const QkvArgs a = { qo, q, k, v, q_norm, k_norm, cos_t, sin_t, seq, row, pos, ldqo, ldq, ldk, ldv, eps, 1.0 / kv->head_dim,
+                        ntok, n_heads, n_pos };
     const auto f = kv->kv_type == ML_F32 ? k_paged_qkv<PG_F32> : kv->kv_type == ML_F16 ? k_paged_qkv<PG_F16> : k_paged_qkv<PG_Q8>;
     hipLaunchKernelGGL(f, dim3(grid), dim3(PG_T), 0, kr_stream(), p, a, lps, kr_fault_word());
     kr_check_launch("paged_qkv");
@@ -366,7 +473,7 @@ extern "C" void krh_paged_load(float *k, size_t ldk, float *v, size_t ldv, const
         pg_refuse(ldk >= kvd && ldv >= kvd && ldk % 4 == 0 && ldv % 4 == 0 && pg_aligned(k) && pg_aligned(v),
                "paged_load: row strides or alignment"))
         return;
-    const int lps = pg_log2(kv->head_dim / 4);
+    const int lps = pg_log2(kv->head_dim / 8);
     const unsigned grid = item_blocks((size_t)n * 2 * kv->n_kv_heads, lps);
     if (pg_refuse(grid > 0, "paged_load: too many rows")) return;
     const auto f = kv->kv_type == ML_F32 ? k_paged_load<PG_F32> : kv->kv_type == ML_F16 ? k_paged_load<PG_F16> : k_paged_load<PG_Q8>;

@@ -67,19 +67,6 @@ __device__ __forceinline__ PaSpan pa_span(const PaArgs &a, int len) {   // len w
     return r;
 }
 
-// Inclusive sums over the wave's lanes, in registers
-template <int CTRL, int ROWS> __device__ __forceinline__ int pa_add_dpp(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int pa_scan(int v) {
-    v = pa_add_dpp<0x111, 0xf>(v);   // from 1, 2, 4 and 8 lanes below in the row of 16
-    v = pa_add_dpp<0x112, 0xf>(v);
-    v = pa_add_dpp<0x114, 0xf>(v);
-    v = pa_add_dpp<0x118, 0xf>(v);
-    v = pa_add_dpp<0x142, 0xa>(v);   // the sums of rows 0 and 2 to rows 1 and 3
-    return pa_add_dpp<0x143, 0xc>(v);   // of the lower half to the upper
-}
-
 // All sequences' tiles, and how many shares they make: share u has tiles
 // [u T / n, (u + 1) T / n). With it the spans of 64 sequences, one a lane.
 struct PaAll {
@@ -91,7 +78,7 @@ __device__ __forceinline__ void pa_fetch(const PgView &p, const PaArgs &a, PaAll
     const int i = base + (int)(threadIdx.x & 63);
     r.base = base;
     r.len = i < p.n_seq ? kr_page_len(a.len[i], a.max_len, bad) : 0;
-    r.sum = pa_scan(i < p.n_seq ? pa_span(a, r.len).tiles : 0);
+    r.sum = pg_scan(i < p.n_seq ? pa_span(a, r.len).tiles : 0);
 }
 __device__ __forceinline__ PaAll pa_all(const PgView &p, const PaArgs &a, int &bad) {
     PaAll r;

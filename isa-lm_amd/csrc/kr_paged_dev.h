@@ -19,6 +19,19 @@ __device__ __forceinline__ int pg_page(const PgView &p, int seq, int row, int &b
     return kr_page_of(p.table + (size_t)seq * p.ld, p.ld, row, p.shift, p.n_pages, bad);
 }
 
+// Inclusive sums over the wave's lanes, in registers
+template <int CTRL, int ROWS> __device__ __forceinline__ int pg_add_dpp(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int pg_scan(int v) {
+    v = pg_add_dpp<0x111, 0xf>(v);   // from 1, 2, 4 and 8 lanes below in the row of 16
+    v = pg_add_dpp<0x112, 0xf>(v);
+    v = pg_add_dpp<0x114, 0xf>(v);
+    v = pg_add_dpp<0x118, 0xf>(v);
+    v = pg_add_dpp<0x142, 0xa>(v);   // the sums of rows 0 and 2 to rows 1 and 3
+    return pg_add_dpp<0x143, 0xc>(v);   // of the lower half to the upper
+}
+
 inline int pg_log2(int v) {
     int l = 0;
     while ((1 << l) < v) l++;

@@ -12,6 +12,7 @@
 namespace {
 
 constexpr int RL_T = 256, RL_N = 4096;
+constexpr int RL_SEEN = 8, RL_BIAS = 2;   // ids a thread reads with the logits
 
 struct RlArgs {
     float *out;
@@ -65,6 +66,13 @@ template <bool VEC> __global__ void __launch_bounds__(RL_T) k_logit_rules(const 
             x[k][0] = i < n ? in[i] : 0.0f;
         }
     }
+    // the row's first ids with them, whether they count or not
+    const int *seen = a.seen + r * a.seen_ld, *ids = a.bias_id + r * a.bias_ld;
+    int sj[RL_SEEN], bj[RL_BIAS];
+#pragma unroll
+    for (int k = 0; k < RL_SEEN; k++) sj[k] = a.seen && k * RL_T + tid < (int)a.seen_ld ? seen[k * RL_T + tid] : -1;
+#pragma unroll
+    for (int k = 0; k < RL_BIAS; k++) bj[k] = a.bias_id && k * RL_T + tid < (int)a.bias_ld ? ids[k * RL_T + tid] : -1;
     const RlRow row = { a.rule[r], a.bias + r * a.bias_ld };
     int bad = 0;
     const int ns = a.seen ? kr_page_len(a.n_seen[r], (int)a.seen_ld, bad) : 0;
@@ -81,16 +89,23 @@ template <bool VEC> __global__ void __launch_bounds__(RL_T) k_logit_rules(const 
             if (nb > 0) ((int4 *)last)[i] = make_int4(-1, -1, -1, -1);
         }
         __syncthreads();
-        const int *seen = a.seen + r * a.seen_ld, *ids = a.bias_id + r * a.bias_ld;
-#pragma unroll 4
-        for (int j = tid; j < ns; j += RL_T) {
-            const int t = seen[j] - i0;
+        auto count = [&](int id) {
+            const int t = id - i0;
             if (t >= 0 && t < n) atomicAdd(&cnt[t], 1);
-        }
-        for (int j = tid; j < nb; j += RL_T) {
-            const int t = ids[j] - i0;
+        };
+        auto note = [&](int id, int j) {
+            const int t = id - i0;
             if (t >= 0 && t < n) atomicMax(&last[t], j);
-        }
+        };
+#pragma unroll
+        for (int k = 0; k < RL_SEEN; k++)
+            if (k * RL_T + tid < ns) count(sj[k]);
+#pragma unroll 4
+        for (int j = RL_SEEN * RL_T + tid; j < ns; j += RL_T) count(seen[j]);
+#pragma unroll
+        for (int k = 0; k < RL_BIAS; k++)
+            if (k * RL_T + tid < nb) note(bj[k], k * RL_T + tid);
+        for (int j = RL_BIAS * RL_T + tid; j < nb; j += RL_T) note(ids[j], j);
         __syncthreads();
     }
     const unsigned *bits = a.masks + (mask >= 0 ? (size_t)mask * (((size_t)a.n + 31) / 32) : 0);
