@@ -389,7 +389,7 @@ size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int m
  * krh_attention_kv (and a Q8 cache's queries stay unquantized): results agree
  * to rounding, and are the same from call to call. Values attended that are not finite
  * give results that are not finite, for the heads that they reach.
- * len[s] <= max_len, which sizes the launch. mass (nullable): mass[(s *
+ * len[s] <= max_len <= 2^29, which sizes the launch; o overlaps no input. mass (nullable): mass[(s *
  * n_kv_heads + h) * mass_ld + r] += the sum of row r's weights over the query
  * heads of KV head h. At most 16 query heads a KV head; q, o and ws 16-byte aligned. */
 void krh_paged_attention(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len, int n_seq,

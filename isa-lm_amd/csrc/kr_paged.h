@@ -13,7 +13,7 @@
 #define KR_HD inline
 #endif
 
-enum { KR_PAGE_MIN = 16, KR_PAGE_MAX = 1024, KR_PAGE_HD_MAX = 256, KR_PAGE_GROUP_MAX = 16 };
+enum { KR_PAGE_MIN = 16, KR_PAGE_MAX = 1024, KR_PAGE_HD_MAX = 256, KR_PAGE_GROUP_MAX = 16, KR_PAGE_LEN_MAX = 1 << 29 };
 
 // what a kernel found: bit i goes to fault word i
 enum { KR_BAD_PAGE = 1, KR_BAD_LEN = 2, KR_BAD_SEQ = 4, KR_BAD_POS = 8, KR_FAULT_WORDS = 4 };

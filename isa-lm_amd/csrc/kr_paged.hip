@@ -18,9 +18,9 @@ constexpr int PG_T = 256;
 // an item takes: with four values a lane 2047 tokens of the 1B shape took 14.7 us
 // normalized into 8 bits, 11 into halves as they are.
 
-// Sums and maxima over the n lanes of an item (n a power of two), in registers:
-// pairs, fours, then the mirrors of 8 and 16 lanes, whose parts agree by then,
-// and the rows and halves swapped.
+// Sums and maxima over the n <= 32 lanes of an item (n a power of two), in
+// registers: pairs, fours, then the mirrors of 8 and 16 lanes, whose parts agree
+// by then, and the two rows of 16 swapped.
 template <int CTRL> __device__ __forceinline__ unsigned pg_dpp(unsigned v) {
     return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
 }
@@ -37,9 +37,8 @@ template <class T, class F> __device__ __forceinline__ T pg_reduce(T v, int n, F
     if (n > 2) v = f(v, other([](unsigned x) { return pg_dpp<0x4e>(x); }));
     if (n > 4) v = f(v, other([](unsigned x) { return pg_dpp<0x141>(x); }));
     if (n > 8) v = f(v, other([](unsigned x) { return pg_dpp<0x140>(x); }));
-    const bool row = threadIdx.x & 16, half = threadIdx.x & 32;
+    const bool row = threadIdx.x & 16;
     if (n > 16) v = f(v, other([&](unsigned x) { const auto s = __builtin_amdgcn_permlane16_swap(x, x, false, false); return row ? s[0] : s[1]; }));
-    if (n > 32) v = f(v, other([&](unsigned x) { const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false); return half ? s[0] : s[1]; }));
     return v;
 }
 __device__ __forceinline__ double pg_sum(double v, int n) {
@@ -455,7 +454,7 @@ extern "C" void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const
         return;
     const int lps = pg_log2(kv->head_dim / 8);
     const unsigned grid = item_blocks((size_t)ntok * (n_heads + 2 * (size_t)kv->n_kv_heads), lps);
-    if (pg_refuse(grid > 0, "paged_qkv: too many tokens")) return;
+    if (pg_refuse(grid > 0, "paged_qkv: too many tokens") || pg_not_ready("paged_qkv before krh_init")) return;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
     const QkvArgs a = { qo, q, k, v, q_norm, k_norm, cos_t, sin_t, seq, row, pos, ldqo, ldq, ldk, ldv, eps, 1.0 / kv->head_dim,
                         ntok, n_heads, n_pos };
@@ -475,7 +474,7 @@ extern "C" void krh_paged_load(float *k, size_t ldk, float *v, size_t ldv, const
         return;
     const int lps = pg_log2(kv->head_dim / 8);
     const unsigned grid = item_blocks((size_t)n * 2 * kv->n_kv_heads, lps);
-    if (pg_refuse(grid > 0, "paged_load: too many rows")) return;
+    if (pg_refuse(grid > 0, "paged_load: too many rows") || pg_not_ready("paged_load before krh_init")) return;
     const auto f = kv->kv_type == ML_F32 ? k_paged_load<PG_F32> : kv->kv_type == ML_F16 ? k_paged_load<PG_F16> : k_paged_load<PG_Q8>;
     hipLaunchKernelGGL(f, dim3(grid), dim3(PG_T), 0, kr_stream(), pg_view(kv, table, table_ld, n_seq), k, ldk, v, ldv, n, seq, row,
                        lps, kr_fault_word());
@@ -492,7 +491,7 @@ extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table
                                 int out_table_ld, int *out_len, float *out_mass, size_t out_ld, void *ws) {
     if (n_seq == 0) return;
     if (pg_refuse(pg_pages_ok(kv), "paged_evict: the pages") ||
-        pg_refuse(n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && keep > 0 && recent >= 0 && recent <= keep && table_ld > 0 &&
+        pg_refuse(n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && max_len <= KR_PAGE_LEN_MAX && keep > 0 && recent >= 0 && recent <= keep && table_ld > 0 &&
                    out_table_ld > 0, "paged_evict sizes") ||
         pg_refuse(table && len && mass && out_table && out_len && out_mass && ws && !((uintptr_t)ws & 3) && out_table != table,
                "paged_evict: a missing array, or the pages onto themselves") ||
@@ -500,6 +499,7 @@ extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table
                "paged_evict: mass rows") ||
         pg_refuse((size_t)out_table_ld * kv->page_size >= (size_t)(keep < max_len ? keep : max_len), "paged_evict: out_table's pages"))
         return;
+    if (pg_not_ready("paged_evict before krh_init")) return;
     int *w = (int *)ws;
     const size_t rows = (size_t)n_seq * kv->n_kv_heads * keep;
     const EvArgs a = { len, mass, mass_ld, max_len, keep, recent, out_table, out_table_ld, out_len, out_mass, out_ld,

@@ -122,6 +122,18 @@ __device__ __forceinline__ int pa_share(const PaAll &all, int t) {
 __device__ __forceinline__ float pa_swap8(float x) {   // the lane 8 away in its row of 16
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
 }
+// tanh within 4 half steps of a float: below 0.6 x + x t P(t), t = x^2, P fitted to
+// (tanh(x) / x - 1) / t for the least of the largest t |error|, 0.1 half steps; from
+// there 1 - 2 / (e^2x + 1). (The C library's tanhf, which the token loop's
+// soft-caps call, is three quotients: a float cache's 10,000 rows 168 us.)
+__device__ __forceinline__ float pa_tanh(float x) {
+    const float t = x * x, y = fabsf(x);
+    const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(-0x1.830bfap-8f, t, 0x1.54e018p-6f), t, -0x1.b89edap-5f),
+                                                  t, 0x1.1109dcp-3f), t, -0x1.55553ep-2f);
+    const float e = __builtin_amdgcn_exp2f(y * 2.8853900817779268f);
+    const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+    return y < 0.6f ? __builtin_fmaf(x * t, p, x) : copysignf(far, x);
+}
 // over the 4 lanes of a column: both halves, then both rows of each, swapped in registers
 __device__ __forceinline__ float pa_max_g(float v) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -284,12 +296,9 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             const char *at = (const char *)p.k + (r + 4 * b) * hd * EB;
 #pragma unroll
             for (int j = 0; j < KS; j++) {
+                // past the head's dims the queries are zero: its first dims again
                 const int d = (j * 4 + g) * KD;
-                const bool in = FULL || d < hd;
-                pa_load(raw.k[b][j], at + (in ? d : 0) * EB);
-                if (!FULL)
-#pragma unroll
-                    for (int i = 0; i < Raw::KB; i++) raw.k[b][j][i] = in ? raw.k[b][j][i] : 0u;
+                pa_load(raw.k[b][j], at + (FULL || d < hd ? d : 0) * EB);
             }
         }
     }
@@ -314,15 +323,15 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             if constexpr (FULL) {
                 pa_load(raw.v[i], at + n * W * EB);
             } else {
-                // 4 dims at a time where a lane has them, else 8 (head_dim is a multiple of 8)
+                // 4 dims at a time where a lane has them, else 8 (head_dim is a
+                // multiple of 8); past the head's dims any, of outputs that are not stored
                 constexpr int P = W < 8 ? W : 8, PW = P * EB / 4;
 #pragma unroll
                 for (int d = 0; d < W; d += P) {
-                    const bool in = n * W + d < hd;
                     unsigned x[PW];
-                    pa_load(x, at + (in ? n * W + d : 0) * EB);
+                    pa_load(x, at + (n * W + d < hd ? n * W + d : 0) * EB);
 #pragma unroll
-                    for (int w = 0; w < PW; w++) raw.v[i][d * EB / 4 + w] = in ? x[w] : 0u;
+                    for (int w = 0; w < PW; w++) raw.v[i][d * EB / 4 + w] = x[w];
                 }
             }
         }
@@ -369,8 +378,9 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             sc[i] = x * (KT == PG_Q8 ? cs * raw.kd[i] : cs);
         }
         if (a.cap > 0.0f) {
+            const float inv_cap = 1.0f / a.cap;
 #pragma unroll
-            for (int i = 0; i < R; i++) sc[i] = a.cap * kr_tanhf(sc[i] / a.cap) * 1.4426950408889634f;
+            for (int i = 0; i < R; i++) sc[i] = pa_tanh(sc[i] * inv_cap) * (a.cap * 1.4426950408889634f);
         }
         if (!whole) {
 #pragma unroll
@@ -676,6 +686,20 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
     const PaParts r = pa_parts(p, a, s, kvh, sp);
     const int r0 = sp.first + block * PJ_ROWS;
     if (r0 >= sp.len) return;
+    const float *z = a.z + ((size_t)s * a.nh + kvh * group) * a.z_ld;
+    float *mass = a.mass + ((size_t)s * p.n_kv + kvh) * a.mass_ld;
+    // the first heads' scores are under way while the maxima are found
+    constexpr int K = PJ_ROWS / PJ_T;
+    float sum[K], old[K], zs[PJ_U][K];
+    int at[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        at[k] = min(r0 + k * PJ_T + tid, sp.len - 1);
+        sum[k] = 0.0f;
+        old[k] = mass[at[k]];
+#pragma unroll
+        for (int h = 0; h < PJ_U; h++) zs[h][k] = h < group ? z[h * a.z_ld + at[k]] : 0.0f;
+    }
     for (int h = tid >> 6; h < group; h += PJ_T / 64) {
         float m, inv;
         pa_stats(a.pml + (r.slot * group + h) * 2, group, r.n, m, inv);
@@ -685,25 +709,21 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
         }
     }
     __syncthreads();
-    const float *z = a.z + ((size_t)s * a.nh + kvh * group) * a.z_ld;
-    float *mass = a.mass + ((size_t)s * p.n_kv + kvh) * a.mass_ld;
-    float sum[PJ_ROWS / PJ_T], old[PJ_ROWS / PJ_T];
 #pragma unroll
-    for (int k = 0; k < PJ_ROWS / PJ_T; k++) {
-        sum[k] = 0.0f;
-        old[k] = mass[min(r0 + k * PJ_T + tid, sp.len - 1)];
-    }
-    for (int h = 0; h < group; h++) {
+    for (int h = 0; h < PJ_U; h++)
+        if (h < group) {
+            const float m = s_m[h] - a.z_up, inv = s_i[h];
+#pragma unroll
+            for (int k = 0; k < K; k++) sum[k] += __builtin_amdgcn_exp2f(zs[h][k] - m) * inv;
+        }
+    for (int h = PJ_U; h < group; h++) {
         const float m = s_m[h] - a.z_up, inv = s_i[h];
 #pragma unroll
-        for (int k = 0; k < PJ_ROWS / PJ_T; k++)
-            sum[k] += __builtin_amdgcn_exp2f(z[h * a.z_ld + min(r0 + k * PJ_T + tid, sp.len - 1)] - m) * inv;
+        for (int k = 0; k < K; k++) sum[k] += __builtin_amdgcn_exp2f(z[h * a.z_ld + at[k]] - m) * inv;
     }
 #pragma unroll
-    for (int k = 0; k < PJ_ROWS / PJ_T; k++) {
-        const int i = r0 + k * PJ_T + tid;
-        if (i < sp.len) mass[i] = old[k] + sum[k];
-    }
+    for (int k = 0; k < K; k++)
+        if (r0 + k * PJ_T + tid < sp.len) mass[at[k]] = old[k] + sum[k];
 }
 
 // Shares in all, of every KV head, so that each SIMD has a wave (8-bit caches:
@@ -739,7 +759,7 @@ PaSizes pa_sizes(const krh_pages *kv, int n_seq, int nh, int max_len, int shares
 }
 
 bool pa_args_ok(const krh_pages *kv, int n_seq, int n_heads, int max_len) {
-    return pg_pages_ok(kv) && n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && max_len <= INT32_MAX / 2 &&
+    return pg_pages_ok(kv) && n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && max_len <= KR_PAGE_LEN_MAX &&
            (long long)n_seq * (max_len / 16 + 1) <= INT32_MAX / 2 && n_heads > 0 &&
            n_heads % kv->n_kv_heads == 0 && n_heads / kv->n_kv_heads <= KR_PAGE_GROUP_MAX;
 }
@@ -776,10 +796,13 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
         pg_refuse(window >= 0 && softcap >= 0.0f && (!mass || mass_ld >= (size_t)max_len),
                   "paged_attention: window, soft-cap or mass rows"))
         return;
+    if (pg_not_ready("paged_attention before krh_init")) return;
     // a window's rows, and those before them in its first tile
     const int rows = window > 0 && window < max_len - 32 ? window + 31 : max_len;
     const int shares = pa_shares(kv, n_seq, rows);
     const PaSizes r = pa_sizes(kv, n_seq, n_heads, max_len, shares, mass != nullptr);
+    const int blocks = mass ? (rows + PJ_ROWS - 1) / PJ_ROWS : 0;
+    if (pg_refuse(n_heads + (long long)kv->n_kv_heads * blocks <= INT32_MAX / PJ_T, "paged_attention: too many rows for a mass")) return;
     float *w = (float *)ws;
     PaArgs a = {};
     a.o = o, a.q = q, a.len = len, a.mass = mass, a.mass_ld = mass_ld;
@@ -793,7 +816,6 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
     hipLaunchKernelGGL(f, dim3(shares, kv->n_kv_heads), dim3(64), 0, kr_stream(), p, a, kr_fault_word());
     kr_check_launch("paged_attention");
     if (shares > 1 || mass) {
-        const int blocks = mass ? (rows + PJ_ROWS - 1) / PJ_ROWS : 0;
         hipLaunchKernelGGL(k_paged_join, dim3(n_heads + kv->n_kv_heads * blocks, n_seq), dim3(PJ_T), 0, kr_stream(), p, a,
                            pg_log2(hd / 4), blocks);
         kr_check_launch("paged_attention");

@@ -59,4 +59,9 @@ inline bool pg_refuse(bool ok, const char *what) {
     if (!ok) kr_fail(ML_E_SHAPE, what, hipSuccess);
     return !ok;
 }
+// a kernel's reports need the fault words
+inline bool pg_not_ready(const char *what) {
+    if (!kr_fault_word()) kr_fail(ML_E_ISA, what, hipSuccess);
+    return !kr_fault_word();
+}
 

@@ -135,7 +135,7 @@ extern "C" void krh_logit_rules(float *out, size_t ldo, const float *logits, siz
                                 const krh_logit_rule *rule, const int *seen, size_t seen_ld, const int *n_seen,
                                 const int *bias_id, const float *bias, size_t bias_ld, const int *n_bias,
                                 const uint32_t *masks, int n_masks) {
-    const bool sizes = n > 0 && rows >= 0 && rows <= KRH_ROWS_MAX && n_masks >= 0 && seen_ld <= INT32_MAX && bias_ld <= INT32_MAX &&
+    const bool sizes = n > 0 && rows >= 0 && rows <= KRH_ROWS_MAX && n_masks >= 0 && seen_ld <= INT32_MAX / 2 && bias_ld <= INT32_MAX / 2 &&
                        ldo >= (size_t)n && ld >= (size_t)n && (out != logits || ldo == ld);
     if (!sizes) {
         kr_fail(ML_E_SHAPE, "logit_rules sizes", hipSuccess);
@@ -144,6 +144,10 @@ extern "C" void krh_logit_rules(float *out, size_t ldo, const float *logits, siz
     if (rows == 0) return;
     if (!out || !logits || !rule || (seen && !n_seen) || (bias_id && (!bias || !n_bias)) || (n_masks > 0 && !masks)) {
         kr_fail(ML_E_SHAPE, "logit_rules: a missing array", hipSuccess);
+        return;
+    }
+    if (!kr_fault_word()) {
+        kr_fail(ML_E_ISA, "logit_rules before krh_init", hipSuccess);
         return;
     }
     const RlArgs a = { out, logits, ldo, ld, rule, seen, n_seen, bias_id, n_bias, bias, seen_ld, bias_ld, masks, n, n_masks };

@@ -209,6 +209,60 @@ def test_attention_many_sequences(dev, kv_type):
     check_attention(dev, kv_type, 4, 2, 64, 16, list(rng.integers(0, 400, 70)), mass=True)
 
 
+@pytest.mark.parametrize("n,most", [(65, 40), (128, 90), (333, 60), (1000, 33)])
+def test_attention_more_sequences_than_lanes(dev, n, most):
+    """past 64 sequences the shares are found over several rounds; runs of empty ones among them"""
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, most, n)
+    lens[40:n // 2] = 0
+    lens[[0, -1]] = 0, most
+    check_attention(dev, K.ML_F16, 2, 1, 64, 16, [int(v) for v in lens], mass=True)
+    check_attention(dev, K.ML_Q8_0, 2, 1, 64, 16, [int(v) for v in lens])
+
+
+def test_attention_many_kv_heads(dev):
+    """more KV heads than waves are wanted: a share holds every sequence"""
+    check_attention(dev, K.ML_F16, 2100, 2100, 8, 16, [40, 3, 0, 70], mass=True)
+
+
+@pytest.mark.parametrize("kv_type,hd", [(K.ML_F32, 256), (K.ML_F16, 256), (K.ML_Q8_0, 256), (K.ML_F32, 208), (K.ML_F16, 136),
+                                        (K.ML_Q8_0, 144)])
+def test_attention_wide_heads(dev, kv_type, hd):
+    """heads past 128 dims: tiles of 16 rows"""
+    check_attention(dev, kv_type, 8, 2, hd, 16, [1, 15, 16, 17, 33, 700, 0, 48], mass=True)
+    check_attention(dev, kv_type, 8, 2, hd, 32, [300, 45], window=37, cap=20.0)
+
+
+def test_offsets_past_32_bits(dev):
+    """pages beyond 2^31 values: rows into them, back, and attended"""
+    n, nkv, hd, page = 270000, 2, 256, 16
+    k, v = (K.DevBuf(4 * n * nkv * hd * page) for _ in range(2))
+    dev.bufs += [k, v]
+    kv = K.KrhPages(k.ptr, v.ptr, None, None, K.ML_F32, n, page, nkv, hd)
+    rng = np.random.default_rng(9)
+    T = 40
+    table = i32([[n - 1, 7, n - 2]])
+    kr, vr, q = f32(rng.standard_normal((T, nkv * hd))), f32(rng.standard_normal((T, nkv * hd))), f32(
+        rng.standard_normal((1, 4, hd)))
+    tb, sb, rb = dev.put(table), dev.zeros(4 * T), dev.put(np.arange(T, dtype=np.int32))
+    kb, vb, ob = dev.put(kr), dev.put(vr), dev.zeros(q.nbytes)
+    ref = C.byref(kv)
+    K.hip.krh_paged_qkv(None, 0, ref, tb.ptr, 3, 1, None, 0, kb.ptr, nkv * hd, vb.ptr, nkv * hd, T, 0, sb.ptr, rb.ptr, None,
+                        None, None, 0.0, None, None, 0)
+    lk, lv = dev.zeros(kr.nbytes), dev.zeros(vr.nbytes)
+    K.hip.krh_paged_load(lk.ptr, nkv * hd, lv.ptr, nkv * hd, ref, tb.ptr, 3, 1, T, sb.ptr, rb.ptr)
+    ws = dev.zeros(K.hip.krh_paged_attention_ws(ref, 1, 4, T, 0))
+    K.hip.krh_paged_attention(ob.ptr, ref, tb.ptr, 3, dev.put(i32([T])).ptr, 1, dev.put(q).ptr, 4, T, 0, 0.0625, 0.0, None, 0,
+                              ws.ptr)
+    ok()
+    assert np.array_equal(lk.get(np.float32, kr.size), kr.reshape(-1)) and np.array_equal(lv.get(np.float32, vr.size), vr.reshape(-1))
+    o = ob.get(np.float32, q.size).reshape(4, hd)
+    k64, v64 = (x.reshape(T, nkv, hd).astype(np.float64) for x in (kr, vr))
+    for h in range(4):
+        w, _, bound, _ = attention(q[0, h].astype(np.float64), k64[:, h // 2], v64[:, h // 2], 0.0625, 0, 0)
+        assert (np.abs(o[h] - w) <= bound).all()
+
+
 def test_attention_shared_pages(dev):
     """two sequences over one prompt's pages, their weights apart"""
     rng = np.random.default_rng(3)

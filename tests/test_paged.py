@@ -57,12 +57,12 @@ CASES += [("krh_paged_attention", ATT, kw) for kw in
           [dict(o=None), dict(q=None), dict(table=None), dict(len=None), dict(ws=None), dict(q=PTR + 4),
            dict(ws=PTR + 8), dict(n_seq=-1), dict(n_seq=70000), dict(n_heads=0), dict(n_heads=5), dict(n_heads=34),
            dict(max_len=0), dict(window=-1), dict(softcap=-1.0), dict(softcap=float("nan")), dict(mass_ld=63),
-           dict(table_ld=0)]]
+           dict(table_ld=0), dict(max_len=2**30), dict(n_seq=60000, max_len=2**29)]]
 CASES += [("krh_paged_evict", EVICT, kw) for kw in
           [dict(table=None), dict(len=None), dict(mass=None), dict(out_table=None), dict(out_len=None),
            dict(out_mass=None), dict(ws=None), dict(out_table=PTR), dict(n_seq=-1), dict(n_seq=70000), dict(max_len=0),
            dict(keep=0), dict(recent=-1), dict(recent=33), dict(mass_ld=63), dict(out_ld=31), dict(out_mass=PTR),
-           dict(table_ld=0), dict(out_table_ld=1)]]
+           dict(table_ld=0), dict(out_table_ld=1), dict(max_len=2**30, mass_ld=2**30)]]
 CASES += [("krh_logit_rules", RULES, kw) for kw in
           [dict(out=None), dict(logits=None), dict(rule=None), dict(n_seen=None), dict(n_bias=None), dict(bias=None),
            dict(masks=None), dict(n=0), dict(rows=-1), dict(rows=70000), dict(n_masks=-1), dict(ldo=99, out=PTR + 4),
@@ -109,3 +109,13 @@ def test_workspaces():
     assert K.hip.krh_paged_attention_ws(C.byref(pages()), 3, 5, 100, 1) == 0
     assert K.hip.krh_paged_evict_ws(3, 2, 7) >= 4 * 3 * 2 * 7
     assert K.hip.krh_paged_evict_ws(3, 2, 0) == 0
+
+
+def test_before_init():
+    """without a device a good call is refused, not launched"""
+    if K.hip.krh_device_cus() > 0:
+        pytest.skip("the device is open")
+    kv = pages()
+    for name, base in (("krh_paged_qkv", QKV), ("krh_paged_load", LOAD), ("krh_paged_attention", ATT),
+                       ("krh_paged_evict", EVICT), ("krh_logit_rules", RULES)):
+        assert call(name, base, kv) == K.ML_E_ISA, name
