@@ -397,8 +397,8 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(const EvArgs a, int *faul
 
 // Rows into the new pages, in units of U bytes, EM_ROWS a workgroup and KV
 // head; their weights, and zeros past them. Bound by HBM: each row read once
-// and written once (16 sequences of up to 4096 rows, 8B shape, half kept: 4.7
-// TB/s).
+// and written once (16 sequences of up to 4096 rows, 8B shape, half kept: 4.3
+// TB/s; with four units a thread read before the first is written, 3.3).
 constexpr int EM_ROWS = 64;
 template <class U> __global__ void __launch_bounds__(PG_T) k_evict_move(const PgView p, const EvArgs a, int rb, int *fault) {
     const int s = blockIdx.z, kvh = blockIdx.y, per = rb / (int)sizeof(U), kept = a.cnt[s], tid = threadIdx.x;

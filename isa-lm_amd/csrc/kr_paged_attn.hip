@@ -1,7 +1,7 @@
 // Attention of one token of each sequence over a paged cache (krh_paged_attention).
 //
 // The rows of all sequences, in tiles of 32 (16), are cut into equal shares, one a
-// wave and KV head (pa_share): the lengths decide on the device, so a batch of all
+// wave and KV head (pa_bound): the lengths decide on the device, so a batch of all
 // lengths loads the chip as one long sequence does. A wave passes over each
 // sequence's part of its share once with the running maximum and sum of the
 // softmax; a sequence within one share is done, the others' parts are joined by a second
@@ -502,25 +502,29 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
         load_v(raw, lo, hi);
     }
 
-    // rows [t0, t1) of the sequence, whole tiles but at its end: at most 64 half tiles, whose
-    // pages are in ids. The first rows are asked for before the queries are.
+    // rows [t0, t1) of the sequence, whole tiles but at its end: at most 64 half
+    // tiles, whose pages are in ids. The first rows are asked for before the queries
+    // are. The rows ahead are asked for without a condition, the last tile's once
+    // more at the end: behind a branch the compiler could not tell them from this
+    // tile's loads in its waits.
     __device__ __forceinline__ void pass(int t0, int t1, bool begin) {
         float sc[R];
+        const int last = t0 + (t1 - t0 - 1) / TILE * TILE;
         if constexpr (pa_two(KT, CL)) {
             Raw x, y;
             load(x, t0);
             if (begin) queries();
-            for (;; t0 += 2 * TILE) {
-                const bool more = t0 + TILE < t1;
-                if (more) load(y, t0 + TILE);
+            for (;;) {
+                load(y, min(t0 + TILE, last));
                 scores(x, sc);
                 rest(x, sc, t0);
-                if (!more) break;
-                const bool again = t0 + 2 * TILE < t1;
-                if (again) load(x, t0 + 2 * TILE);
+                t0 += TILE;
+                if (t0 > last) break;
+                load(x, min(t0 + TILE, last));
                 scores(y, sc);
-                rest(y, sc, t0 + TILE);
-                if (!again) break;
+                rest(y, sc, t0);
+                t0 += TILE;
+                if (t0 > last) break;
             }
         } else {
             Raw x;
@@ -528,16 +532,14 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             rows_of(t0, lo, hi);
             load_k(x, lo, hi);
             if (begin) queries();
-            for (;; t0 += TILE) {
+            for (;;) {
                 load_v(x, lo, hi);
                 scores(x, sc);
-                const bool more = t0 + TILE < t1;
-                if (more) {
-                    rows_of(t0 + TILE, lo, hi);
-                    load_k(x, lo, hi);
-                }
+                rows_of(min(t0 + TILE, last), lo, hi);
+                load_k(x, lo, hi);
                 rest(x, sc, t0);
-                if (!more) break;
+                t0 += TILE;
+                if (t0 > last) break;
             }
         }
     }
@@ -726,21 +728,27 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
         if (r0 + k * PJ_T + tid < sp.len) mass[at[k]] = old[k] + sum[k];
 }
 
-// Shares in all, of every KV head, so that each SIMD has a wave (8-bit caches:
-// two, their waves work more and read less), fewer where the rows are few: a
-// share is worth PA_BYTES of K and V at least. The lengths are the device's, so
-// this is what they may be at most.
-// Measured (us, 1024 / 2048 waves): 8B shape, 16 sequences 30.2 / 32.7, one of
-// 120,001 rows 98 / 105; 8-bit heads of 64 31.9 / 27.8. With 16, 32 and 64 KB:
-// one sequence of 4000 rows 15.5, 13.7, 13.7; 64 of up to 300 23.5, 23.0, 25.4.
-constexpr int PA_WAVES = 1024, PA_BYTES = 32 * 1024;
+// Shares in all, of every KV head: a wave a SIMD, which has the next tile's
+// rows under way. 8-bit rows of up to 64 dims take three, their waves work more and
+// read less. Fewer where the rows are few: a share is worth PA_BYTES of K and V at
+// least (halves: twice that). The lengths are the device's, so this is what
+// they may be at most.
+// Measured (us, 1024 / 2048 / 3072 waves): 8B shape, 16 sequences 28.9 / 34.6 /
+// 35.5, one of 120,001 rows 95 / 101 / 108; 8 bits, 24 sequences of 64 dims 28.7 /
+// 26.8 / 26.2 and with the mass 45.4 / 40.2 / 35.7, of 128 dims 27.3 / 31.3 / 34.1.
+// 16 / 32 KB: halves, one sequence of 4000 rows 14.6 / 12.4; floats of 48 dims, 8
+// of up to 250 9.8 / 11.6; 8 bits of 48 dims, 16 of up to 8000 17.4 / 19.8.
+constexpr int PA_WAVES = 1024, PA_BYTES = 16 * 1024;
 int pa_least(const krh_pages *kv) {
-    const int tile = 2 * pa_tile(kv->head_dim) * kv->head_dim * (kv->kv_type == ML_F32 ? 4 : kv->kv_type == ML_F16 ? 2 : 1);
-    return tile < PA_BYTES ? PA_BYTES / tile : 1;
+    const bool f16 = kv->kv_type == ML_F16;
+    const int tile = 2 * pa_tile(kv->head_dim) * kv->head_dim * (f16 ? 2 : kv->kv_type == ML_F32 ? 4 : 1);
+    const int bytes = f16 ? 2 * PA_BYTES : PA_BYTES;
+    return tile < bytes ? bytes / tile : 1;
 }
 int pa_shares(const krh_pages *kv, int n_seq, int rows) {
     const long long tile = pa_tile(kv->head_dim), tiles = n_seq * ((rows + tile - 1) / tile), least = pa_least(kv);
-    const long long most = (tiles + least - 1) / least, want = (kv->kv_type == ML_Q8_0 ? 2 * PA_WAVES : PA_WAVES) / kv->n_kv_heads;
+    const int waves = kv->kv_type == ML_Q8_0 && kv->head_dim <= 64 ? 3 * PA_WAVES : PA_WAVES;
+    const long long most = (tiles + least - 1) / least, want = waves / kv->n_kv_heads;
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
