@@ -18,8 +18,8 @@
 // The halves' products are exact in 32 bits, so a float operand is split in
 // two halves, x = hi + lo with |x - hi - lo| <= 2^-22 |x|: the queries (scaled by a
 // power of two a head) and the weights (scaled by 2^14, so that weights 2^-28
-// of the largest keep hi and lo whole). A KV head of up to 8 query heads has the
-// hi parts in columns 0-7 and the lo parts in 8-15 of one product. int8 rows become halves
+// of the largest keep hi and lo whole). The products of both parts are in the same sums (with both in the columns
+// of one product, where a KV head has at most 8 query heads, 1 to 4% more time for their exchange). int8 rows become halves
 // exactly (their scale multiplies the score, or the weight); F32 caches take
 // the 32-bit product, whose rate still passes what HBM delivers.
 #include <type_traits>
@@ -119,9 +119,6 @@ __device__ __forceinline__ int pa_share(const PaAll &all, int t) {
     return (int)((((long long)t + 1) * all.shares - 1) / all.tiles);
 }
 
-__device__ __forceinline__ float pa_swap8(float x) {   // the lane 8 away in its row of 16
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
-}
 // tanh within 4 half steps of a float: below 0.6 x + x t P(t), t = x^2, P fitted to
 // (tanh(x) / x - 1) / t for the least of the largest t |error|, 0.1 half steps; from
 // there 1 - 2 / (e^2x + 1). (The C library's tanhf, which the token loop's
@@ -194,7 +191,7 @@ template <int N> __device__ __forceinline__ void pa_load(unsigned (&x)[N], const
 constexpr bool pa_two(int kt, int cl) { return cl <= (kt == PG_F32 ? 64 : 128) || kt == PG_Q8; }
 constexpr int pa_waves(int kt, int cl) { return cl > (kt == PG_Q8 ? 128 : 64) ? 1 : 2; }   // a SIMD
 
-template <int KT, int CL, int NB, bool FULL> struct PaWave {
+template <int KT, int CL, bool FULL> struct PaWave {
     using Raw = PaRaw<KT, CL>;
     static constexpr int W = Raw::W, KS = Raw::KS, NT = Raw::NT, R = Raw::R, TILE = 16 * NT, EB = KT == PG_F32 ? 4 : KT == PG_F16 ? 2 : 1;
     static constexpr int KD = KT == PG_F32 ? 4 : 8;   // dims a K load
@@ -202,8 +199,9 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
 
     const PgView &p;
     const PaArgs &a;
-    const int lane, n, g, kvh, hd, group, col;
-    const bool live, is_lo;
+    static constexpr int NB = HALF ? 2 : 1;           // operands of the queries: hi and lo
+    const int lane, n, g, kvh, hd, group;
+    const bool live;   // whether this lane's column is a query head
     int seq, t_ids, bad;
     PaSpan sp;
     int ids;   // the pages of 64 half tiles from t_ids on, one a lane
@@ -214,10 +212,9 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
 
     __device__ __forceinline__ PaWave(const PgView &p_, const PaArgs &a_, int kvh_)
         : p(p_), a(a_), lane(threadIdx.x & 63), n(lane & 15), g(lane >> 4), kvh(kvh_), hd(FULL ? CL : p_.hd),
-          group(a_.nh / p_.n_kv), col(NB == 1 && HALF ? n & 7 : n), live(col < group), is_lo(NB == 1 && HALF && n >= 8),
-          bad(0) {}
+          group(a_.nh / p_.n_kv), live(n < group), bad(0) {}
 
-    __device__ __forceinline__ size_t head() const { return (size_t)seq * a.nh + kvh * group + (live ? col : 0); }
+    __device__ __forceinline__ size_t head() const { return (size_t)seq * a.nh + kvh * group + (live ? n : 0); }
 
     // the pages of the half tiles from row t0 on that have rows attended; 0 elsewhere
     __device__ __forceinline__ void find(int t0) {
@@ -268,12 +265,8 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
                     h[i] = (_Float16)y;
                     l[i] = (_Float16)(y - (float)h[i]);
                 }
-                if constexpr (NB == 1) {
-                    qf[j][0] = is_lo ? l : h;
-                } else {
-                    qf[j][0] = h;
-                    qf[j][1] = l;
-                }
+                qf[j][0] = h;
+                qf[j][1] = l;
             }
         } else {
 #pragma unroll
@@ -337,7 +330,7 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
         }
     }
 
-    // products of the tile's rows R g + i with the queries of head `col`
+    // products of the tile's rows R g + i with query head n
     __device__ __forceinline__ void scores(const Raw &raw, float (&sc)[R]) const {
 #pragma unroll
         for (int b = 0; b < NT; b++) {
@@ -372,11 +365,7 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
         const int r0 = t0 + R * g;
         float m_tile = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-            float x = sc[i];
-            if (NB == 1 && HALF) x += pa_swap8(x);
-            sc[i] = x * (KT == PG_Q8 ? cs * raw.kd[i] : cs);
-        }
+        for (int i = 0; i < R; i++) sc[i] *= KT == PG_Q8 ? cs * raw.kd[i] : cs;
         if (a.cap > 0.0f) {
             const float inv_cap = 1.0f / a.cap;
 #pragma unroll
@@ -398,7 +387,7 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
         }
 #pragma unroll
         for (int i = 0; i < R; i++) m_tile = fmaxf(m_tile, sc[i]);
-        if (a.z && live && !is_lo) {
+        if (a.z && live) {
             float *z = a.z + head() * a.z_ld + r0;
 #pragma unroll
             for (int i = 0; i < R; i += 4) *(float4v *)(z + i) = float4v{ sc[i], sc[i + 1], sc[i + 2], sc[i + 3] };
@@ -428,7 +417,7 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
         // the weights as operands: R halves, or floats
         typedef _Float16 halfr __attribute__((ext_vector_type(R)));
         typedef unsigned uintr __attribute__((ext_vector_type(R / 2)));
-        halfr ph[NB], pl;
+        halfr ph[2];
         float pf[R];
 #pragma unroll
         for (int i = 0; i < R; i++) {
@@ -444,17 +433,9 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
             if constexpr (HALF) {
                 const _Float16 hi = (_Float16)x;
                 ph[0][i] = hi;
-                pl[i] = (_Float16)(x - (float)hi);
+                ph[1][i] = (_Float16)(x - (float)hi);
             } else {
                 pf[i] = x;
-            }
-        }
-        if constexpr (HALF) {
-            if constexpr (NB == 1) {
-                const uintr x = __builtin_bit_cast(uintr, ph[0]), y = __builtin_bit_cast(uintr, pl);
-                ph[0] = __builtin_bit_cast(halfr, is_lo ? y : x);
-            } else {
-                ph[1] = pl;
             }
         }
         if constexpr (KT == PG_F32) {
@@ -471,7 +452,7 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
                 for (int i = 0; i < R / 2; i++)
                     w[i] = __builtin_amdgcn_perm(raw.v[2 * i + 1][c / 2], raw.v[2 * i][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                for (int x = 0; x < NB; x++) o[c] = pa_weigh(__builtin_bit_cast(halfr, w), ph[x], o[c]);
+                for (int x = 0; x < 2; x++) o[c] = pa_weigh(__builtin_bit_cast(halfr, w), ph[x], o[c]);
             }
         } else {
 #pragma unroll
@@ -489,7 +470,7 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
 #pragma unroll
-                    for (int x = 0; x < NB; x++) o[c4 + c] = pa_weigh(__builtin_bit_cast(halfr, w[c]), ph[x], o[c4 + c]);
+                    for (int x = 0; x < 2; x++) o[c4 + c] = pa_weigh(__builtin_bit_cast(halfr, w[c]), ph[x], o[c4 + c]);
                 }
             }
         }
@@ -560,35 +541,29 @@ template <int KT, int CL, int NB, bool FULL> struct PaWave {
                 pass(r, min(r1, r + (64 / NT) * TILE), r == r0);
             }
         }
-        if (NB == 1 && HALF) {
-#pragma unroll
-            for (int c = 0; c < W; c++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[c][i] += pa_swap8(o[c][i]);
-        }
         const float l = pa_sum_g(l_run);
         float f = alone ? 1.0f / l : 1.0f;
         if (KT == PG_Q8) f = ldexpf(f, ev);
         if (sp.len == 0) f = 0.0f;
-        if (g == 0 && live && !is_lo && (!alone || a.z)) {
-            *(float2v *)(a.pml + (slot * group + col) * 2) = float2v{ m_run, l };
+        if (g == 0 && live && (!alone || a.z)) {
+            *(float2v *)(a.pml + (slot * group + n) * 2) = float2v{ m_run, l };
         }
-        float *out = alone ? a.o + head() * hd : a.part + (slot * group + col) * hd;
+        float *out = alone ? a.o + head() * hd : a.part + (slot * group + n) * hd;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int d0 = (4 * g + i) * W;
 #pragma unroll
             for (int c = 0; c < W; c += 4)
-                if (live && !is_lo && (FULL || d0 + c < hd))
+                if (live && (FULL || d0 + c < hd))
                     *(float4v *)(out + d0 + c) = float4v{ o[c][i] * f, o[c + 1][i] * f, o[c + 2][i] * f, o[c + 3][i] * f };
         }
     }
 };
 
-template <int KT, int CL, int NB, bool FULL>
+template <int KT, int CL, bool FULL>
 __global__ void __launch_bounds__(64, pa_waves(KT, CL)) k_paged_shares(const PgView p, const PaArgs a, int *fault) {
     const int u = blockIdx.x, kvh = blockIdx.y;
-    PaWave<KT, CL, NB, FULL> w(p, a, kvh);
+    PaWave<KT, CL, FULL> w(p, a, kvh);
     PaAll all = pa_all(p, a, w.bad);
     if (u < all.shares) {
         int left = pa_bound(all, u + 1) - pa_bound(all, u), t = pa_bound(all, u);
@@ -774,17 +749,11 @@ bool pa_args_ok(const krh_pages *kv, int n_seq, int n_heads, int max_len) {
 
 using PaKernel = void (*)(const PgView, const PaArgs, int *);
 
-template <int KT, int CL> PaKernel pa_kernel(int group, int hd) {
-    if constexpr (KT == PG_F32) {
-        return hd == CL ? k_paged_shares<KT, CL, 1, true> : k_paged_shares<KT, CL, 1, false>;
-    } else {
-        if (hd != CL) return k_paged_shares<KT, CL, 2, false>;
-        return group <= 8 ? k_paged_shares<KT, CL, 1, true> : k_paged_shares<KT, CL, 2, true>;
-    }
-}
-template <int KT> PaKernel pa_kernel(int group, int hd) {
-    return hd <= 64 ? pa_kernel<KT, 64>(group, hd) : hd <= 128 ? pa_kernel<KT, 128>(group, hd) : pa_kernel<KT, 256>(group, hd);
-}
+// Heads take the next width of 64, 128 and 256 dims; a kernel of its own has them
+// where they fill it (without, halves take 0 to 2% more, 8 bits 0 to 6, floats 1 and of
+// 256 dims 7).
+template <int KT, int CL> PaKernel pa_kernel(int hd) { return hd == CL ? k_paged_shares<KT, CL, true> : k_paged_shares<KT, CL, false>; }
+template <int KT> PaKernel pa_kernel(int hd) { return hd <= 64 ? pa_kernel<KT, 64>(hd) : hd <= 128 ? pa_kernel<KT, 128>(hd) : pa_kernel<KT, 256>(hd); }
 
 }  // namespace
 
@@ -818,9 +787,9 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
     a.nh = n_heads, a.max_len = max_len, a.window = window, a.shares = shares, a.least = pa_least(kv), a.tl = pg_log2(pa_tile(kv->head_dim));
     a.scale = scale, a.cap = softcap, a.z_up = kv->kv_type == ML_F32 ? 0.0f : PA_UP;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
-    const int group = n_heads / kv->n_kv_heads, hd = kv->head_dim;
-    const PaKernel f = kv->kv_type == ML_F32 ? pa_kernel<PG_F32>(group, hd) : kv->kv_type == ML_F16 ? pa_kernel<PG_F16>(group, hd)
-                                                                                                    : pa_kernel<PG_Q8>(group, hd);
+    const int hd = kv->head_dim;
+    const PaKernel f = kv->kv_type == ML_F32 ? pa_kernel<PG_F32>(hd) : kv->kv_type == ML_F16 ? pa_kernel<PG_F16>(hd)
+                                                                                                    : pa_kernel<PG_Q8>(hd);
     hipLaunchKernelGGL(f, dim3(shares, kv->n_kv_heads), dim3(64), 0, kr_stream(), p, a, kr_fault_word());
     kr_check_launch("paged_attention");
     if (shares > 1 || mass) {
