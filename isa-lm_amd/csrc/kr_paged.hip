@@ -1,9 +1,6 @@
 // Several sequences over one paged cache: the rows of new tokens into their
 // pages (per-head norm and rotation on the way), attention of one token of each
 // sequence, and eviction by accumulated attention weight.
-#include "kr_internal.h"
-#include "kr_numerics.h"
-#include "kr_paged.h"
 #include "kr_paged_dev.h"
 
 namespace {
@@ -38,7 +35,11 @@ template <class T, class F> __device__ __forceinline__ T pg_reduce(T v, int n, F
     if (n > 4) v = f(v, other([](unsigned x) { return pg_dpp<0x141>(x); }));
     if (n > 8) v = f(v, other([](unsigned x) { return pg_dpp<0x140>(x); }));
     const bool row = threadIdx.x & 16;
-    if (n > 16) v = f(v, other([&](unsigned x) { const auto s = __builtin_amdgcn_permlane16_swap(x, x, false, false); return row ? s[0] : s[1]; }));
+    if (n > 16)
+        v = f(v, other([&](unsigned x) {
+            const auto s = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+            return row ? s[0] : s[1];
+        }));
     return v;
 }
 __device__ __forceinline__ double pg_sum(double v, int n) {
@@ -85,7 +86,8 @@ __device__ __forceinline__ void pg_put(float *p, const Pg8 &x) {
 // the conversions of krh_store_kv, but that an 8-bit row's factor is 127 times
 // the rounded reciprocal of its maximum, as tensor libraries form 127 / max (a
 // step of the factor at most: an element next to a border may fall on its other side)
-template <int KT> __device__ __forceinline__ void pg_store(void *dst, float *d, size_t at, int hd, const Pg8 &x, int l, bool live, int n) {
+template <int KT>
+__device__ __forceinline__ void pg_store(void *dst, float *d, size_t at, int hd, const Pg8 &x, int l, bool live, int n) {
     const size_t e = at * hd + 8 * l;
     if constexpr (KT == PG_F32) {
         if (live) pg_put((float *)dst + e, x);
@@ -181,8 +183,9 @@ template <int KT> __device__ __forceinline__ Pg8 pg_load8(const void *src, const
     }
 }
 
-template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_load(const PgView p, float *k, size_t ldk, float *v, size_t ldv,
-                                                                       int n_rows, const int *seqs, const int *rows, int lps, int *fault) {
+template <int KT>
+__global__ void __launch_bounds__(PG_T) k_paged_load(const PgView p, float *k, size_t ldk, float *v, size_t ldv, int n_rows,
+                                                     const int *seqs, const int *rows, int lps, int *fault) {
     const unsigned n = 1u << lps, per = 2 * p.n_kv, item = (blockIdx.x * PG_T + threadIdx.x) >> lps;
     const int l = (int)(threadIdx.x & (n - 1));
     if (item >= n_rows * per || 8 * l >= p.hd) return;
@@ -446,26 +449,33 @@ extern "C" void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const
     if (ntok == 0) return;
     const size_t kvd = (size_t)kv->n_kv_heads * kv->head_dim, qd = (size_t)n_heads * kv->head_dim;
     if (pg_refuse(table && k && v && seq && row && (n_heads == 0 || (q && qo)) && (!cos_t) == (!sin_t) &&
-                   (!cos_t || (pos && n_pos > 0)) && (n_heads == 0 || (!q_norm) == (!k_norm)), "paged_qkv: a missing array") ||
-        pg_refuse(ldk >= kvd && ldv >= kvd && ldk % 4 == 0 && ldv % 4 == 0 && pg_aligned(k) && pg_aligned(v) && pg_aligned(k_norm) &&
-                   pg_aligned(cos_t) && pg_aligned(sin_t) &&
-                   (n_heads == 0 || (ldq >= qd && ldqo >= qd && ldq % 4 == 0 && ldqo % 4 == 0 && pg_aligned(q) &&
-                                     pg_aligned(qo) && pg_aligned(q_norm))), "paged_qkv: row strides or alignment"))
+                      (!cos_t || (pos && n_pos > 0)) && (n_heads == 0 || (!q_norm) == (!k_norm)),
+                  "paged_qkv: a missing array") ||
+        pg_refuse(ldk >= kvd && ldv >= kvd && ldk % 4 == 0 && ldv % 4 == 0 && pg_aligned(k) && pg_aligned(v) &&
+                      pg_aligned(k_norm) && pg_aligned(cos_t) && pg_aligned(sin_t) &&
+                      (n_heads == 0 || (ldq >= qd && ldqo >= qd && ldq % 4 == 0 && ldqo % 4 == 0 && pg_aligned(q) &&
+                                        pg_aligned(qo) && pg_aligned(q_norm))),
+                  "paged_qkv: row strides or alignment"))
         return;
     const int lps = pg_log2(kv->head_dim / 8);
     const unsigned grid = item_blocks((size_t)ntok * (n_heads + 2 * (size_t)kv->n_kv_heads), lps);
     if (pg_refuse(grid > 0, "paged_qkv: too many tokens") || pg_not_ready("paged_qkv before krh_init")) return;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
-    const QkvArgs a = { qo, q, k, v, q_norm, k_norm, cos_t, sin_t, seq, row, pos, ldqo, ldq, ldk, ldv, eps, 1.0 / kv->head_dim,
+    const QkvArgs a = { qo,  q,    k,   v,   q_norm, k_norm, cos_t, sin_t, seq, row,
+                        pos, ldqo, ldq, ldk, ldv,    eps,    1.0 / kv->head_dim,
                         ntok, n_heads, n_pos };
-    const auto f = kv->kv_type == ML_F32 ? k_paged_qkv<PG_F32> : kv->kv_type == ML_F16 ? k_paged_qkv<PG_F16> : k_paged_qkv<PG_Q8>;
+    const auto f = kv->kv_type == ML_F32   ? k_paged_qkv<PG_F32>
+                   : kv->kv_type == ML_F16 ? k_paged_qkv<PG_F16>
+                                           : k_paged_qkv<PG_Q8>;
     hipLaunchKernelGGL(f, dim3(grid), dim3(PG_T), 0, kr_stream(), p, a, lps, kr_fault_word());
     kr_check_launch("paged_qkv");
 }
 
 extern "C" void krh_paged_load(float *k, size_t ldk, float *v, size_t ldv, const krh_pages *kv, const int *table,
                                int table_ld, int n_seq, int n, const int *seq, const int *row) {
-    if (pg_refuse(pg_pages_ok(kv), "paged_load: the pages") || pg_refuse(n >= 0 && n_seq > 0 && table_ld > 0, "paged_load sizes")) return;
+    if (pg_refuse(pg_pages_ok(kv), "paged_load: the pages") ||
+        pg_refuse(n >= 0 && n_seq > 0 && table_ld > 0, "paged_load sizes"))
+        return;
     if (n == 0) return;
     const size_t kvd = (size_t)kv->n_kv_heads * kv->head_dim;
     if (pg_refuse(table && k && v && seq && row, "paged_load: a missing array") ||
@@ -475,9 +485,11 @@ extern "C" void krh_paged_load(float *k, size_t ldk, float *v, size_t ldv, const
     const int lps = pg_log2(kv->head_dim / 8);
     const unsigned grid = item_blocks((size_t)n * 2 * kv->n_kv_heads, lps);
     if (pg_refuse(grid > 0, "paged_load: too many rows") || pg_not_ready("paged_load before krh_init")) return;
-    const auto f = kv->kv_type == ML_F32 ? k_paged_load<PG_F32> : kv->kv_type == ML_F16 ? k_paged_load<PG_F16> : k_paged_load<PG_Q8>;
-    hipLaunchKernelGGL(f, dim3(grid), dim3(PG_T), 0, kr_stream(), pg_view(kv, table, table_ld, n_seq), k, ldk, v, ldv, n, seq, row,
-                       lps, kr_fault_word());
+    const auto f = kv->kv_type == ML_F32   ? k_paged_load<PG_F32>
+                   : kv->kv_type == ML_F16 ? k_paged_load<PG_F16>
+                                           : k_paged_load<PG_Q8>;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(PG_T), 0, kr_stream(), pg_view(kv, table, table_ld, n_seq), k, ldk, v, ldv,
+                       n, seq, row, lps, kr_fault_word());
     kr_check_launch("paged_load");
 }
 
@@ -491,13 +503,16 @@ extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table
                                 int out_table_ld, int *out_len, float *out_mass, size_t out_ld, void *ws) {
     if (n_seq == 0) return;
     if (pg_refuse(pg_pages_ok(kv), "paged_evict: the pages") ||
-        pg_refuse(n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && max_len <= KR_PAGE_LEN_MAX && keep > 0 && recent >= 0 && recent <= keep && table_ld > 0 &&
+        pg_refuse(n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && max_len <= KR_PAGE_LEN_MAX && keep > 0 &&
+                   recent >= 0 && recent <= keep && table_ld > 0 &&
                    out_table_ld > 0, "paged_evict sizes") ||
-        pg_refuse(table && len && mass && out_table && out_len && out_mass && ws && !((uintptr_t)ws & 3) && out_table != table,
+        pg_refuse(table && len && mass && out_table && out_len && out_mass && ws && !((uintptr_t)ws & 3) &&
+                   out_table != table,
                "paged_evict: a missing array, or the pages onto themselves") ||
         pg_refuse(mass_ld >= (size_t)max_len && out_ld >= (size_t)keep && (out_mass != mass || out_ld == mass_ld),
                "paged_evict: mass rows") ||
-        pg_refuse((size_t)out_table_ld * kv->page_size >= (size_t)(keep < max_len ? keep : max_len), "paged_evict: out_table's pages"))
+        pg_refuse((size_t)out_table_ld * kv->page_size >= (size_t)(keep < max_len ? keep : max_len),
+                   "paged_evict: out_table's pages"))
         return;
     if (pg_not_ready("paged_evict before krh_init")) return;
     int *w = (int *)ws;
@@ -506,7 +521,8 @@ extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table
                        w + 2 * rows, w, (float *)(w + rows) };
     hipLaunchKernelGGL(k_evict_select, dim3(kv->n_kv_heads, n_seq), dim3(EV_T), 0, kr_stream(), a, kr_fault_word());
     kr_check_launch("paged_evict");
-    const int rb = kv->head_dim * (kv->kv_type == ML_F32 ? 4 : kv->kv_type == ML_F16 ? 2 : 1), most = keep < max_len ? keep : max_len;
+    const int rb = kv->head_dim * (kv->kv_type == ML_F32 ? 4 : kv->kv_type == ML_F16 ? 2 : 1);
+    const int most = keep < max_len ? keep : max_len;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
     hipLaunchKernelGGL(rb % 16 ? k_evict_move<uint2> : k_evict_move<uint4>,
                        dim3((most + EM_ROWS - 1) / EM_ROWS, kv->n_kv_heads, n_seq), dim3(PG_T), 0, kr_stream(), p, a, rb,

@@ -1,27 +1,37 @@
-// Attention of one token of each sequence over a paged cache (krh_paged_attention).
+// Attention of one token of each sequence over a paged cache
+// (krh_paged_attention).
 //
-// The rows of all sequences, in tiles of 32 (16), are cut into equal shares, one a
-// wave and KV head (pa_bound): the lengths decide on the device, so a batch of all
-// lengths loads the chip as one long sequence does. A wave passes over each
-// sequence's part of its share once with the running maximum and sum of the
-// softmax; a sequence within one share is done, the others' parts are joined by a second
-// launch (k_paged_join), which finds them by the same arithmetic.
+// The rows of all sequences, in tiles of 32 (16), are cut into equal shares, one
+// a wave and KV head (pa_bound): the lengths decide on the device, so a batch of
+// all lengths loads the chip as one long sequence does. A wave passes over each
+// sequence's part of its share once, with the running maximum and sum of the
+// softmax. A sequence within one share is then done; the others' parts are
+// joined by a second launch (k_paged_join), which finds them by the same
+// arithmetic. Where all are short each is a share, and there is no second launch. (Joined by the last share to end instead, whose parts pass between
+// the dies' caches: 20 to 40 us more with atomics that pass those caches, 60 to
+// 90 with fences.)
 //
 // Both products run on the matrix cores, transposed so that nothing passes
-// through LDS: S^T = K Q^T has rows as the tile's rows and query heads as its
-// columns, and the lane that holds a head's scores of 8 (4) consecutive rows holds
-// them as the operand P^T of O^T = V^T P^T. K's rows are read straight into
+// through LDS: S^T = K Q^T has the tile's rows as rows and query heads as
+// columns, and the lane that holds a head's scores of 8 (4) consecutive rows
+// holds them as the operand P^T of O^T = V^T P^T. K's rows are read straight into
 // operand registers (the order of the contraction is free, so a lane reads 8
-// dims at a time); V's are transposed 2 by 2 in registers by byte permutes
-// (F32: none, a float is an operand by itself).
+// dims at a time); V's are transposed 2 by 2 in registers by byte permutes (F32:
+// none, a float is an operand by itself).
 //
-// The halves' products are exact in 32 bits, so a float operand is split in
-// two halves, x = hi + lo with |x - hi - lo| <= 2^-22 |x|: the queries (scaled by a
-// power of two a head) and the weights (scaled by 2^14, so that weights 2^-28
-// of the largest keep hi and lo whole). The products of both parts are in the same sums (with both in the columns
-// of one product, where a KV head has at most 8 query heads, 1 to 4% more time for their exchange). int8 rows become halves
-// exactly (their scale multiplies the score, or the weight); F32 caches take
-// the 32-bit product, whose rate still passes what HBM delivers.
+// The halves' products are exact in 32 bits, so a float operand is split in two
+// halves, x = hi + lo with |x - hi - lo| <= 2^-22 |x|: the queries (scaled by a
+// power of two a head) and the weights (scaled by 2^14, so that weights 2^-28 of
+// the largest keep hi and lo whole). The products of both are in the same sums
+// (hi and lo as columns of one product, for up to 8 query heads a KV head, took
+// 1 to 4% more, for their exchange). int8 rows become halves exactly; their scale
+// multiplies the score, or the weight. F32 caches take the 32-bit product, whose
+// rate still passes what HBM delivers.
+//
+// Bound by HBM where the rows are many: 8B shape, F16, 64 sequences of up to 6144
+// rows 125 us (5.5 TB/s; the chip's plain read rate is 5.6), one of 120,001 rows
+// 93 (5.3), 16 of up to 4001 24 (4.9). 8-bit rows by a tile's latency and
+// instructions: 24 sequences of 64 dims 22 us (4.2).
 #include <type_traits>
 #include "kr_paged_dev.h"
 
@@ -49,7 +59,8 @@ struct PaArgs {
     float *pml;     // [n_kv][n_seq + shares][group][2]: their maximum (log2) and weight
     float *z;       // [n_seq][nh][z_ld]: the scores (log2), for the mass
     size_t z_ld;
-    int nh, max_len, window, shares, tl, least;   // tl: log2 of a tile's rows; least: tiles a share is worth
+    int nh, max_len, window, shares;
+    int whole, tl, least;     // whole: a share a sequence; tl: log2 of a tile's rows; least: tiles a share is worth
     float scale, cap, z_up;   // z_up: log2 of the weights' scale in the sums
 };
 
@@ -125,8 +136,10 @@ __device__ __forceinline__ int pa_share(const PaAll &all, int t) {
 // soft-caps call, is three quotients: a float cache's 10,000 rows 168 us.)
 __device__ __forceinline__ float pa_tanh(float x) {
     const float t = x * x, y = fabsf(x);
-    const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(-0x1.830bfap-8f, t, 0x1.54e018p-6f), t, -0x1.b89edap-5f),
-                                                  t, 0x1.1109dcp-3f), t, -0x1.55553ep-2f);
+    float p = __builtin_fmaf(-0x1.830bfap-8f, t, 0x1.54e018p-6f);
+    p = __builtin_fmaf(p, t, -0x1.b89edap-5f);
+    p = __builtin_fmaf(p, t, 0x1.1109dcp-3f);
+    p = __builtin_fmaf(p, t, -0x1.55553ep-2f);
     const float e = __builtin_amdgcn_exp2f(y * 2.8853900817779268f);
     const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
     return y < 0.6f ? __builtin_fmaf(x * t, p, x) : copysignf(far, x);
@@ -145,8 +158,12 @@ __device__ __forceinline__ float pa_sum_g(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-__device__ __forceinline__ float4v pa_weigh(half8 v, half8 p, float4v o) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, o, 0, 0, 0); }
-__device__ __forceinline__ float4v pa_weigh(half4 v, half4 p, float4v o) { return __builtin_amdgcn_mfma_f32_16x16x16f16(v, p, o, 0, 0, 0); }
+__device__ __forceinline__ float4v pa_weigh(half8 v, half8 p, float4v o) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, o, 0, 0, 0);
+}
+__device__ __forceinline__ float4v pa_weigh(half4 v, half4 p, float4v o) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(v, p, o, 0, 0, 0);
+}
 
 // halves of 4 int8 (xor 0x80: 0..255) as 1024 + u - 1152, exact
 __device__ __forceinline__ unsigned pa_h2(unsigned u, unsigned sel) {
@@ -193,7 +210,8 @@ constexpr int pa_waves(int kt, int cl) { return cl > (kt == PG_Q8 ? 128 : 64) ? 
 
 template <int KT, int CL, bool FULL> struct PaWave {
     using Raw = PaRaw<KT, CL>;
-    static constexpr int W = Raw::W, KS = Raw::KS, NT = Raw::NT, R = Raw::R, TILE = 16 * NT, EB = KT == PG_F32 ? 4 : KT == PG_F16 ? 2 : 1;
+    static constexpr int W = Raw::W, KS = Raw::KS, NT = Raw::NT, R = Raw::R, TILE = 16 * NT;
+    static constexpr int EB = KT == PG_F32 ? 4 : KT == PG_F16 ? 2 : 1;
     static constexpr int KD = KT == PG_F32 ? 4 : 8;   // dims a K load
     static constexpr bool HALF = KT != PG_F32;
 
@@ -216,7 +234,7 @@ template <int KT, int CL, bool FULL> struct PaWave {
 
     __device__ __forceinline__ size_t head() const { return (size_t)seq * a.nh + kvh * group + (live ? n : 0); }
 
-    // the pages of the half tiles from row t0 on that have rows attended; 0 elsewhere
+    // the pages of the half tiles from row t0 on that have rows attended; -1 elsewhere
     __device__ __forceinline__ void find(int t0) {
         t_ids = t0;
         const int r = t0 + 16 * lane;
@@ -351,7 +369,8 @@ template <int KT, int CL, bool FULL> struct PaWave {
                 } else {
 #pragma unroll
                     for (int c = 0; c < 4; c++)
-                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(raw.k[b][j][c]), qf[j][0][c], acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(raw.k[b][j][c]), qf[j][0][c], acc, 0,
+                                                                   0, 0);
                 }
             }
 #pragma unroll
@@ -450,7 +469,8 @@ template <int KT, int CL, bool FULL> struct PaWave {
                 uintr w;
 #pragma unroll
                 for (int i = 0; i < R / 2; i++)
-                    w[i] = __builtin_amdgcn_perm(raw.v[2 * i + 1][c / 2], raw.v[2 * i][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+                    w[i] = __builtin_amdgcn_perm(raw.v[2 * i + 1][c / 2], raw.v[2 * i][c / 2],
+                                                 c & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                 for (int x = 0; x < 2; x++) o[c] = pa_weigh(__builtin_bit_cast(halfr, w), ph[x], o[c]);
             }
@@ -461,7 +481,8 @@ template <int KT, int CL, bool FULL> struct PaWave {
 #pragma unroll
                 for (int i = 0; i < R / 2; i++) {
                     const unsigned x = raw.v[2 * i][c4 / 4] ^ 0x80808080u, y = raw.v[2 * i + 1][c4 / 4] ^ 0x80808080u;
-                    const unsigned u = __builtin_amdgcn_perm(y, x, 0x05010400u), v = __builtin_amdgcn_perm(y, x, 0x07030602u);
+                    const unsigned u = __builtin_amdgcn_perm(y, x, 0x05010400u);
+                    const unsigned v = __builtin_amdgcn_perm(y, x, 0x07030602u);
                     w[0][i] = pa_h2(u, 0x04010400);
                     w[1][i] = pa_h2(u, 0x04030402);
                     w[2][i] = pa_h2(v, 0x04010400);
@@ -564,6 +585,13 @@ template <int KT, int CL, bool FULL>
 __global__ void __launch_bounds__(64, pa_waves(KT, CL)) k_paged_shares(const PgView p, const PaArgs a, int *fault) {
     const int u = blockIdx.x, kvh = blockIdx.y;
     PaWave<KT, CL, FULL> w(p, a, kvh);
+    if (a.whole) {
+        w.seq = u;
+        w.sp = pa_span(a, kr_page_len(a.len[u], a.max_len, w.bad));
+        w.part(0, w.sp.tiles, 0);
+        kr_report(fault, w.bad);
+        return;
+    }
     PaAll all = pa_all(p, a, w.bad);
     if (u < all.shares) {
         int left = pa_bound(all, u + 1) - pa_bound(all, u), t = pa_bound(all, u);
@@ -727,6 +755,20 @@ int pa_shares(const krh_pages *kv, int n_seq, int rows) {
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
+// Rows up to which a sequence is one wave's, a KV head, and there is no second
+// launch (it is not known how many of them are used, and the mass takes the launch
+// anyway). About 0.7 us a tile of halves or 8 bits of 128 dims, twice that for
+// floats of 64, against the join's 4 to 10 us, the more the more sequences. Measured
+// (us, shares / whole): 8B shape, halves, one sequence of 256 rows 10.2 / 9.9, of 384
+// 10.2 / 12.9, 64 of up to 512 25.8 / 18.7; 8 bits of 64 dims, 256 rows 11.3 / 9.3,
+// 384 11.3 / 12.3; floats of 48 dims, 128 rows 9.5 / 8.5, 192 9.4 / 11.0; halves of
+// 256 dims, 128 rows, 1 and 8 sequences 10.6 / 11.3 and 13.0 / 11.1.
+constexpr int PA_WHOLE = 256, PA_WHOLE_MANY = 128;
+int pa_whole(const krh_pages *kv, int n_seq) {
+    const int rows = PA_WHOLE * 128 / ((kv->head_dim <= 128 ? 128 : 256) * (kv->kv_type != ML_F32 ? 1 : kv->head_dim <= 64 ? 2 : 4));
+    return (long long)n_seq * kv->n_kv_heads >= PA_WHOLE_MANY ? 2 * rows : rows;
+}
+
 // the workspace's pieces, in floats
 struct PaSizes {
     size_t part, pml, z_ld, z;
@@ -752,8 +794,12 @@ using PaKernel = void (*)(const PgView, const PaArgs, int *);
 // Heads take the next width of 64, 128 and 256 dims; a kernel of its own has them
 // where they fill it (without, halves take 0 to 2% more, 8 bits 0 to 6, floats 1 and of
 // 256 dims 7).
-template <int KT, int CL> PaKernel pa_kernel(int hd) { return hd == CL ? k_paged_shares<KT, CL, true> : k_paged_shares<KT, CL, false>; }
-template <int KT> PaKernel pa_kernel(int hd) { return hd <= 64 ? pa_kernel<KT, 64>(hd) : hd <= 128 ? pa_kernel<KT, 128>(hd) : pa_kernel<KT, 256>(hd); }
+template <int KT, int CL> PaKernel pa_kernel(int hd) {
+    return hd == CL ? k_paged_shares<KT, CL, true> : k_paged_shares<KT, CL, false>;
+}
+template <int KT> PaKernel pa_kernel(int hd) {
+    return hd <= 64 ? pa_kernel<KT, 64>(hd) : hd <= 128 ? pa_kernel<KT, 128>(hd) : pa_kernel<KT, 256>(hd);
+}
 
 }  // namespace
 
@@ -776,15 +822,20 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
     if (pg_not_ready("paged_attention before krh_init")) return;
     // a window's rows, and those before them in its first tile
     const int rows = window > 0 && window < max_len - 32 ? window + 31 : max_len;
-    const int shares = pa_shares(kv, n_seq, rows);
-    const PaSizes r = pa_sizes(kv, n_seq, n_heads, max_len, shares, mass != nullptr);
+    const bool whole = !mass && rows <= pa_whole(kv, n_seq);
+    const int shares = whole ? n_seq : pa_shares(kv, n_seq, rows);
+    const PaSizes r = pa_sizes(kv, n_seq, n_heads, max_len, whole ? 1 : shares, mass != nullptr);
     const int blocks = mass ? (rows + PJ_ROWS - 1) / PJ_ROWS : 0;
-    if (pg_refuse(n_heads + (long long)kv->n_kv_heads * blocks <= INT32_MAX / PJ_T, "paged_attention: too many rows for a mass")) return;
+    if (pg_refuse(n_heads + (long long)kv->n_kv_heads * blocks <= INT32_MAX / PJ_T,
+                  "paged_attention: too many rows for a mass"))
+        return;
     float *w = (float *)ws;
     PaArgs a = {};
     a.o = o, a.q = q, a.len = len, a.mass = mass, a.mass_ld = mass_ld;
     a.part = w, a.pml = w + r.part, a.z = mass ? w + r.part + r.pml : nullptr, a.z_ld = r.z_ld;
-    a.nh = n_heads, a.max_len = max_len, a.window = window, a.shares = shares, a.least = pa_least(kv), a.tl = pg_log2(pa_tile(kv->head_dim));
+    a.nh = n_heads, a.max_len = max_len, a.window = window, a.shares = shares, a.least = pa_least(kv);
+    a.tl = pg_log2(pa_tile(kv->head_dim));
+    a.whole = whole;
     a.scale = scale, a.cap = softcap, a.z_up = kv->kv_type == ML_F32 ? 0.0f : PA_UP;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
     const int hd = kv->head_dim;
@@ -792,7 +843,7 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
                                                                                                     : pa_kernel<PG_Q8>(hd);
     hipLaunchKernelGGL(f, dim3(shares, kv->n_kv_heads), dim3(64), 0, kr_stream(), p, a, kr_fault_word());
     kr_check_launch("paged_attention");
-    if (shares > 1 || mass) {
+    if ((shares > 1 && !whole) || mass) {
         hipLaunchKernelGGL(k_paged_join, dim3(n_heads + kv->n_kv_heads * blocks, n_seq), dim3(PJ_T), 0, kr_stream(), p, a,
                            pg_log2(hd / 4), blocks);
         kr_check_launch("paged_attention");

@@ -51,8 +51,8 @@ inline bool pg_aligned(const void *p) { return !((uintptr_t)p & 15); }
 
 inline PgView pg_view(const krh_pages *kv, const int *table, int ld, int n_seq) {
     const bool q8 = kv->kv_type == ML_Q8_0;
-    return { kv->k, kv->v, q8 ? kv->kd : nullptr, q8 ? kv->vd : nullptr, table, ld, n_seq, kv->n_pages, pg_log2(kv->page_size),
-             kv->n_kv_heads, kv->head_dim };
+    return { kv->k, kv->v, q8 ? kv->kd : nullptr, q8 ? kv->vd : nullptr, table, ld, n_seq, kv->n_pages,
+             pg_log2(kv->page_size), kv->n_kv_heads, kv->head_dim };
 }
 
 inline bool pg_refuse(bool ok, const char *what) {

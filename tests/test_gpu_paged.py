@@ -220,6 +220,22 @@ def test_attention_more_sequences_than_lanes(dev, n, most):
     check_attention(dev, K.ML_Q8_0, 2, 1, 64, 16, [int(v) for v in lens])
 
 
+@pytest.mark.parametrize("kv_type,hd,most", [(K.ML_F16, 128, 256), (K.ML_Q8_0, 64, 256), (K.ML_F16, 256, 128), (K.ML_F32, 64, 128),
+                                             (K.ML_F32, 128, 64), (K.ML_F32, 256, 32)])
+@pytest.mark.parametrize("many", [False, True])
+def test_attention_whole_sequences(dev, kv_type, hd, most, many):
+    """each side of the length up to which a sequence is one wave's, for few sequences and for many"""
+    rng = np.random.default_rng(hd)
+    n, top = (70, 2 * most) if many else (3, most)
+    lens = [int(v) for v in rng.integers(0, top, n)]
+    lens[1] = 0
+    for extra in (0, 1):
+        lens[0] = top + extra
+        check_attention(dev, kv_type, 4, 2, hd, 16, lens)
+        check_attention(dev, kv_type, 4, 2, hd, 16, lens, mass=True)
+    check_attention(dev, kv_type, 4, 2, hd, 16, [300, 7, 0, 900], window=most - 31)
+
+
 def test_attention_many_kv_heads(dev):
     """more KV heads than waves are wanted: a share holds every sequence"""
     check_attention(dev, K.ML_F16, 2100, 2100, 8, 16, [40, 3, 0, 70], mass=True)
