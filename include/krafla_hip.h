@@ -333,18 +333,18 @@ void krh_sample(krh_sampler *s, int *tok, float *logits, int n, int *pos, int *l
 uint64_t krh_sampler_rng(const krh_sampler *s);
 
 /* ---- several sequences over one paged cache ----
- * A pool of pages for one layer, shared by any number of sequences. Row r of a
- * sequence (its r-th cached token; a rotated key keeps its position when rows
- * before it go) lies in page table[seq * table_ld + r / page_size], slot r %
- * page_size. A page holds [n_kv_heads][page_size][head_dim]: one KV head's rows
- * are contiguous, so a page is read by whole cache lines whatever the head's
- * width. Sequences may share pages (a common prompt); entries past a
- * sequence's rows are not read.
+ * No counterpart in the reference. A pool of pages for one layer, shared by any
+ * number of sequences. Row r of a sequence (its r-th cached token; a rotated key
+ * keeps its position when rows before it go) lies in page table[seq * table_ld +
+ * r / page_size], slot r % page_size. A page holds [n_kv_heads][page_size]
+ * [head_dim]: one KV head's rows are contiguous, so a page is read by whole cache
+ * lines whatever the head's width. Sequences may share pages (a common prompt);
+ * entries past a sequence's rows are not read.
  *
- * Tables, lengths, rows and positions are device data. One out of range is
- * never used as an address: what it names is replaced by the pool's first page
- * (a bad length by 0, a bad token is left out), the results for that sequence
- * hold no meaning, and the next krh_sync reports ML_E_SHAPE.
+ * Tables, lengths, rows and positions are device data. One out of range is never
+ * used as an address: the pool's first page stands in for what it names (length
+ * 0 for a bad length; a bad token is left out), the results of that sequence hold
+ * no meaning, and the next krh_sync reports ML_E_SHAPE.
  *
  * Every call works on the library stream, allocates nothing, and can be captured
  * into a graph. A workspace holds nothing between calls: calls on the one
@@ -359,75 +359,81 @@ typedef struct {
     int head_dim;       /* a multiple of 8, 8 to 256 */
 } krh_pages;
 /* The rows of ntok tokens into their pages: token t is row row[t] of sequence
- * seq[t], at position pos[t]. Query heads q (t * ldq; ldqo in qo) and key heads k are
- * RMS-normalized with q_norm / k_norm when those are non-NULL, and rotated by row pos[t] of
- * the n_pos-row tables when cos_t is non-NULL (krh_heads_norm_rope; head_dim /
- * 2 floats a row); keys and values are converted as krh_store_kv does (F32 as they are). The
- * same bits as those calls, but that the norm's sum of squares is formed in 64
- * bits instead of in index order in 32, and a Q8 row's factor as 127 times the
- * reciprocal of its maximum instead of their quotient (an element next to a border
- * may round to its other side). n_heads 0: no queries (q, qo unused); qo may be q. q, qo,
- * k, v, the norms and tables 16-byte aligned, row strides multiples of 4; the rows
- * of a call are distinct. pos may be NULL without tables. */
+ * seq[t], at position pos[t]. Query heads q (t * ldq; ldqo in qo) and key heads k
+ * (t * ldk) are RMS-normalized with q_norm / k_norm when those are non-NULL, and
+ * rotated by row pos[t] of the n_pos-row tables (head_dim / 2 floats a row) when
+ * cos_t is non-NULL, as krh_heads_norm_rope does; keys and values (t * ldv) are
+ * converted as krh_store_kv does (F32 as they are). The same bits as those calls
+ * but for two: the norm's sum of squares is formed in 64 bits instead of in index
+ * order in 32, and a Q8 row's factor as 127 times the reciprocal of its maximum
+ * instead of their quotient (an element next to a border may round to its other
+ * side). n_heads 0: no queries (q, qo unused). qo may be q; nothing else
+ * overlaps. pos may be NULL without tables. The rows of a call are distinct. q,
+ * qo, k, v, the norms and the tables 16-byte aligned, row strides multiples of 4. */
 void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const int *table, int table_ld, int n_seq,
                    const float *q, size_t ldq, const float *k, size_t ldk, const float *v, size_t ldv, int ntok,
                    int n_heads, const int *seq, const int *row, const int *pos, const float *q_norm,
                    const float *k_norm, float eps, const float *cos_t, const float *sin_t, int n_pos);
-/* Rows back as floats: k, v (n * ldk, n * ldv; [n_kv_heads][head_dim] a row) of row
- * row[i] of sequence seq[i], i < n; a bad one gets zeros. Alignment as above. */
+/* Rows back as floats: k, v (i * ldk, i * ldv; [n_kv_heads][head_dim] a row) of
+ * row row[i] of sequence seq[i], i < n; a bad one gets zeros. Alignment as above. */
 void krh_paged_load(float *k, size_t ldk, float *v, size_t ldv, const krh_pages *kv, const int *table, int table_ld,
                     int n_seq, int n, const int *seq, const int *row);
-/* Bytes of workspace that krh_paged_attention takes for these sizes (0 for
- * sizes that it refuses); mass: whether it is given a mass array. */
+/* Bytes of workspace that krh_paged_attention takes for these sizes and any
+ * window (0 for sizes that it refuses); mass: whether it is given a mass array. */
 size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int max_len, int mass);
 /* Attention of one new token of each sequence, its last row: o, q [n_seq]
- * [n_heads * head_dim]. Sequence s attends its len[s] rows, or with window > 0
- * the last window ones: softmax of scale * (q . K), soft-capped first (cap *
- * tanh(score / cap)) when softcap > 0, over V. A sequence of no rows gets
- * zeros. Scores, sums and weights are held in 32 bits; the cache's length is
- * split over the chip and the parts joined, so sums are not in the order of
- * krh_attention_kv (and a Q8 cache's queries stay unquantized): results agree
- * to rounding, and are the same from call to call. Values attended that are not finite
- * give results that are not finite, for the heads that they reach.
- * len[s] <= max_len <= 2^29, which sizes the launch; o overlaps no input. mass (nullable): mass[(s *
- * n_kv_heads + h) * mass_ld + r] += the sum of row r's weights over the query
- * heads of KV head h. At most 16 query heads a KV head; q, o and ws 16-byte aligned. */
+ * [n_heads * head_dim], o apart from every input. Sequence s attends its len[s]
+ * rows, or with window > 0 the last window ones: softmax of scale * (q . K),
+ * soft-capped first (cap * tanh(score / cap)) when softcap > 0, over V. A
+ * sequence of no rows gets zeros. len[s] <= max_len <= 2^29, which sizes the
+ * launch. At most 16 query heads a KV head; q, o and ws 16-byte aligned.
+ *
+ * Scores, sums and weights are held in 32 bits, a Q8 cache's queries unquantized.
+ * The rows are split over the chip and the parts joined, so sums are not in the
+ * order of krh_attention_kv: results agree to rounding, and are the same from
+ * call to call. Values attended that are not finite give results that are not
+ * finite, for the heads that they reach; rows not attended may hold anything.
+ *
+ * mass (nullable): mass[(s * n_kv_heads + h) * mass_ld + r] += the sum of row r's
+ * weights over the query heads of KV head h, for the rows attended. */
 void krh_paged_attention(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len, int n_seq,
                          const float *q, int n_heads, int max_len, int window, float scale, float softcap,
                          float *mass, size_t mass_ld, void *ws);
 /* Bytes of workspace that krh_paged_evict takes */
 size_t krh_paged_evict_ws(int n_seq, int n_kv_heads, int keep);
-/* Eviction by accumulated weight: of sequence s's len[s] rows each KV head
- * keeps the last `recent` and the keep - recent with the largest mass of the
- * others (equal masses: the lower row; a NaN counts as the largest), and a sequence of at most `keep` rows
- * keeps all. The kept rows go, in their order, to rows 0.. of the sequence in the
- * pages of out_table, which no table of the call names; out_len[s] = min(len[s], keep),
- * and out_mass (rows of out_ld >= keep) receives the kept masses, then zeros as far as the row and the larger of
- * keep and max_len go.
- * out_len may be len, and out_mass mass where out_ld is mass_ld. Heads keep different rows; every
- * head has the same number. */
+/* Eviction by accumulated weight. Of sequence s's len[s] <= max_len <= 2^29 rows
+ * each KV head keeps the last `recent` and the keep - recent with the largest
+ * mass of the others (equal masses: the lower row; a NaN counts as the largest);
+ * a sequence of at most `keep` rows keeps all. Heads keep different rows, each
+ * head the same number. The kept rows go, in their order, to rows 0.. of the
+ * sequence in the pages of out_table, which no table of the call names. out_len[s]
+ * = min(len[s], keep), and out_mass (rows of out_ld >= keep) receives the kept
+ * masses, then zeros as far as the row and the larger of keep and max_len go.
+ * out_len may be len, and out_mass mass where out_ld is mass_ld. */
 void krh_paged_evict(const krh_pages *kv, const int *table, int table_ld, const int *len, const float *mass,
                      size_t mass_ld, int n_seq, int max_len, int keep, int recent, const int *out_table,
                      int out_table_ld, int *out_len, float *out_mass, size_t out_ld, void *ws);
 
 /* ---- rules on a batch of logit rows ----
- * What a caller asks of the next token, before krh_sample or krh_argmax draws
- * it (the sampler's own penalty, model/sampler.c:39-48, looks back over one
- * sequence's last ids only). A device array, one a row: */
+ * No counterpart in the reference but the sampler's own penalty
+ * (model/sampler.c:39-48), which looks back over one sequence's last ids: what a
+ * caller asks of the next token, before krh_sample or krh_argmax draws it. A
+ * device array, one a row: */
 typedef struct {
     float repeat;       /* ids seen: a positive logit over it, any other times it (1: off) */
     float presence;     /* taken off an id seen at all (0: off) */
     float frequency;    /* taken off once for each time an id was seen (0: off) */
     int mask;           /* this row's token mask, or -1 */
 } krh_logit_rule;
-/* out[r][i] (r * ldo) for the n logits of each row (r * ld), in this order:
- * the penalties for the ids of seen[r][0 .. n_seen[r]) (r * seen_ld); plus the
- * bias of id i (bias_id, bias: r * bias_ld, n_bias[r] pairs; the last of an
- * id's pairs holds); minus infinity where bit i % 32 of masks[mask][i / 32] is
- * clear (n_masks rows of (n + 31) / 32 words). Ids outside [0, n) are passed
- * over, as the sampler passes over them; counts outside [0, seen_ld] and [0, bias_ld] and masks outside
- * [-1, n_masks) are errors that krh_sync reports (counts taken as 0, masks as none). seen, bias_id and masks may be
- * NULL (with n_masks 0): none. out may be logits where ldo is ld. */
+/* out[r][i] (r * ldo) for the n logits of each row (r * ld), in this order: the
+ * penalties for the ids of seen[r][0 .. n_seen[r]) (r * seen_ld); plus the bias of
+ * id i (bias_id, bias: r * bias_ld, n_bias[r] pairs; the last of an id's pairs
+ * holds); minus infinity where bit i % 32 of masks[mask][i / 32] is clear (n_masks
+ * rows of (n + 31) / 32 words). Ids outside [0, n) are passed over, as the sampler
+ * passes over them. Counts outside [0, seen_ld] and [0, bias_ld] and masks outside
+ * [-1, n_masks) are errors that the next krh_sync reports (counts taken as 0,
+ * masks as none). seen, bias_id, and masks with n_masks 0, may be NULL: none. out
+ * may be logits where ldo is ld. Allocates nothing; can be captured. */
 void krh_logit_rules(float *out, size_t ldo, const float *logits, size_t ld, int n, int rows,
                      const krh_logit_rule *rule, const int *seen, size_t seen_ld, const int *n_seen,
                      const int *bias_id, const float *bias, size_t bias_ld, const int *n_bias, const uint32_t *masks,

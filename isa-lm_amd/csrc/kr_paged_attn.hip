@@ -731,17 +731,19 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
         if (r0 + k * PJ_T + tid < sp.len) mass[at[k]] = old[k] + sum[k];
 }
 
-// Shares in all, of every KV head: a wave a SIMD, which has the next tile's
-// rows under way. 8-bit rows of up to 64 dims take three, their waves work more and
-// read less. Fewer where the rows are few: a share is worth PA_BYTES of K and V at
-// least (halves: twice that). The lengths are the device's, so this is what
-// they may be at most.
-// Measured (us, 1024 / 2048 / 3072 waves): 8B shape, 16 sequences 28.9 / 34.6 /
-// 35.5, one of 120,001 rows 95 / 101 / 108; 8 bits, 24 sequences of 64 dims 28.7 /
-// 26.8 / 26.2 and with the mass 45.4 / 40.2 / 35.7, of 128 dims 27.3 / 31.3 / 34.1.
+// Shares in all, of every KV head: three waves a CU, which have the next tile's
+// rows under way, keep HBM busy. 8-bit rows, which take a tile's work to read half
+// as much, have four, and twelve up to 64 dims. Fewer where the rows are few: a
+// share is worth PA_BYTES of K and V at least (halves: twice that). The lengths
+// are the device's, so this is what they may be at most.
+// Measured from HBM (us, 512 / 768 / 1024 / 2048 / 3072 waves): 8B shape, halves, 16
+// sequences 32.8 / 32.8 / 33.0 / 37.6 / 40.5, 64 129.6 / 129.5 / 132.8 / 136.0 / 140.5,
+// one of 120,001 rows 91.7 / 92.0 / 94.8 / 101.6 / 108.3; 8 bits, 24 sequences of 64 dims
+// 46.0 / 36.9 / 32.0 / 30.4 / 30.6 and with the mass 57.6 / 47.2 / 49.3 / 46.2 / 42.9,
+// 16 of 128 dims 34.0 / 29.7 / 29.2 / 33.2 / 36.7.
 // 16 / 32 KB: halves, one sequence of 4000 rows 14.6 / 12.4; floats of 48 dims, 8
 // of up to 250 9.8 / 11.6; 8 bits of 48 dims, 16 of up to 8000 17.4 / 19.8.
-constexpr int PA_WAVES = 1024, PA_BYTES = 16 * 1024;
+constexpr int PA_CUS = 256, PA_BYTES = 16 * 1024;
 int pa_least(const krh_pages *kv) {
     const bool f16 = kv->kv_type == ML_F16;
     const int tile = 2 * pa_tile(kv->head_dim) * kv->head_dim * (f16 ? 2 : kv->kv_type == ML_F32 ? 4 : 1);
@@ -750,7 +752,7 @@ int pa_least(const krh_pages *kv) {
 }
 int pa_shares(const krh_pages *kv, int n_seq, int rows) {
     const long long tile = pa_tile(kv->head_dim), tiles = n_seq * ((rows + tile - 1) / tile), least = pa_least(kv);
-    const int waves = kv->kv_type == ML_Q8_0 && kv->head_dim <= 64 ? 3 * PA_WAVES : PA_WAVES;
+    const int waves = PA_CUS * (kv->kv_type != ML_Q8_0 ? 3 : kv->head_dim > 64 ? 4 : 12);
     const long long most = (tiles + least - 1) / least, want = waves / kv->n_kv_heads;
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }

@@ -574,6 +574,35 @@ def test_evict(dev, kv_type, hd, kind, keep, recent, inplace):
         assert np.array_equal(got[name].view(np.uint8), want[name].view(np.uint8)), name
 
 
+@pytest.mark.parametrize("kind", ["spread", "ties", "equal", "odd"])
+@pytest.mark.parametrize("keep,recent", [(6000, 100), (1, 1), (1, 0), (19999, 5)])
+def test_evict_many_rows(dev, kind, keep, recent):
+    """more rows of one first digit than a wave holds apart, and fewer"""
+    rng = np.random.default_rng(keep)
+    lens, nkv, page, hd = [20000, 9001], 2, 64, 8
+    kept = [min(n, keep) for n in lens]
+    p = Pool(dev, rng, K.ML_F16, lens, page, nkv, hd, spare=sum(-(-n // page) for n in kept))
+    out = np.full((2, -(-keep // page)), -1, np.int32)
+    free = list(p.free)
+    for i, n in enumerate(kept):
+        out[i, :-(-n // page)] = [free.pop() for _ in range(-(-n // page))]
+    p.put()
+    w = weights(rng, kind, (2, nkv, 20000))
+    nb, mb = dev.zeros(8), dev.zeros(2 * nkv * keep * 4)
+    K.hip.krh_paged_evict(p.ref, p.tab.ptr, p.ld, dev.put(i32(lens)).ptr, dev.put(w).ptr, 20000, 2, 20000, keep, recent,
+                          dev.put(out).ptr, out.shape[1], nb.ptr, mb.ptr, keep,
+                          dev.zeros(K.hip.krh_paged_evict_ws(2, nkv, keep)).ptr)
+    ok()
+    assert nb.get(np.int32, 2).tolist() == kept
+    om, got = mb.get(np.float32, 2 * nkv * keep).reshape(2, nkv, keep), p.get("k")
+    for i, n in enumerate(lens):
+        for g in range(nkv):
+            r = evicted(w[i, g], n, keep, recent)
+            j = np.arange(len(r))
+            assert np.array_equal(bits(om[i, g, :len(r)]), bits(w[i, g, r])) and (om[i, g, len(r):] == 0).all()
+            assert np.array_equal(got[out[i, j // page], g, j % page], p.a["k"][p.table[i, r // page], g, r % page])
+
+
 def test_evict_bad(dev):
     """a length or a new page out of range is reported; the other sequences are as they should be"""
     rng = np.random.default_rng(1)
@@ -609,7 +638,7 @@ def rules(x, n, rep, pre, frq, seen, bias, bits_):
 
 
 @pytest.mark.parametrize("n,rows,seen_ld,bias_ld,n_masks", [(1, 1, 1, 1, 1), (31, 2, 5, 3, 1), (33, 1, 0, 0, 0), (4096, 3, 700, 40, 2),
-                                                            (4097, 2, 64, 0, 3), (32000, 4, 70, 5, 0), (151936, 5, 9000, 300, 4),
+                                                            (4097, 2, 64, 0, 3), (32000, 4, 70, 5, 0), (151936, 5, 9000, 300, 4), (5000, 2, 2049, 1500, 1),
                                                             (50001, 70, 300, 17, 8)])
 @pytest.mark.parametrize("inplace", [False, True])
 def test_rules(dev, n, rows, seen_ld, bias_ld, n_masks, inplace):
@@ -676,6 +705,55 @@ def test_rules_bad_counts(dev):
         assert K.hip.krh_sync() == K.ML_E_SHAPE
         K.hip.krh_clear_error()
         assert np.array_equal(bits(ob.get(np.float32, 400)), bits(x).reshape(-1))
+
+
+def test_captured_as_eager(dev):
+    """attention with its mass, eviction and the rules in one graph over one workspace, replayed with other inputs and
+    with eager calls over the same workspace between: each replay gives what the calls give"""
+    rng = np.random.default_rng(21)
+    S, nh, nkv, hd, page, ml, n = 3, 8, 2, 64, 16, 700, 4100
+    lens = [700, 33, 400]
+    p = Pool(dev, rng, K.ML_F16, lens, page, nkv, hd, spare=3 * 4)
+    out = np.full((S, 4), -1, np.int32)
+    for i, v in enumerate(lens):
+        out[i, :-(-min(v, 50) // page)] = p.free[4 * i:4 * i + -(-min(v, 50) // page)]
+    p.put()
+    lb, ub, qb = dev.put(i32(lens)), dev.put(out), dev.zeros(S * nh * hd * 4)
+    rule = (K.LogitRule * S)(*[K.LogitRule(1.3, 0.2, 0.1, -1)] * S)
+    rb, seen, ns, xb = dev.put(np.frombuffer(bytes(rule), np.uint8)), dev.put(i32(rng.integers(0, n, (S, 90)))), dev.put(
+        i32([90, 0, 40])), dev.zeros(S * n * 4)
+    ws = dev.zeros(max(K.hip.krh_paged_attention_ws(p.ref, S, nh, ml, 1), K.hip.krh_paged_evict_ws(S, nkv, 50)))
+    m0 = dev.put(f32(rng.random((S, nkv, ml))))
+
+    def outputs():
+        return [dev.zeros(v) for v in (S * nh * hd * 4, S * nkv * ml * 4, 4 * S, S * nkv * 50 * 4, S * n * 4)]
+
+    def calls(o, m, ln, om, y):
+        K.hip.krh_copy_d2d_async(m.ptr, m0.ptr, m.nbytes)
+        K.hip.krh_paged_attention(o.ptr, p.ref, p.tab.ptr, p.ld, lb.ptr, S, qb.ptr, nh, ml, 0, 0.125, 0.0, m.ptr, ml, ws.ptr)
+        K.hip.krh_paged_evict(p.ref, p.tab.ptr, p.ld, lb.ptr, m.ptr, ml, S, ml, 50, 10, ub.ptr, 4, ln.ptr, om.ptr, 50, ws.ptr)
+        K.hip.krh_logit_rules(y.ptr, n, xb.ptr, n, n, S, rb.ptr, seen.ptr, 90, ns.ptr, None, None, 0, None, None, 0)
+
+    a, b = outputs(), outputs()
+    calls(*a)
+    ok()
+    g = C.c_void_p()
+    K.check(K.hip.krh_graph_begin())
+    calls(*b)
+    K.check(K.hip.krh_graph_end(C.byref(g)))
+    for _ in range(4):
+        q, x = f32(rng.standard_normal((S, nh, hd))), f32(rng.standard_normal((S, n)))
+        for buf, v in ((qb, q), (xb, x)):
+            K.check(K.hip.krh_copy_h2d(buf.ptr, v.ctypes.data, v.nbytes))
+        K.check(K.hip.krh_graph_launch(g))
+        ok()
+        pages = [p.get(v).copy() for v in "kv"]
+        calls(*a)
+        ok()
+        for u, v in zip(a, b):
+            assert np.array_equal(u.get(np.uint8, u.nbytes), v.get(np.uint8, v.nbytes))
+        assert all(np.array_equal(u, p.get(v)) for u, v in zip(pages, "kv"))
+    K.hip.krh_graph_free(g)
 
 
 @pytest.mark.parametrize("kv_type", TYPES)
