@@ -40,6 +40,9 @@ namespace {
 // Rows of a tile: 32, and 16 for heads past 128 dims, whose rows fill the registers
 constexpr int pa_tile(int hd) { return hd > 128 ? 16 : 32; }
 constexpr float PA_UP = 14.0f;     // the weights' scale (log2; halves end at 2^16)
+// the least power of two that 8-bit rows' weights and sums are over: with it a
+// sum of 2^29 weights stays within 32 bits, and the scale 0 of rows of zeros has one
+constexpr int PA_EV = -80;
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
@@ -225,7 +228,8 @@ template <int KT, int CL, bool FULL> struct PaWave {
     int ids;   // the pages of 64 half tiles from t_ids on, one a lane
     std::conditional_t<HALF, half8, float4v> qf[KS][NB];   // the queries as operands
     float cs, m_run, l_run;
-    int ev;    // Q8: the weights carry the V scales over 2^ev
+    int ev;        // Q8: weights and sums are over 2^ev,
+    float v_end;   // which all V scales so far are below
     float4v o[W];
 
     __device__ __forceinline__ PaWave(const PgView &p_, const PaArgs &a_, int kvh_)
@@ -411,28 +415,30 @@ template <int KT, int CL, bool FULL> struct PaWave {
 #pragma unroll
             for (int i = 0; i < R; i += 4) *(float4v *)(z + i) = float4v{ sc[i], sc[i + 1], sc[i + 2], sc[i + 3] };
         }
-        m_tile = pa_max_g(m_tile);
-        int ev_new = ev;
+        // The maximum, one for a column's four lanes, moves where a lane has a
+        // larger score; with it what the weights are scaled by, for the 8-bit
+        // rows' scales that they carry to end in halves: 2^-ev, in the sums too.
+        float v_tile = 0.0f;
         if constexpr (KT == PG_Q8) {
-            float vm = 0.0f;
 #pragma unroll
-            for (int i = 0; i < R; i++) vm = fmaxf(vm, fabsf(raw.vd[i]));
-            vm = pa_max_g(vm);
-            ev_new = max(ev, min((int)(__float_as_uint(vm) >> 23) - 126, 120));
+            for (int i = 0; i < R; i++) v_tile = fmaxf(v_tile, fabsf(raw.vd[i]));
         }
-        if (__any(m_tile > m_run || ev_new > ev)) {
-            const float m_new = fmaxf(m_run, m_tile);
-            const float f = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-            const float fo = KT == PG_Q8 ? ldexpf(f, ev - ev_new) : f;
+        if (__any(m_tile > m_run || (KT == PG_Q8 && v_tile >= v_end))) {
+            const float m_new = fmaxf(m_run, pa_max_g(m_tile));
+            float f = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+            if constexpr (KT == PG_Q8) {
+                const int e = max(ev, min((int)(__float_as_uint(pa_max_g(v_tile)) >> 23) - 126, 120));   // v_tile < 2^e
+                f = ldexpf(f, ev - e);
+                ev = e;
+                v_end = ldexpf(1.0f, ev);
+            }
             m_run = m_new;
-            ev = ev_new;
             l_run *= f;
 #pragma unroll
-            for (int c = 0; c < W; c++) o[c] *= fo;
+            for (int c = 0; c < W; c++) o[c] *= f;
         }
         // weights of no finite maximum: 0 for -inf, NaN for NaN
-        const float base = (m_run == -INFINITY ? 0.0f : m_run) - (HALF ? PA_UP : 0.0f);
-        const float vs = KT == PG_Q8 ? ldexpf(1.0f, -ev) : 1.0f;
+        const float base = (m_run == -INFINITY ? 0.0f : m_run) - (HALF ? PA_UP - (float)(KT == PG_Q8 ? ev : 0) : 0.0f);
         // the weights as operands: R halves, or floats
         typedef _Float16 halfr __attribute__((ext_vector_type(R)));
         typedef unsigned uintr __attribute__((ext_vector_type(R / 2)));
@@ -446,7 +452,7 @@ template <int KT, int CL, bool FULL> struct PaWave {
                 // a rounded product: left to itself the compiler rounds it to a
                 // half twice, once from the exact product, and at a tie the hi
                 // that is multiplied is not the one taken off for lo
-                x *= raw.vd[i] * vs;
+                x *= raw.vd[i];
                 asm("" : "+v"(x));
             }
             if constexpr (HALF) {
@@ -550,7 +556,8 @@ template <int KT, int CL, bool FULL> struct PaWave {
     __device__ __forceinline__ void part(int t, int end, size_t slot) {
         m_run = -INFINITY;
         l_run = 0.0f;
-        ev = -120;
+        ev = PA_EV;
+        v_end = 0.0f;
 #pragma unroll
         for (int c = 0; c < W; c++) o[c] = float4v{ 0, 0, 0, 0 };
         const bool alone = t == 0 && end == sp.tiles;
@@ -562,9 +569,8 @@ template <int KT, int CL, bool FULL> struct PaWave {
                 pass(r, min(r1, r + (64 / NT) * TILE), r == r0);
             }
         }
-        const float l = pa_sum_g(l_run);
-        float f = alone ? 1.0f / l : 1.0f;
-        if (KT == PG_Q8) f = ldexpf(f, ev);
+        const float s = pa_sum_g(l_run), l = KT == PG_Q8 ? ldexpf(s, ev) : s;
+        float f = alone ? 1.0f / s : KT == PG_Q8 ? ldexpf(1.0f, ev) : 1.0f;
         if (sp.len == 0) f = 0.0f;
         if (g == 0 && live && (!alone || a.z)) {
             *(float2v *)(a.pml + (slot * group + n) * 2) = float2v{ m_run, l };

@@ -204,6 +204,39 @@ def test_attention_scales(dev, kv_type, kscale, vscale, peak):
 
 
 @pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("ml", [100, 3000])
+def test_attention_rows_of_zeros(dev, kv_type, ml):
+    """values of zeros, whose 8-bit scale is 0, in all rows of a sequence, in its first ones or in some; and scales far
+    apart"""
+    rng = np.random.default_rng(31)
+    lens = [100, 90, 64, 77, 3000 if ml == 3000 else 50]
+    p = Pool(dev, rng, kv_type, lens, 16, 2, 64)
+    for i, rows in enumerate([range(100), range(40), range(0, 64, 3), [], []]):
+        for r in rows:
+            at = (p.table[i, r // 16], slice(None), r % 16)
+            p.a["v"][at] = 0
+            if kv_type == K.ML_Q8_0:
+                p.a["vd"][at] = 0
+    if kv_type == K.ML_Q8_0:
+        p.a["vd"][p.table[3, :3]] *= np.float32(2.0 ** -60)
+        p.a["vd"][p.table[4, :2]] *= np.float32(2.0 ** 40)
+    p.put()
+    S, nh = len(lens), 6
+    q = f32(rng.standard_normal((S, nh, 64)))
+    ob, ws = dev.zeros(q.nbytes), dev.zeros(K.hip.krh_paged_attention_ws(p.ref, S, nh, ml, 0))
+    K.hip.krh_paged_attention(ob.ptr, p.ref, p.tab.ptr, p.ld, dev.put(i32(lens)).ptr, S, dev.put(q).ptr, nh, ml, 0, 0.125,
+                              0.0, None, 0, ws.ptr)
+    ok()
+    o = ob.get(np.float32, q.size).reshape(q.shape)
+    assert (o[0] == 0).all()
+    for i, n in enumerate(lens):
+        k, v = p.rows("k", i, n), p.rows("v", i, n)
+        for h in range(nh):
+            w, _, bound, _ = attention(q[i, h].astype(np.float64), k[:, h // 3], v[:, h // 3], 0.125, 0, 0)
+            assert (np.abs(o[i, h] - w) <= bound).all(), (i, h)
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
 def test_attention_many_sequences(dev, kv_type):
     rng = np.random.default_rng(5)
     check_attention(dev, kv_type, 4, 2, 64, 16, list(rng.integers(0, 400, 70)), mass=True)
