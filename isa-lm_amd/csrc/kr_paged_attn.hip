@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
 // as much, have four, and twelve up to 64 dims. Fewer where the rows are few: a
 // share is worth PA_BYTES of K and V at least (halves: twice that). The lengths
 // are the device's, so this is what they may be at most.
-// Measured from HBM (us, 512 / 768 / 1024 / 2048 / 3072 waves): 8B shape, halves, 16
+// Measured from HBM (us, 2 / 3 / 4 / 8 / 12 waves a CU): 8B shape, halves, 16
 // sequences 32.8 / 32.8 / 33.0 / 37.6 / 40.5, 64 129.6 / 129.5 / 132.8 / 136.0 / 140.5,
 // one of 120,001 rows 91.7 / 92.0 / 94.8 / 101.6 / 108.3; 8 bits, 24 sequences of 64 dims
 // 46.0 / 36.9 / 32.0 / 30.4 / 30.6 and with the mass 57.6 / 47.2 / 49.3 / 46.2 / 42.9,
