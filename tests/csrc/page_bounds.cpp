@@ -6,7 +6,8 @@
 #include <climits>
 #include <cstdio>
 #include <cstdlib>
-#include <vector>
+#include <sys/mman.h>
+#include <unistd.h>
 
 static unsigned long long st = 88172645463325252ull;
 static unsigned rnd() {
@@ -18,14 +19,18 @@ static unsigned rnd() {
 
 int main(int argc, char **argv) {
     const int trials = argc > 1 ? atoi(argv[1]) : 100000;
+    // a page with nothing behind it, nor before it: a read past a table that ends there faults
+    const size_t ps = (size_t)sysconf(_SC_PAGESIZE);
+    char *map = (char *)mmap(nullptr, 3 * ps, PROT_NONE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
+    if (map == MAP_FAILED || mprotect(map + ps, ps, PROT_READ | PROT_WRITE)) return 9;
     const int odd[] = { INT_MIN, -1, 0, 1, INT_MAX, 1 << 30, 65536 };
     for (int i = 0; i < trials; i++) {
         const int shift = 4 + rnd() % 7, ld = 1 + rnd() % 9, n_pages = 1 + rnd() % 20, n_kv = 1 + rnd() % 8;
-        std::vector<int> table(ld);   // exactly ld entries: a read past them is the sanitizer's to find
-        for (int &v : table) v = rnd() % 4 ? (int)(rnd() % n_pages) : odd[rnd() % 7] + (int)(rnd() % 3 == 0 ? n_pages : 0u);
+        int *table = (int *)(i & 1 ? map + ps : map + 2 * ps - ld * sizeof(int));
+        for (int j = 0; j < ld; j++) table[j] = rnd() % 4 ? (int)(rnd() % n_pages) : odd[rnd() % 7] + (int)(rnd() % 3 == 0 ? n_pages : 0u);
         const int row = rnd() % 3 ? (int)(rnd() % (unsigned)((ld + 1) << shift)) : INT_MAX - (int)(rnd() % 100);
         int bad = 0;
-        const int id = kr_page_of(table.data(), ld, row, shift, n_pages, bad);
+        const int id = kr_page_of(table, ld, row, shift, n_pages, bad);
         const bool good = (row >> shift) < ld && table[row >> shift] >= 0 && table[row >> shift] < n_pages;
         const int kvh = rnd() % n_kv;
         const size_t at = kr_page_row(id, n_kv, kvh, shift, row), rows = ((size_t)n_pages * n_kv) << shift;
