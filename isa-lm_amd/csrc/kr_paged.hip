@@ -209,6 +209,11 @@ __device__ __forceinline__ unsigned ev_key(float w) {
     return w != w ? 0xffffffffu : u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
 
+// and back, where it was no NaN and no -0
+__device__ __forceinline__ float ev_weight(unsigned u) {
+    return __uint_as_float(u ^ ((unsigned)((int)~u >> 31) | 0x80000000u));
+}
+
 constexpr int EV_T = 1024, EV_W = EV_T / 64, EV_D = 11, EV_B = 1 << EV_D;   // radix digits of 11, 11 and 10 bits
 constexpr int EV_U = 8;   // rows a lane reads ahead
 
@@ -227,12 +232,10 @@ struct EvArgs {
     float *w;   // [n_seq][n_kv][keep]: their weights
 };
 
-// Sums of a count over the waves before this one; all of them read at once
+// Sums of a count over the waves before this one
 __device__ __forceinline__ int ev_before(const int *s, int wave) {
-    int sum = 0;
-#pragma unroll
-    for (int i = 0; i < EV_W; i++) sum += i < wave ? s[i] : 0;
-    return sum;
+    const int sum = pg_scan(s[threadIdx.x & (EV_W - 1)]);
+    return wave ? __builtin_amdgcn_readlane(sum, wave - 1) : 0;
 }
 
 // Rows r0 .. r1 - 1, EV_U x 64 at a time, a lane's reads side by side
@@ -254,6 +257,11 @@ template <class F> __device__ __forceinline__ void ev_rows(const float *mass, in
 #pragma unroll
     for (int k = 0; k < EV_U; k++)
         if (r + 64 * k < r1) f(r + lane + 64 * k, r + lane + 64 * k < r1, w[k]);
+}
+
+// How many of the lanes below this one are in `m`
+__device__ __forceinline__ int ev_below(unsigned long long m) {
+    return __builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0));
 }
 
 // From the heaviest digit down: the one where the counts' sum reaches `need`,
@@ -281,8 +289,9 @@ __device__ __forceinline__ void ev_digit(int *hist, int *s_sum, int *s_res, int 
 // lowest row on. Each wave has an even part of the rows. The rows with the
 // first digit's bits go to LDS, where they are few (each wave up to EV_C), and the
 // other digits look at those. Bound by the one CU's instructions, three passes over
-// the rows: 32,001 rows, 8 workgroups, 102 us with one lane looking through the
-// counts and barriers every 1024 rows; 45 with five passes over all rows.
+// the rows: 8 workgroups, 60,000 rows 32 us, 120,000 65; 32,001 rows 23.4, 102 with
+// one lane looking through the counts and barriers every 1024 rows, 45 with five
+// passes over all rows.
 constexpr int EV_C = 512;
 __global__ void __launch_bounds__(EV_T) k_evict_select(const EvArgs a, int *fault) {
     __shared__ int hist[EV_B];
@@ -396,6 +405,148 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(const EvArgs a, int *faul
         ties += __popcll(bt);
         at += __popcll(bk);
     });
+}
+
+__device__ __forceinline__ unsigned ev_load(__amdgpu_buffer_rsrc_t rows, int r, int k) {
+    return __builtin_amdgcn_raw_buffer_load_b32(rows, r * 4 + k * 256, 0, 0);
+}
+
+// The same where all rows but the recent ones fit LDS, by their keys: one pass
+// over the weights, the others over LDS. A launch on few rows is bound by its
+// code's way from memory, so there is one copy for all digits and none for
+// tails: rows past the last have the key 0, below any weight's. On many it is
+// bound by the CU's instructions, 10 or so a row: 32,001 rows, 8 workgroups, 16.5
+// us (the select above: 23.4); 16 sequences of up to 4096, 7.6 (10.9).
+template <int R> __global__ void __launch_bounds__(EV_T) k_evict_select_lds(const EvArgs a, int *fault) {
+    __shared__ int hist[EV_B];
+    __shared__ unsigned s_key[R];
+    __shared__ int s_sum[EV_W], s_res[2], s_odd[EV_W], s_take[EV_W], s_tie[EV_W];
+    const int kvh = blockIdx.x, s = blockIdx.y, n_kv = gridDim.x, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int bad = 0;
+    const int len = __builtin_amdgcn_readfirstlane(kr_page_len(a.len[s], a.max_len, bad));
+    for (int i = tid; i < EV_B; i += EV_T) hist[i] = 0;
+    if (tid == 0) kr_report(fault, bad);
+    const size_t sh = (size_t)s * n_kv + kvh;
+    const float *mass = a.mass + sh * a.mass_ld;
+    int *idx = a.idx + sh * a.keep;
+    float *ow = a.w + sh * a.keep;
+    const int kept = min(len, a.keep), old = len <= a.keep ? 0 : len - a.recent, want = kept - (len - old);
+    if (kvh == 0 && tid == 0) a.cnt[s] = kept;
+#pragma unroll 1
+    for (int r = tid; r < len - old; r += EV_T) {
+        idx[want + r] = old + r;
+        ow[want + r] = mass[old + r];
+    }
+    if (want == 0) return;   // 0 < want < old after this
+    constexpr int N = 4, B = 64 * N;   // 256 rows at a time: 512 left waves idle (17.2, 8.3 us)
+    const int part = ((old + EV_W - 1) / EV_W + B - 1) / B * B, r0 = wave * part, r1 = min(r0 + part, (old + B - 1) / B * B);
+    __syncthreads();
+    // zeros, which rows that no head looks at all have, count together
+    int zeros = 0, odd = 0;   // odd: weights that their keys do not give back
+    const auto rows = __builtin_amdgcn_make_buffer_rsrc((void *)mass, 0, old * 4, 0x00020000);   // 0 past them
+    unsigned w[N], next[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) next[k] = ev_load(rows, r0 + lane, k);
+#pragma unroll 1
+    for (int r = r0; r < r1; r += B) {
+#pragma unroll
+        for (int k = 0; k < N; k++) w[k] = next[k];
+#pragma unroll
+        for (int k = 0; k < N; k++) next[k] = ev_load(rows, r + B + lane, k);
+        unsigned long long o = 0;
+#pragma unroll
+        for (int k = 0; k < N; k++)   // NaN, -0
+            o |= __builtin_amdgcn_ballot_w64(__builtin_amdgcn_classf(__uint_as_float(w[k]), 0x23));
+        if (__builtin_expect(o != 0, 0)) {
+#pragma unroll
+            for (int k = 0; k < N; k++) w[k] = w[k] << 1 > 0xff000000u ? 0x7fffffffu : w[k] == 0x80000000u ? 0 : w[k];
+            odd = 1;
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const unsigned u = w[k], key = u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+            s_key[r + lane + 64 * k] = key;
+            zeros += __popcll(__builtin_amdgcn_ballot_w64(u == 0));
+            if (u != 0) atomicAdd(&hist[key >> (32 - EV_D)], 1);
+        }
+    }
+    if (r1 > max(r0, old)) {   // rows past the last, read as zeros
+        zeros -= r1 - max(r0, old);
+        for (int r = max(r0, old) + lane; r < r1; r += 64) s_key[r] = 0;
+    }
+    if (lane == 0) {
+        if (zeros) atomicAdd(&hist[0x80000000u >> (32 - EV_D)], zeros);
+        s_odd[wave] = odd;
+    }
+    int need = want, digit;
+    unsigned prefix = 0;
+#pragma unroll 1
+    for (int b = 32 - EV_D;;) {   // bits 21 to 31, 10 to 20, 0 to 9
+        ev_digit(hist, s_sum, s_res, digit, need);
+        digit = __builtin_amdgcn_readfirstlane(digit);
+        prefix |= (unsigned)digit << b;
+        if (b == 0) break;
+        const int top = b;
+        b = max(0, b - EV_D);
+        const unsigned pre = prefix >> top, mask = (1u << (top - b)) - 1;
+#pragma unroll 1
+        for (int r = r0; r < r1; r += B) {
+            unsigned u[N];
+#pragma unroll
+            for (int k = 0; k < N; k++) u[k] = s_key[r + 64 * k + lane];
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (u[k] >> top == pre) atomicAdd(&hist[u[k] >> b & mask], 1);
+        }
+    }
+    // rows above `prefix`, and the first `need` of those at it
+    int take = 0, ties = 0;
+#pragma unroll 1
+    for (int r = r0; r < r1; r += B) {
+        unsigned u[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) u[k] = s_key[r + 64 * k + lane];
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            take += __popcll(__builtin_amdgcn_ballot_w64(u[k] > prefix));
+            ties += __popcll(__builtin_amdgcn_ballot_w64(u[k] == prefix));
+        }
+    }
+    if (lane == 0) {
+        s_take[wave] = take;
+        s_tie[wave] = ties;
+    }
+    __syncthreads();
+    ties = ev_before(s_tie, wave);
+    int at = ev_before(s_take, wave) + min(ties, need);
+    const bool give = !__any(s_odd[lane & (EV_W - 1)]);
+#pragma unroll 1
+    for (int r = r0; r < r1; r += B) {
+        unsigned u[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) u[k] = s_key[r + 64 * k + lane];
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const unsigned long long bt = __builtin_amdgcn_ballot_w64(u[k] == prefix);
+            bool got = u[k] >= prefix;
+            if (bt) {
+                if (ties + __popcll(bt) > need) got = got && (u[k] != prefix || ties + ev_below(bt) < need);
+                ties += __popcll(bt);
+            }
+            const unsigned long long bk = __builtin_amdgcn_ballot_w64(got);
+            if (got) {
+                const unsigned j = 4 * (at + ev_below(bk));
+                *(int *)((char *)idx + j) = r + 64 * k + lane;
+                *(float *)((char *)ow + j) = ev_weight(u[k]);
+            }
+            at += __popcll(bk);
+        }
+    }
+    if (give) return;
+    __syncthreads();
+#pragma unroll 1
+    for (int j = tid; j < want; j += EV_T) ow[j] = mass[idx[j]];
 }
 
 // Rows into the new pages, in units of U bytes, EM_ROWS a workgroup and KV
@@ -519,7 +670,13 @@ extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table
     const size_t rows = (size_t)n_seq * kv->n_kv_heads * keep;
     const EvArgs a = { len, mass, mass_ld, max_len, keep, recent, out_table, out_table_ld, out_len, out_mass, out_ld,
                        w + 2 * rows, w, (float *)(w + rows) };
-    hipLaunchKernelGGL(k_evict_select, dim3(kv->n_kv_heads, n_seq), dim3(EV_T), 0, kr_stream(), a, kr_fault_word());
+    // 40 KB of LDS leave room for a second workgroup on the CU: 64 sequences of up to 4000 rows, 9.4 us (136 KB: 12.7);
+    // past 32768 rows the weights are read three times: 60,000, 32 us
+    const int most_old = max_len - recent;
+    const auto select = most_old <= 8192    ? k_evict_select_lds<8192>
+                        : most_old <= 32768 ? k_evict_select_lds<32768>
+                                            : k_evict_select;
+    hipLaunchKernelGGL(select, dim3(kv->n_kv_heads, n_seq), dim3(EV_T), 0, kr_stream(), a, kr_fault_word());
     kr_check_launch("paged_evict");
     const int rb = kv->head_dim * (kv->kv_type == ML_F32 ? 4 : kv->kv_type == ML_F16 ? 2 : 1);
     const int most = keep < max_len ? keep : max_len;

@@ -636,6 +636,45 @@ def test_evict_many_rows(dev, kind, keep, recent):
             assert np.array_equal(got[out[i, j // page], g, j % page], p.a["k"][p.table[i, r // page], g, r % page])
 
 
+@pytest.mark.parametrize("rows", [65, 256, 257, 4097, 8192, 8193, 28001, 32768, 32769, 40000])
+@pytest.mark.parametrize("kind", ["zeros", "negative", "odd", "spread"])
+def test_evict_sizes(dev, rows, kind):
+    """rows that fill the select's LDS, one more and one less; a few weights among zeros, with as many rows kept as
+    are left then; no weight above zero; every row but one"""
+    rng = np.random.default_rng(rows)
+    nkv, page, hd, recent = 2, 64, 8, rows % 7
+    n = rows + recent
+    lens = [n, n - 1, n // 3, n // 17 + 2, n]
+    for keep in (recent + rows // 2, recent + rows - 1, recent + 1):
+        kept = [min(m, keep) for m in lens]
+        p = Pool(dev, rng, K.ML_F16, lens, page, nkv, hd, spare=sum(-(-m // page) for m in kept))
+        out = np.full((len(lens), -(-keep // page)), -1, np.int32)
+        free = list(p.free)
+        for i, m in enumerate(kept):
+            out[i, :-(-m // page)] = [free.pop() for _ in range(-(-m // page))]
+        p.put()
+        w = weights(rng, "spread" if kind == "negative" else kind, (len(lens), nkv, n)) if kind != "zeros" else (
+            np.where(rng.random((len(lens), nkv, n)) < 0.02, rng.random((len(lens), nkv, n)), 0).astype(np.float32))
+        if kind == "negative":
+            w = -np.abs(w)
+            w[:, :, ::5] = -0.0
+        w[4] = 0
+        nb, mb = dev.zeros(len(lens) * 4), dev.zeros(len(lens) * nkv * keep * 4)
+        K.hip.krh_paged_evict(p.ref, p.tab.ptr, p.ld, dev.put(i32(lens)).ptr, dev.put(w).ptr, n, len(lens), n, keep, recent,
+                              dev.put(out).ptr, out.shape[1], nb.ptr, mb.ptr, keep,
+                              dev.zeros(K.hip.krh_paged_evict_ws(len(lens), nkv, keep)).ptr)
+        ok()
+        assert nb.get(np.int32, len(lens)).tolist() == kept
+        om, got = mb.get(np.float32, len(lens) * nkv * keep).reshape(len(lens), nkv, keep), p.get("k")
+        for i, m in enumerate(lens):
+            for g in range(nkv):
+                r = evicted(w[i, g], m, keep, recent)
+                j = np.arange(len(r))
+                assert np.array_equal(bits(om[i, g, :len(r)]), bits(w[i, g, r])), (keep, i, g)
+                assert (om[i, g, len(r):] == 0).all()
+                assert np.array_equal(got[out[i, j // page], g, j % page], p.a["k"][p.table[i, r // page], g, r % page])
+
+
 def test_evict_bad(dev):
     """a length or a new page out of range is reported; the other sequences are as they should be"""
     rng = np.random.default_rng(1)
