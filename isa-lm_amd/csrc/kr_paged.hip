@@ -549,20 +549,23 @@ template <int R> __global__ void __launch_bounds__(EV_T) k_evict_select_lds(cons
     for (int j = tid; j < want; j += EV_T) ow[j] = mass[idx[j]];
 }
 
-// Rows into the new pages, in units of U bytes, EM_ROWS a workgroup and KV
-// head; their weights, and zeros past them. Bound by HBM: each row read once
-// and written once (16 sequences of up to 4096 rows, 8B shape, half kept: 4.3
-// TB/s; with four units a thread read before the first is written, 3.3).
-constexpr int EM_ROWS = 64;
-template <class U> __global__ void __launch_bounds__(PG_T) k_evict_move(const PgView p, const EvArgs a, int rb, int *fault) {
+// Rows into the new pages, in units of U bytes, as many rows a workgroup as its
+// threads have units; their weights, and zeros past them. Bound by HBM: each row
+// read once and written once (16 sequences of up to 4096 rows, 8B shape, half
+// kept: 4.6 TB/s; with four units a thread one after another 4.3, all read before
+// the first is written 3.3. Stores past the caches reach 5.0, but the attention
+// that reads the new pages next loses as much).
+constexpr unsigned EM_BLOCKS = 1 << 16;
+template <class U> __global__ void __launch_bounds__(PG_T) k_evict_move(const PgView p, const EvArgs a, int rb, int rows, int *fault) {
     const int s = blockIdx.z, kvh = blockIdx.y, per = rb / (int)sizeof(U), kept = a.cnt[s], tid = threadIdx.x;
     const size_t sh = (size_t)s * p.n_kv + kvh;
     const int *idx = a.idx + sh * a.keep, *ot = a.out_table + (size_t)s * a.out_ld;
     if (blockIdx.x == 0 && kvh == 0 && tid == 0) a.out_len[s] = kept;
     int bad = 0;
-    const int j0 = blockIdx.x * EM_ROWS, n = min(kept - j0, EM_ROWS) * per;
-    for (int e = tid; e < n; e += PG_T) {
-        const int j = j0 + e / per, u = e % per, r = idx[j];
+    for (int j0 = blockIdx.x * rows; j0 < kept; j0 += gridDim.x * rows) {
+        const int j = j0 + tid / per, u = tid % per;
+        if (tid >= rows * per || j >= kept) continue;
+        const int r = idx[j];
         int b = 0;
         const size_t from = kr_page_row(pg_page(p, s, r, b), p.n_kv, kvh, p.shift, r);
         const size_t to = kr_page_row(kr_page_of(ot, a.out_ld, j, p.shift, p.n_pages, b), p.n_kv, kvh, p.shift, j);
@@ -681,8 +684,11 @@ extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table
     const int rb = kv->head_dim * (kv->kv_type == ML_F32 ? 4 : kv->kv_type == ML_F16 ? 2 : 1);
     const int most = keep < max_len ? keep : max_len;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
+    const int units = rb / (rb % 16 ? 8 : 16), each = PG_T / units;   // rows a workgroup
+    static_assert(PG_T >= KR_PAGE_HD_MAX * 4 / 8, "a row's units");
+    const unsigned blocks = ((unsigned)most + each - 1) / each;
     hipLaunchKernelGGL(rb % 16 ? k_evict_move<uint2> : k_evict_move<uint4>,
-                       dim3((most + EM_ROWS - 1) / EM_ROWS, kv->n_kv_heads, n_seq), dim3(PG_T), 0, kr_stream(), p, a, rb,
-                       kr_fault_word());
+                       dim3(blocks < EM_BLOCKS ? blocks : EM_BLOCKS, kv->n_kv_heads, n_seq), dim3(PG_T), 0, kr_stream(), p,
+                       a, rb, each, kr_fault_word());
     kr_check_launch("paged_evict");
 }
