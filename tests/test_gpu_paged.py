@@ -675,6 +675,26 @@ def test_evict_sizes(dev, rows, kind):
                 assert np.array_equal(got[out[i, j // page], g, j % page], p.a["k"][p.table[i, r // page], g, r % page])
 
 
+def test_evict_wide_rows(dev):
+    """more kept rows than the copy has workgroups for, of the widest rows"""
+    rng = np.random.default_rng(5)
+    n, keep, page, hd = 18000, 17001, 64, 256
+    p = Pool(dev, rng, K.ML_F32, [n], page, 1, hd, spare=-(-keep // page))
+    out = np.array([list(p.free)[:-(-keep // page)]], np.int32)
+    p.put()
+    w = weights(rng, "spread", (1, 1, n))
+    nb, mb = dev.zeros(4), dev.zeros(keep * 4)
+    K.hip.krh_paged_evict(p.ref, p.tab.ptr, p.ld, dev.put(i32([n])).ptr, dev.put(w).ptr, n, 1, n, keep, 500,
+                          dev.put(out).ptr, out.shape[1], nb.ptr, mb.ptr, keep,
+                          dev.zeros(K.hip.krh_paged_evict_ws(1, 1, keep)).ptr)
+    ok()
+    r, j = evicted(w[0, 0], n, keep, 500), np.arange(keep)
+    assert nb.get(np.int32, 1).tolist() == [keep]
+    assert np.array_equal(bits(mb.get(np.float32, keep)), bits(w[0, 0, r]))
+    for name in "kv":
+        assert np.array_equal(p.get(name)[out[0, j // page], 0, j % page], p.a[name][p.table[0, r // page], 0, r % page])
+
+
 def test_evict_bad(dev):
     """a length or a new page out of range is reported; the other sequences are as they should be"""
     rng = np.random.default_rng(1)
