@@ -556,7 +556,8 @@ template <int R> __global__ void __launch_bounds__(EV_T) k_evict_select_lds(cons
 // the first is written 3.3. Stores past the caches reach 5.0, but the attention
 // that reads the new pages next loses as much).
 constexpr unsigned EM_BLOCKS = 1 << 12;   // past it a workgroup takes more rows
-template <class U> __global__ void __launch_bounds__(PG_T) k_evict_move(const PgView p, const EvArgs a, int rb, int rows, int *fault) {
+template <class U> __global__ void __launch_bounds__(PG_T) k_evict_move(const PgView p, const EvArgs a, int rb, int rows,
+                                                                        int *fault) {
     const int s = blockIdx.z, kvh = blockIdx.y, per = rb / (int)sizeof(U), kept = a.cnt[s], tid = threadIdx.x;
     const size_t sh = (size_t)s * p.n_kv + kvh;
     const int *idx = a.idx + sh * a.keep, *ot = a.out_table + (size_t)s * a.out_ld;

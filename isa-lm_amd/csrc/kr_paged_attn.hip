@@ -7,9 +7,10 @@
 // sequence's part of its share once, with the running maximum and sum of the
 // softmax. A sequence within one share is then done; the others' parts are
 // joined by a second launch (k_paged_join), which finds them by the same
-// arithmetic. Where all are short each is a share, and there is no second launch. (Joined by the last share to end instead, whose parts pass between
-// the dies' caches: 20 to 40 us more with atomics that pass those caches, 60 to
-// 90 with fences.)
+// arithmetic. Where all are short each is a share, and there is no second launch.
+// (Joined by the last share to end instead, whose parts pass between the dies'
+// caches: 20 to 40 us more with atomics that pass those caches, 60 to 90 with
+// fences.)
 //
 // Both products run on the matrix cores, transposed so that nothing passes
 // through LDS: S^T = K Q^T has the tile's rows as rows and query heads as
@@ -773,7 +774,8 @@ int pa_shares(const krh_pages *kv, int n_seq, int rows) {
 // 256 dims, 128 rows, 1 and 8 sequences 10.6 / 11.3 and 13.0 / 11.1.
 constexpr int PA_WHOLE = 256, PA_WHOLE_MANY = 128;
 int pa_whole(const krh_pages *kv, int n_seq) {
-    const int rows = PA_WHOLE * 128 / ((kv->head_dim <= 128 ? 128 : 256) * (kv->kv_type != ML_F32 ? 1 : kv->head_dim <= 64 ? 2 : 4));
+    const int rows =
+        PA_WHOLE * 128 / ((kv->head_dim <= 128 ? 128 : 256) * (kv->kv_type != ML_F32 ? 1 : kv->head_dim <= 64 ? 2 : 4));
     return (long long)n_seq * kv->n_kv_heads >= PA_WHOLE_MANY ? 2 * rows : rows;
 }
 
