@@ -58,6 +58,10 @@ KR_HD int kr_page_in(int i, int n, int what, int &bad) {
     return i;
 }
 
+// entry j of a list that counts n of them, -1 past those: what lies behind the
+// counted ones, up to the row's stride, may belong to no allocation
+KR_HD int kr_id_at(const int *ids, int j, int n) { return j < n ? ids[j] : -1; }
+
 #ifdef __HIPCC__
 // any thread that found something bad; a store a word, so that none is lost
 __device__ __forceinline__ void kr_report(int *fault, int bad) {

@@ -71,17 +71,19 @@ template <bool VEC> __global__ void __launch_bounds__(RL_T) k_logit_rules(const 
             x[k][0] = i < n ? in[i] : 0.0f;
         }
     }
-    // the row's first ids with them, whether they count or not
+    // the row's first ids, as many as count
+    const RlRow row = { a.rule[r], a.bias + r * a.bias_ld };
+    int n_seen = a.n_seen[r], n_bias = a.n_bias[r];
+    asm("" : "+s"(n_seen), "+s"(n_bias));   // waited for together
+    int bad = 0;
+    const int ns = kr_page_len(a.seen ? n_seen : 0, (int)a.seen_ld, bad);
+    const int nb = kr_page_len(a.bias_id ? n_bias : 0, (int)a.bias_ld, bad);
     const int *seen = a.seen + r * a.seen_ld, *ids = a.bias_id + r * a.bias_ld;
     int sj[RL_SEEN], bj[RL_BIAS];
 #pragma unroll
-    for (int k = 0; k < RL_SEEN; k++) sj[k] = a.seen && k * RL_T + tid < (int)a.seen_ld ? seen[k * RL_T + tid] : -1;
+    for (int k = 0; k < RL_SEEN; k++) sj[k] = kr_id_at(seen, k * RL_T + tid, ns);
 #pragma unroll
-    for (int k = 0; k < RL_BIAS; k++) bj[k] = a.bias_id && k * RL_T + tid < (int)a.bias_ld ? ids[k * RL_T + tid] : -1;
-    const RlRow row = { a.rule[r], a.bias + r * a.bias_ld };
-    int bad = 0;
-    const int ns = a.seen ? kr_page_len(a.n_seen[r], (int)a.seen_ld, bad) : 0;
-    const int nb = a.bias_id ? kr_page_len(a.n_bias[r], (int)a.bias_ld, bad) : 0;
+    for (int k = 0; k < RL_BIAS; k++) bj[k] = kr_id_at(ids, k * RL_T + tid, nb);
     int mask = row.p.mask;
     if (mask < -1 || mask >= a.n_masks) {
         bad |= KR_BAD_LEN;
@@ -156,8 +158,11 @@ extern "C" void krh_logit_rules(float *out, size_t ldo, const float *logits, siz
         kr_fail(ML_E_ISA, "logit_rules before krh_init", hipSuccess);
         return;
     }
-    const RlArgs a = { out,    logits, ldo,  ld,      rule,    seen,  n_seen, bias_id,
-                       n_bias, bias,   seen_ld, bias_ld, masks, n,      n_masks };
+    // where there is no list, any readable words stand for its counts, so that a
+    // launch asks for both without a branch
+    const int *none = (const int *)rule;
+    const RlArgs a = { out,    logits, ldo,     ld,      rule,  seen, seen ? n_seen : none, bias_id, bias_id ? n_bias : none,
+                       bias,   seen_ld, bias_ld, masks, n,    n_masks };
     const bool vec = !(((uintptr_t)out | (uintptr_t)logits) & 15) && ldo % 4 == 0 && ld % 4 == 0;
     hipLaunchKernelGGL(vec ? k_logit_rules<true> : k_logit_rules<false>, dim3((n + RL_N - 1) / RL_N, rows), dim3(RL_T),
                        0, kr_stream(), a, kr_fault_word());
