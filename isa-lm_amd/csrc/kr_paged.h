@@ -19,10 +19,10 @@ enum { KR_PAGE_MIN = 16, KR_PAGE_MAX = 1024, KR_PAGE_HD_MAX = 256, KR_PAGE_GROUP
 enum { KR_BAD_PAGE = 1, KR_BAD_LEN = 2, KR_BAD_SEQ = 4, KR_BAD_POS = 8, KR_FAULT_WORDS = 4 };
 
 // The page that holds `row` of a sequence: an id in [0, n_pages), n_pages >= 1,
-// whatever the table holds. row >= 0; only the table's ld entries are read.
+// whatever the table holds and `row` is; only the table's ld entries are read.
 KR_HD int kr_page_of(const int *table, int ld, int row, int shift, int n_pages, int &bad) {
-    const int i = row >> shift;
-    if (i >= ld) {
+    const unsigned i = (unsigned)row >> shift;   // a negative row is past every table
+    if (i >= (unsigned)ld) {
         bad |= KR_BAD_PAGE;
         return 0;
     }

@@ -17,3 +17,7 @@ def host_check(tmp_path, name, trials):
 
 def test_lists_are_read_to_their_counts(tmp_path):
     host_check(tmp_path, "list_bounds", 1000)
+
+
+def test_negative_rows_are_out_of_range(tmp_path):
+    host_check(tmp_path, "row_bounds", 100000)
