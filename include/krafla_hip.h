@@ -367,9 +367,10 @@ typedef struct {
  * but for two: the norm's sum of squares is formed in 64 bits instead of in index
  * order in 32, and a Q8 row's factor as 127 times the reciprocal of its maximum
  * instead of their quotient (an element next to a border may round to its other
- * side). n_heads 0: no queries (q, qo unused). qo may be q; nothing else
- * overlaps. pos may be NULL without tables. The rows of a call are distinct. q,
- * qo, k, v, the norms and the tables 16-byte aligned, row strides multiples of 4. */
+ * side). n_heads 0: no queries (q, qo unused). qo may be q where ldqo is ldq;
+ * nothing else overlaps. pos may be NULL without tables. The rows of a call are
+ * distinct. q, qo, k, v, the norms and the tables 16-byte aligned, row strides
+ * multiples of 4. */
 void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const int *table, int table_ld, int n_seq,
                    const float *q, size_t ldq, const float *k, size_t ldk, const float *v, size_t ldv, int ntok,
                    int n_heads, const int *seq, const int *row, const int *pos, const float *q_norm,

@@ -610,7 +610,9 @@ extern "C" void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const
                       pg_aligned(k_norm) && pg_aligned(cos_t) && pg_aligned(sin_t) &&
                       (n_heads == 0 || (ldq >= qd && ldqo >= qd && ldq % 4 == 0 && ldqo % 4 == 0 && pg_aligned(q) &&
                                         pg_aligned(qo) && pg_aligned(q_norm))),
-                  "paged_qkv: row strides or alignment"))
+                  "paged_qkv: row strides or alignment") ||
+        // tokens pass in no order: with strides apart one's output would lie on another's query
+        pg_refuse(n_heads == 0 || ntok == 1 || qo != q || ldqo == ldq, "paged_qkv: queries in place with another stride"))
         return;
     const int lps = pg_log2(kv->head_dim / 8);
     const unsigned grid = item_blocks((size_t)ntok * (n_heads + 2 * (size_t)kv->n_kv_heads), lps);

@@ -1,10 +1,13 @@
 """The paged cache's operators and the logit rules without a device, at the
 edges of what their calls allow: the bounds of lists and rows, and refusals."""
+import ctypes as C
 import os
 import subprocess
 
+import pytest
 
-from test_paged import HERE, ROOT
+import krafla as K
+from test_paged import HERE, PTR, QKV, ROOT, call, pages
 
 
 def host_check(tmp_path, name, trials):
@@ -15,9 +18,32 @@ def host_check(tmp_path, name, trials):
     assert r.returncode == 0 and r.stdout.startswith("ok"), (r.returncode, r.stdout + r.stderr)
 
 
+def refused(name, args, kv):
+    """what a refused call says"""
+    K.hip.krh_clear_error()
+    a = dict(args)
+    if "kv" in a:
+        a["kv"] = C.byref(kv)
+    getattr(K.hip, name)(*a.values())
+    said = K.hip.krh_last_error()
+    K.hip.krh_clear_error()
+    return said
+
+
 def test_lists_are_read_to_their_counts(tmp_path):
     host_check(tmp_path, "list_bounds", 1000)
 
 
 def test_negative_rows_are_out_of_range(tmp_path):
     host_check(tmp_path, "row_bounds", 100000)
+
+
+@pytest.mark.parametrize("ldqo", [260, 512])
+def test_queries_in_place_have_one_stride(ldqo):
+    """tokens pass in no order, so one's output would lie on another's query"""
+    assert call("krh_paged_qkv", dict(QKV, qo=PTR, q=PTR, ldq=256, ldqo=ldqo), pages()) == K.ML_E_SHAPE
+    assert b"in place" in refused("krh_paged_qkv", dict(QKV, qo=PTR, q=PTR, ldq=256, ldqo=ldqo), pages())
+    # apart, or without queries, the strides are the caller's
+    if K.hip.krh_device_cus() == 0:
+        assert call("krh_paged_qkv", dict(QKV, qo=PTR + 65536, ldqo=ldqo), pages()) == K.ML_E_ISA
+        assert call("krh_paged_qkv", dict(QKV, n_heads=0, q_norm=None, ldqo=ldqo), pages()) == K.ML_E_ISA
