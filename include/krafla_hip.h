@@ -343,8 +343,8 @@ uint64_t krh_sampler_rng(const krh_sampler *s);
  *
  * Tables, lengths, rows and positions are device data. One out of range is never
  * used as an address: the pool's first page stands in for what it names (length
- * 0 for a bad length; a bad token is left out), the results of that sequence hold
- * no meaning, and the next krh_sync reports ML_E_SHAPE.
+ * 0 for a bad length; of a bad token neither row is stored), the results of that
+ * sequence hold no meaning, and the next krh_sync reports ML_E_SHAPE.
  *
  * Every call works on the library stream, allocates nothing, and can be captured
  * into a graph. A workspace holds nothing between calls: calls on the one

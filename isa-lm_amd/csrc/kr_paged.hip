@@ -122,11 +122,14 @@ template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_qkv(const PgVi
                            : (isk ? a.k + (size_t)t * a.ldk : a.v + (size_t)t * a.ldv) + (size_t)kvh * hd;
     Pg8 x = pg_get(src + d);
     int bad = 0, row = 0, page = 0;
+    int pos = a.cs ? a.pos[t] : 0;
     if (!isq) {
         const int seq = kr_page_in(a.seq[t], p.n_seq, KR_BAD_SEQ, bad);
         row = kr_page_in(a.row[t], INT_MAX, KR_BAD_PAGE, bad);
         page = pg_page(p, seq, row, bad);
     }
+    // the value looks at the position too: of a bad token neither row is stored
+    if (a.cs) pos = kr_page_in(pos, a.n_pos, KR_BAD_POS, bad);
     const bool keep = bad == 0;
     if (isq || isk) {
         const float *w = isq ? a.qw : a.kw;
@@ -141,7 +144,7 @@ template <int KT> __global__ void __launch_bounds__(PG_T) k_paged_qkv(const PgVi
             for (int i = 0; i < 8; i++) x.v[i] = kr_fmul(kr_fmul(x.v[i], inv), g.v[i]);
         }
         if (a.cs) {
-            const size_t at = (size_t)kr_page_in(a.pos[t], a.n_pos, KR_BAD_POS, bad) * (hd >> 1) + d / 2;
+            const size_t at = (size_t)pos * (hd >> 1) + d / 2;
             const float4 c4 = *(const float4 *)(a.cs + at), s4 = *(const float4 *)(a.sn + at);
             const float c[4] = { c4.x, c4.y, c4.z, c4.w }, s[4] = { s4.x, s4.y, s4.z, s4.w };
 #pragma unroll

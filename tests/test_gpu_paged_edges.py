@@ -5,7 +5,7 @@ import pytest
 
 import krafla as K
 from test_gpu_kernels import bits, f32, ok
-from test_gpu_paged import U, dev, device, i32, rules  # noqa: F401  (dev, device: fixtures)
+from test_gpu_paged import TYPES, Pool, U, dev, device, i32, rules, tables  # noqa: F401  (dev, device: fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,27 @@ def test_rules_last_row_to_its_count(dev, n, seen_ld, bias_ld, n_seen, n_bias): 
         assert (np.abs(o[r] - want) <= 6 * U * big).all()
         same = np.setdiff1d(np.arange(n), np.concatenate([seen[s], b_id[b]]))
         assert np.array_equal(bits(o[r][same]), bits(x[r][same]))
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("at", [5, -1, 2**31 - 1])
+def test_qkv_bad_position_stores_nothing(dev, kv_type, at):  # noqa: F811
+    """a token whose position is outside the tables leaves both its rows as they were, and is reported"""
+    rng = np.random.default_rng(3)
+    p = Pool(dev, rng, kv_type, [20, 20], 16, 2, 64).put()
+    seq, row, pos = i32([0, 1, 1]), i32([3, 4, 19]), i32([0, at, 4])
+    k, v = f32(rng.standard_normal((3, 128))), f32(rng.standard_normal((3, 128)))
+    q = f32(rng.standard_normal((3, 256)))
+    cs, sn = dev.put(np.ones((5, 32), np.float32)), dev.put(np.zeros((5, 32), np.float32))
+    K.hip.krh_paged_qkv(dev.zeros(q.nbytes).ptr, 256, p.ref, p.tab.ptr, p.ld, 2, dev.put(q).ptr, 256, dev.put(k).ptr, 128,
+                        dev.put(v).ptr, 128, 3, 4, dev.put(seq).ptr, dev.put(row).ptr, dev.put(pos).ptr, None, None, 0.0, cs.ptr,
+                        sn.ptr, 5)
+    assert K.hip.krh_sync() == K.ML_E_SHAPE and b"position" in K.hip.krh_last_error()
+    K.hip.krh_clear_error()
+    for name in p.a:
+        got, want = p.get(name), p.a[name].copy()
+        for t in (0, 2):
+            x = (p.table[seq[t], row[t] // 16], slice(None), row[t] % 16)
+            assert not np.array_equal(got[x], want[x])
+            want[x] = got[x]
+        assert np.array_equal(got, want), name
