@@ -22,8 +22,9 @@
 //
 // The halves' products are exact in 32 bits, so a float operand is split in two
 // halves, x = hi + lo with |x - hi - lo| <= 2^-22 |x|: the queries (scaled by a
-// power of two a head) and the weights (scaled by 2^14, so that weights 2^-28 of
-// the largest keep hi and lo whole). The products of both are in the same sums
+// power of two a head) and the weights (times 2^15 after the power, which is exact:
+// lo is a whole half down to 2^-17 of the largest weight, and below that weights
+// err by up to 2^-40 of it). The products of both are in the same sums
 // (hi and lo as columns of one product, for up to 8 query heads a KV head, took
 // 1 to 4% more, for their exchange). int8 rows become halves exactly; their scale
 // multiplies the score, or the weight. F32 caches take the 32-bit product, whose
@@ -40,9 +41,9 @@ namespace {
 
 // Rows of a tile: 32, and 16 for heads past 128 dims, whose rows fill the registers
 constexpr int pa_tile(int hd) { return hd > 128 ? 16 : 32; }
-constexpr float PA_UP = 14.0f;     // the weights' scale (log2; halves end at 2^16)
-// the least power of two that 8-bit rows' weights and sums are over: with it a
-// sum of 2^29 weights stays within 32 bits, and the scale 0 of rows of zeros has one
+constexpr int PA_UP = 15;   // the weights' scale (log2; halves end at 2^16)
+// the least power of two that 8-bit rows' weights are over: the scale 0 of rows of
+// zeros has one with it
 constexpr int PA_EV = -80;
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -65,7 +66,7 @@ struct PaArgs {
     size_t z_ld;
     int nh, max_len, window, shares;
     int whole, tl, least;     // whole: a share a sequence; tl: log2 of a tile's rows; least: tiles a share is worth
-    float scale, cap, z_up;   // z_up: log2 of the weights' scale in the sums
+    float scale, cap;
 };
 
 // rows [first, len) of a sequence, in tiles from the one that holds `first`; a
@@ -229,7 +230,7 @@ template <int KT, int CL, bool FULL> struct PaWave {
     int ids;   // the pages of 64 half tiles from t_ids on, one a lane
     std::conditional_t<HALF, half8, float4v> qf[KS][NB];   // the queries as operands
     float cs, m_run, l_run;
-    int ev;        // Q8: weights and sums are over 2^ev,
+    int ev;        // Q8: weights times V scales, and o, are over 2^ev,
     float v_end;   // which all V scales so far are below
     float4v o[W];
 
@@ -417,8 +418,8 @@ template <int KT, int CL, bool FULL> struct PaWave {
             for (int i = 0; i < R; i += 4) *(float4v *)(z + i) = float4v{ sc[i], sc[i + 1], sc[i + 2], sc[i + 3] };
         }
         // The maximum, one for a column's four lanes, moves where a lane has a
-        // larger score; with it what the weights are scaled by, for the 8-bit
-        // rows' scales that they carry to end in halves: 2^-ev, in the sums too.
+        // larger score; with it what the 8-bit rows' weights are over, for the
+        // scales that they carry to end in halves: 2^ev, o's sums too.
         float v_tile = 0.0f;
         if constexpr (KT == PG_Q8) {
 #pragma unroll
@@ -427,6 +428,7 @@ template <int KT, int CL, bool FULL> struct PaWave {
         if (__any(m_tile > m_run || (KT == PG_Q8 && v_tile >= v_end))) {
             const float m_new = fmaxf(m_run, pa_max_g(m_tile));
             float f = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+            l_run *= f;
             if constexpr (KT == PG_Q8) {
                 const int e = max(ev, min((int)(__float_as_uint(pa_max_g(v_tile)) >> 23) - 126, 120));   // v_tile < 2^e
                 f = ldexpf(f, ev - e);
@@ -434,12 +436,12 @@ template <int KT, int CL, bool FULL> struct PaWave {
                 v_end = ldexpf(1.0f, ev);
             }
             m_run = m_new;
-            l_run *= f;
 #pragma unroll
             for (int c = 0; c < W; c++) o[c] *= f;
         }
         // weights of no finite maximum: 0 for -inf, NaN for NaN
-        const float base = (m_run == -INFINITY ? 0.0f : m_run) - (HALF ? PA_UP - (float)(KT == PG_Q8 ? ev : 0) : 0.0f);
+        const float base = m_run == -INFINITY ? 0.0f : m_run;
+        const float up = KT == PG_Q8 ? ldexpf(1.0f, PA_UP - ev) : (float)(1 << PA_UP);
         // the weights as operands: R halves, or floats
         typedef _Float16 halfr __attribute__((ext_vector_type(R)));
         typedef unsigned uintr __attribute__((ext_vector_type(R / 2)));
@@ -457,6 +459,7 @@ template <int KT, int CL, bool FULL> struct PaWave {
                 asm("" : "+v"(x));
             }
             if constexpr (HALF) {
+                x *= up;
                 const _Float16 hi = (_Float16)x;
                 ph[0][i] = hi;
                 ph[1][i] = (_Float16)(x - (float)hi);
@@ -570,8 +573,9 @@ template <int KT, int CL, bool FULL> struct PaWave {
                 pass(r, min(r1, r + (64 / NT) * TILE), r == r0);
             }
         }
-        const float s = pa_sum_g(l_run), l = KT == PG_Q8 ? ldexpf(s, ev) : s;
-        float f = alone ? 1.0f / s : KT == PG_Q8 ? ldexpf(1.0f, ev) : 1.0f;
+        const float l = pa_sum_g(l_run);
+        float f = alone ? 1.0f / l : 1.0f;
+        if constexpr (HALF) f = ldexpf(f, KT == PG_Q8 ? ev - PA_UP : -PA_UP);
         if (sp.len == 0) f = 0.0f;
         if (g == 0 && live && (!alone || a.z)) {
             *(float2v *)(a.pml + (slot * group + n) * 2) = float2v{ m_run, l };
@@ -724,12 +728,12 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
 #pragma unroll
     for (int h = 0; h < PJ_U; h++)
         if (h < group) {
-            const float m = s_m[h] - a.z_up, inv = s_i[h];
+            const float m = s_m[h], inv = s_i[h];
 #pragma unroll
             for (int k = 0; k < K; k++) sum[k] += __builtin_amdgcn_exp2f(zs[h][k] - m) * inv;
         }
     for (int h = PJ_U; h < group; h++) {
-        const float m = s_m[h] - a.z_up, inv = s_i[h];
+        const float m = s_m[h], inv = s_i[h];
 #pragma unroll
         for (int k = 0; k < K; k++) sum[k] += __builtin_amdgcn_exp2f(z[h * a.z_ld + at[k]] - m) * inv;
     }
@@ -846,7 +850,7 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
     a.nh = n_heads, a.max_len = max_len, a.window = window, a.shares = shares, a.least = pa_least(kv);
     a.tl = pg_log2(pa_tile(kv->head_dim));
     a.whole = whole;
-    a.scale = scale, a.cap = softcap, a.z_up = kv->kv_type == ML_F32 ? 0.0f : PA_UP;
+    a.scale = scale, a.cap = softcap;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
     const int hd = kv->head_dim;
     const PaKernel f = kv->kv_type == ML_F32 ? pa_kernel<PG_F32>(hd) : kv->kv_type == ML_F16 ? pa_kernel<PG_F16>(hd)

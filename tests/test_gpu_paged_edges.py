@@ -67,3 +67,104 @@ def test_qkv_bad_position_stores_nothing(dev, kv_type, at):  # noqa: F811
             assert not np.array_equal(got[x], want[x])
             want[x] = got[x]
         assert np.array_equal(got, want), name
+
+
+def attend(d, p, lens, q, nh, mass, scale=1.0, cap=0.0, max_len=None):
+    """the outputs, and the masses from zero (or None), of one call"""
+    S, ml = len(lens), max_len or max(lens)
+    ob, mb = d.zeros(q.nbytes), d.zeros(S * p.nkv * ml * 4)
+    ws = d.zeros(K.hip.krh_paged_attention_ws(p.ref, S, nh, ml, int(mass)))
+    K.hip.krh_paged_attention(ob.ptr, p.ref, p.tab.ptr, p.ld, d.put(i32(lens)).ptr, S, d.put(f32(q)).ptr, nh, ml, 0, scale, cap,
+                              mb.ptr if mass else None, ml, ws.ptr)
+    ok()
+    return (ob.get(np.float32, q.size).reshape(S, nh, p.hd).astype(np.float64),
+            mb.get(np.float32, S * p.nkv * ml).reshape(S, p.nkv, ml).astype(np.float64) if mass else None)
+
+
+def along_first(p, z, rows, seq):
+    """K of the sequence's rows: z (for a query of ones times the first unit vector) on the first dim, nothing on the others"""
+    at = (p.table[seq, rows // p.page], slice(None), rows % p.page)
+    p.a["k"][at] = 0
+    if p.kv_type == K.ML_Q8_0:
+        p.a["k"][at + (0,)] = np.sign(z).astype(np.int8)[:, None]
+        p.a["kd"][at] = np.abs(z)[:, None]
+    else:
+        p.a["k"][at + (0,)] = np.asarray(z)[:, None]
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("n", [33, 3000])
+@pytest.mark.parametrize("mass", [False, True])
+def test_attention_of_large_equal_scores(dev, kv_type, n, mass):  # noqa: F811
+    """scores past 2^24, whose steps are larger than the weights' scale: rows of one score share their weight, whatever it is"""
+    rng = np.random.default_rng(n)
+    scores = [c * 2.0 ** e for e in (20, 24, 25, 26, 27, 28, 30) for c in (1.0, 1.125, 1.5, 1.875)]
+    lens = [n if i < 2 else 33 for i in range(len(scores))]
+    p = Pool(dev, rng, kv_type, lens, 16, 1, 64)
+    q = np.zeros((len(scores), 1, 64), np.float32)
+    for i, z in enumerate(scores):
+        rows = np.arange(lens[i])
+        along_first(p, np.where(rows % 3 == 1, -1.0, 1.0), rows, i)   # every third row far below the others
+        q[i, 0, 0] = z
+    p.put()
+    o, m = attend(dev, p, lens, q, 1, mass)
+    for i, ln in enumerate(lens):
+        high = np.arange(ln) % 3 != 1
+        a = high / high.sum()
+        v = p.rows("v", i, ln)[:, 0]
+        # equal weights are 1 before their sum: what is left are the sums over n rows and the quotient
+        rel = 2 * (ln + 64) * U
+        assert (np.abs(o[i, 0] - a @ v) <= rel * (a @ np.abs(v))).all(), (i, scores[i])
+        if mass:
+            assert (np.abs(m[i, 0, :ln] - a) <= rel * a).all() and (m[i, 0, ln:] == 0).all()
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("mass", [False, True])
+def test_attention_weights_keep_their_bits(dev, kv_type, mass):  # noqa: F811
+    """Two rows, whose weights' quotient e^-t, 0 < t < 1, the outputs show.
+
+    In half steps U, at most: the score's factor and product (8 bits: one product more) 2 (3) t, the power 2 (a step of a
+    value over 1/2), the operand's two halves 2 (a half step of the lower one), the two outputs' products 2. Spread evenly
+    within these, but for the power's which may lie on one side: a root mean square of 2.6 U, with a tenth for the sample."""
+    rng = np.random.default_rng(1)
+    S = 1000
+    p = Pool(dev, rng, kv_type, [2] * S, 16, 1, 64, fill=False)
+    t = rng.random(S) * 0.98 + 0.01
+    t = (t.astype(np.float16) if kv_type == K.ML_F16 else f32(t)).astype(np.float64)
+    for i in range(S):
+        along_first(p, np.array([0.0, -t[i]]), np.arange(2), i)
+        at = p.table[i, 0]
+        p.a["v"][at, 0, [0, 1], [0, 1]] = 64 if kv_type == K.ML_Q8_0 else 1
+        if kv_type == K.ML_Q8_0:
+            p.a["vd"][at, 0, :2] = 2.0 ** -6
+    p.put()
+    q = np.zeros((S, 1, 64), np.float32)
+    q[:, 0, 0] = 1
+    o, m = attend(dev, p, [2] * S, q, 1, mass)
+    for x, y in [(o[:, 0, 0], o[:, 0, 1])] + ([(m[:, 0, 0], m[:, 0, 1])] if mass else []):
+        err = y / x / np.exp(-t) - 1
+        assert np.abs(err).max() <= 9 * U, np.abs(err).max() / U
+        assert np.sqrt((err ** 2).mean()) <= 2.9 * U, np.sqrt((err ** 2).mean()) / U
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_attention_small_weights(dev, kv_type):  # noqa: F811
+    """Weights down to 2^-36 of the largest, each on a dim of its own: to 2^-22 (two halves) and the score's roundings
+    of their value, and below 2^-17 of the largest to 2^-39 of it"""
+    rng = np.random.default_rng(2)
+    n = 64
+    p = Pool(dev, rng, kv_type, [n], 16, 1, 64, fill=False)
+    r = np.arange(n)
+    t = (r * 0.4).astype(np.float16).astype(np.float64)
+    along_first(p, -t, r, 0)
+    p.a["v"][p.table[0, r // 16], 0, r % 16, r] = 64 if kv_type == K.ML_Q8_0 else 1
+    if kv_type == K.ML_Q8_0:
+        p.a["vd"][p.table[0, r // 16], 0, r % 16] = 2.0 ** -6
+    p.put()
+    q = np.zeros((1, 1, 64), np.float32)
+    q[0, 0, 0] = 1
+    o, _ = attend(dev, p, [n], q, 1, False)
+    a = np.exp(-t)
+    a /= a.sum()
+    assert (np.abs(o[0, 0] - a) <= (3 * t + 80) * U * a + 2.0 ** -39 * a.max()).all()
