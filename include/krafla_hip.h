@@ -391,8 +391,9 @@ size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int m
  *
  * Scores, the softmax's maximum and sum, and all sums of products are held in 32
  * bits, a Q8 cache's queries unquantized. For the products of an F16 or Q8 cache
- * queries and weights are two halves each: to 2^-22 of their value, or to 2^-38 of
- * the head's largest where that is more. An F32 cache's are floats.
+ * queries and weights (Q8: weights times their V scales) are two halves each: to
+ * 2^-22 of their value, or to 2^-38 of the head's largest where that is more. An
+ * F32 cache's are floats.
  * The rows are split over the chip and the parts joined, so sums are not in the
  * order of krh_attention_kv: results agree to rounding, and are the same from
  * call to call. Values attended that are not finite give results that are not

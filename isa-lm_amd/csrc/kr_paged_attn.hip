@@ -230,8 +230,10 @@ template <int KT, int CL, bool FULL> struct PaWave {
     int ids;   // the pages of 64 half tiles from t_ids on, one a lane
     std::conditional_t<HALF, half8, float4v> qf[KS][NB];   // the queries as operands
     float cs, m_run, l_run;
-    int ev;        // Q8: weights times V scales, and o, are over 2^ev,
-    float v_end;   // which all V scales so far are below
+    // Q8: the largest weight times V scale so far (of the maximum now); with o's
+    // sums they are over 2^ev = v_end, which it is below
+    float v_run, v_end;
+    int ev;
     float4v o[W];
 
     __device__ __forceinline__ PaWave(const PgView &p_, const PaArgs &a_, int kvh_)
@@ -417,30 +419,48 @@ template <int KT, int CL, bool FULL> struct PaWave {
 #pragma unroll
             for (int i = 0; i < R; i += 4) *(float4v *)(z + i) = float4v{ sc[i], sc[i + 1], sc[i + 2], sc[i + 3] };
         }
-        // The maximum, one for a column's four lanes, moves where a lane has a
-        // larger score; with it what the 8-bit rows' weights are over, for the
-        // scales that they carry to end in halves: 2^ev, o's sums too.
-        float v_tile = 0.0f;
-        if constexpr (KT == PG_Q8) {
-#pragma unroll
-            for (int i = 0; i < R; i++) v_tile = fmaxf(v_tile, fabsf(raw.vd[i]));
-        }
-        if (__any(m_tile > m_run || (KT == PG_Q8 && v_tile >= v_end))) {
+        // the maximum, one for a column's four lanes, moves where a lane has a larger score
+        const bool moved = __any(m_tile > m_run);
+        float f = 1.0f;
+        if (moved) {
             const float m_new = fmaxf(m_run, pa_max_g(m_tile));
-            float f = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-            l_run *= f;
-            if constexpr (KT == PG_Q8) {
-                const int e = max(ev, min((int)(__float_as_uint(pa_max_g(v_tile)) >> 23) - 126, 120));   // v_tile < 2^e
-                f = ldexpf(f, ev - e);
-                ev = e;
-                v_end = ldexpf(1.0f, ev);
-            }
+            f = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
             m_run = m_new;
-#pragma unroll
-            for (int c = 0; c < W; c++) o[c] *= f;
+            l_run *= f;
         }
         // weights of no finite maximum: 0 for -inf, NaN for NaN
         const float base = m_run == -INFINITY ? 0.0f : m_run;
+        float v_tile = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            sc[i] = __builtin_amdgcn_exp2f(sc[i] - base);
+            l_run += sc[i];
+            if constexpr (KT == PG_Q8) {
+                // a rounded product: left to itself the compiler rounds it to a
+                // half twice, once from the exact product, and at a tie the hi
+                // that is multiplied is not the one taken off for lo
+                sc[i] *= raw.vd[i];
+                asm("" : "+v"(sc[i]));
+                v_tile = fmaxf(v_tile, fabsf(sc[i]));
+            }
+        }
+        // 8-bit rows' weights carry their V scales, and what both are over to end in
+        // halves goes by their product: a large scale without weight moves nothing,
+        // and it comes down again with the weights of an earlier maximum
+        if constexpr (KT == PG_Q8) {
+            if (moved || __any(v_tile >= v_end)) {
+                v_run = fmaxf(v_run * f, pa_max_g(v_tile));
+                const int e = max(PA_EV, (int)(__float_as_uint(v_run) >> 23) - 126);   // v_run < 2^e
+                f = ldexpf(f, ev - e);
+                ev = e;
+                v_end = ldexpf(1.0f, e);
+#pragma unroll
+                for (int c = 0; c < W; c++) o[c] *= f;
+            }
+        } else if (moved) {
+#pragma unroll
+            for (int c = 0; c < W; c++) o[c] *= f;
+        }
         const float up = KT == PG_Q8 ? ldexpf(1.0f, PA_UP - ev) : (float)(1 << PA_UP);
         // the weights as operands: R halves, or floats
         typedef _Float16 halfr __attribute__((ext_vector_type(R)));
@@ -449,15 +469,7 @@ template <int KT, int CL, bool FULL> struct PaWave {
         float pf[R];
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            float x = __builtin_amdgcn_exp2f(sc[i] - base);
-            l_run += x;
-            if constexpr (KT == PG_Q8) {
-                // a rounded product: left to itself the compiler rounds it to a
-                // half twice, once from the exact product, and at a tie the hi
-                // that is multiplied is not the one taken off for lo
-                x *= raw.vd[i];
-                asm("" : "+v"(x));
-            }
+            float x = sc[i];
             if constexpr (HALF) {
                 x *= up;
                 const _Float16 hi = (_Float16)x;
@@ -561,7 +573,7 @@ template <int KT, int CL, bool FULL> struct PaWave {
         m_run = -INFINITY;
         l_run = 0.0f;
         ev = PA_EV;
-        v_end = 0.0f;
+        v_run = v_end = 0.0f;
 #pragma unroll
         for (int c = 0; c < W; c++) o[c] = float4v{ 0, 0, 0, 0 };
         const bool alone = t == 0 && end == sp.tiles;

@@ -5,7 +5,7 @@ import pytest
 
 import krafla as K
 from test_gpu_kernels import bits, f32, ok
-from test_gpu_paged import TYPES, Pool, U, dev, device, i32, rules, tables  # noqa: F401  (dev, device: fixtures)
+from test_gpu_paged import TYPES, Pool, U, attention, dev, device, i32, rules, tables  # noqa: F401  (dev, device: fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +168,52 @@ def test_attention_small_weights(dev, kv_type):  # noqa: F811
     a = np.exp(-t)
     a /= a.sum()
     assert (np.abs(o[0, 0] - a) <= (3 * t + 80) * U * a + 2.0 ** -39 * a.max()).all()
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** 20, 2.0 ** 30, 2.0 ** 60])
+@pytest.mark.parametrize("n,far", [(250, 0), (250, 100), (250, 249), (5000, 3), (5000, 2600)])
+def test_attention_large_scale_without_weight(dev, ratio, n, far):  # noqa: F811
+    """an 8-bit row of a large scale that no head looks at takes no bits of the others, wherever it lies"""
+    rng = np.random.default_rng(n + far)
+    lens = [n, 40]
+    p = Pool(dev, rng, K.ML_Q8_0, lens, 16, 2, 64)
+    q = f32(np.abs(rng.standard_normal((2, 4, 64))) + 0.1)
+    at = (p.table[0, far // 16], slice(None), far % 16)
+    p.a["vd"][at] *= np.float32(ratio)
+    p.a["k"][at], p.a["kd"][at] = -127, 8.0     # a score under -100 for every head
+    p.put()
+    o, _ = attend(dev, p, lens, q, 4, n == 250, scale=0.125)
+    for i, ln in enumerate(lens):
+        k, v = p.rows("k", i, ln), p.rows("v", i, ln)
+        for h in range(4):
+            keep = np.ones(ln, bool)
+            if i == 0:      # the row has no weight at all, and its own score's error is no other row's
+                z = (k[:, h // 2] @ q[0, h]) * 0.125
+                assert z[far] - z.max() < -100
+                keep[far] = False
+            w, _, bound, _ = attention(q[i, h].astype(np.float64), k[keep, h // 2], v[keep, h // 2], 0.125, 0, 0)
+            assert (np.abs(o[i, h] - w) <= bound).all(), (i, h, (np.abs(o[i, h] - w) / bound).max())
+
+
+@pytest.mark.parametrize("mass", [False, True])
+def test_attention_scales_behind_a_new_maximum(dev, mass):  # noqa: F811
+    """rows of large scales first, then rows of small scales whose scores leave those without weight, and the other way round"""
+    rng = np.random.default_rng(11)
+    lens = [200, 200, 64, 3000]
+    p = Pool(dev, rng, K.ML_Q8_0, lens, 16, 1, 64)
+    q = np.zeros((4, 1, 64), np.float32)
+    q[:, 0, 0] = 1
+    for i, n in enumerate(lens):
+        r = np.arange(n)
+        late = r >= n // 2 if i != 1 else r < n // 2
+        along_first(p, np.where(late, 90.0, 0.5) + rng.random(n), r, i)
+        at = (p.table[i, r // 16], 0, r % 16)
+        p.a["vd"][at] *= f32(np.where(late, 2.0 ** -20, 2.0 ** 20))
+    p.put()
+    o, m = attend(dev, p, lens, q, 1, mass)
+    for i, n in enumerate(lens):
+        k, v = p.rows("k", i, n)[:, 0], p.rows("v", i, n)[:, 0]
+        w, a, bound, rel = attention(q[i, 0].astype(np.float64), k, v, 1.0, 0, 0)
+        assert (np.abs(o[i, 0] - w) <= bound).all(), (i, (np.abs(o[i, 0] - w) / bound).max())
+        if mass:
+            assert (np.abs(m[i, 0, :n] - a) <= rel * a + 1e-30).all()
