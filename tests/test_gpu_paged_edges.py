@@ -5,7 +5,7 @@ import pytest
 
 import krafla as K
 from test_gpu_kernels import bits, f32, ok
-from test_gpu_paged import TYPES, Pool, U, attention, dev, device, i32, rules, tables  # noqa: F401  (dev, device: fixtures)
+from test_gpu_paged import NP, TYPES, Pool, U, attention, dev, device, i32, rules, tables  # noqa: F401  (dev, device: fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -217,3 +217,52 @@ def test_attention_scales_behind_a_new_maximum(dev, mass):  # noqa: F811
         assert (np.abs(o[i, 0] - w) <= bound).all(), (i, (np.abs(o[i, 0] - w) / bound).max())
         if mass:
             assert (np.abs(m[i, 0, :n] - a) <= rel * a + 1e-30).all()
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 64), (8, 1, 128), (3, 3, 48), (2, 1, 256)])
+def test_qkv_normed_rows(dev, kv_type, nh, nkv, hd):  # noqa: F811
+    """Normalized heads: values are stored as without a norm, bit for bit; 8-bit keys' scales are their rows' maxima over
+    127, and scale times element is the key within half a step.
+
+    In 32 bits a normalized and rotated value errs by at most 10 U of its row's largest before the rotation (the factor, two
+    products, then two products and a sum of two values), its maximum by as much; the element's factor and product by 4 U."""
+    rng = np.random.default_rng(hd)
+    T, page = 30, 16
+    p = Pool(dev, rng, kv_type, [T], page, nkv, hd).put()
+    k, v, q = (f32(rng.standard_normal((T, n * hd)) * 3) for n in (nkv, nkv, nh))
+    v[4] = 0
+    pos = i32(rng.integers(0, 50, T))
+    cs, sn = tables(rng, 50, hd)
+    kw = f32(1 + 0.1 * rng.standard_normal(hd))
+    K.hip.krh_paged_qkv(dev.zeros(q.nbytes).ptr, nh * hd, p.ref, p.tab.ptr, p.ld, 1, dev.put(q).ptr, nh * hd, dev.put(k).ptr,
+                        nkv * hd, dev.put(v).ptr, nkv * hd, T, nh, dev.zeros(4 * T).ptr, dev.put(i32(np.arange(T))).ptr,
+                        dev.put(pos).ptr, dev.put(kw).ptr, dev.put(kw).ptr, 1e-6, dev.put(cs).ptr, dev.put(sn).ptr, 50)
+    ok()
+    got = {n: p.get(n) for n in p.a}
+    for t in range(T):
+        at = (p.table[0, t // page], slice(None), t % page)
+        x = v[t].reshape(nkv, hd)
+        if kv_type == K.ML_Q8_0:
+            m = np.abs(x).max(1, keepdims=True)
+            assert np.array_equal(bits(got["vd"][at]), bits(m[:, 0] / np.float32(127)))
+            with np.errstate(divide="ignore", invalid="ignore"):
+                e = np.trunc(x * (np.float32(127) * (np.float32(1) / m)) + np.copysign(np.float32(0.5), x))
+            assert np.array_equal(got["v"][at], np.where(m < 1e-30, 0, e).astype(np.int8))
+        else:
+            assert np.array_equal(got["v"][at].view(np.uint8), np.ascontiguousarray(x.astype(NP[kv_type])).view(np.uint8))
+        x = k[t].reshape(nkv, hd).astype(np.float64)
+        x = x / np.sqrt((x ** 2).mean(1, keepdims=True) + 1e-6) * kw
+        pre = np.abs(x).max(1)
+        a, b, c, s = x[:, 0::2], x[:, 1::2], cs[pos[t]], sn[pos[t]]
+        y = np.empty_like(x)
+        y[:, 0::2], y[:, 1::2] = a * c - b * s, a * s + b * c
+        g = got["k"][at].astype(np.float64)
+        if kv_type == K.ML_Q8_0:
+            d = got["kd"][at].astype(np.float64)
+            assert (np.abs(d - np.abs(y).max(1) / 127) <= 11 * U * pre / 127).all()
+            assert (np.abs(g * d[:, None] - y) <= d[:, None] * (0.5 + 127 * 4 * U) + 10 * U * pre[:, None]).all()
+            assert (np.abs(g).max(1) == 127).all()
+        else:
+            step = 2.0 ** -11 if kv_type == K.ML_F16 else 0.0
+            assert (np.abs(g - y) <= step * np.abs(y) + 12 * U * pre[:, None] + (2.0 ** -25 if step else 0)).all()
