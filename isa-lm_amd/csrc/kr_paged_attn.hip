@@ -34,6 +34,7 @@
 // rows 125 us (5.5 TB/s; the chip's plain read rate is 5.6), one of 120,001 rows
 // 93 (5.3), 16 of up to 4001 24 (4.9). 8-bit rows by a tile's latency and
 // instructions: 24 sequences of 64 dims 22 us (4.2).
+#include <cfloat>
 #include <type_traits>
 #include "kr_paged_dev.h"
 
@@ -842,7 +843,9 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
     if (pg_refuse(pa_args_ok(kv, n_seq, n_heads, max_len), "paged_attention sizes") ||
         pg_refuse(o && table && table_ld > 0 && len && q && ws && pg_aligned(o) && pg_aligned(q) && pg_aligned(ws),
                   "paged_attention: a missing or unaligned array") ||
-        pg_refuse(window >= 0 && softcap >= 0.0f && (!mass || mass_ld >= (size_t)max_len),
+        // a soft-cap whose reciprocal is a float: with infinity every score would be 0 times it
+        pg_refuse(window >= 0 && (softcap == 0.0f || (softcap >= FLT_MIN && softcap <= FLT_MAX)) &&
+                      (!mass || mass_ld >= (size_t)max_len),
                   "paged_attention: window, soft-cap or mass rows"))
         return;
     if (pg_not_ready("paged_attention before krh_init")) return;

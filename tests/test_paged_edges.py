@@ -7,7 +7,7 @@ import subprocess
 import pytest
 
 import krafla as K
-from test_paged import HERE, PTR, QKV, ROOT, call, pages
+from test_paged import ATT, HERE, PTR, QKV, ROOT, call, pages
 
 
 def host_check(tmp_path, name, trials):
@@ -47,3 +47,12 @@ def test_queries_in_place_have_one_stride(ldqo):
     if K.hip.krh_device_cus() == 0:
         assert call("krh_paged_qkv", dict(QKV, qo=PTR + 65536, ldqo=ldqo), pages()) == K.ML_E_ISA
         assert call("krh_paged_qkv", dict(QKV, n_heads=0, q_norm=None, ldqo=ldqo), pages()) == K.ML_E_ISA
+
+
+@pytest.mark.parametrize("cap", [float("inf"), 1e-40, 1e-45])
+def test_soft_caps_without_a_reciprocal_refused(cap):
+    """infinity times a score's tanh, 0 there, is no number, and the smallest floats' reciprocals are infinite"""
+    assert call("krh_paged_attention", dict(ATT, softcap=cap), pages()) == K.ML_E_SHAPE
+    if K.hip.krh_device_cus() == 0:
+        assert call("krh_paged_attention", dict(ATT, softcap=3e38), pages()) == K.ML_E_ISA
+        assert call("krh_paged_attention", dict(ATT, softcap=1.2e-38), pages()) == K.ML_E_ISA
