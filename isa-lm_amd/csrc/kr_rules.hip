@@ -96,13 +96,14 @@ template <bool VEC> __global__ void __launch_bounds__(RL_T) k_logit_rules(const 
             if (nb > 0) ((int4 *)last)[i] = make_int4(-1, -1, -1, -1);
         }
         __syncthreads();
+        // ids below i0, negative ones among them, wrap past n: i0 + n <= 2^31
         auto count = [&](int id) {
-            const int t = id - i0;
-            if (t >= 0 && t < n) atomicAdd(&cnt[t], 1);
+            const unsigned t = (unsigned)id - (unsigned)i0;
+            if (t < (unsigned)n) atomicAdd(&cnt[t], 1);
         };
         auto note = [&](int id, int j) {
-            const int t = id - i0;
-            if (t >= 0 && t < n) atomicMax(&last[t], j);
+            const unsigned t = (unsigned)id - (unsigned)i0;
+            if (t < (unsigned)n) atomicMax(&last[t], j);
         };
 #pragma unroll
         for (int k = 0; k < RL_SEEN; k++)
@@ -164,7 +165,7 @@ extern "C" void krh_logit_rules(float *out, size_t ldo, const float *logits, siz
     const RlArgs a = { out,    logits, ldo,     ld,      rule,  seen, seen ? n_seen : none, bias_id, bias_id ? n_bias : none,
                        bias,   seen_ld, bias_ld, masks, n,    n_masks };
     const bool vec = !(((uintptr_t)out | (uintptr_t)logits) & 15) && ldo % 4 == 0 && ld % 4 == 0;
-    hipLaunchKernelGGL(vec ? k_logit_rules<true> : k_logit_rules<false>, dim3((n + RL_N - 1) / RL_N, rows), dim3(RL_T),
+    hipLaunchKernelGGL(vec ? k_logit_rules<true> : k_logit_rules<false>, dim3(((unsigned)n + RL_N - 1) / RL_N, rows), dim3(RL_T),
                        0, kr_stream(), a, kr_fault_word());
     kr_check_launch("logit_rules");
 }

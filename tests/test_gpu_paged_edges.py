@@ -266,3 +266,26 @@ def test_qkv_normed_rows(dev, kv_type, nh, nkv, hd):  # noqa: F811
         else:
             step = 2.0 ** -11 if kv_type == K.ML_F16 else 0.0
             assert (np.abs(g - y) <= step * np.abs(y) + 12 * U * pre[:, None] + (2.0 ** -25 if step else 0)).all()
+
+
+def test_rules_on_most_ids(dev):  # noqa: F811
+    """as many ids as an int counts, and ids at both ends of the ints, on a row in place"""
+    n = 2 ** 31 - 1
+    xb = K.DevBuf(4 * n)
+    dev.bufs.append(xb)
+    at = [0, 1, 5, 4095, 4096, n - 4097, n - 4096, n - 2, n - 1]
+    for i in at:
+        v = f32([i % 97 + 1])
+        K.check(K.hip.krh_copy_h2d(xb.ptr + 4 * i, v.ctypes.data, 4))
+    seen = i32([0, n - 1, 5, -1, -2 ** 31, 5, 2 ** 31 - 1, n - 4097, -2 ** 31 + 1])   # n itself is passed over
+    b_id, bias = i32([n - 2, -2 ** 31, 4096, -1, n - 2]), f32([9, 100, 2, 100, 4])
+    rule = K.LogitRule(2.0, 0.25, 0.5, -1)
+    K.hip.krh_logit_rules(xb.ptr, n, xb.ptr, n, n, 1, dev.put(np.frombuffer(bytes(rule), np.uint8)).ptr, dev.put(seen).ptr, 9,
+                          dev.put(i32([9])).ptr, dev.put(b_id).ptr, dev.put(bias).ptr, 5, dev.put(i32([5])).ptr, None, 0)
+    ok()
+    for i in at:
+        v = np.empty(1, np.float32)
+        K.check(K.hip.krh_copy_d2h(v.ctypes.data, xb.ptr + 4 * i, 4))
+        c = int((seen == i).sum())
+        want = (i % 97 + 1) / (2 if c else 1) - 0.5 * c - (0.25 if c else 0) + {n - 2: 4, 4096: 2}.get(i, 0)
+        assert v[0] == want, i
