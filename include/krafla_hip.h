@@ -404,13 +404,13 @@ size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int m
 void krh_paged_attention(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len, int n_seq,
                          const float *q, int n_heads, int max_len, int window, float scale, float softcap,
                          float *mass, size_t mass_ld, void *ws);
-/* Bytes of workspace that krh_paged_evict takes */
+/* Bytes of workspace that krh_paged_evict takes (0 for sizes that it refuses) */
 size_t krh_paged_evict_ws(int n_seq, int n_kv_heads, int keep);
 /* Eviction by accumulated weight. Of sequence s's len[s] <= max_len <= 2^29 rows
- * each KV head keeps the last `recent` and the keep - recent with the largest
- * mass of the others (equal masses: the lower row; a NaN counts as the largest);
- * a sequence of at most `keep` rows keeps all. Heads keep different rows, each
- * head the same number. The kept rows go, in their order, to rows 0.. of the
+ * each KV head keeps the last `recent` and the keep - recent (keep <= 2^29) with
+ * the largest mass of the others (equal masses: the lower row; a NaN counts as the
+ * largest); a sequence of at most `keep` rows keeps all. Heads keep different rows,
+ * each head the same number. The kept rows go, in their order, to rows 0.. of the
  * sequence in the pages of out_table, which no table of the call names. out_len[s]
  * = min(len[s], keep), and out_mass (rows of out_ld >= keep) receives the kept
  * masses, then zeros as far as the row and the larger of keep and max_len go.

@@ -654,7 +654,7 @@ extern "C" void krh_paged_load(float *k, size_t ldk, float *v, size_t ldv, const
 }
 
 extern "C" size_t krh_paged_evict_ws(int n_seq, int n_kv_heads, int keep) {
-    if (n_seq <= 0 || n_kv_heads <= 0 || keep <= 0) return 0;
+    if (n_seq <= 0 || n_kv_heads <= 0 || keep <= 0 || keep > KR_PAGE_LEN_MAX) return 0;
     return sizeof(int) * (2 * (size_t)n_seq * n_kv_heads * keep + n_seq);
 }
 
@@ -664,6 +664,7 @@ extern "C" void krh_paged_evict(const krh_pages *kv, const int *table, int table
     if (n_seq == 0) return;
     if (pg_refuse(pg_pages_ok(kv), "paged_evict: the pages") ||
         pg_refuse(n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && max_len <= KR_PAGE_LEN_MAX && keep > 0 &&
+                   keep <= KR_PAGE_LEN_MAX &&   // the copy's steps past the last mass stay within an int
                    recent >= 0 && recent <= keep && table_ld > 0 &&
                    out_table_ld > 0, "paged_evict sizes") ||
         pg_refuse(table && len && mass && out_table && out_len && out_mass && ws && !((uintptr_t)ws & 3) &&

@@ -7,7 +7,7 @@ import subprocess
 import pytest
 
 import krafla as K
-from test_paged import ATT, HERE, PTR, QKV, ROOT, call, pages
+from test_paged import ATT, EVICT, HERE, PTR, QKV, ROOT, call, pages
 
 
 def host_check(tmp_path, name, trials):
@@ -56,3 +56,13 @@ def test_soft_caps_without_a_reciprocal_refused(cap):
     if K.hip.krh_device_cus() == 0:
         assert call("krh_paged_attention", dict(ATT, softcap=3e38), pages()) == K.ML_E_ISA
         assert call("krh_paged_attention", dict(ATT, softcap=1.2e-38), pages()) == K.ML_E_ISA
+
+
+@pytest.mark.parametrize("keep", [2**29 + 1, 2**31 - 1])
+def test_more_rows_kept_than_a_sequence_has_refused(keep):
+    """the masses' zeros go as far as `keep`, and steps past an int's last value would come out below the row"""
+    assert call("krh_paged_evict", dict(EVICT, keep=keep, out_ld=2**31), pages()) == K.ML_E_SHAPE
+    assert K.hip.krh_paged_evict_ws(1, 2, keep) == 0
+    if K.hip.krh_device_cus() == 0:
+        assert call("krh_paged_evict", dict(EVICT, keep=2**29, out_table_ld=4, out_ld=2**31), pages()) == K.ML_E_ISA
+    assert K.hip.krh_paged_evict_ws(1, 2, 2**29) == 4 * (4 * 2**29 + 1)
