@@ -385,8 +385,8 @@ size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int m
 /* Attention of one new token of each sequence, its last row: o, q [n_seq]
  * [n_heads * head_dim], o apart from every input. Sequence s attends its len[s]
  * rows, or with window > 0 the last window ones: softmax of scale * (q . K),
- * soft-capped first (cap * tanh(score / cap)) when softcap > 0 (a normal float),
- * over V. A sequence of no rows gets zeros. len[s] <= max_len <= 2^29, which sizes
+ * soft-capped first (cap * tanh(score / cap)) when softcap > 0 (a normal float, at
+ * most 2^126), over V. A sequence of no rows gets zeros. len[s] <= max_len <= 2^29, which sizes
  * the launch. At most 16 query heads a KV head; q, o and ws 16-byte aligned.
  *
  * Scores, the softmax's maximum and sum, and all sums of products are held in 32

@@ -843,8 +843,8 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
     if (pg_refuse(pa_args_ok(kv, n_seq, n_heads, max_len), "paged_attention sizes") ||
         pg_refuse(o && table && table_ld > 0 && len && q && ws && pg_aligned(o) && pg_aligned(q) && pg_aligned(ws),
                   "paged_attention: a missing or unaligned array") ||
-        // a soft-cap whose reciprocal is a float: with infinity every score would be 0 times it
-        pg_refuse(window >= 0 && (softcap == 0.0f || (softcap >= FLT_MIN && softcap <= FLT_MAX)) &&
+        // a soft-cap that is a normal float with its reciprocal and its log2 e times
+        pg_refuse(window >= 0 && (softcap == 0.0f || (softcap >= FLT_MIN && softcap <= 0x1p126f)) &&
                       (!mass || mass_ld >= (size_t)max_len),
                   "paged_attention: window, soft-cap or mass rows"))
         return;

@@ -289,3 +289,19 @@ def test_rules_on_most_ids(dev):  # noqa: F811
         c = int((seen == i).sum())
         want = (i % 97 + 1) / (2 if c else 1) - 0.5 * c - (0.25 if c else 0) + {n - 2: 4, 4096: 2}.get(i, 0)
         assert v[0] == want, i
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("cap", [2.0 ** 126, 2.0 ** -126])
+def test_attention_extreme_soft_caps(dev, kv_type, cap):  # noqa: F811
+    """a cap far above the scores leaves them (to a step of 2^-149 times the cap), one far below gives every row the same weight"""
+    rng = np.random.default_rng(4)
+    p = Pool(dev, rng, kv_type, [50, 7], 16, 2, 64).put()
+    q = f32(rng.standard_normal((2, 4, 64)))
+    o, _ = attend(dev, p, [50, 7], q, 4, False, scale=0.125, cap=cap)
+    for i, n in enumerate((50, 7)):
+        k, v = p.rows("k", i, n), p.rows("v", i, n)
+        for h in range(4):
+            w, _, bound, _ = attention(q[i, h].astype(np.float64) * (cap > 1), k[:, h // 2], v[:, h // 2], 0.125, 0, 0)
+            more = 2 * 2.0 ** -149 * cap * np.abs(v[:, h // 2]).max() if cap > 1 else 0
+            assert (np.abs(o[i, h] - w) <= bound + more + 8 * U * np.abs(v[:, h // 2]).max()).all(), (i, h)

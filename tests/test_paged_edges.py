@@ -49,12 +49,13 @@ def test_queries_in_place_have_one_stride(ldqo):
         assert call("krh_paged_qkv", dict(QKV, n_heads=0, q_norm=None, ldqo=ldqo), pages()) == K.ML_E_ISA
 
 
-@pytest.mark.parametrize("cap", [float("inf"), 1e-40, 1e-45])
+@pytest.mark.parametrize("cap", [float("inf"), 3e38, 1e-40, 1e-45])
 def test_soft_caps_without_a_reciprocal_refused(cap):
-    """infinity times a score's tanh, 0 there, is no number, and the smallest floats' reciprocals are infinite"""
+    """Infinity times a score's tanh, 0 there, is no number, and the smallest floats' reciprocals are infinite. 3e38 times
+    log2 e, by which powers are taken, is infinite too."""
     assert call("krh_paged_attention", dict(ATT, softcap=cap), pages()) == K.ML_E_SHAPE
     if K.hip.krh_device_cus() == 0:
-        assert call("krh_paged_attention", dict(ATT, softcap=3e38), pages()) == K.ML_E_ISA
+        assert call("krh_paged_attention", dict(ATT, softcap=8e37), pages()) == K.ML_E_ISA
         assert call("krh_paged_attention", dict(ATT, softcap=1.2e-38), pages()) == K.ML_E_ISA
 
 
