@@ -360,14 +360,14 @@ typedef struct {
 } krh_pages;
 /* The rows of ntok tokens into their pages: token t is row row[t] of sequence
  * seq[t], at position pos[t]. Query heads q (t * ldq; ldqo in qo) and key heads k
- * (t * ldk) are RMS-normalized with q_norm / k_norm when those are non-NULL, and
- * rotated by row pos[t] of the n_pos-row tables (head_dim / 2 floats a row) when
- * cos_t is non-NULL, as krh_heads_norm_rope does; keys and values (t * ldv) are
- * converted as krh_store_kv does (F32 as they are). The same bits as those calls
- * but for two: the norm's sum of squares is formed in 64 bits instead of in index
- * order in 32, and a Q8 row's factor as 127 times the reciprocal of its maximum
- * instead of their quotient (an element next to a border may round to its other
- * side). n_heads 0: no queries (q, qo unused). qo may be q where ldqo is ldq;
+ * (t * ldk) are RMS-normalized with q_norm / k_norm when those are non-NULL (where
+ * there are queries, both or neither), and rotated by row pos[t] of the n_pos-row
+ * tables (head_dim / 2 floats a row) when cos_t is non-NULL, as krh_heads_norm_rope
+ * does; keys and values (t * ldv) are converted as krh_store_kv does (F32 as they
+ * are). The same bits as those calls but for two: the norm's sum of squares is
+ * formed in 64 bits instead of in index order in 32, and a Q8 row's factor as 127
+ * times the reciprocal of its maximum instead of their quotient (an element next to
+ * a border may round to its other side). n_heads 0: no queries (q, qo unused). qo may be q where ldqo is ldq;
  * nothing else overlaps. pos may be NULL without tables. The rows of a call are
  * distinct. q, qo, k, v, the norms and the tables 16-byte aligned, row strides
  * multiples of 4. */
@@ -380,7 +380,8 @@ void krh_paged_qkv(float *qo, size_t ldqo, const krh_pages *kv, const int *table
 void krh_paged_load(float *k, size_t ldk, float *v, size_t ldv, const krh_pages *kv, const int *table, int table_ld,
                     int n_seq, int n, const int *seq, const int *row);
 /* Bytes of workspace that krh_paged_attention takes for these sizes and any
- * window (0 for sizes that it refuses); mass: whether it is given a mass array. */
+ * window (0 for sizes that it refuses); mass: whether it is given a mass array,
+ * which takes a float a query head and row of max_len. */
 size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int max_len, int mass);
 /* Attention of one new token of each sequence, its last row: o, q [n_seq]
  * [n_heads * head_dim], o apart from every input. Sequence s attends its len[s]
@@ -394,10 +395,12 @@ size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int m
  * queries and weights (Q8: weights times their V scales) are two halves each: to
  * 2^-22 of their value, or to 2^-38 of the head's largest where that is more. An
  * F32 cache's are floats.
+ *
  * The rows are split over the chip and the parts joined, so sums are not in the
  * order of krh_attention_kv: results agree to rounding, and are the same from
- * call to call. Values attended that are not finite give results that are not
- * finite, for the heads that they reach; rows not attended may hold anything.
+ * call to call. A NaN or an infinite value attended gives results that are not
+ * finite, for the heads that it reaches; an infinite key those, or the softmax of
+ * its score (minus infinity: no weight). Rows not attended may hold anything.
  *
  * mass (nullable): mass[(s * n_kv_heads + h) * mass_ld + r] += the sum of row r's
  * weights over the query heads of KV head h, for the rows attended. */

@@ -419,7 +419,7 @@ __device__ __forceinline__ unsigned ev_load(__amdgpu_buffer_rsrc_t rows, int r, 
 // code's way from memory, so there is one copy for all digits and none for
 // tails: rows past the last have the key 0, below any weight's. On many it is
 // bound by the CU's instructions, 10 or so a row: 32,001 rows, 8 workgroups, 16.5
-// us (the select above: 23.4); 16 sequences of up to 4096, 7.6 (10.9).
+// us, 17.2 on another card (the select above: 23.4); 16 sequences of up to 4096, 7.5 (10.9).
 template <int R> __global__ void __launch_bounds__(EV_T) k_evict_select_lds(const EvArgs a, int *fault) {
     __shared__ int hist[EV_B];
     __shared__ unsigned s_key[R];

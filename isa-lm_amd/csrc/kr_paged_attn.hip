@@ -31,9 +31,9 @@
 // rate still passes what HBM delivers.
 //
 // Bound by HBM where the rows are many: 8B shape, F16, 64 sequences of up to 6144
-// rows 125 us (5.5 TB/s; the chip's plain read rate is 5.6), one of 120,001 rows
-// 93 (5.3), 16 of up to 4001 24 (4.9). 8-bit rows by a tile's latency and
-// instructions: 24 sequences of 64 dims 22 us (4.2).
+// rows 123 us (5.5 TB/s; plain reads of 4 GB reach 5.3 to 6.5 by their grid), one of
+// 120,001 rows 91 (5.4), 16 of up to 4001 24 (5.0). 8-bit rows by a tile's latency
+// and instructions: 24 sequences of 64 dims 23 us (4.0).
 #include <cfloat>
 #include <type_traits>
 #include "kr_paged_dev.h"
@@ -757,7 +757,8 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
 
 // Shares in all, of every KV head: three waves a CU, which have the next tile's
 // rows under way, keep HBM busy. 8-bit rows, which take a tile's work to read half
-// as much, have four, and twelve up to 64 dims. Fewer where the rows are few: a
+// as much, have four, and twelve up to 64 dims (measured at 64; the kernel of narrower
+// heads has eight resident). Fewer where the rows are few: a
 // share is worth PA_BYTES of K and V at least (halves: twice that). The lengths
 // are the device's, so this is what they may be at most.
 // Measured from HBM (us, 2 / 3 / 4 / 8 / 12 waves a CU): 8B shape, halves, 16
@@ -767,6 +768,7 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
 // 16 of 128 dims 34.0 / 29.7 / 29.2 / 33.2 / 36.7.
 // 16 / 32 KB: halves, one sequence of 4000 rows 14.6 / 12.4; floats of 48 dims, 8
 // of up to 250 9.8 / 11.6; 8 bits of 48 dims, 16 of up to 8000 17.4 / 19.8.
+// PA_CUS is a constant so that a workspace has one size before and after krh_init.
 constexpr int PA_CUS = 256, PA_BYTES = 16 * 1024;
 int pa_least(const krh_pages *kv) {
     const bool f16 = kv->kv_type == ML_F16;

@@ -5,7 +5,7 @@
 // counts the row's seen ids that fall among them in LDS (integer atomics: the order
 // does not matter) and finds the last bias pair of each (a maximum of pair
 // numbers). Bound by HBM, 8 bytes a logit, when the seen ids are few: 64 rows of
-// 151,936 with 2000 seen 17.7 us, 4.4 TB/s (33 with the ids read after the
+// 151,936 with 2000 seen 17.0 us, 4.6 TB/s (33 with the ids read after the
 // logits, one logit a lane). 512 threads on 4096 ids fill a CU with waves; 256 threads
 // 21.6 us, 1024 19.6, 512 on 8192 ids 22.7; 256 on 2048 as fast, at twice the reads of
 // the seen ids.
@@ -46,7 +46,7 @@ __device__ __forceinline__ float rl_apply(const RlRow &r, float x, int c, int b,
 }
 
 // VEC: rows of the logits and the output 16-byte aligned, four ids a lane and
-// step (64 rows of 151,936 ids 17.7 us; one at a time 19.5)
+// step (64 rows of 151,936 ids 17.0 us; one at a time 19.5)
 template <bool VEC> __global__ void __launch_bounds__(RL_T) k_logit_rules(const RlArgs a, int *fault) {
     constexpr int V = VEC ? 4 : 1, STEPS = RL_N / (RL_T * V);
     __shared__ __align__(16) int cnt[RL_N];
