@@ -447,6 +447,53 @@ void krh_logit_rules(float *out, size_t ldo, const float *logits, size_t ld, int
                      const int *bias_id, const float *bias, size_t bias_ld, const int *n_bias, const uint32_t *masks,
                      int n_masks);
 
+/* ---- 8-bit products with a scale a token and a scale an output ----
+ * No counterpart in the reference, whose products have a scale every 32 values: a
+ * matrix as krh_quantize_row_rows leaves its rows, and tokens as that call or
+ * krh_block_norm leaves them. */
+typedef struct {
+    const int8_t *q;    /* [rows] rows ld apart, 16-byte aligned, all of rows * ld readable; what lies behind a row's
+                         * cols values may be anything */
+    const float *d;     /* [rows] */
+    size_t ld;          /* a multiple of 16 */
+    int rows, cols;     /* cols up to 131071, whose sums end within 32 bits */
+} krh_mat8;
+/* Y[t * ldy + r] = S xd[t] W->d[r] + bias[r], S = sum_k W->q[r][k] xq[t * ldx + k]
+ * the whole number; accumulate != 0: added to Y. T tokens (up to KRH_ROWS_MAX), xq
+ * as a matrix's rows: 16-byte aligned, ldx a multiple of 16, all of T * ldx
+ * readable. bias may be NULL. The same bits for every T: S to a float, times xd,
+ * times d, then the bias, then Y. Y overlaps no input. Allocates nothing; can be
+ * captured. */
+void krh_matmul_i8(float *Y, size_t ldy, const krh_mat8 *W, const int8_t *xq, size_t ldx, const float *xd,
+                   const float *bias, int T, int accumulate);
+/* H[t * ldh + r] = silu(g) u of the two products g (w1) and u (w3) of the same
+ * sizes, as krh_matmul_i8 and krh_silu_mul leave it */
+void krh_matmul_i8_swiglu(float *H, size_t ldh, const krh_mat8 *w1, const krh_mat8 *w3, const int8_t *xq, size_t ldx,
+                          const float *xd, int T);
+
+/* ---- between two blocks of a layer ----
+ * The norm of a block's output, its gate, the residual add and the next block's
+ * norm, for `rows` rows of n <= 16384 (the family steps' krh_rmsnorm_rows and
+ * krh_add_rows in one launch, with gate and scale, and 8-bit rows):
+ *
+ *   x' = x + alpha (gate (y / rms(y)) post)     xo = x'
+ *   z  = (x' / rms(x')) pre                     z, or q and d: z's 8-bit row and its scale
+ *
+ * rms(v) = sqrt(mean v^2 + eps), the mean in 64 bits, its reciprocal rounded to 32;
+ * the products from the left, each rounded, alpha last. Without y x' is x; post, gate (ldg 0: one
+ * for all rows) and pre may be NULL: without those factors, and without pre neither z nor q. Outputs
+ * that are NULL are not stored; q and d come together, as krh_quantize_row_rows
+ * leaves z, but that a row with a NaN has the scale NaN. xo and z may be x or y
+ * with its stride; nothing else overlaps. Any alignment; rows that are all 16-byte
+ * aligned (q 4) with strides and n multiples of 4 are read and written four values
+ * at a time. Allocates nothing; can be captured. */
+void krh_block_norm(float *xo, size_t ldxo, const float *x, size_t ldx, const float *y, size_t ldy, const float *post,
+                    const float *gate, size_t ldg, float alpha, const float *pre, float eps, float *z, size_t ldz,
+                    int8_t *q, size_t ldq, float *d, int n, int rows);
+/* such rows back as floats: x[r * ldx + i] = q[r * ldq + i] d[r * ldd], i < n */
+void krh_dequantize_row_rows(float *x, size_t ldx, const int8_t *q, size_t ldq, const float *d, size_t ldd, int n,
+                             int rows);
+
 /* ---- the reference's unfused kernels (the ml_k_<op>_hip op table) ----
  * Each computes the scalar kernel of kernels/scalar/k_scalar.c in its float
  * order, on device pointers. */

@@ -59,6 +59,11 @@ class KrhPages(C.Structure):
                 ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
 
 
+class KrhMat8(C.Structure):
+    """krh_mat8: an int8 matrix with a scale a row, device pointers"""
+    _fields_ = [("q", C.c_void_p), ("d", C.c_void_p), ("ld", C.c_size_t), ("rows", C.c_int), ("cols", C.c_int)]
+
+
 class LogitRule(C.Structure):
     """krh_logit_rule: one row's penalties and token mask"""
     _fields_ = [("repeat", C.c_float), ("presence", C.c_float), ("frequency", C.c_float), ("mask", C.c_int)]
@@ -197,6 +202,11 @@ for name, res, args in [
                                C.c_int, _P, C.c_int, _P, _P, C.c_size_t, _P]),
     ("krh_logit_rules", None, [_P, C.c_size_t, _P, C.c_size_t, C.c_int, C.c_int, _P, _P, C.c_size_t, _P, _P, _P,
                                C.c_size_t, _P, _P, C.c_int]),
+    ("krh_matmul_i8", None, [_P, C.c_size_t, C.POINTER(KrhMat8), _P, C.c_size_t, _P, _P, C.c_int, C.c_int]),
+    ("krh_matmul_i8_swiglu", None, [_P, C.c_size_t, C.POINTER(KrhMat8), C.POINTER(KrhMat8), _P, C.c_size_t, _P, C.c_int]),
+    ("krh_block_norm", None, [_P, C.c_size_t, _P, C.c_size_t, _P, C.c_size_t, _P, _P, C.c_size_t, C.c_float, _P, C.c_float,
+                              _P, C.c_size_t, _P, C.c_size_t, _P, C.c_int, C.c_int]),
+    ("krh_dequantize_row_rows", None, [_P, C.c_size_t, _P, C.c_size_t, _P, C.c_size_t, C.c_int, C.c_int]),
     ("krh_tanhf_range", None, [_P, C.c_uint32, C.c_size_t]),
     ("krh_rmsnorm_q8_t", None, [_P, _P, C.c_int, _P, _P, _P, C.c_int, C.c_float, C.c_int]),
     ("krh_quantize_q8_t", None, [_P, _P, C.c_int, _P, C.c_int, C.c_int]),

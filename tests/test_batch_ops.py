@@ -1,0 +1,73 @@
+"""8-bit products, the norms between blocks and the attention over shared rows
+without a device: what the calls refuse."""
+import ctypes as C
+
+import pytest
+
+import krafla as K
+
+PTR = 0x100000   # an address that a refused call never reads
+
+
+def mat(**kw):
+    return K.KrhMat8(**dict(dict(q=PTR, d=PTR, ld=64, rows=24, cols=50), **kw))
+
+
+I8 = dict(Y=PTR, ldy=24, W=mat(), xq=PTR, ldx=64, xd=PTR, bias=PTR, T=3, accumulate=0)
+GLU = dict(H=PTR, ldh=24, w1=mat(), w3=mat(), xq=PTR, ldx=64, xd=PTR, T=3)
+NORM = dict(xo=PTR, ldxo=64, x=PTR, ldx=64, y=PTR + 4096, ldy=64, post=PTR, gate=PTR, ldg=0, alpha=1.0, pre=PTR, eps=1e-6,
+            z=PTR + 8192, ldz=64, q=PTR, ldq=64, d=PTR, n=64, rows=3)
+DEQ = dict(x=PTR, ldx=64, q=PTR, ldq=64, d=PTR, ldd=1, n=64, rows=3)
+
+BAD_MATS = [dict(q=None), dict(d=None), dict(q=PTR + 8), dict(ld=48), dict(ld=56), dict(rows=0), dict(rows=-1),
+            dict(rows=2**31 - 1), dict(cols=0), dict(cols=-5), dict(cols=65), dict(cols=1 << 17, ld=1 << 17)]
+
+CASES = [("krh_matmul_i8", I8, kw) for kw in
+         [dict(Y=None), dict(xq=None), dict(xd=None), dict(W=None), dict(T=-1), dict(T=70000), dict(ldy=23), dict(ldx=48),
+          dict(ldx=72), dict(xq=PTR + 4)] + [dict(W=mat(**b)) for b in BAD_MATS]]
+CASES += [("krh_matmul_i8_swiglu", GLU, kw) for kw in
+          [dict(H=None), dict(xq=None), dict(xd=None), dict(w1=None), dict(w3=None), dict(T=-1), dict(T=70000), dict(ldh=23),
+           dict(ldx=48), dict(ldx=72), dict(xq=PTR + 8), dict(w3=mat(rows=25)), dict(w1=mat(cols=49))] +
+          [dict(w1=mat(**b)) for b in BAD_MATS] + [dict(w3=mat(**b)) for b in BAD_MATS]]
+CASES += [("krh_block_norm", NORM, kw) for kw in
+          [dict(x=None), dict(xo=None, z=None, q=None, d=None), dict(pre=None), dict(y=None), dict(q=None), dict(d=None),
+           dict(n=0), dict(n=16385), dict(rows=-1), dict(rows=70000), dict(ldx=63), dict(ldxo=63, xo=PTR + 64), dict(ldy=60),
+           dict(ldg=32), dict(ldz=8), dict(ldq=63), dict(ldxo=68), dict(z=PTR, ldz=68), dict(z=PTR + 4096, ldz=68),
+           dict(xo=PTR + 4096, ldxo=72)]]
+CASES += [("krh_dequantize_row_rows", DEQ, kw) for kw in
+          [dict(x=None), dict(q=None), dict(d=None), dict(n=-1), dict(rows=-1), dict(rows=70000), dict(ldx=63)]]
+
+
+def call(name, args, **kw):
+    a = dict(args, **kw)
+    K.hip.krh_clear_error()
+    getattr(K.hip, name)(*[C.byref(v) if isinstance(v, C.Structure) else v for v in a.values()])
+    st = K.hip.krh_status()
+    K.hip.krh_clear_error()
+    return st
+
+
+@pytest.mark.parametrize("name,base,kw", CASES, ids=["%s-%d" % (n[4:], i) for i, (n, _, _) in enumerate(CASES)])
+def test_refused(name, base, kw):
+    assert call(name, base, **kw) == K.ML_E_SHAPE
+
+
+def test_nothing_to_do():
+    assert call("krh_matmul_i8", I8, T=0) == K.ML_OK
+    assert call("krh_matmul_i8_swiglu", GLU, T=0) == K.ML_OK
+    assert call("krh_block_norm", NORM, rows=0) == K.ML_OK
+    assert call("krh_dequantize_row_rows", DEQ, rows=0) == K.ML_OK
+    assert call("krh_dequantize_row_rows", DEQ, n=0) == K.ML_OK
+
+
+def test_before_init():
+    """without a device a good call is refused, not launched"""
+    if K.hip.krh_device_cus() > 0:
+        pytest.skip("the device is open")
+    for name, base, more in (("krh_matmul_i8", I8, [dict(bias=None), dict(accumulate=1)]), ("krh_matmul_i8_swiglu", GLU, []),
+                             ("krh_block_norm", NORM, [dict(y=None, post=None, gate=None), dict(q=None, d=None),
+                                                       dict(pre=None, z=None, q=None, d=None), dict(xo=None), dict(rows=1, ldxo=68),
+                                                       dict(ldg=64)]),
+                             ("krh_dequantize_row_rows", DEQ, [dict(rows=1, ldx=0)])):
+        for kw in [{}] + more:
+            assert call(name, base, **kw) == K.ML_E_ISA, (name, kw)
