@@ -407,6 +407,28 @@ size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int m
 void krh_paged_attention(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len, int n_seq,
                          const float *q, int n_heads, int max_len, int window, float scale, float softcap,
                          float *mass, size_t mass_ld, void *ws);
+/* Bytes of workspace that krh_paged_attention_shared takes for these sizes and
+ * any window (0 for sizes that it refuses) */
+size_t krh_paged_attention_shared_ws(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_groups,
+                                     int max_shared);
+/* krh_paged_attention of sequences that begin alike (a common prompt's pages),
+ * the common rows read once for all of them. Sequences group[g] .. group[g + 1] - 1,
+ * g < n_groups <= 64, share their first shared[g] <= max_shared rows: their tables
+ * name the same pages for these, or pages of the same rows, and the first one's
+ * are read, as far as any of the group attends; len counts them. group ascends
+ * within [0, n_seq]; sequences before group[0] and from group[n_groups] on share
+ * nothing. group and shared are device data, checked as lengths and sequences are;
+ * max_shared sizes the launch. A sequence may be shorter than its group's shared
+ * rows, or have none.
+ *
+ * The results are krh_paged_attention's to rounding, the same from call to call;
+ * what that call states of arguments, precision and not finite values holds here
+ * too, but that a NaN or an infinite value in a shared row that some sequence
+ * attends may reach its group's other heads of the KV head. */
+void krh_paged_attention_shared(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len,
+                                int n_seq, const int *group, const int *shared, int n_groups, int max_shared,
+                                const float *q, int n_heads, int max_len, int window, float scale, float softcap,
+                                void *ws);
 /* Bytes of workspace that krh_paged_evict takes (0 for sizes that it refuses) */
 size_t krh_paged_evict_ws(int n_seq, int n_kv_heads, int keep);
 /* Eviction by accumulated weight. Of sequence s's len[s] <= max_len <= 2^29 rows

@@ -1,0 +1,696 @@
+// Attention of one token of each sequence over a paged cache in which groups of
+// sequences begin with the same rows (krh_paged_attention_shared).
+//
+// With few sequences a shared row is read by each (krh_paged_attention); with
+// many a group's shared rows are passed over once for all of its query heads
+// (k_shared_rows), its sequences' own rows as krh_paged_attention passes over a
+// window (kr_paged_wave.h), and a last launch joins the parts: with each part's
+// maximum m (in log2), sum l and unscaled output o, out = sum 2^(m - M) o / sum 2^(m - M) l.
+//
+// The shared rows are a matrix product with as many columns as the group has
+// query heads of the KV head. A workgroup's waves have 32 columns each and the
+// same rows, 32 at a time, which pass through LDS: S^T = K Q^T has rows as rows, so
+// the lane that holds a column's scores of rows 4 h + 8 j + (0..3), h its half of
+// the wave, has them as the operand P^T of O^T = V^T P^T as they are, in the order
+// of rows in which V is laid down transposed (F32: a float is an operand by itself,
+// so V's rows lie as they are). All products are those of kr_paged_wave.h: a float operand
+// is two halves, x = hi + lo, F32 caches take the 32-bit product.
+//
+// The tiles of all (group, column tile) pairs are cut into equal shares, one a
+// workgroup and KV head, by the lengths that the device has; a share's sums of a
+// column tile are a part.
+#include <cfloat>
+#include "kr_paged_wave.h"
+
+namespace {
+
+typedef float float16v __attribute__((ext_vector_type(16)));
+
+constexpr int SH_R = 32;   // rows a tile
+struct ShArgs : PaShared {
+    float *spart, *spml;   // [n_kv][column tiles + shares][CT][hd] and [2]: the shared rows' parts
+    int sshares, sleast, slots, ct;   // ct: columns of a workgroup
+    int *fault;
+};
+
+// The groups, one a lane
+struct ShGroups {
+    int s0, s1, rows;   // sequences [s0, s1), which share `rows` rows
+};
+// Starts that do not ascend within the batch leave no group; a group of one sequence is none.
+__device__ __forceinline__ ShGroups sh_groups(const PgView &p, const PaShared &a, int &bad) {
+    const int g = (int)(threadIdx.x & 63), i = min(g, a.n_groups - 1);
+    ShGroups r = { a.group[i], a.group[i + 1], kr_page_len(a.shared[i], a.max_shared, bad) };
+    if (__any(r.s0 < 0 || r.s1 < r.s0 || r.s1 > p.n_seq)) {
+        bad |= KR_BAD_SEQ;
+        r.s0 = r.s1 = 0;
+    }
+    if (g >= a.n_groups || r.s1 - r.s0 < 2) r.rows = 0;
+    return r;
+}
+__device__ __forceinline__ int pa_skip(const PgView &p, const PaShared &a, int i, int &bad) {
+    const ShGroups r = sh_groups(p, a, bad);
+    int skip = 0;
+    for (int g = 0; g < a.n_groups; g++) {
+        const int rows = __builtin_amdgcn_readlane(r.rows, g);
+        if (i >= __builtin_amdgcn_readlane(r.s0, g) && i < __builtin_amdgcn_readlane(r.s1, g)) skip = rows;
+    }
+    return skip;
+}
+
+// The tiles of the groups, one group a lane: `cts` column tiles of the rows from
+// `begin` on in `rts` row tiles; `sum`, `csum`: inclusive sums of all tiles and of
+// the column tiles
+struct ShTiles {
+    ShGroups g;
+    int begin, rts, cts, sum, csum, shares;
+};
+__device__ __forceinline__ ShTiles sh_tiles(const PgView &p, const ShArgs &a, int &bad) {
+    ShTiles r;
+    r.g = sh_groups(p, a, bad);
+    const int lane = (int)(threadIdx.x & 63), group = a.nh / p.n_kv;
+    r.begin = 0;
+    if (a.window > 0) {
+        // of a window the first row that any sequence of the group attends
+        for (int g = 0; g < a.n_groups; g++) {
+            if (__builtin_amdgcn_readlane(r.g.rows, g) == 0) continue;
+            const int s1 = __builtin_amdgcn_readlane(r.g.s1, g);
+            int least = INT_MAX;
+            for (int s = __builtin_amdgcn_readlane(r.g.s0, g) + lane; s < s1; s += 64) {
+                const int len = kr_page_len(a.len[s], a.max_len, bad);
+                if (len > 0) least = min(least, max(0, len - a.window));
+            }
+            for (int o = 32; o >= 1; o >>= 1) least = min(least, __shfl_xor(least, o));
+            if (lane == g) r.begin = min(least, r.g.rows) & -SH_R;
+        }
+    }
+    r.rts = (r.g.rows - r.begin + SH_R - 1) / SH_R;
+    r.cts = r.g.rows > 0 ? ((r.g.s1 - r.g.s0) * group + a.ct - 1) / a.ct : 0;
+    r.sum = pg_scan(r.rts * r.cts);
+    r.csum = pg_scan(r.cts);
+    const int all = __builtin_amdgcn_readlane(r.sum, 63);
+    r.shares = max(1, min(a.sshares, (all + a.sleast - 1) / a.sleast));
+    return r;
+}
+
+__device__ __forceinline__ float sh_other(float v) {   // the same column's value in the other half of the wave
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(threadIdx.x & 32 ? s[0] : s[1]);
+}
+
+template <int KT, int CL> struct ShLds {
+    static constexpr int EB = KT == PG_F32 ? 4 : 2;
+    alignas(16) char k[2][SH_R * CL * EB];
+    alignas(16) char v[2][SH_R * CL * EB];
+    alignas(16) float kd[2][KT == PG_Q8 ? SH_R : 4], vd[2][KT == PG_Q8 ? SH_R : 4];
+    int range[2];
+};
+
+// where 16 bytes of a K row lie (F32: of a V row too): 16 rows of one chunk in all banks
+template <int NC> __device__ __forceinline__ int sh_at(int row, int c) {
+    return (row * NC + (c ^ (NC >= 16 ? row & 15 : (row >> 1) & 7))) * 16;
+}
+// 4 rows (8 c16 + 4 h + 16 s + 0..3, quad = 4 s + 2 p + h) of one dim of V in halves
+__device__ __forceinline__ int sh_vt(int dim, int chunk) { return dim * 64 + ((chunk ^ ((dim >> 2) & 3)) << 4); }
+
+constexpr int sh_waves(int kt, int cl, int wc) { return wc == 1 || cl > 128 || (kt == PG_F32 && cl > 64) ? 1 : 2; }   // a SIMD
+
+template <int KT, int CL, int WC> struct ShWork {
+    static constexpr bool HALF = KT != PG_F32;
+    static constexpr int NTH = 64 * WC, CT = 32 * WC;
+    static constexpr int KC = HALF ? CL / 8 : CL / 4;          // LDS chunks of 16 bytes a row
+    static constexpr int KN = (SH_R * KC + NTH - 1) / NTH;     // K chunks a thread
+    static constexpr int VU = HALF ? 8 * (CL / 4) : SH_R * KC; // V's pieces: 4 rows of 4 dims, or a chunk
+    static constexpr int VN = (VU + NTH - 1) / NTH;
+    static constexpr int KW = KT == PG_Q8 ? 2 : 4;             // words of a K chunk in the pool
+    static constexpr int VW = KT == PG_F32 ? 4 : KT == PG_F16 ? 8 : 4;
+    static constexpr int KS = HALF ? CL / 16 : CL / 8;         // K operands of a row
+    static constexpr int DT = CL / 32;
+
+    const PgView &p;
+    const ShArgs &a;
+    ShLds<KT, CL> &lds;
+    const int lane, h, wave, kvh, hd, group;
+    int bad;
+    // the piece: rows [row0, row1) in tiles, of which [vf, vl) are attended by a column here
+    int lead, vf, vl;
+    bool live;
+    int first, last, wf, wl;   // the column's rows; all columns of the wave have [wf, wl)
+    int ids, ids_at;
+    unsigned kr[KN][KW], vr[VN][VW];
+    float sr;
+    std::conditional_t<HALF, half8, float4v> qf[KS][HALF ? 2 : 1];
+    float cs, m_run, l_run, v_run, v_end;
+    int ev;
+    float16v o[DT];
+
+    __device__ __forceinline__ ShWork(const PgView &p_, const ShArgs &a_, ShLds<KT, CL> &l, int kvh_)
+        : p(p_), a(a_), lds(l), lane(threadIdx.x & 63), h(lane >> 5),
+          wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))), kvh(kvh_), hd(p_.hd), group(a_.nh / p_.n_kv), bad(0) {}
+
+    // this lane's column: head `head` of all, or none
+    __device__ __forceinline__ void column(int s0, int s1, int rows, int ct, size_t &head) {
+        const int c = ct * CT + wave * 32 + (lane & 31), s = s0 + c / group;
+        live = s < s1;
+        head = live ? (size_t)s * a.nh + kvh * group + c % group : (size_t)s0 * a.nh + kvh * group;
+        const int len = live ? kr_page_len(a.len[s], a.max_len, bad) : 0;
+        last = min(len, rows);
+        first = a.window > 0 && len > a.window ? min(len - a.window, rows) : 0;
+        const bool some = live && first < last;
+        int f = some ? first : INT_MAX, l = some ? last : 0;
+        wf = live ? first : 0;
+        wl = live ? last : INT_MAX;
+        for (int o = 16; o >= 1; o >>= 1) {
+            f = min(f, __shfl_xor(f, o));
+            l = max(l, __shfl_xor(l, o));
+            wf = max(wf, __shfl_xor(wf, o));
+            wl = min(wl, __shfl_xor(wl, o));
+        }
+        wf = __builtin_amdgcn_readfirstlane(wf);
+        wl = __builtin_amdgcn_readfirstlane(wl);
+        __syncthreads();   // the piece before has been read
+        if (threadIdx.x == 0) lds.range[0] = INT_MAX, lds.range[1] = 0;
+        __syncthreads();
+        if (lane == 0) {
+            atomicMin(&lds.range[0], f);
+            atomicMax(&lds.range[1], l);
+        }
+        __syncthreads();
+        vf = __builtin_amdgcn_readfirstlane(lds.range[0]);
+        vl = __builtin_amdgcn_readfirstlane(lds.range[1]);
+    }
+
+    // the pages of the 64 half tiles from r0 on
+    __device__ __forceinline__ void find(int r0) {
+        ids_at = r0;
+        const int r = r0 + 16 * lane;
+        ids = r + 16 > vf && r < vl ? pg_page(p, lead, r, bad) : -1;
+    }
+
+    // asks for the rows of the tile at r0
+    __device__ __forceinline__ void fetch(int r0) {
+        if (r0 - ids_at >= 64 * 16) find(r0);
+        const int i = (r0 - ids_at) >> 4;
+        const int a0 = __builtin_amdgcn_readlane(ids, i), a1 = __builtin_amdgcn_readlane(ids, i + 1);
+        const size_t lo = kr_page_row(max(a0 >= 0 ? a0 : a1, 0), p.n_kv, kvh, p.shift, r0);
+        const size_t hi = kr_page_row(max(a1 >= 0 ? a1 : a0, 0), p.n_kv, kvh, p.shift, r0 + 16) - 16;
+        constexpr int EB = KT == PG_F32 ? 4 : KT == PG_F16 ? 2 : 1, KD = HALF ? 8 : 4;
+#pragma unroll
+        for (int j = 0; j < KN; j++) {
+            const int u = j * NTH + (int)threadIdx.x, row = u / KC, d = u % KC * KD;
+            // past the head's dims: zeros, which meet the queries' zeros
+#pragma unroll
+            for (int w = 0; w < KW; w++) kr[j][w] = 0;
+            if ((SH_R * KC % NTH == 0 || row < SH_R) && d < hd)
+                pa_load(kr[j], (const char *)p.k + ((row < 16 ? lo : hi) + row) * hd * EB + d * EB);
+        }
+#pragma unroll
+        for (int j = 0; j < VN; j++) {
+            const int u = j * NTH + (int)threadIdx.x;
+#pragma unroll
+            for (int w = 0; w < VW; w++) vr[j][w] = 0;
+            if (VU % NTH != 0 && u >= VU) continue;
+            if constexpr (HALF) {
+                const int quad = u / (CL / 4), d = u % (CL / 4) * 4;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int row = quad * 4 + i;
+                    unsigned x[VW / 4] = {};
+                    // rows that no column attends may hold anything
+                    if (d < hd && r0 + row >= vf && r0 + row < vl)
+                        pa_load(x, (const char *)p.v + ((row < 16 ? lo : hi) + row) * hd * EB + d * EB);
+#pragma unroll
+                    for (int w = 0; w < VW / 4; w++) vr[j][i * (VW / 4) + w] = x[w];
+                }
+            } else {
+                const int row = u / KC, d = u % KC * 4;
+                if (d < hd && r0 + row >= vf && r0 + row < vl)
+                    pa_load(vr[j], (const char *)p.v + ((row < 16 ? lo : hi) + row) * hd * EB + d * EB);
+            }
+        }
+        if constexpr (KT == PG_Q8) {
+            const int row = lane & 31;
+            sr = 0.0f;
+            if (wave == 0 && r0 + row >= vf && r0 + row < vl)
+                sr = (lane < 32 ? p.kd : p.vd)[(row < 16 ? lo : hi) + row];
+        }
+    }
+
+    // and lays them down
+    __device__ __forceinline__ void put(int buf) {
+#pragma unroll
+        for (int j = 0; j < KN; j++) {
+            const int u = j * NTH + (int)threadIdx.x, row = u / KC, c = u % KC;
+            if (SH_R * KC % NTH != 0 && row >= SH_R) continue;
+            uint4v w;
+            if constexpr (KT == PG_Q8) {
+                const unsigned x = kr[j][0] ^ 0x80808080u, y = kr[j][1] ^ 0x80808080u;
+                w = uint4v{ pa_h2(x, 0x04010400), pa_h2(x, 0x04030402), pa_h2(y, 0x04010400), pa_h2(y, 0x04030402) };
+            } else {
+                w = uint4v{ kr[j][0], kr[j][1], kr[j][2], kr[j][3] };
+            }
+            *(uint4v *)(lds.k[buf] + sh_at<KC>(row, c)) = w;
+        }
+#pragma unroll
+        for (int j = 0; j < VN; j++) {
+            const int u = j * NTH + (int)threadIdx.x;
+            if (VU % NTH != 0 && u >= VU) continue;
+            if constexpr (HALF) {
+                const int quad = u / (CL / 4), d = u % (CL / 4) * 4;
+                const int chunk = (quad >> 2) * 2 + (quad & 1), half = (quad >> 1) & 1;
+                uint2v t[4];
+                if constexpr (KT == PG_F16) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const unsigned sel = c & 1 ? 0x07060302u : 0x05040100u;
+                        t[c] = uint2v{ __builtin_amdgcn_perm(vr[j][2 + c / 2], vr[j][c / 2], sel),
+                                       __builtin_amdgcn_perm(vr[j][6 + c / 2], vr[j][4 + c / 2], sel) };
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const unsigned x = vr[j][2 * i] ^ 0x80808080u, y = vr[j][2 * i + 1] ^ 0x80808080u;
+                        const unsigned lo = __builtin_amdgcn_perm(y, x, 0x05010400u), hi = __builtin_amdgcn_perm(y, x, 0x07030602u);
+                        t[0][i] = pa_h2(lo, 0x04010400);
+                        t[1][i] = pa_h2(lo, 0x04030402);
+                        t[2][i] = pa_h2(hi, 0x04010400);
+                        t[3][i] = pa_h2(hi, 0x04030402);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++) *(uint2v *)(lds.v[buf] + sh_vt(d + c, chunk) + 8 * half) = t[c];
+            } else {
+                const int row = u / KC, c = u % KC;
+                // rows 4 apart, which the two halves of a wave read together, in different banks
+                *(uint4v *)(lds.v[buf] + (row * KC + (c ^ ((row >> 2 & 1) << 3))) * 16) =
+                    uint4v{ vr[j][0], vr[j][1], vr[j][2], vr[j][3] };
+            }
+        }
+        if constexpr (KT == PG_Q8) {
+            if (wave == 0) (lane < 32 ? lds.kd : lds.vd)[buf][lane & 31] = sr;
+        }
+    }
+
+    __device__ __forceinline__ void queries(size_t head) {
+        const float *q = a.q + head * hd;
+        int e = 0;
+        if constexpr (HALF) {
+            float x[KS][8], m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                const int d = j * 16 + h * 8;
+#pragma unroll
+                for (int i = 0; i < 8; i += 4) {
+                    const float4v t = live && d < hd ? *(const float4v *)(q + d + i) : float4v{ 0, 0, 0, 0 };
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        x[j][i + c] = t[c];
+                        m = fmaxf(m, fabsf(t[c]));
+                    }
+                }
+            }
+            m = fmaxf(m, sh_other(m));
+            if (m > 0.0f && m < INFINITY) e = 13 - ilogbf(m);
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                half8 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float y = ldexpf(x[j][i], e);
+                    hi[i] = (_Float16)y;
+                    lo[i] = (_Float16)(y - (float)hi[i]);
+                }
+                qf[j][0] = hi;
+                qf[j][1] = lo;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                const int d = j * 8 + h * 4;
+                qf[j][0] = live && d < hd ? *(const float4v *)(q + d) : float4v{ 0, 0, 0, 0 };
+            }
+        }
+        cs = ldexpf(a.cap > 0.0f ? a.scale : a.scale * 1.4426950408889634f, -e);
+    }
+
+    // the tile at row r0, in LDS
+    __device__ __forceinline__ void tile(int buf, int r0) {
+        float16v s = {};
+#pragma unroll
+        for (int j = 0; j < KS; j++) {
+            const uint4v w = *(const uint4v *)(lds.k[buf] + sh_at<KC>(lane & 31, 2 * j + h));
+            if constexpr (HALF) {
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, w), qf[j][x], s, 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[c]), qf[j][0][c], s, 0, 0, 0);
+            }
+        }
+        // value i is row (i & 3) + 8 (i >> 2) + 4 h
+        if constexpr (KT == PG_Q8) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float4v d = *(const float4v *)(lds.kd[buf] + 2 * i + 4 * h);
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[i + c] *= cs * d[c];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[i] *= cs;
+        }
+        if (a.cap > 0.0f) {
+            const float inv_cap = 1.0f / a.cap;
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[i] = pa_tanh(s[i] * inv_cap) * (a.cap * 1.4426950408889634f);
+        }
+        if (r0 < wf || r0 + SH_R > wl) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int r = r0 + (i & 3) + 8 * (i >> 2) + 4 * h;
+                s[i] = r >= first && r < last ? s[i] : -INFINITY;
+            }
+        }
+        float m_tile = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; i++) m_tile = fmaxf(m_tile, s[i]);
+        const bool moved = __any(m_tile > m_run);
+        float f = 1.0f;
+        if (moved) {
+            const float m_new = fmaxf(m_run, fmaxf(m_tile, sh_other(m_tile)));
+            f = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= f;
+        }
+        const float base = m_run == -INFINITY ? 0.0f : m_run;
+        float v_tile = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            s[i] = __builtin_amdgcn_exp2f(s[i] - base);
+            l_run += s[i];
+        }
+        if constexpr (KT == PG_Q8) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float4v d = *(const float4v *)(lds.vd[buf] + 2 * i + 4 * h);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    // a rounded product: hi and lo are of the same value
+                    float x = s[i + c] * d[c];
+                    asm("" : "+v"(x));
+                    s[i + c] = x;
+                    v_tile = fmaxf(v_tile, fabsf(x));
+                }
+            }
+            // what the weights times their scales are over, as kr_paged_wave.h has it
+            if (moved || __any(v_tile >= v_end)) {
+                v_run = fmaxf(v_run * f, fmaxf(v_tile, sh_other(v_tile)));
+                const int e = max(PA_EV, (int)(__float_as_uint(v_run) >> 23) - 126);
+                f = ldexpf(f, ev - e);
+                ev = e;
+                v_end = ldexpf(1.0f, e);
+#pragma unroll
+                for (int t = 0; t < DT; t++) o[t] *= f;
+            }
+        } else if (moved) {
+#pragma unroll
+            for (int t = 0; t < DT; t++) o[t] *= f;
+        }
+        if constexpr (HALF) {
+            const float up = KT == PG_Q8 ? ldexpf(1.0f, PA_UP - ev) : (float)(1 << PA_UP);
+            half8 w[2][2];   // [16 rows][hi, lo]
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float x = s[i] * up;
+                const _Float16 hi = (_Float16)x;
+                w[i >> 3][0][i & 7] = hi;
+                w[i >> 3][1][i & 7] = (_Float16)(x - (float)hi);
+            }
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const half8 v = *(const half8 *)(lds.v[buf] + sh_vt(32 * t + (lane & 31), 2 * c + h));
+#pragma unroll
+                    for (int x = 0; x < 2; x++) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[c][x], o[t], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int row = (i & 3) + 8 * (i >> 2) + 4 * h, dim = 32 * t + (lane & 31);
+                    const float v = *(const float *)(lds.v[buf] + (row * KC + ((dim >> 2) ^ ((row >> 2 & 1) << 3))) * 16 + (dim & 3) * 4);
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[i], o[t], 0, 0, 0);
+                }
+        }
+    }
+
+    // row tiles at rows [r0, r1) of a group's column tile ct, and the part's sums
+    __device__ __forceinline__ void part(int s0, int s1, int rows, int ct, int r0, int r1, size_t slot) {
+        size_t head;
+        column(s0, s1, rows, ct, head);
+        lead = s0;
+        m_run = -INFINITY;
+        l_run = 0.0f;
+        ev = PA_EV;
+        v_run = v_end = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; t++) o[t] = float16v{};
+        // tiles that no column here attends are passed over
+        r0 = max(r0, vf & -SH_R);
+        r1 = min(r1, vl);
+        if (r0 < r1) {
+            find(r0);
+            fetch(r0);
+            queries(head);
+            put(0);
+            __syncthreads();
+            for (int buf = 0; r0 < r1; r0 += SH_R, buf ^= 1) {
+                const bool more = r0 + SH_R < r1;
+                if (more) fetch(r0 + SH_R);
+                tile(buf, r0);
+                if (more) put(buf ^ 1);
+                __syncthreads();
+            }
+        }
+        const float l = l_run + sh_other(l_run);
+        const float f = HALF ? ldexpf(1.0f, KT == PG_Q8 ? ev - PA_UP : -PA_UP) : 1.0f;
+        if (!live) return;
+        const size_t at = slot * CT + wave * 32 + (lane & 31);
+        if (h == 0) *(float2v *)(a.spml + at * 2) = float2v{ m_run, l };
+        float *out = a.spart + at * hd;
+#pragma unroll
+        for (int t = 0; t < DT; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int d = 32 * t + 2 * i + 4 * h;
+                if (d < hd) *(float4v *)(out + d) = float4v{ o[t][i] * f, o[t][i + 1] * f, o[t][i + 2] * f, o[t][i + 3] * f };
+            }
+    }
+};
+
+template <int KT, int CL, int WC>
+__global__ void __launch_bounds__(64 * WC, sh_waves(KT, CL, WC)) k_shared_rows(const PgView p, const ShArgs a) {
+    __shared__ ShLds<KT, CL> lds;
+    const int u = blockIdx.x, kvh = blockIdx.y;
+    ShWork<KT, CL, WC> w(p, a, lds, kvh);
+    const ShTiles all = sh_tiles(p, a, w.bad);
+    const int tiles = __builtin_amdgcn_readlane(all.sum, 63);
+    if (u < all.shares && tiles > 0) {
+        const int end = (int)((long long)tiles * (u + 1) / all.shares);
+        for (int t = (int)((long long)tiles * u / all.shares); t < end;) {
+            const int g = __popcll(__ballot(all.sum <= t));
+            const int rts = __builtin_amdgcn_readlane(all.rts, g), cts = __builtin_amdgcn_readlane(all.cts, g);
+            const int at = t - (__builtin_amdgcn_readlane(all.sum, g) - rts * cts), ct = at / rts, r = at % rts;
+            const int n = min(rts - r, end - t), begin = __builtin_amdgcn_readlane(all.begin, g);
+            const int rows = __builtin_amdgcn_readlane(all.g.rows, g);
+            const size_t slot = (size_t)kvh * a.slots + __builtin_amdgcn_readlane(all.csum, g) - cts + ct + u;
+            w.part(__builtin_amdgcn_readlane(all.g.s0, g), __builtin_amdgcn_readlane(all.g.s1, g), rows, ct, begin + r * SH_R,
+                   min(rows, begin + (r + n) * SH_R), slot);
+            t += n;
+        }
+    }
+    kr_report(a.fault, w.bad);
+}
+
+template <int KT, int CL, bool FULL>
+__global__ void __launch_bounds__(64, pa_waves(KT, CL)) k_shared_own(const PgView p, const PaShared a, int *fault) {
+    const int u = blockIdx.x, kvh = blockIdx.y;
+    PaWave<KT, CL, FULL, PaShared> w(p, a, kvh);
+    PaAll all = pa_all(p, a, w.bad);
+    if (u < all.shares) {
+        int left = pa_bound(all, u + 1) - pa_bound(all, u), t = pa_bound(all, u);
+        for (w.seq = pa_find(p, a, all, t, w.bad); left > 0; w.seq++, t = 0) {
+            w.sp = pa_of(p, a, all, w.seq, w.bad);
+            const int end = min(w.sp.tiles, t + left);
+            w.part(t, end, (size_t)kvh * (p.n_seq + a.shares) + w.seq + u);
+            left -= end - t;
+        }
+    }
+    kr_report(fault, w.bad);
+}
+
+// A head of a sequence a workgroup: its own rows' parts, then the shared ones'
+// (2^dl lanes hold its dims four at a time, the workgroup's other factor the parts
+// side by side)
+constexpr int SJ_T = 256;
+__global__ void __launch_bounds__(SJ_T) k_shared_join(const PgView p, const ShArgs a, int dl) {
+    __shared__ float4v s_o[SJ_T];
+    const int s = blockIdx.y, x = blockIdx.x, tid = threadIdx.x, group = a.nh / p.n_kv, kvh = x / group, col = x % group;
+    int bad = 0;   // reported by the other launches
+    PaSpan sp;
+    const PaParts r = pa_parts(p, a, s, kvh, sp);
+    const float *ml0 = a.pml + (r.slot * group + col) * 2, *part0 = a.part + (r.slot * group + col) * p.hd;
+    const float *ml1 = nullptr, *part1 = nullptr;
+    int n1 = 0;
+    const ShTiles all = sh_tiles(p, a, bad);
+    const unsigned long long in = __ballot(all.g.rows > 0 && s >= all.g.s0 && s < all.g.s1);
+    if (in) {
+        const int g = __builtin_ctzll(in), rts = __builtin_amdgcn_readlane(all.rts, g), cts = __builtin_amdgcn_readlane(all.cts, g);
+        const int c = (s - __builtin_amdgcn_readlane(all.g.s0, g)) * group + col, ct = c / a.ct;
+        if (rts > 0) {
+            const int tiles = __builtin_amdgcn_readlane(all.sum, 63);
+            const int t0 = __builtin_amdgcn_readlane(all.sum, g) - rts * cts + ct * rts;
+            const auto share = [&](int t) { return (int)((((long long)t + 1) * all.shares - 1) / tiles); };
+            const int u0 = share(t0);
+            n1 = share(t0 + rts - 1) - u0 + 1;
+            const size_t slot = (size_t)kvh * a.slots + __builtin_amdgcn_readlane(all.csum, g) - cts + ct + u0;
+            ml1 = a.spml + (slot * a.ct + c % a.ct) * 2;
+            part1 = a.spart + (slot * a.ct + c % a.ct) * p.hd;
+        }
+    }
+    const int n = r.n + n1;
+    const auto get = [&](int i) {
+        return *(const float2v *)(i < r.n ? ml0 + (size_t)i * group * 2 : ml1 + (size_t)(i - r.n) * a.ct * 2);
+    };
+    const auto at = [&](int i) { return i < r.n ? part0 + (size_t)i * group * p.hd : part1 + (size_t)(i - r.n) * a.ct * p.hd; };
+    const int lane = tid & 63;
+    float m = -INFINITY, l = 0.0f;
+    for (int i = lane; i < n; i += 64) m = fmaxf(m, get(i).x);
+    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const auto weight = [&](float v) { return v == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v - m); };
+    for (int i = lane; i < n; i += 64) {
+        const float2v v = get(i);
+        l += v.y * weight(v.x);
+    }
+    for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
+    const float inv = sp.len == 0 ? 0.0f : 1.0f / l;
+    const int q = tid & ((1 << dl) - 1), lanes = SJ_T >> dl, d = 4 * q < p.hd ? 4 * q : 0;
+    float4v acc = { 0, 0, 0, 0 };
+    for (int i = tid >> dl; i < n; i += lanes) acc += *(const float4v *)(at(i) + d) * weight(get(i).x);
+    s_o[tid] = acc;
+    for (int k = lanes >> 1; k >= 1; k >>= 1) {
+        __syncthreads();
+        if ((tid >> dl) < k) s_o[tid] = acc = acc + s_o[tid + (k << dl)];
+    }
+    if (tid >> dl == 0 && 4 * q < p.hd) *(float4v *)(a.o + ((size_t)s * a.nh + x) * p.hd + d) = acc * inv;
+}
+
+// ---- the host's side ----
+
+constexpr int SH_CUS = 256;
+int sh_wc(const krh_pages *kv, int n_seq, int nh, int n_groups) {
+    const long long cols = ((long long)n_seq + n_groups - 1) / n_groups * (nh / kv->n_kv_heads);
+    return cols > 32 || kv->head_dim > 128 ? 4 : 1;
+}
+
+struct ShSizes {
+    int wc, shares, sshares, slots;
+    size_t part, pml, spart, spml;   // floats
+};
+ShSizes sh_sizes(const krh_pages *kv, int n_seq, int nh, int max_len, int n_groups, int max_shared) {
+    ShSizes r;
+    const int group = nh / kv->n_kv_heads;
+    r.wc = sh_wc(kv, n_seq, nh, n_groups);
+    const int ct = 32 * r.wc;
+    const long long cts = (long long)n_seq * group / ct + n_groups, tiles = cts * ((max_shared + SH_R - 1) / SH_R);
+    const long long waves = SH_CUS * 8 / r.wc / kv->n_kv_heads;
+    r.sshares = (int)(waves < 1 ? 1 : waves < tiles ? waves : tiles);
+    r.slots = (int)(cts + r.sshares);
+    r.shares = SH_CUS * 3 / kv->n_kv_heads > 0 ? SH_CUS * 3 / kv->n_kv_heads : 1;
+    const size_t own = (size_t)kv->n_kv_heads * (n_seq + r.shares) * group;
+    const size_t both = (size_t)kv->n_kv_heads * r.slots * ct;
+    r.part = own * kv->head_dim;
+    r.pml = (own * 2 + 3) & ~(size_t)3;
+    r.spart = both * kv->head_dim;
+    r.spml = both * 2;
+    return r;
+}
+
+bool sh_args_ok(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_groups, int max_shared) {
+    return pg_pages_ok(kv) && n_seq > 0 && n_seq <= KRH_ROWS_MAX && max_len > 0 && max_len <= KR_PAGE_LEN_MAX &&
+           n_heads > 0 && n_heads % kv->n_kv_heads == 0 && n_heads / kv->n_kv_heads <= KR_PAGE_GROUP_MAX &&
+           (long long)n_seq * (max_len / 16 + 1) <= INT32_MAX / 2 && n_groups >= 0 && n_groups <= PA_GROUPS &&
+           max_shared >= 0 && max_shared <= max_len &&
+           // tiles of all column tiles
+           ((long long)n_seq * (n_heads / kv->n_kv_heads) / 32 + n_groups) * (max_shared / SH_R + 1) <= INT32_MAX / 2;
+}
+
+using ShRows = void (*)(const PgView, const ShArgs);
+template <int KT, int CL> ShRows sh_rows(int wc) {
+    if constexpr (CL <= 128) {
+        if (wc == 1) return k_shared_rows<KT, CL, 1>;
+    }
+    return k_shared_rows<KT, CL, 4>;
+}
+template <int KT> ShRows sh_rows(int hd, int wc) {
+    return hd <= 64 ? sh_rows<KT, 64>(wc) : hd <= 128 ? sh_rows<KT, 128>(wc) : sh_rows<KT, 256>(wc);
+}
+using ShOwn = void (*)(const PgView, const PaShared, int *);
+template <int KT, int CL> ShOwn sh_own(int hd) { return hd == CL ? k_shared_own<KT, CL, true> : k_shared_own<KT, CL, false>; }
+template <int KT> ShOwn sh_own(int hd) { return hd <= 64 ? sh_own<KT, 64>(hd) : hd <= 128 ? sh_own<KT, 128>(hd) : sh_own<KT, 256>(hd); }
+
+}  // namespace
+
+extern "C" size_t krh_paged_attention_shared_ws(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_groups,
+                                                int max_shared) {
+    if (!sh_args_ok(kv, n_seq, n_heads, max_len, n_groups, max_shared)) return 0;
+    const size_t base = krh_paged_attention_ws(kv, n_seq, n_heads, max_len, 0);
+    if (n_groups == 0 || max_shared == 0) return base;
+    const ShSizes r = sh_sizes(kv, n_seq, n_heads, max_len, n_groups, max_shared);
+    const size_t b = sizeof(float) * (r.part + r.pml + r.spart + r.spml + 4);
+    return b > base ? b : base;
+}
+
+extern "C" void krh_paged_attention_shared(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len,
+                                           int n_seq, const int *group, const int *shared, int n_groups, int max_shared,
+                                           const float *q, int n_heads, int max_len, int window, float scale,
+                                           float softcap, void *ws) {
+    if (n_seq == 0) return;
+    if (pg_refuse(sh_args_ok(kv, n_seq, n_heads, max_len, n_groups, max_shared), "paged_attention_shared sizes") ||
+        pg_refuse(o && table && table_ld > 0 && len && q && ws && pg_aligned(o) && pg_aligned(q) && pg_aligned(ws) &&
+                      (n_groups == 0 || (group && shared)),
+                  "paged_attention_shared: a missing or unaligned array") ||
+        pg_refuse(window >= 0 && (softcap == 0.0f || (softcap >= FLT_MIN && softcap <= 0x1p126f)),
+                  "paged_attention_shared: window or soft-cap"))
+        return;
+    if (n_groups == 0 || max_shared == 0) {
+        krh_paged_attention(o, kv, table, table_ld, len, n_seq, q, n_heads, max_len, window, scale, softcap, nullptr, 0, ws);
+        return;
+    }
+    if (pg_not_ready("paged_attention_shared before krh_init")) return;
+    const ShSizes r = sh_sizes(kv, n_seq, n_heads, max_len, n_groups, max_shared);
+    float *w = (float *)ws;
+    ShArgs a = {};
+    a.o = o, a.q = q, a.len = len;
+    a.part = w, a.pml = w + r.part, a.spart = a.pml + r.pml, a.spml = a.spart + r.spart;
+    a.nh = n_heads, a.max_len = max_len, a.window = window, a.shares = r.shares, a.tl = pg_log2(pa_tile(kv->head_dim));
+    a.least = 1;
+    a.scale = scale, a.cap = softcap;
+    a.group = group, a.shared = shared, a.n_groups = n_groups, a.max_shared = max_shared;
+    a.sshares = r.sshares, a.sleast = 4, a.slots = r.slots, a.ct = 32 * r.wc, a.fault = kr_fault_word();
+    const PgView p = pg_view(kv, table, table_ld, n_seq);
+    const int hd = kv->head_dim;
+    const ShRows f = kv->kv_type == ML_F32 ? sh_rows<PG_F32>(hd, r.wc) : kv->kv_type == ML_F16 ? sh_rows<PG_F16>(hd, r.wc)
+                                                                                              : sh_rows<PG_Q8>(hd, r.wc);
+    hipLaunchKernelGGL(f, dim3(r.sshares, kv->n_kv_heads), dim3(64 * r.wc), 0, kr_stream(), p, a);
+    kr_check_launch("paged_attention_shared");
+    const ShOwn g = kv->kv_type == ML_F32 ? sh_own<PG_F32>(hd) : kv->kv_type == ML_F16 ? sh_own<PG_F16>(hd) : sh_own<PG_Q8>(hd);
+    hipLaunchKernelGGL(g, dim3(r.shares, kv->n_kv_heads), dim3(64), 0, kr_stream(), p, (const PaShared &)a, kr_fault_word());
+    kr_check_launch("paged_attention_shared");
+    hipLaunchKernelGGL(k_shared_join, dim3(n_heads, n_seq), dim3(SJ_T), 0, kr_stream(), p, a, pg_log2(hd / 4));
+    kr_check_launch("paged_attention_shared");
+}

@@ -71,3 +71,44 @@ def test_before_init():
                              ("krh_dequantize_row_rows", DEQ, [dict(rows=1, ldx=0)])):
         for kw in [{}] + more:
             assert call(name, base, **kw) == K.ML_E_ISA, (name, kw)
+
+
+# ---- attention over shared rows ----
+
+def pages(**kw):
+    f = dict(k=PTR, v=PTR, kd=None, vd=None, kv_type=K.ML_F16, n_pages=4, page_size=16, n_kv_heads=2, head_dim=64)
+    return K.KrhPages(**dict(f, **kw))
+
+
+SHARE = dict(o=PTR, kv=pages(), table=PTR, table_ld=4, len=PTR, n_seq=20, group=PTR, shared=PTR, n_groups=2, max_shared=48, q=PTR,
+             n_heads=4, max_len=64, window=0, scale=1.0, softcap=0.0, ws=PTR)
+
+
+@pytest.mark.parametrize("kw", [dict(o=None), dict(table=None), dict(len=None), dict(group=None), dict(shared=None), dict(q=None),
+                                dict(ws=None), dict(o=PTR + 8), dict(q=PTR + 4), dict(ws=PTR + 8), dict(n_seq=-1),
+                                dict(n_seq=70000), dict(n_groups=-1), dict(n_groups=65), dict(max_shared=-1),
+                                dict(max_shared=65), dict(n_heads=0), dict(n_heads=5), dict(n_heads=34), dict(max_len=0),
+                                dict(max_len=2**30), dict(n_seq=60000, max_len=2**29), dict(table_ld=0), dict(window=-1),
+                                dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(softcap=1e-40),
+                                dict(kv=None), dict(kv=pages(k=None)), dict(kv=pages(kv_type=K.ML_Q8_0)),
+                                dict(kv=pages(page_size=24)), dict(kv=pages(head_dim=12))],
+                         ids=lambda kw: "-".join(kw))
+def test_shared_attention_refused(kw):
+    assert call("krh_paged_attention_shared", SHARE, **kw) == K.ML_E_SHAPE
+
+
+def test_shared_attention_nothing_to_do():
+    assert call("krh_paged_attention_shared", SHARE, n_seq=0) == K.ML_OK
+    if K.hip.krh_device_cus() == 0:
+        for kw in ({}, dict(n_groups=0, group=None, shared=None), dict(max_shared=0), dict(n_groups=64), dict(max_shared=64)):
+            assert call("krh_paged_attention_shared", SHARE, **kw) == K.ML_E_ISA, kw
+
+
+def test_shared_attention_workspaces():
+    ws = K.hip.krh_paged_attention_shared_ws
+    kv = C.byref(pages())
+    assert ws(kv, 20, 4, 64, 2, 48) >= K.hip.krh_paged_attention_ws(kv, 20, 4, 64, 0) > 0
+    assert ws(kv, 20, 4, 64, 0, 0) == K.hip.krh_paged_attention_ws(kv, 20, 4, 64, 0)
+    for bad in ((kv, 0, 4, 64, 2, 48), (kv, 20, 5, 64, 2, 48), (kv, 20, 4, 64, 65, 48), (kv, 20, 4, 64, 2, 65),
+                (None, 20, 4, 64, 2, 48)):
+        assert ws(*bad) == 0
