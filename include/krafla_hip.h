@@ -477,21 +477,26 @@ typedef struct {
     const int8_t *q;    /* [rows] rows ld apart, 16-byte aligned, all of rows * ld readable; what lies behind a row's
                          * cols values may be anything */
     const float *d;     /* [rows] */
-    size_t ld;          /* a multiple of 16 */
+    size_t ld;          /* a multiple of 16, at most 2^23 */
     int rows, cols;     /* cols up to 131071, whose sums end within 32 bits */
 } krh_mat8;
 /* Y[t * ldy + r] = S xd[t] W->d[r] + bias[r], S = sum_k W->q[r][k] xq[t * ldx + k]
  * the whole number; accumulate != 0: added to Y. T tokens (up to KRH_ROWS_MAX), xq
- * as a matrix's rows: 16-byte aligned, ldx a multiple of 16, all of T * ldx
- * readable. bias may be NULL. The same bits for every T: S to a float, times xd,
+ * as a matrix's rows: 16-byte aligned, ldx a multiple of 16, at most 2^23, all of
+ * T * ldx readable. bias may be NULL. The same bits for every T: S to a float, times xd,
  * times d, then the bias, then Y. Y overlaps no input. Allocates nothing; can be
  * captured. */
 void krh_matmul_i8(float *Y, size_t ldy, const krh_mat8 *W, const int8_t *xq, size_t ldx, const float *xd,
                    const float *bias, int T, int accumulate);
 /* H[t * ldh + r] = silu(g) u of the two products g (w1) and u (w3) of the same
- * sizes, as krh_matmul_i8 and krh_silu_mul leave it */
+ * sizes, each as krh_matmul_i8 leaves it, silu(g) = g / (1 + e^-g) and its product
+ * within 8 half steps of a float (1e-35 where e^-g leaves the floats) */
 void krh_matmul_i8_swiglu(float *H, size_t ldh, const krh_mat8 *w1, const krh_mat8 *w3, const int8_t *xq, size_t ldx,
                           const float *xd, int T);
+/* The tiles that krh_matmul_i8 takes for these sizes, or krh_matmul_i8_swiglu for a
+ * pair of matrices: 0 to 7 (kr_matmul_i8.hip's forms), -1 for no size. The results
+ * are the same bits whatever they are. */
+int krh_matmul_i8_form(int rows, int cols, int ntok, int swiglu);
 
 /* ---- between two blocks of a layer ----
  * The norm of a block's output, its gate, the residual add and the next block's

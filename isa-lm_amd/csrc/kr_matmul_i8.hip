@@ -4,6 +4,8 @@
 // The sums are exact in 32 bits whatever their order, so the reduction is split
 // and its parts are joined freely, and every form gives the same bits: one
 // float conversion and two products an output.
+#include <cfloat>
+#include <cmath>
 #include "kr_internal.h"
 #include "kr_numerics.h"
 
@@ -12,6 +14,7 @@ namespace {
 typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr int I8_COLS = (1 << 17) - 1;   // 2^14 * cols < 2^31
+constexpr size_t I8_LD = 1 << 23;        // a tile's rows within 32-bit offsets
 
 struct I8Args {
     float *y;
@@ -25,86 +28,424 @@ struct I8Args {
     int rows, cols, ntok, add;
 };
 
-// 16 bytes of a row from k on; those past its end are zeros (the row's stride
-// holds whole 16 bytes)
-__device__ __forceinline__ v4i i8_get(const int8_t *row, int k, int cols) {
-    v4i v = {};
-    if (k < cols) v = *(const v4i *)(row + k);
+// the first n of 16 bytes, then zeros
+__device__ __forceinline__ v4i i8_cut(v4i v, int n) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int left = cols - k - 4 * i;
+        const int left = n - 4 * i;
         if (left < 4) v[i] = left <= 0 ? 0 : v[i] & (int)((1u << 8 * left) - 1);
     }
     return v;
 }
-
 __device__ __forceinline__ float i8_scaled(int sum, float xd, float wd) { return kr_fmul(kr_fmul((float)sum, xd), wd); }
+// silu(g) u = g / (1 + e^-g) u within 8 half steps. The power of two takes the product g log2 e in two parts;
+// below -88, where e^-g leaves the floats, silu is 0 (to 6e-37). (The C library's
+// expf and the division, which krh_silu_mul takes, are 90 instructions an output and
+// would be a third of a prompt's time.)
 __device__ __forceinline__ float i8_silu_mul(float g, float u) {
-    return kr_fmul(kr_fdiv(g, kr_fadd(1.0f, kr_expf(-g))), u);
-}
-// the output of token t and row r from its sums
-template <bool GLU> __device__ __forceinline__ void i8_out(const I8Args &a, int t, int r, int s0, int s1) {
-    float v = i8_scaled(s0, a.xd[t], a.wd[0][r]);
-    float *y = a.y + (size_t)t * a.ldy + r;
-    if constexpr (GLU) {
-        *y = i8_silu_mul(v, i8_scaled(s1, a.xd[t], a.wd[1][r]));
-    } else {
-        if (a.bias) v = kr_fadd(v, a.bias[r]);
-        *y = a.add ? kr_fadd(*y, v) : v;
-    }
+    const float x = fminf(fmaxf(g, -88.0f), 88.0f);
+    const float t = x * -1.44269502f;
+    const float lo = __builtin_fmaf(x, -1.92596299e-8f, __builtin_fmaf(x, -1.44269502f, -t));
+    float e = __builtin_amdgcn_exp2f(t);
+    e = __builtin_fmaf(e, lo * 0.693147182f, e);
+    const float s = g < -88.0f ? 0.0f : __builtin_amdgcn_rcpf(1.0f + e);
+    return kr_fmul(kr_fmul(g, s), u);
 }
 
-// Few tokens: a workgroup has 16 rows (of both matrices) and 16 NT tokens, its
-// waves parts of the reduction, each read straight into operand registers; the
-// parts' sums meet in LDS.
-constexpr int FEW_W = 8, FEW_T = 64 * FEW_W;
-template <int NT, bool GLU> __global__ void __launch_bounds__(FEW_T) k_i8_few(const I8Args a) {
-    constexpr int M = GLU ? 2 : 1;
-    __shared__ v4i s_sum[FEW_W][M][NT][64];
+// Up to 16 tokens: a workgroup has 16 rows, its waves parts of
+// the reduction: lines of 128 values in turn, read straight into operand
+// registers, FEW_D steps of 64 values ahead. The parts' sums meet in LDS. Bound by
+// HBM: one token, 4096 rows of 14,336 12.0 us (4.9 TB/s), of 4096 5.7. A lane's 16
+// bytes are a row's of its own, which a CU reads at about 16 bytes a clock, so
+// with more tokens their reads take longer than W's (16: 17.0 us).
+constexpr int FEW_W = 8, FEW_T = 64 * FEW_W, FEW_D = 8;
+__global__ void __launch_bounds__(FEW_T) k_i8_few(const I8Args a) {
+    static_assert(FEW_D % 2 == 0, "whole lines");
+    __shared__ v4i s_sum[FEW_W][64];
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int r0 = blockIdx.x * 16, t0 = blockIdx.y * 16 * NT;
-    const int8_t *w[M], *x[NT];
+    const int r0 = blockIdx.x * 16;
+    const int8_t *xb = a.x, *wb = a.w[0] + (size_t)r0 * a.ldw[0];
+    const unsigned wo = (unsigned)min(n, a.rows - 1 - r0) * (unsigned)a.ldw[0];
+    const unsigned xo = (unsigned)min(n, a.ntok - 1) * (unsigned)a.ldx;
+    const int last = (a.cols - 1) & ~15;   // the last 16 bytes with a value, which are read for those past them
+    // this wave's step u is half of its line u / 2
+    auto at = [&](int u) { return ((u >> 1) * FEW_W + wave) * 128 + (u & 1) * 64 + 16 * g; };
+    v4i w[FEW_D], x[FEW_D], acc = {};
+    auto load = [&](int u, v4i &w, v4i &x) {
+        const unsigned k = min(at(u), last);
+        w = *(const v4i *)(wb + (wo + k));
+        x = *(const v4i *)(xb + (xo + k));
+    };
+    const int lines = (a.cols + 127) / 128, steps = wave < lines ? 2 * ((lines - wave + FEW_W - 1) / FEW_W) : 0;
+    if (steps > 0) {
 #pragma unroll
-    for (int m = 0; m < M; m++) w[m] = a.w[m] + (size_t)min(r0 + n, a.rows - 1) * a.ldw[m];
+        for (int i = 0; i < FEW_D; i++) load(i, w[i], x[i]);
+        int u = 0;
+        for (; u + FEW_D < steps; u += FEW_D) {
 #pragma unroll
-    for (int j = 0; j < NT; j++) x[j] = a.x + (size_t)min(t0 + 16 * j + n, a.ntok - 1) * a.ldx;
-    v4i acc[M][NT] = {};
-    // 64 values a step, steps in turn over the waves
-    for (int k0 = wave * 64; k0 < a.cols; k0 += FEW_W * 64) {
-        const int k = k0 + 16 * g;
-        v4i xv[NT];
+            for (int i = 0; i < FEW_D; i++) {
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], x[i], acc, 0, 0, 0);
+                load(u + FEW_D + i, w[i], x[i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // the last steps, of which some end within the row or lie past it
 #pragma unroll
-        for (int j = 0; j < NT; j++) xv[j] = i8_get(x[j], k, a.cols);
+        for (int i = 0; i < FEW_D; i++)
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(i8_cut(w[i], a.cols - at(u + i)), x[i], acc, 0, 0, 0);
+    }
+    s_sum[wave][lane] = acc;
+    __syncthreads();
+    // one wave has four rows of a token a lane
+    if (wave > 0) return;
+    v4i sum = {};
 #pragma unroll
-        for (int m = 0; m < M; m++) {
-            const v4i wv = i8_get(w[m], k, a.cols);
+    for (int v = 0; v < FEW_W; v++) sum += s_sum[v][lane];
+    const int r = r0 + 4 * g;
+    if (n >= a.ntok) return;
+    const float xd = a.xd[n];
+    float *y = a.y + (size_t)n * a.ldy + r;
 #pragma unroll
-            for (int j = 0; j < NT; j++) acc[m][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, xv[j], acc[m][j], 0, 0, 0);
+    for (int c = 0; c < 4; c++) {
+        if (r + c >= a.rows) break;
+        float v = i8_scaled(sum[c], xd, a.wd[0][r + c]);
+        if (a.bias) v = kr_fadd(v, a.bias[r + c]);
+        y[c] = a.add ? kr_fadd(y[c], v) : v;
+    }
+}
+
+// Tiles of BT tokens and BR rows (GLU: 32 rows of each matrix in turn), WT x WR
+// waves with an even part each, or WK times as many, each with a part of the
+// reduction. That goes in stages of BK values, which pass from memory to LDS
+// without registers, NB stages in a ring: one barrier a stage, and a stage's loads
+// are under way while the NB - 1 before it are worked on. A row's 16-byte chunks lie
+// in LDS in an order of the row's own, so that the rows that a wave reads one chunk
+// of are in different banks; the order is taken from the source's side, as the
+// loads fill LDS in lane order.
+//
+// What bounds them. The largest tile (256 x 256, waves of 128 x 64): LDS, 192 KB of
+// reads and 64 KB of loads a stage of 128 values, about 2500 clocks beside 2048 of
+// products; its loop reaches 2.4 POP/s of the 5.0 that the matrix cores have, and 2047
+// tokens of the 8B shape's w1 and w3 take 252 us (1.9 POP/s; 267 with waves of 128 x 128,
+// one a SIMD; 333 in tiles of 128 x 128). Small tiles: the way of a stage's operands from
+// LDS, with a wave a SIMD 0.4 us a stage, which the split of the reduction over 8 waves
+// shares out: 64 tokens, 4096 rows of 4096, 7.6 us (18.4 in tiles of 64 x 64 without it,
+// 12.5 with operands from memory).
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+// 16 bytes a lane from base + off to LDS at `to` (one address a wave) + 16 lane.
+// No register waits for it: a wait on the vector memory counter ends it. (The
+// compiler does not see into it, so it holds the 5 clocks that a load waits for an
+// address register which a vector instruction has written.)
+__device__ __forceinline__ void i8_to_lds(unsigned to, const int8_t *base, unsigned off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+}
+// all but the last N of this wave's loads have ended, and all waves are here
+template <int N> __device__ __forceinline__ void i8_stage_wait() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+template <int KC> __device__ __forceinline__ int i8_chunk(int row, int c) { return c ^ (KC == 8 ? (row >> 1) & 7 : row & 15); }
+
+template <int BT_, int BR_, int WT_, int WR_, int BK_, int NB_, int WK_ = 1> struct I8Tile {
+    static constexpr int BT = BT_, BR = BR_, WT = WT_, WR = WR_, BK = BK_, NB = NB_, WK = WK_;
+    static constexpr int WAVES = WT * WR * WK, T = 64 * WAVES, KC = BK / 16, MT = BT / WT / 32, NT = BR / WR / 32;
+    static constexpr int PER = 64 / KC;                            // rows a wave's load covers
+    static constexpr int LX = BT / PER / WAVES, LW = BR / PER / WAVES;   // loads a wave and stage
+    static_assert(LX * PER * WAVES == BT && LW * PER * WAVES == BR && 32 % PER == 0 && BK % 64 == 0, "whole loads");
+};
+
+// the schedule of P products with R reads spread evenly behind them
+template <int P, int R, int I = 0> __device__ __forceinline__ void i8_schedule() {
+    if constexpr (I < P) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr ((I + 1) * R / P > I * R / P) __builtin_amdgcn_sched_group_barrier(0x100, (I + 1) * R / P - I * R / P, 0);
+        i8_schedule<P, R, I + 1>();
+    }
+}
+
+template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(const I8Args a, int nt, int nr) {
+    constexpr int KC = S::KC, BK = S::BK, NB = S::NB;
+    constexpr int XB = S::BT * BK, WB = S::BR * BK;
+    __shared__ alignas(16) int8_t s_ring[NB * (XB + WB)];
+    int8_t *const s_x = s_ring, *const s_w = s_ring + NB * XB;
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    // Consecutive workgroups go to the dies in turn: each die has consecutive tiles,
+    // 8 token tiles of a row tile after one another, which share what its L2 holds
+    const int all = nt * nr, q = all / 8, rem = all % 8, die = blockIdx.x % 8;
+    const int l = die * q + min(die, rem) + (int)blockIdx.x / 8;
+    const int band = l / (8 * nr) * 8, wide = min(8, nt - band), in = l - band * nr;
+    const int t0 = (band + in % wide) * S::BT, r0 = in / wide * (GLU ? S::BR / 2 : S::BR);
+    // where this lane's chunks of a stage are: byte offsets from the tile's first row
+    const int8_t *xb = a.x + (size_t)t0 * a.ldx;
+    const int8_t *w0 = a.w[0] + (size_t)r0 * a.ldw[0], *w1 = GLU ? a.w[1] + (size_t)r0 * a.ldw[1] : nullptr;
+    unsigned xo[S::LX], wo[S::LW];
+    const int sub = lane / KC, slot = lane % KC;
+#pragma unroll
+    for (int j = 0; j < S::LX; j++) {
+        const int row = (j * S::WAVES + wave) * S::PER + sub;
+        xo[j] = (unsigned)min(row, a.ntok - 1 - t0) * (unsigned)a.ldx + i8_chunk<KC>(row, slot) * 16;
+    }
+    auto second = [&](int j) { return GLU && ((j * S::WAVES + wave) * S::PER >> 5 & 1); };
+    auto ldw = [&](int j) { return (unsigned)(second(j) ? a.ldw[1] : a.ldw[0]); };
+    auto mrow = [&](int row) { return min(GLU ? ((row >> 6) << 5) + (row & 31) : row, a.rows - 1 - r0); };
+#pragma unroll
+    for (int j = 0; j < S::LW; j++) {
+        const int row = (j * S::WAVES + wave) * S::PER + sub;
+        wo[j] = (unsigned)mrow(row) * ldw(j) + i8_chunk<KC>(row, slot) * 16;
+    }
+    const unsigned lx = (unsigned)(uintptr_t)(__attribute__((address_space(3))) int8_t *)s_x;
+    const unsigned lw = (unsigned)(uintptr_t)(__attribute__((address_space(3))) int8_t *)s_w;
+    const int stages = (a.cols + BK - 1) / BK;
+    auto load = [&](int st) {
+        const int k = st * BK, buf = st % NB;
+        const bool whole = k + BK <= a.cols;
+#pragma unroll
+        for (int j = 0; j < S::LX; j++) {
+            const int g = j * S::WAVES + wave;
+            unsigned off = xo[j];
+            if (!whole) {   // past the row's stride: any of its values, which meet zeros
+                const int c = i8_chunk<KC>(g * S::PER + sub, slot) * 16;
+                if (k + c >= (int)a.ldx) off -= c;
+            }
+            i8_to_lds(lx + buf * XB + g * 1024, xb + k, off);
+        }
+#pragma unroll
+        for (int j = 0; j < S::LW; j++) {
+            const int g = j * S::WAVES + wave;
+            unsigned off = wo[j];
+            if (!whole) {
+                const int c = i8_chunk<KC>(g * S::PER + sub, slot) * 16;
+                if (k + c >= (int)ldw(j)) off -= c;
+            }
+            i8_to_lds(lw + buf * WB + g * 1024, (second(j) ? w1 : w0) + k, off);
+        }
+    };
+    // zeros for what the last stage's rows of W have past their end, so that nothing there counts
+    auto clear = [&](int st) {
+        const int left = a.cols - st * BK;
+        for (int i = threadIdx.x; i < S::BR * KC; i += S::T) {
+            const int c = i8_chunk<KC>(i / KC, i % KC) * 16;
+            v4i *p = (v4i *)(s_w + st % NB * WB + i * 16);
+            if (c >= left) {
+                *p = v4i{};
+            } else if (c + 16 > left) {
+                *p = i8_cut(*p, left - c);
+            }
+        }
+        __syncthreads();
+    };
+    v16i acc[S::MT][S::NT] = {};
+    const int wk = wave / (S::WT * S::WR), wg = wave % (S::WT * S::WR), wt = wg / S::WR, wr = wg % S::WR, n = lane & 31;
+    constexpr int KS = BK / 32 / S::WK;   // steps of a stage, of which the wave's are wk * KS ..
+    // Small tiles ask for a stage's operands at once, whose way from LDS would else
+    // be most of a step; larger ones for the next step's among a step's products
+    constexpr bool ALL = S::MT * S::NT <= 2 || S::WK > 1;
+    constexpr int D = ALL ? KS : 2;
+    v4i xv[D][S::MT], wv[D][S::NT];
+    // the operands of 32 values, step k of a stage
+    auto read = [&](int st, int k, v4i (&x)[S::MT], v4i (&w)[S::NT]) {
+        const int c = i8_chunk<KC>(n, 2 * (wk * KS + k) + h) * 16;
+        const int8_t *sx = s_x + st % NB * XB + (wt * S::MT * 32 + n) * BK + c;
+        const int8_t *sw = s_w + st % NB * WB + (wr * S::NT * 32 + n) * BK + c;
+#pragma unroll
+        for (int m = 0; m < S::MT; m++) x[m] = *(const v4i *)(sx + m * 32 * BK);
+#pragma unroll
+        for (int m = 0; m < S::NT; m++) w[m] = *(const v4i *)(sw + m * 32 * BK);
+    };
+    auto products = [&](const v4i (&x)[S::MT], const v4i (&w)[S::NT]) {
+#pragma unroll
+        for (int m = 0; m < S::MT; m++)
+#pragma unroll
+            for (int c = 0; c < S::NT; c++) acc[m][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[m], w[c], acc[m][c], 0, 0, 0);
+    };
+#pragma unroll
+    for (int st = 0; st < NB - 1; st++)
+        if (st < stages) load(st);
+    const int cut = a.cols % BK ? stages - 1 : -1;
+    for (int st = 0; st < stages; st++) {
+        if (NB > 2 && st + NB - 2 < stages - 1) {
+            i8_stage_wait<(NB - 2) * (S::LX + S::LW)>();
+        } else {
+            i8_stage_wait<0>();
+        }
+        if (st == cut) clear(cut);
+        if (st + NB - 1 < stages) load(st + NB - 1);
+        if constexpr (ALL) {
+#pragma unroll
+            for (int k = 0; k < KS; k++) read(st, k, xv[k], wv[k]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < KS; k++) products(xv[k], wv[k]);
+        } else {
+            read(st, 0, xv[0], wv[0]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                if (k + 1 < KS) read(st, k + 1, xv[(k + 1) & 1], wv[(k + 1) & 1]);
+                products(xv[k & 1], wv[k & 1]);
+                i8_schedule<S::MT * S::NT, S::MT + S::NT>();
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
+    // value i of a tile is token (i & 3) + 8 (i >> 2) + 4 h, and row n
+    constexpr int M = GLU ? 2 : 1;
+    const bool whole = t0 + S::BT <= a.ntok && r0 + S::BR / M <= a.rows;
+    // values i0 .. i0 + 3 of the token tile at tm, rows r + n
+    auto quad = [&](int tm, int r, const float (&xd)[4], const v4i &s0, const v4i &s1, const float *wd, float bias) {
+        float *y = a.y + (size_t)tm * a.ldy + r;
+        float v[4];
 #pragma unroll
-    for (int m = 0; m < M; m++)
+        for (int i = 0; i < 4; i++) {
+            v[i] = i8_scaled(s0[i], xd[i], wd[0]);
+            if constexpr (GLU) v[i] = i8_silu_mul(v[i], i8_scaled(s1[i], xd[i], wd[1]));
+        }
+        if (!GLU && a.bias) {
 #pragma unroll
-        for (int j = 0; j < NT; j++) s_sum[wave][m][j][lane] = acc[m][j];
-    __syncthreads();
-    // an output a thread: row r of the tile is component r % 4 of lane 16 (r / 4) + token
-    for (int i = threadIdx.x; i < 256 * NT; i += FEW_T) {
-        const int r = i & 15, t = i >> 4, l = 16 * (r >> 2) + (t & 15);
-        int sum[2] = { 0, 0 };
+            for (int i = 0; i < 4; i++) v[i] = kr_fadd(v[i], bias);
+        }
+        auto live = [&](int i) { return whole || (r < a.rows && tm + i < a.ntok); };
+        if (!GLU && a.add) {
+            float old[4];
 #pragma unroll
-        for (int v = 0; v < FEW_W; v++)
+            for (int i = 0; i < 4; i++) old[i] = live(i) ? y[i * a.ldy] : 0.0f;
 #pragma unroll
-            for (int m = 0; m < M; m++) sum[m] += ((const int *)&s_sum[v][m][t >> 4][l])[r & 3];
-        if (r0 + r < a.rows && t0 + t < a.ntok) i8_out<GLU>(a, t0 + t, r0 + r, sum[0], sum[1]);
+            for (int i = 0; i < 4; i++) v[i] = kr_fadd(old[i], v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (live(i)) y[i * a.ldy] = v[i];
+    };
+    int r[S::NT / M];
+    float wd[S::NT / M][M], bias[S::NT / M];
+#pragma unroll
+    for (int c = 0; c < S::NT / M; c++) {
+        r[c] = r0 + (wr * S::NT / M + c) * 32 + n;
+        const int at = min(r[c], a.rows - 1);
+        wd[c][0] = a.wd[0][at];
+        if constexpr (GLU) wd[c][1] = a.wd[1][at];
+        bias[c] = !GLU && a.bias ? a.bias[at] : 0.0f;
     }
+    auto part = [](const v16i &v, int q) { return v4i{ v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3] }; };
+    auto tokens = [&](int m, int q) { return t0 + (wt * S::MT + m) * 32 + 8 * q + 4 * h; };
+    auto scales = [&](int tm, float (&xd)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) xd[i] = a.xd[min(tm + i, a.ntok - 1)];
+    };
+    if constexpr (S::WK == 1) {
+#pragma unroll
+        for (int m = 0; m < S::MT; m++) {
+            float xd[4][4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) scales(tokens(m, q), xd[q]);
+#pragma unroll
+            for (int c = 0; c < S::NT / M; c++)
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    quad(tokens(m, q), r[c], xd[q], part(acc[m][c * M], q), part(acc[m][c * M + M - 1], q), wd[c], bias[c]);
+        }
+    } else {
+        // the parts' sums meet in the ring, RM tiles at a time, and each wave has its share of the values
+        constexpr int NC = S::NT / M, P = S::MT * NC, ROOM = NB * (XB + WB) / (S::WAVES * M * 4096), RM = ROOM >= P ? P : ROOM >= 4 ? 4 : ROOM >= 2 ? 2 : 1;
+        static_assert(ROOM > 0 && P % RM == 0, "the parts fit");
+        v4i *const s_part = (v4i *)s_ring;
+#pragma unroll
+        for (int p0 = 0; p0 < P; p0 += RM) {
+            __syncthreads();
+#pragma unroll
+            for (int p = 0; p < RM; p++)
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int c = 0; c < M; c++)
+                        s_part[(((wave * RM + p) * 4 + q) * M + c) * 64 + lane] = part(acc[(p0 + p) / NC][(p0 + p) % NC * M + c], q);
+            __syncthreads();
+#pragma unroll
+            for (int p = 0; p < RM; p++) {
+                // quads of the tile in turn over the parts' waves
+                for (int q = (wk - p * 4 % S::WK + S::WK) % S::WK; q < 4; q += S::WK) {
+                    float xd[4];
+                    const int tm = tokens((p0 + p) / NC, q), cc = (p0 + p) % NC;
+                    scales(tm, xd);
+                    v4i sum[M] = {};
+#pragma unroll
+                    for (int k = 0; k < S::WK; k++)
+#pragma unroll
+                        for (int c = 0; c < M; c++)
+                            sum[c] += s_part[(((k * S::WT * S::WR + wg) * RM + p) * 4 + q) * M * 64 + c * 64 + lane];
+                    quad(tm, r[cc], xd, sum[0], sum[M - 1], wd[cc], bias[cc]);
+                }
+            }
+        }
+    }
+}
+
+// The forms, and what they take: with n tiles a CU, base + n out + (n == 1 ? one : n many) cols / 4096
+// us, as measured (4096 rows of 4096 and 14,336, pairs of 14,336 and 8192 rows, 1 to 2047
+// tokens; the estimates are within 10% of those but where rounds are not whole).
+// At 4096 rows of 4096 in us, 32 x 32 / 64 x 32 / 64 x 64 / 128 x 64 / 128 x 128 split /
+// whole / 256 x 256: 64 tokens 7.7 / 8.3 / 10.6 / 14.5 / 22 / 23 / 49, 256 18.0 / 15.7 / 12.1 / 15.7 / 22.6 /
+// 23.9 / 50, 512 33 / 29 / 21 / 17.4 / 23.7 / 24.7 / 51, 2047 112 / 103 / 70 / 57 / 49 / 39 / 56.
+enum { I8_FEW, I8_32x32, I8_64x32, I8_64x64, I8_128x64, I8_128x128_SPLIT, I8_128x128, I8_256x256, I8_FORMS };
+struct I8Cost {
+    int bt, br;
+    float base, out, one, many;
+};
+constexpr I8Cost I8_COST[I8_FORMS] = { { 16, 16, 3.2f, 0, 2.5f, 2.5f },  { 32, 32, 2.3f, 1.0f, 4.2f, 3.0f },
+                                       { 64, 32, 2.8f, 1.2f, 5.0f, 5.0f }, { 64, 64, 2.0f, 3.2f, 6.2f, 6.2f },
+                                       { 128, 64, 4.8f, 1.6f, 11, 11 },  { 128, 128, 7.0f, 1.2f, 19, 19 },
+                                       { 128, 128, 4.0f, 0.2f, 23, 19.5f }, { 256, 256, 4.5f, 6.0f, 58, 58 } };
+// Operands from memory up to 8 tokens (4096 rows of 4096 in us, against tiles of 32 x 32: one
+// token 5.7 / 7.1, 16 7.0 / 7.3; 896 rows of 4864 6.4 / 7.4 and 8.7 / 7.7; a pair of 8192 rows of 2048
+// 11.5 / 8.0); else the least estimate.
+constexpr int I8_FEW_MAX = 8;
+int i8_form(int rows, int cols, int ntok, bool glu) {
+    if (ntok <= I8_FEW_MAX && !glu) return I8_FEW;
+    int best = I8_32x32;
+    float least = FLT_MAX;
+    for (int f = I8_32x32; f < I8_FORMS; f++) {
+        const I8Cost &c = I8_COST[f];
+        if (glu && f == I8_64x64) continue;   // with 32 rows of each matrix at least, that is 64 x 32
+        const int br = f < I8_128x64 ? c.br : glu ? c.br / 2 : c.br;
+        const double tiles = (double)((ntok + c.bt - 1) / c.bt) * ((rows + (long long)br - 1) / br);
+        // a pair's tile of 32 rows is twice the work
+        const float n = (float)ceil(tiles / 256), k = cols / 4096.0f * (glu && f < I8_128x64 ? 1.5f : 1.0f);
+        const float us = c.base + n * c.out + (n == 1 ? c.one : n * c.many) * k;
+        if (us < least) least = us, best = f;
+    }
+    return best;
+}
+
+// a launch holds 2^32 - 1 threads
+template <class F, class... A> void i8_start(F f, const char *what, long long blocks, int threads, const A &...args) {
+    if (blocks > UINT32_MAX / threads) {
+        kr_fail(ML_E_SHAPE, what, hipSuccess);
+        return;
+    }
+    hipLaunchKernelGGL(f, dim3((unsigned)blocks), dim3(threads), 0, kr_stream(), args...);
+    kr_check_launch(what);
+}
+template <class S, bool GLU> void i8_tiles(const I8Args &a, const char *what) {
+    const int nt = (a.ntok + S::BT - 1) / S::BT, nr = (a.rows + (GLU ? S::BR / 2 : S::BR) - 1) / (GLU ? S::BR / 2 : S::BR);
+    i8_start(k_i8_tile<S, GLU>, what, (long long)nt * nr, S::T, a, nt, nr);
 }
 
 template <bool GLU> void i8_launch(const I8Args &a, const char *what) {
-    const int nt = a.ntok <= 16 ? 1 : a.ntok <= 32 ? 2 : 4;
-    const auto f = nt == 1 ? k_i8_few<1, GLU> : nt == 2 ? k_i8_few<2, GLU> : k_i8_few<4, GLU>;
-    hipLaunchKernelGGL(f, dim3((a.rows + 15) / 16, (a.ntok + 16 * nt - 1) / (16 * nt)), dim3(FEW_T), 0, kr_stream(), a);
-    kr_check_launch(what);
+    constexpr int R = GLU ? 64 : 32;   // 32 rows of a matrix
+    switch (i8_form(a.rows, a.cols, a.ntok, GLU)) {
+    case I8_32x32: return i8_tiles<I8Tile<32, R, 1, 1, 256, 4, 8>, GLU>(a, what);
+    case I8_64x32: return i8_tiles<I8Tile<64, R, 1, 1, 256, GLU ? 3 : 4, 8>, GLU>(a, what);
+    case I8_128x64: return i8_tiles<I8Tile<128, 64, 2, 1, 256, 3, 4>, GLU>(a, what);
+    case I8_128x128_SPLIT: return i8_tiles<I8Tile<128, 128, 2, 2, 128, 4, 2>, GLU>(a, what);
+    case I8_128x128: return i8_tiles<I8Tile<128, 128, 4, 2, 128, 2>, GLU>(a, what);
+    case I8_256x256: return i8_tiles<I8Tile<256, 256, 2, 4, 128, 2>, GLU>(a, what);
+    default:
+        if constexpr (!GLU) {
+            if (i8_form(a.rows, a.cols, a.ntok, GLU) == I8_64x64) return i8_tiles<I8Tile<64, 64, 1, 1, 256, 4, 8>, GLU>(a, what);
+            i8_start(k_i8_few, what, (a.rows + 15) / 16, FEW_T, a);
+        }
+    }
 }
 
 bool i8_refuse(bool ok, const char *what) {
@@ -118,13 +459,17 @@ bool i8_not_ready(const char *what) {
 bool i8_aligned(const void *p) { return !((uintptr_t)p & 15); }
 bool i8_mat_ok(const krh_mat8 *w) {
     return w && w->q && w->d && i8_aligned(w->q) && w->rows > 0 && w->rows <= INT32_MAX - 1024 && w->cols > 0 &&
-           w->cols <= I8_COLS && w->ld % 16 == 0 && w->ld >= (size_t)w->cols;
+           w->cols <= I8_COLS && w->ld % 16 == 0 && w->ld >= (size_t)w->cols && w->ld <= I8_LD;
 }
 bool i8_args_ok(const krh_mat8 *w, const float *y, size_t ldy, const int8_t *xq, size_t ldx, const float *xd) {
-    return y && xq && xd && i8_aligned(xq) && ldy >= (size_t)w->rows && ldx % 16 == 0 && ldx >= (size_t)w->cols;
+    return y && xq && xd && i8_aligned(xq) && ldy >= (size_t)w->rows && ldx % 16 == 0 && ldx >= (size_t)w->cols && ldx <= I8_LD;
 }
 
 }  // namespace
+
+extern "C" int krh_matmul_i8_form(int rows, int cols, int ntok, int swiglu) {
+    return rows > 0 && cols > 0 && cols <= I8_COLS && ntok > 0 ? i8_form(rows, cols, ntok, swiglu != 0) : -1;
+}
 
 extern "C" void krh_matmul_i8(float *Y, size_t ldy, const krh_mat8 *W, const int8_t *xq, size_t ldx, const float *xd,
                               const float *bias, int T, int accumulate) {

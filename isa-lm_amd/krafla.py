@@ -207,6 +207,7 @@ for name, res, args in [
                                C.c_size_t, _P, _P, C.c_int]),
     ("krh_matmul_i8", None, [_P, C.c_size_t, C.POINTER(KrhMat8), _P, C.c_size_t, _P, _P, C.c_int, C.c_int]),
     ("krh_matmul_i8_swiglu", None, [_P, C.c_size_t, C.POINTER(KrhMat8), C.POINTER(KrhMat8), _P, C.c_size_t, _P, C.c_int]),
+    ("krh_matmul_i8_form", C.c_int, [C.c_int] * 4),
     ("krh_block_norm", None, [_P, C.c_size_t, _P, C.c_size_t, _P, C.c_size_t, _P, _P, C.c_size_t, C.c_float, _P, C.c_float,
                               _P, C.c_size_t, _P, C.c_size_t, _P, C.c_int, C.c_int]),
     ("krh_dequantize_row_rows", None, [_P, C.c_size_t, _P, C.c_size_t, _P, C.c_size_t, C.c_int, C.c_int]),

@@ -105,25 +105,69 @@ def test_i8_largest_sums(dev, T, rows):
 @pytest.mark.parametrize("T", TOKENS)
 @pytest.mark.parametrize("rows,cols", [(1, 3), (16, 64), (37, 130), (130, 1000), (300, 272)])
 def test_i8_swiglu(dev, T, rows, cols):
-    """the bits of two products and krh_silu_mul_rows, and the definition in 64 bits"""
+    """the definition in 64 bits from the products as krh_matmul_i8 leaves them"""
+    check_swiglu(dev, T, rows, cols)
+
+
+def check_swiglu(dev, T, rows, cols):
     rng = np.random.default_rng(T + rows)
     w1, w3, x = Mat(dev, rng, rows, cols), Mat(dev, rng, rows, cols, 48), Mat(dev, rng, T, cols)
     ldh = rows + 3
     h0 = np.full((T, ldh), 55.0, np.float32)
-    hb, gb, ub = dev.put(h0), dev.zeros(4 * T * rows), dev.zeros(4 * T * rows)
+    hb = dev.put(h0)
     K.hip.krh_matmul_i8_swiglu(hb.ptr, ldh, w1.ref, w3.ref, x.qb.ptr, x.ld, x.sb.ptr, T)
-    K.hip.krh_matmul_i8(gb.ptr, rows, w1.ref, x.qb.ptr, x.ld, x.sb.ptr, None, T, 0)
-    K.hip.krh_matmul_i8(ub.ptr, rows, w3.ref, x.qb.ptr, x.ld, x.sb.ptr, None, T, 0)
-    K.hip.krh_silu_mul_rows(gb.ptr, rows, ub.ptr, rows, rows, T)
     ok()
     h = hb.get(np.float32, h0.size).reshape(h0.shape)
     assert (h[:, rows:] == 55.0).all()
-    assert np.array_equal(bits(h[:, :rows]), bits(gb.get(np.float32, T * rows).reshape(T, rows)))
     g, u = product(w1, x).astype(np.float64), product(w3, x).astype(np.float64)
     want = g / (1 + np.exp(-g)) * u
-    # from g and u as they are: a float's exponential, sum, quotient and product, at most 4 half steps of the result
-    # (the exponential's share of 1 + e is less than 1), and where e^-g overflows 0
-    assert (np.abs(h[:, :rows] - want) <= 4.01 * U * np.abs(want) + 1e-30).all()
+    # half steps: the power 2 (the instruction's last bit) and 1 (its second part's sum), whose share of 1 + e^-g is less
+    # than 1; the sum 1, the reciprocal 2, the two products 1 each
+    assert (np.abs(h[:, :rows] - want) <= 8.01 * U * np.abs(want) + 1e-30).all()
+    # a token's bits do not depend on the others
+    hb2 = dev.zeros(4 * rows)
+    t = T // 2
+    K.hip.krh_matmul_i8_swiglu(hb2.ptr, rows, w1.ref, w3.ref, x.qb.ptr + t * x.ld, x.ld, x.sb.ptr + 4 * t, 1)
+    ok()
+    assert np.array_equal(bits(hb2.get(np.float32, rows)), bits(h[t, :rows]))
+
+
+@pytest.mark.parametrize("scale", [0.02, 0.3, 3.0, 1e4, 1e30])
+def test_i8_swiglu_range(dev, scale):
+    """from products near zero to those whose power leaves the floats, both signs"""
+    rng = np.random.default_rng(3)
+    w1, w3, x = Mat(dev, rng, 64, 100), Mat(dev, rng, 64, 100), Mat(dev, rng, 40, 100)
+    for m, f in ((w1, scale), (w3, min(scale, 1.0))):
+        m.s = f32(m.s * f)
+        m.sb = dev.put(m.s)
+        m.d.d = m.sb.ptr
+    hb = dev.zeros(4 * 40 * 64)
+    K.hip.krh_matmul_i8_swiglu(hb.ptr, 64, w1.ref, w3.ref, x.qb.ptr, x.ld, x.sb.ptr, 40)
+    ok()
+    h = hb.get(np.float32, 40 * 64).reshape(40, 64)
+    g, u = product(w1, x).astype(np.float64), product(w3, x).astype(np.float64)
+    with np.errstate(over="ignore"):
+        want = g / (1 + np.exp(-g)) * u
+    assert (np.abs(h - want) <= 8.01 * U * np.abs(want) + 1e-35 * (1 + np.abs(u))).all()
+
+
+FORMS = [(0, 5, 40, 100), (1, 20, 40, 300), (2, 33, 4100, 300), (3, 33, 9000, 700), (4, 130, 6000, 1500), (5, 200, 9000, 5000),
+         (6, 1030, 3000, 200), (7, 2050, 6000, 2100)]
+PAIR_FORMS = [(1, 5, 40, 300), (2, 33, 4100, 700), (4, 100, 4100, 2100), (5, 100, 9000, 5000), (6, 700, 2100, 130),
+              (7, 1500, 4100, 2100)]
+
+
+@pytest.mark.parametrize("form,T,rows,cols", FORMS)
+def test_i8_forms(dev, form, T, rows, cols):
+    """each of the forms, by sizes that take it"""
+    assert K.hip.krh_matmul_i8_form(rows, cols, T, 0) == form
+    check_i8(dev, T, rows, cols, bias=True, add=True, ldy=rows + 3)
+
+
+@pytest.mark.parametrize("form,T,rows,cols", PAIR_FORMS)
+def test_i8_swiglu_forms(dev, form, T, rows, cols):
+    assert K.hip.krh_matmul_i8_form(rows, cols, T, 1) == form
+    check_swiglu(dev, T, rows, cols)
 
 
 def test_i8_captured(dev):
