@@ -125,6 +125,11 @@ template <int KT, int CL, int WC> struct ShWork {
     static constexpr int KW = KT == PG_Q8 ? 2 : 4;             // words of a K chunk in the pool
     static constexpr int VW = KT == PG_F32 ? 4 : KT == PG_F16 ? 8 : 4;
     static constexpr int KS = HALF ? CL / 16 : CL / 8;         // K operands of a row
+    static constexpr int EB = KT == PG_F32 ? 4 : KT == PG_F16 ? 2 : 1, KD = HALF ? 8 : 4, VC = CL / 4;
+    static_assert(16 % (64 / (KC < 64 ? KC : 64)) == 0 && 16 % (64 * (HALF ? 4 : 1) / VC) == 0, "a wave's pieces in one half of a tile");
+    // log2 of what the weights are over, and by how much (log2) one may pass the maximum that it is taken from before
+    // that moves: 2^13 2^2 are within the halves, and a weight's lo a whole half down to 2^-15 of the largest
+    static constexpr int UP = KT == PG_F16 ? 13 : 0, SLACK = 2;
     static constexpr int DT = CL / 32;
 
     const PgView &p;
@@ -138,6 +143,7 @@ template <int KT, int CL, int WC> struct ShWork {
     int first, last, wf, wl;   // the column's rows; all columns of the wave have [wf, wl)
     int ids, ids_at;
     unsigned kr[KN][KW], vr[VN][VW];
+    unsigned ko[KN], vo[VN];   // this thread's pieces of a tile, bytes from the row that its half of the tile starts at
     float sr;
     std::conditional_t<HALF, half8, float4v> qf[KS][HALF ? 2 : 1];
     float cs, m_run, l_run, v_run, v_end;
@@ -146,7 +152,21 @@ template <int KT, int CL, int WC> struct ShWork {
 
     __device__ __forceinline__ ShWork(const PgView &p_, const ShArgs &a_, ShLds<KT, CL> &l, int kvh_)
         : p(p_), a(a_), lds(l), lane(threadIdx.x & 63), h(lane >> 5),
-          wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))), kvh(kvh_), hd(p_.hd), group(a_.nh / p_.n_kv), bad(0) {}
+          wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))), kvh(kvh_), hd(p_.hd), group(a_.nh / p_.n_kv), bad(0) {
+        // past the head's dims its first ones, which meet zeros (K) or come to nothing (V)
+#pragma unroll
+        for (int j = 0; j < KN; j++) {
+            const int u = j * NTH + (int)threadIdx.x, row = u / KC, d = u % KC * KD;
+            ko[j] = ((row & 15) * hd + (d < hd ? d : 0)) * EB;
+        }
+#pragma unroll
+        for (int j = 0; j < VN; j++) {
+            const int u = j * NTH + (int)threadIdx.x, row = vrow(u), d = u % VC * 4;
+            vo[j] = ((row & 15) * hd + (d < hd ? d : 0)) * EB;
+        }
+    }
+    // the first row of a V piece, one of VC beside each other
+    static __device__ __forceinline__ int vrow(int u) { return HALF ? u / VC * 4 : u / VC; }
 
     // this lane's column: head `head` of all, or none
     __device__ __forceinline__ void column(int s0, int s1, int rows, int ct, size_t &head) {
@@ -193,51 +213,41 @@ template <int KT, int CL, int WC> struct ShWork {
         const int i = (r0 - ids_at) >> 4;
         const int a0 = __builtin_amdgcn_readlane(ids, i), a1 = __builtin_amdgcn_readlane(ids, i + 1);
         const size_t lo = kr_page_row(max(a0 >= 0 ? a0 : a1, 0), p.n_kv, kvh, p.shift, r0);
-        const size_t hi = kr_page_row(max(a1 >= 0 ? a1 : a0, 0), p.n_kv, kvh, p.shift, r0 + 16) - 16;
-        constexpr int EB = KT == PG_F32 ? 4 : KT == PG_F16 ? 2 : 1, KD = HALF ? 8 : 4;
+        const size_t hi = kr_page_row(max(a1 >= 0 ? a1 : a0, 0), p.n_kv, kvh, p.shift, r0 + 16);
+        const char *const k0 = (const char *)p.k + lo * hd * EB, *const k1 = (const char *)p.k + hi * hd * EB;
+        const char *const v0 = (const char *)p.v + lo * hd * EB, *const v1 = (const char *)p.v + hi * hd * EB;
+        const int first_u = wave * 64;   // of the wave, whose pieces lie in one half of the tile
 #pragma unroll
         for (int j = 0; j < KN; j++) {
-            const int u = j * NTH + (int)threadIdx.x, row = u / KC, d = u % KC * KD;
-            // past the head's dims: zeros, which meet the queries' zeros
-#pragma unroll
-            for (int w = 0; w < KW; w++) kr[j][w] = 0;
-            if ((SH_R * KC % NTH == 0 || row < SH_R) && d < hd)
-                pa_load(kr[j], (const char *)p.k + ((row < 16 ? lo : hi) + row) * hd * EB + d * EB);
+            const int row = (j * NTH + first_u) / KC;
+            if (SH_R * KC % NTH == 0 || row < SH_R) pa_load(kr[j], (row < 16 ? k0 : k1) + ko[j]);
         }
 #pragma unroll
         for (int j = 0; j < VN; j++) {
-            const int u = j * NTH + (int)threadIdx.x;
-#pragma unroll
-            for (int w = 0; w < VW; w++) vr[j][w] = 0;
-            if (VU % NTH != 0 && u >= VU) continue;
+            if (VU % NTH != 0 && j * NTH + first_u >= VU) continue;
+            const char *const at = (vrow(j * NTH + first_u) < 16 ? v0 : v1) + vo[j];
             if constexpr (HALF) {
-                const int quad = u / (CL / 4), d = u % (CL / 4) * 4;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int row = quad * 4 + i;
-                    unsigned x[VW / 4] = {};
-                    // rows that no column attends may hold anything
-                    if (d < hd && r0 + row >= vf && r0 + row < vl)
-                        pa_load(x, (const char *)p.v + ((row < 16 ? lo : hi) + row) * hd * EB + d * EB);
+                for (int r = 0; r < 4; r++) {
+                    unsigned x[VW / 4];
+                    pa_load(x, at + r * hd * EB);
 #pragma unroll
-                    for (int w = 0; w < VW / 4; w++) vr[j][i * (VW / 4) + w] = x[w];
+                    for (int w = 0; w < VW / 4; w++) vr[j][r * (VW / 4) + w] = x[w];
                 }
             } else {
-                const int row = u / KC, d = u % KC * 4;
-                if (d < hd && r0 + row >= vf && r0 + row < vl)
-                    pa_load(vr[j], (const char *)p.v + ((row < 16 ? lo : hi) + row) * hd * EB + d * EB);
+                pa_load(vr[j], at);
             }
         }
         if constexpr (KT == PG_Q8) {
             const int row = lane & 31;
-            sr = 0.0f;
-            if (wave == 0 && r0 + row >= vf && r0 + row < vl)
-                sr = (lane < 32 ? p.kd : p.vd)[(row < 16 ? lo : hi) + row];
+            if (wave == 0) sr = (lane < 32 ? p.kd : p.vd)[row < 16 ? lo + row : hi + (row - 16)];
         }
     }
 
-    // and lays them down
-    __device__ __forceinline__ void put(int buf) {
+    // and lays them down; rows that no column attends may hold anything, so of V they are zeros
+    __device__ __forceinline__ void put(int buf, int r0) {
+        const bool whole = r0 >= vf && r0 + SH_R <= vl;
+        auto in = [&](int row) { return r0 + row >= vf && r0 + row < vl; };
 #pragma unroll
         for (int j = 0; j < KN; j++) {
             const int u = j * NTH + (int)threadIdx.x, row = u / KC, c = u % KC;
@@ -255,8 +265,12 @@ template <int KT, int CL, int WC> struct ShWork {
         for (int j = 0; j < VN; j++) {
             const int u = j * NTH + (int)threadIdx.x;
             if (VU % NTH != 0 && u >= VU) continue;
+            if (!whole && KT != PG_Q8) {
+#pragma unroll
+                for (int w = 0; w < VW; w++) vr[j][w] = in(vrow(u) + (HALF ? w / (VW / 4) : 0)) ? vr[j][w] : 0u;
+            }
             if constexpr (HALF) {
-                const int quad = u / (CL / 4), d = u % (CL / 4) * 4;
+                const int quad = u / VC, d = u % VC * 4;
                 const int chunk = (quad >> 2) * 2 + (quad & 1), half = (quad >> 1) & 1;
                 uint2v t[4];
                 if constexpr (KT == PG_F16) {
@@ -287,12 +301,16 @@ template <int KT, int CL, int WC> struct ShWork {
             }
         }
         if constexpr (KT == PG_Q8) {
-            if (wave == 0) (lane < 32 ? lds.kd : lds.vd)[buf][lane & 31] = sr;
+            // 8-bit rows are numbers whatever they hold; their scales may be none
+            if (wave == 0) (lane < 32 ? lds.kd : lds.vd)[buf][lane & 31] = whole || in(lane & 31) ? sr : 0.0f;
         }
     }
 
     __device__ __forceinline__ void queries(size_t head) {
         const float *q = a.q + head * hd;
+        // the scores' factor is positive, so that the largest product is the largest score: its sign is the queries', and
+        // of 0 so are the zeros
+        const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : a.scale;
         int e = 0;
         if constexpr (HALF) {
             float x[KS][8], m = 0.0f;
@@ -304,7 +322,7 @@ template <int KT, int CL, int WC> struct ShWork {
                     const float4v t = live && d < hd ? *(const float4v *)(q + d + i) : float4v{ 0, 0, 0, 0 };
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
-                        x[j][i + c] = t[c];
+                        x[j][i + c] = t[c] * sign;
                         m = fmaxf(m, fabsf(t[c]));
                     }
                 }
@@ -327,27 +345,47 @@ template <int KT, int CL, int WC> struct ShWork {
 #pragma unroll
             for (int j = 0; j < KS; j++) {
                 const int d = j * 8 + h * 4;
-                qf[j][0] = live && d < hd ? *(const float4v *)(q + d) : float4v{ 0, 0, 0, 0 };
+                qf[j][0] = live && d < hd ? *(const float4v *)(q + d) * sign : float4v{ 0, 0, 0, 0 };
             }
         }
-        cs = ldexpf(a.cap > 0.0f ? a.scale : a.scale * 1.4426950408889634f, -e);
+        const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+        cs = ldexpf(a.cap > 0.0f ? scale : scale * 1.4426950408889634f, -e);
     }
 
     // the tile at row r0, in LDS
     __device__ __forceinline__ void tile(int buf, int r0) {
         float16v s = {};
+        // eight operands are asked for at once: one by one their way from LDS would be most of a tile's time
+        constexpr int G = 8;
 #pragma unroll
-        for (int j = 0; j < KS; j++) {
-            const uint4v w = *(const uint4v *)(lds.k[buf] + sh_at<KC>(lane & 31, 2 * j + h));
-            if constexpr (HALF) {
+        for (int j0 = 0; j0 < KS; j0 += G) {
+            uint4v w[G];
 #pragma unroll
-                for (int x = 0; x < 2; x++)
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, w), qf[j][x], s, 0, 0, 0);
-            } else {
+            for (int j = 0; j < G && j0 + j < KS; j++) w[j] = *(const uint4v *)(lds.k[buf] + sh_at<KC>(lane & 31, 2 * (j0 + j) + h));
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[c]), qf[j][0][c], s, 0, 0, 0);
+            for (int j = 0; j < G && j0 + j < KS; j++) {
+                if constexpr (HALF) {
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, w[j]), qf[j0 + j][x], s, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[j][c]), qf[j0 + j][0][c], s, 0, 0, 0);
+                }
             }
+        }
+        // V's first operands, on their way meanwhile
+        constexpr int VG = HALF ? (DT < 4 ? DT : 4) : 0;
+        half8 vf8[HALF ? VG : 1][2];
+        auto v_read = [&](int t, int c) { return *(const half8 *)(lds.v[buf] + sh_vt(32 * t + (lane & 31), 2 * c + h)); };
+        if constexpr (HALF) {
+#pragma unroll
+            for (int t = 0; t < VG; t++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) vf8[t][c] = v_read(t, c);
+            __builtin_amdgcn_sched_barrier(0);
         }
         // value i is row (i & 3) + 8 (i >> 2) + 4 h
         if constexpr (KT == PG_Q8) {
@@ -355,16 +393,15 @@ template <int KT, int CL, int WC> struct ShWork {
             for (int i = 0; i < 16; i += 4) {
                 const float4v d = *(const float4v *)(lds.kd[buf] + 2 * i + 4 * h);
 #pragma unroll
-                for (int c = 0; c < 4; c++) s[i + c] *= cs * d[c];
+                for (int c = 0; c < 4; c++) s[i + c] *= d[c];
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[i] *= cs;
         }
+        float ce = cs;   // a score's power of two is s ce
         if (a.cap > 0.0f) {
-            const float inv_cap = 1.0f / a.cap;
+            const float inv_cap = cs / a.cap;
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = pa_tanh(s[i] * inv_cap) * (a.cap * 1.4426950408889634f);
+            for (int i = 0; i < 16; i++) s[i] = pa_tanh(s[i] * inv_cap);
+            ce = a.cap * 1.4426950408889634f;
         }
         if (r0 < wf || r0 + SH_R > wl) {
 #pragma unroll
@@ -376,7 +413,9 @@ template <int KT, int CL, int WC> struct ShWork {
         float m_tile = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; i++) m_tile = fmaxf(m_tile, s[i]);
-        const bool moved = __any(m_tile > m_run);
+        m_tile *= ce;
+        // what the weights are taken from moves where a score passes it by more than SLACK (and at the first)
+        const bool moved = __any(m_tile > m_run + SLACK);
         float f = 1.0f;
         if (moved) {
             const float m_new = fmaxf(m_run, fmaxf(m_tile, sh_other(m_tile)));
@@ -384,14 +423,15 @@ template <int KT, int CL, int WC> struct ShWork {
             m_run = m_new;
             l_run *= f;
         }
-        const float base = m_run == -INFINITY ? 0.0f : m_run;
-        float v_tile = 0.0f;
+        // weights of no finite maximum: 0 for -inf, NaN for NaN
+        const float base = UP - (m_run == -INFINITY ? 0.0f : m_run);
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            s[i] = __builtin_amdgcn_exp2f(s[i] - base);
+            s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], ce, base));
             l_run += s[i];
         }
         if constexpr (KT == PG_Q8) {
+            float v_tile = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const float4v d = *(const float4v *)(lds.vd[buf] + 2 * i + 4 * h);
@@ -414,37 +454,46 @@ template <int KT, int CL, int WC> struct ShWork {
 #pragma unroll
                 for (int t = 0; t < DT; t++) o[t] *= f;
             }
+            const float up = ldexpf(1.0f, PA_UP - ev);
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[i] *= up;
         } else if (moved) {
 #pragma unroll
             for (int t = 0; t < DT; t++) o[t] *= f;
         }
         if constexpr (HALF) {
-            const float up = KT == PG_Q8 ? ldexpf(1.0f, PA_UP - ev) : (float)(1 << PA_UP);
             half8 w[2][2];   // [16 rows][hi, lo]
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const float x = s[i] * up;
-                const _Float16 hi = (_Float16)x;
+                const _Float16 hi = (_Float16)s[i];
                 w[i >> 3][0][i & 7] = hi;
-                w[i >> 3][1][i & 7] = (_Float16)(x - (float)hi);
+                w[i >> 3][1][i & 7] = (_Float16)__builtin_fmaf((float)hi, -1.0f, s[i]);
             }
 #pragma unroll
-            for (int t = 0; t < DT; t++)
+            for (int t0 = 0; t0 < DT; t0 += VG) {
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const half8 v = *(const half8 *)(lds.v[buf] + sh_vt(32 * t + (lane & 31), 2 * c + h));
+                for (int t = 0; t < VG; t++)
 #pragma unroll
-                    for (int x = 0; x < 2; x++) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[c][x], o[t], 0, 0, 0);
-                }
+                    for (int c = 0; c < 2; c++) {
+#pragma unroll
+                        for (int x = 0; x < 2; x++)
+                            o[t0 + t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf8[t][c], w[c][x], o[t0 + t], 0, 0, 0);
+                        if (t0 + VG < DT) vf8[t][c] = v_read(t0 + VG + t, c);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         } else {
 #pragma unroll
-            for (int t = 0; t < DT; t++)
+            for (int t = 0; t < DT; t++) {
+                float v[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int row = (i & 3) + 8 * (i >> 2) + 4 * h, dim = 32 * t + (lane & 31);
-                    const float v = *(const float *)(lds.v[buf] + (row * KC + ((dim >> 2) ^ ((row >> 2 & 1) << 3))) * 16 + (dim & 3) * 4);
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[i], o[t], 0, 0, 0);
+                    v[i] = *(const float *)(lds.v[buf] + (row * KC + ((dim >> 2) ^ ((row >> 2 & 1) << 3))) * 16 + (dim & 3) * 4);
                 }
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[i], s[i], o[t], 0, 0, 0);
+            }
         }
     }
 
@@ -466,18 +515,17 @@ template <int KT, int CL, int WC> struct ShWork {
             find(r0);
             fetch(r0);
             queries(head);
-            put(0);
+            put(0, r0);
             __syncthreads();
             for (int buf = 0; r0 < r1; r0 += SH_R, buf ^= 1) {
                 const bool more = r0 + SH_R < r1;
                 if (more) fetch(r0 + SH_R);
                 tile(buf, r0);
-                if (more) put(buf ^ 1);
+                if (more) put(buf ^ 1, r0 + SH_R);
                 __syncthreads();
             }
         }
-        const float l = l_run + sh_other(l_run);
-        const float f = HALF ? ldexpf(1.0f, KT == PG_Q8 ? ev - PA_UP : -PA_UP) : 1.0f;
+        const float l = ldexpf(l_run + sh_other(l_run), -UP), f = ldexpf(1.0f, KT == PG_Q8 ? ev - PA_UP : -UP);
         if (!live) return;
         const size_t at = slot * CT + wave * 32 + (lane & 31);
         if (h == 0) *(float2v *)(a.spml + at * 2) = float2v{ m_run, l };
