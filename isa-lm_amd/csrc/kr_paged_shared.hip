@@ -20,6 +20,7 @@
 // workgroup and KV head, by the lengths that the device has; a share's sums of a
 // column tile are a part.
 #include <cfloat>
+#include <cmath>
 #include "kr_paged_wave.h"
 
 namespace {
@@ -27,9 +28,10 @@ namespace {
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int SH_R = 32;   // rows a tile
+constexpr int SH_WC = 4, SH_CT = 32 * SH_WC;   // waves and columns of a workgroup
 struct ShArgs : PaShared {
-    float *spart, *spml;   // [n_kv][column tiles + shares][CT][hd] and [2]: the shared rows' parts
-    int sshares, sleast, slots, ct;   // ct: columns of a workgroup
+    float *spart, *spml;   // [n_kv][column tiles + shares][SH_CT][hd] and [2]: the shared rows' parts
+    int sshares, sleast, slots;
     int *fault;
 };
 
@@ -85,7 +87,7 @@ __device__ __forceinline__ ShTiles sh_tiles(const PgView &p, const ShArgs &a, in
         }
     }
     r.rts = (r.g.rows - r.begin + SH_R - 1) / SH_R;
-    r.cts = r.g.rows > 0 ? ((r.g.s1 - r.g.s0) * group + a.ct - 1) / a.ct : 0;
+    r.cts = r.g.rows > 0 ? ((r.g.s1 - r.g.s0) * group + SH_CT - 1) / SH_CT : 0;
     r.sum = pg_scan(r.rts * r.cts);
     r.csum = pg_scan(r.cts);
     const int all = __builtin_amdgcn_readlane(r.sum, 63);
@@ -113,11 +115,11 @@ template <int NC> __device__ __forceinline__ int sh_at(int row, int c) {
 // 4 rows (8 c16 + 4 h + 16 s + 0..3, quad = 4 s + 2 p + h) of one dim of V in halves
 __device__ __forceinline__ int sh_vt(int dim, int chunk) { return dim * 64 + ((chunk ^ ((dim >> 2) & 3)) << 4); }
 
-constexpr int sh_waves(int kt, int cl, int wc) { return wc == 1 || cl > 128 || (kt == PG_F32 && cl > 64) ? 1 : 2; }   // a SIMD
+constexpr int sh_waves(int kt, int cl) { return cl > 128 || (kt == PG_F32 && cl > 64) ? 1 : 2; }   // a SIMD
 
-template <int KT, int CL, int WC> struct ShWork {
+template <int KT, int CL> struct ShWork {
     static constexpr bool HALF = KT != PG_F32;
-    static constexpr int NTH = 64 * WC, CT = 32 * WC;
+    static constexpr int NTH = 64 * SH_WC, CT = SH_CT;
     static constexpr int KC = HALF ? CL / 8 : CL / 4;          // LDS chunks of 16 bytes a row
     static constexpr int KN = (SH_R * KC + NTH - 1) / NTH;     // K chunks a thread
     static constexpr int VU = HALF ? 8 * (CL / 4) : SH_R * KC; // V's pieces: 4 rows of 4 dims, or a chunk
@@ -139,12 +141,12 @@ template <int KT, int CL, int WC> struct ShWork {
     int bad;
     // the piece: rows [row0, row1) in tiles, of which [vf, vl) are attended by a column here
     int lead, vf, vl;
-    bool live;
+    bool live, busy;   // the lane's column, or any of the wave's, is a query head's
     int first, last, wf, wl;   // the column's rows; all columns of the wave have [wf, wl)
     int ids, ids_at;
     unsigned kr[KN][KW], vr[VN][VW];
     unsigned ko[KN], vo[VN];   // this thread's pieces of a tile, bytes from the row that its half of the tile starts at
-    float sr;
+    float sr, minus;   // minus: -1, which the compiler does not see, so that a lo is one instruction
     std::conditional_t<HALF, half8, float4v> qf[KS][HALF ? 2 : 1];
     float cs, m_run, l_run, v_run, v_end;
     int ev;
@@ -152,7 +154,8 @@ template <int KT, int CL, int WC> struct ShWork {
 
     __device__ __forceinline__ ShWork(const PgView &p_, const ShArgs &a_, ShLds<KT, CL> &l, int kvh_)
         : p(p_), a(a_), lds(l), lane(threadIdx.x & 63), h(lane >> 5),
-          wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))), kvh(kvh_), hd(p_.hd), group(a_.nh / p_.n_kv), bad(0) {
+          wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))), kvh(kvh_), hd(p_.hd), group(a_.nh / p_.n_kv), bad(0), sr(0.0f), minus(-1.0f) {
+        asm("" : "+v"(minus));
         // past the head's dims its first ones, which meet zeros (K) or come to nothing (V)
 #pragma unroll
         for (int j = 0; j < KN; j++) {
@@ -172,6 +175,7 @@ template <int KT, int CL, int WC> struct ShWork {
     __device__ __forceinline__ void column(int s0, int s1, int rows, int ct, size_t &head) {
         const int c = ct * CT + wave * 32 + (lane & 31), s = s0 + c / group;
         live = s < s1;
+        busy = __any(live);
         head = live ? (size_t)s * a.nh + kvh * group + c % group : (size_t)s0 * a.nh + kvh * group;
         const int len = live ? kr_page_len(a.len[s], a.max_len, bad) : 0;
         last = min(len, rows);
@@ -467,7 +471,7 @@ template <int KT, int CL, int WC> struct ShWork {
             for (int i = 0; i < 16; i++) {
                 const _Float16 hi = (_Float16)s[i];
                 w[i >> 3][0][i & 7] = hi;
-                w[i >> 3][1][i & 7] = (_Float16)__builtin_fmaf((float)hi, -1.0f, s[i]);
+                w[i >> 3][1][i & 7] = (_Float16)__builtin_fmaf((float)hi, minus, s[i]);
             }
 #pragma unroll
             for (int t0 = 0; t0 < DT; t0 += VG) {
@@ -520,7 +524,7 @@ template <int KT, int CL, int WC> struct ShWork {
             for (int buf = 0; r0 < r1; r0 += SH_R, buf ^= 1) {
                 const bool more = r0 + SH_R < r1;
                 if (more) fetch(r0 + SH_R);
-                tile(buf, r0);
+                if (busy) tile(buf, r0);
                 if (more) put(buf ^ 1, r0 + SH_R);
                 __syncthreads();
             }
@@ -540,11 +544,32 @@ template <int KT, int CL, int WC> struct ShWork {
     }
 };
 
-template <int KT, int CL, int WC>
-__global__ void __launch_bounds__(64 * WC, sh_waves(KT, CL, WC)) k_shared_rows(const PgView p, const ShArgs a) {
+// The first workgroups' waves have shares of the sequences' own rows, the others shares of the
+// shared ones: the former wait for HBM, the latter for the matrix cores (and
+// for power: 64 sequences behind 32,000 rows run at 1.6 GHz), so they are one launch.
+template <int KT, int CL>
+__global__ void __launch_bounds__(64 * SH_WC, sh_waves(KT, CL)) k_shared_rows(const PgView p, const ShArgs a, int own) {
     __shared__ ShLds<KT, CL> lds;
-    const int u = blockIdx.x, kvh = blockIdx.y;
-    ShWork<KT, CL, WC> w(p, a, lds, kvh);
+    // KV heads in turn, so that a die has few of them (of eight one), whose rows its L2 holds for all columns
+    const int kvh = (int)blockIdx.x % p.n_kv, block = (int)blockIdx.x / p.n_kv;
+    if (block < own) {
+        const int u = block * SH_WC + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+        PaWave<KT, CL, false, ShArgs> w(p, a, kvh);
+        PaAll all = pa_all(p, a, w.bad);
+        if (u < all.shares) {
+            int left = pa_bound(all, u + 1) - pa_bound(all, u), t = pa_bound(all, u);
+            for (w.seq = pa_find(p, a, all, t, w.bad); left > 0; w.seq++, t = 0) {
+                w.sp = pa_of(p, a, all, w.seq, w.bad);
+                const int end = min(w.sp.tiles, t + left);
+                w.part(t, end, (size_t)kvh * (p.n_seq + a.shares) + w.seq + u);
+                left -= end - t;
+            }
+        }
+        kr_report(a.fault, w.bad);
+        return;
+    }
+    const int u = block - own;
+    ShWork<KT, CL> w(p, a, lds, kvh);
     const ShTiles all = sh_tiles(p, a, w.bad);
     const int tiles = __builtin_amdgcn_readlane(all.sum, 63);
     if (u < all.shares && tiles > 0) {
@@ -564,23 +589,6 @@ __global__ void __launch_bounds__(64 * WC, sh_waves(KT, CL, WC)) k_shared_rows(c
     kr_report(a.fault, w.bad);
 }
 
-template <int KT, int CL, bool FULL>
-__global__ void __launch_bounds__(64, pa_waves(KT, CL)) k_shared_own(const PgView p, const PaShared a, int *fault) {
-    const int u = blockIdx.x, kvh = blockIdx.y;
-    PaWave<KT, CL, FULL, PaShared> w(p, a, kvh);
-    PaAll all = pa_all(p, a, w.bad);
-    if (u < all.shares) {
-        int left = pa_bound(all, u + 1) - pa_bound(all, u), t = pa_bound(all, u);
-        for (w.seq = pa_find(p, a, all, t, w.bad); left > 0; w.seq++, t = 0) {
-            w.sp = pa_of(p, a, all, w.seq, w.bad);
-            const int end = min(w.sp.tiles, t + left);
-            w.part(t, end, (size_t)kvh * (p.n_seq + a.shares) + w.seq + u);
-            left -= end - t;
-        }
-    }
-    kr_report(fault, w.bad);
-}
-
 // A head of a sequence a workgroup: its own rows' parts, then the shared ones'
 // (2^dl lanes hold its dims four at a time, the workgroup's other factor the parts
 // side by side)
@@ -598,7 +606,7 @@ __global__ void __launch_bounds__(SJ_T) k_shared_join(const PgView p, const ShAr
     const unsigned long long in = __ballot(all.g.rows > 0 && s >= all.g.s0 && s < all.g.s1);
     if (in) {
         const int g = __builtin_ctzll(in), rts = __builtin_amdgcn_readlane(all.rts, g), cts = __builtin_amdgcn_readlane(all.cts, g);
-        const int c = (s - __builtin_amdgcn_readlane(all.g.s0, g)) * group + col, ct = c / a.ct;
+        const int c = (s - __builtin_amdgcn_readlane(all.g.s0, g)) * group + col, ct = c / SH_CT;
         if (rts > 0) {
             const int tiles = __builtin_amdgcn_readlane(all.sum, 63);
             const int t0 = __builtin_amdgcn_readlane(all.sum, g) - rts * cts + ct * rts;
@@ -606,15 +614,15 @@ __global__ void __launch_bounds__(SJ_T) k_shared_join(const PgView p, const ShAr
             const int u0 = share(t0);
             n1 = share(t0 + rts - 1) - u0 + 1;
             const size_t slot = (size_t)kvh * a.slots + __builtin_amdgcn_readlane(all.csum, g) - cts + ct + u0;
-            ml1 = a.spml + (slot * a.ct + c % a.ct) * 2;
-            part1 = a.spart + (slot * a.ct + c % a.ct) * p.hd;
+            ml1 = a.spml + (slot * SH_CT + c % SH_CT) * 2;
+            part1 = a.spart + (slot * SH_CT + c % SH_CT) * p.hd;
         }
     }
     const int n = r.n + n1;
     const auto get = [&](int i) {
-        return *(const float2v *)(i < r.n ? ml0 + (size_t)i * group * 2 : ml1 + (size_t)(i - r.n) * a.ct * 2);
+        return *(const float2v *)(i < r.n ? ml0 + (size_t)i * group * 2 : ml1 + (size_t)(i - r.n) * SH_CT * 2);
     };
-    const auto at = [&](int i) { return i < r.n ? part0 + (size_t)i * group * p.hd : part1 + (size_t)(i - r.n) * a.ct * p.hd; };
+    const auto at = [&](int i) { return i < r.n ? part0 + (size_t)i * group * p.hd : part1 + (size_t)(i - r.n) * SH_CT * p.hd; };
     const int lane = tid & 63;
     float m = -INFINITY, l = 0.0f;
     for (int i = lane; i < n; i += 64) m = fmaxf(m, get(i).x);
@@ -640,32 +648,56 @@ __global__ void __launch_bounds__(SJ_T) k_shared_join(const PgView p, const ShAr
 // ---- the host's side ----
 
 constexpr int SH_CUS = 256;
-int sh_wc(const krh_pages *kv, int n_seq, int nh, int n_groups) {
-    const long long cols = ((long long)n_seq + n_groups - 1) / n_groups * (nh / kv->n_kv_heads);
-    return cols > 32 || kv->head_dim > 128 ? 4 : 1;
-}
 
 struct ShSizes {
-    int wc, shares, sshares, slots;
+    int shares, sshares, slots;
     size_t part, pml, spart, spml;   // floats
 };
-ShSizes sh_sizes(const krh_pages *kv, int n_seq, int nh, int max_len, int n_groups, int max_shared) {
+ShSizes sh_sizes(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_shared) {
     ShSizes r;
     const int group = nh / kv->n_kv_heads;
-    r.wc = sh_wc(kv, n_seq, nh, n_groups);
-    const int ct = 32 * r.wc;
-    const long long cts = (long long)n_seq * group / ct + n_groups, tiles = cts * ((max_shared + SH_R - 1) / SH_R);
-    const long long waves = SH_CUS * 8 / r.wc / kv->n_kv_heads;
-    r.sshares = (int)(waves < 1 ? 1 : waves < tiles ? waves : tiles);
+    const long long cts = (long long)n_seq * group / SH_CT + n_groups, tiles = cts * ((max_shared + SH_R - 1) / SH_R);
+    // as many workgroups as the chip holds at once, a quarter of them for the sequences' own rows
+    const int wgs = SH_CUS * sh_waves(kv->kv_type, kv->head_dim), want = wgs * 3 / 4 / kv->n_kv_heads;
+    r.sshares = (int)(want < 1 ? 1 : want < tiles ? want : tiles);
     r.slots = (int)(cts + r.sshares);
-    r.shares = SH_CUS * 3 / kv->n_kv_heads > 0 ? SH_CUS * 3 / kv->n_kv_heads : 1;
+    r.shares = SH_WC * (wgs / 4 / kv->n_kv_heads > 0 ? wgs / 4 / kv->n_kv_heads : 1);
     const size_t own = (size_t)kv->n_kv_heads * (n_seq + r.shares) * group;
-    const size_t both = (size_t)kv->n_kv_heads * r.slots * ct;
+    const size_t both = (size_t)kv->n_kv_heads * r.slots * SH_CT;
     r.part = own * kv->head_dim;
     r.pml = (own * 2 + 3) & ~(size_t)3;
     r.spart = both * kv->head_dim;
     r.spml = both * 2;
     return r;
+}
+
+// Tiles that a share is worth: two, whose parts are fewer to join (8B shape, halves, 16
+// sequences behind 1024 rows in us, of 1 / 2 / 4: 20.8 / 18.4 / 19.7, 64 31.8 / 30.9 / 27.8); one of those
+// that take long (floats of 256 dims, 32 behind 1024 rows 50.7 / 60 / 83.5, of 128 30.7 / 29.4 / 37.7;
+// halves of 256 dims 27.3 / 27.9 / 35.7).
+int sh_least(const krh_pages *kv) { return kv->kv_type == ML_F32 || kv->head_dim > 128 ? 1 : 2; }
+
+// Whether the shared rows are better passed over once, by estimated times in us. Each
+// sequence by itself (krh_paged_attention): 11.5, and all sequences' rows at the rate at which
+// dies read what others read too (TB/s: halves 14, floats 11, 8 bits 7). Once for
+// all: 13, 0.1 a sequence, and a workgroup's tiles, `tile` each. Measured, each / once,
+// sequences of up to 200 rows behind 256 / 1024 / 4096 / 16,384: 8B shape, halves, 8 13.0 / 15.2, 15.7 /
+// 16.1, 23.6 / 22.5, 49.9 / 32.5, 64 17.1 / 23.8, 37.8 / 30.9, 93 / 38.6, 307 / 67; 1B shape, 8 bits, 16 14.2 / 14.4,
+// 15.5 / 15.3, 22.9 / 21.5, 49.6 / 33.7; floats of 256 dims, 32 23.3 / 37.2, 43.6 / 50.7, 121 / 85.5, 408 / 248.
+bool sh_pays(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_shared, int window) {
+    static const float rate[3] = { 11e6f, 14e6f, 7e6f };                                     // bytes a us: F32, F16, Q8
+    static const float tile[3][3] = { { 1.8f, 4.2f, 20 }, { 1.4f, 1.8f, 6 }, { 1.6f, 2.3f, 8 } };
+    const int t = kv->kv_type == ML_F32 ? 0 : kv->kv_type == ML_F16 ? 1 : 2, c = kv->head_dim <= 64 ? 0 : kv->head_dim <= 128 ? 1 : 2;
+    const double rows = window > 0 && window < max_shared ? window : max_shared;
+    const double row = (double)kv->n_kv_heads * kv->head_dim * (t == 0 ? 8 : t == 1 ? 4 : 2) + (t == 2 ? 8 * kv->n_kv_heads : 0);
+    const double cts = ceil((double)n_seq * (nh / kv->n_kv_heads) / SH_CT);
+    const double tiles = ceil(cts * ceil(rows / SH_R) * kv->n_kv_heads / (SH_CUS * sh_waves(kv->kv_type, kv->head_dim) * 3 / 4));
+    return n_seq > n_groups && 11.5 + n_seq * rows * row / rate[t] > 13.0 + 0.1 * n_seq + tiles * tile[t][c];
+}
+// a workspace is sized without a window, so what it takes has to hold for that too
+bool sh_shared(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_shared, int window) {
+    return n_groups > 0 && max_shared > 0 && sh_pays(kv, n_seq, nh, n_groups, max_shared, 0) &&
+           (window == 0 || sh_pays(kv, n_seq, nh, n_groups, max_shared, window));
 }
 
 bool sh_args_ok(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_groups, int max_shared) {
@@ -677,28 +709,25 @@ bool sh_args_ok(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_
            ((long long)n_seq * (n_heads / kv->n_kv_heads) / 32 + n_groups) * (max_shared / SH_R + 1) <= INT32_MAX / 2;
 }
 
-using ShRows = void (*)(const PgView, const ShArgs);
-template <int KT, int CL> ShRows sh_rows(int wc) {
-    if constexpr (CL <= 128) {
-        if (wc == 1) return k_shared_rows<KT, CL, 1>;
-    }
-    return k_shared_rows<KT, CL, 4>;
+using ShRows = void (*)(const PgView, const ShArgs, int);
+template <int KT> ShRows sh_rows(int hd) {
+    return hd <= 64 ? k_shared_rows<KT, 64> : hd <= 128 ? k_shared_rows<KT, 128> : k_shared_rows<KT, 256>;
 }
-template <int KT> ShRows sh_rows(int hd, int wc) {
-    return hd <= 64 ? sh_rows<KT, 64>(wc) : hd <= 128 ? sh_rows<KT, 128>(wc) : sh_rows<KT, 256>(wc);
-}
-using ShOwn = void (*)(const PgView, const PaShared, int *);
-template <int KT, int CL> ShOwn sh_own(int hd) { return hd == CL ? k_shared_own<KT, CL, true> : k_shared_own<KT, CL, false>; }
-template <int KT> ShOwn sh_own(int hd) { return hd <= 64 ? sh_own<KT, 64>(hd) : hd <= 128 ? sh_own<KT, 128>(hd) : sh_own<KT, 256>(hd); }
 
 }  // namespace
+
+extern "C" int krh_paged_attention_shared_form(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_groups,
+                                               int max_shared, int window) {
+    if (!sh_args_ok(kv, n_seq, n_heads, max_len, n_groups, max_shared)) return -1;
+    return sh_shared(kv, n_seq, n_heads, n_groups, max_shared, window);
+}
 
 extern "C" size_t krh_paged_attention_shared_ws(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_groups,
                                                 int max_shared) {
     if (!sh_args_ok(kv, n_seq, n_heads, max_len, n_groups, max_shared)) return 0;
     const size_t base = krh_paged_attention_ws(kv, n_seq, n_heads, max_len, 0);
-    if (n_groups == 0 || max_shared == 0) return base;
-    const ShSizes r = sh_sizes(kv, n_seq, n_heads, max_len, n_groups, max_shared);
+    if (!sh_shared(kv, n_seq, n_heads, n_groups, max_shared, 0)) return base;
+    const ShSizes r = sh_sizes(kv, n_seq, n_heads, n_groups, max_shared);
     const size_t b = sizeof(float) * (r.part + r.pml + r.spart + r.spml + 4);
     return b > base ? b : base;
 }
@@ -715,12 +744,12 @@ extern "C" void krh_paged_attention_shared(float *o, const krh_pages *kv, const 
         pg_refuse(window >= 0 && (softcap == 0.0f || (softcap >= FLT_MIN && softcap <= 0x1p126f)),
                   "paged_attention_shared: window or soft-cap"))
         return;
-    if (n_groups == 0 || max_shared == 0) {
+    if (!sh_shared(kv, n_seq, n_heads, n_groups, max_shared, window)) {
         krh_paged_attention(o, kv, table, table_ld, len, n_seq, q, n_heads, max_len, window, scale, softcap, nullptr, 0, ws);
         return;
     }
     if (pg_not_ready("paged_attention_shared before krh_init")) return;
-    const ShSizes r = sh_sizes(kv, n_seq, n_heads, max_len, n_groups, max_shared);
+    const ShSizes r = sh_sizes(kv, n_seq, n_heads, n_groups, max_shared);
     float *w = (float *)ws;
     ShArgs a = {};
     a.o = o, a.q = q, a.len = len;
@@ -729,15 +758,11 @@ extern "C" void krh_paged_attention_shared(float *o, const krh_pages *kv, const 
     a.least = 1;
     a.scale = scale, a.cap = softcap;
     a.group = group, a.shared = shared, a.n_groups = n_groups, a.max_shared = max_shared;
-    a.sshares = r.sshares, a.sleast = 4, a.slots = r.slots, a.ct = 32 * r.wc, a.fault = kr_fault_word();
+    a.sshares = r.sshares, a.sleast = sh_least(kv), a.slots = r.slots, a.fault = kr_fault_word();
     const PgView p = pg_view(kv, table, table_ld, n_seq);
-    const int hd = kv->head_dim;
-    const ShRows f = kv->kv_type == ML_F32 ? sh_rows<PG_F32>(hd, r.wc) : kv->kv_type == ML_F16 ? sh_rows<PG_F16>(hd, r.wc)
-                                                                                              : sh_rows<PG_Q8>(hd, r.wc);
-    hipLaunchKernelGGL(f, dim3(r.sshares, kv->n_kv_heads), dim3(64 * r.wc), 0, kr_stream(), p, a);
-    kr_check_launch("paged_attention_shared");
-    const ShOwn g = kv->kv_type == ML_F32 ? sh_own<PG_F32>(hd) : kv->kv_type == ML_F16 ? sh_own<PG_F16>(hd) : sh_own<PG_Q8>(hd);
-    hipLaunchKernelGGL(g, dim3(r.shares, kv->n_kv_heads), dim3(64), 0, kr_stream(), p, (const PaShared &)a, kr_fault_word());
+    const int hd = kv->head_dim, own = (r.shares + SH_WC - 1) / SH_WC;
+    const ShRows f = kv->kv_type == ML_F32 ? sh_rows<PG_F32>(hd) : kv->kv_type == ML_F16 ? sh_rows<PG_F16>(hd) : sh_rows<PG_Q8>(hd);
+    hipLaunchKernelGGL(f, dim3((own + r.sshares) * kv->n_kv_heads), dim3(64 * SH_WC), 0, kr_stream(), p, a, own);
     kr_check_launch("paged_attention_shared");
     hipLaunchKernelGGL(k_shared_join, dim3(n_heads, n_seq), dim3(SJ_T), 0, kr_stream(), p, a, pg_log2(hd / 4));
     kr_check_launch("paged_attention_shared");

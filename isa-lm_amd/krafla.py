@@ -197,6 +197,7 @@ for name, res, args in [
     ("krh_paged_attention_ws", C.c_size_t, [C.POINTER(KrhPages), C.c_int, C.c_int, C.c_int, C.c_int]),
     ("krh_paged_attention", None, [_P, C.POINTER(KrhPages), _P, C.c_int, _P, C.c_int, _P, C.c_int, C.c_int, C.c_int,
                                    C.c_float, C.c_float, _P, C.c_size_t, _P]),
+    ("krh_paged_attention_shared_form", C.c_int, [C.POINTER(KrhPages)] + [C.c_int] * 6),
     ("krh_paged_attention_shared_ws", C.c_size_t, [C.POINTER(KrhPages), C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     ("krh_paged_attention_shared", None, [_P, C.POINTER(KrhPages), _P, C.c_int, _P, C.c_int, _P, _P, C.c_int, C.c_int, _P,
                                           C.c_int, C.c_int, C.c_int, C.c_float, C.c_float, _P]),

@@ -80,17 +80,25 @@ class Batch:
                 x[t, :, used.get(t, 0):] = np.nan if name == "v" else np.inf
         return self
 
-    def put(self, max_len=None, max_shared=None):
+    def put(self, max_len=None, max_shared=None, window=0):
+        """the bounds that the host gives as they are, or so large that sharing pays by them, whatever the lengths are"""
         self.p.put()
         S = len(self.lens)
         self.max_len = max_len or max(max(self.lens), 1)
         self.max_shared = min(self.max_len, max(self.shared)) if max_shared is None else max_shared
+        while max_len is None and self.max_len < 2 ** 19 and not self.form(window):
+            self.max_len *= 2
+            self.max_shared = self.max_len - 1
         self.qb, self.lb = self.dev.put(self.q), self.dev.put(i32(self.lens))
         self.gb, self.sb = self.dev.put(i32(self.start)), self.dev.put(i32([min(s, self.max_shared) for s in self.shared]))
         self.ob = self.dev.put(np.full(self.q.size + 64, 777.0, np.float32))
         self.nb = K.hip.krh_paged_attention_shared_ws(self.p.ref, S, self.nh, self.max_len, len(self.shared), self.max_shared)
         self.ws = self.dev.put(np.full(self.nb + 256, 0xEE, np.uint8))
         return self
+
+    def form(self, window=0):
+        return K.hip.krh_paged_attention_shared_form(self.p.ref, len(self.lens), self.nh, self.max_len, len(self.shared),
+                                                     self.max_shared, window)
 
     def run(self, window=0, cap=0.0, ws=None):
         K.hip.krh_paged_attention_shared(self.ob.ptr, self.p.ref, self.p.tab.ptr, self.p.ld, self.lb.ptr, len(self.lens),
@@ -122,9 +130,10 @@ class Batch:
         assert su == 0 or np.sqrt(sq / su) <= 4 * U * np.sqrt(self.hd + max(self.lens))
 
 
-def check(dev, kv_type, nh, nkv, hd, page, groups, own, window=0, cap=0.0, alone=(0, 0), copies=False, max_len=None, seed=0):
+def check(dev, kv_type, nh, nkv, hd, page, groups, own, window=0, cap=0.0, alone=(0, 0), copies=False, max_len=None, seed=0, form=1):
     rng = np.random.default_rng(seed + hd + 7 * nh + len(own))
-    b = Batch(dev, rng, kv_type, nh, nkv, hd, page, groups, own, alone, copies).spoil().put(max_len)
+    b = Batch(dev, rng, kv_type, nh, nkv, hd, page, groups, own, alone, copies).spoil().put(max_len, window=window)
+    assert form is None or b.form(window) == form
     outs = []
     for _ in range(2):
         b.run(window, cap)
@@ -140,14 +149,16 @@ def own_rows(rng, n, most):
 
 
 HEADS = [(6, 6, 48), (14, 2, 64), (8, 2, 128), (3, 1, 80), (4, 1, 96), (8, 4, 256), (16, 1, 64), (9, 1, 128), (5, 5, 8),
-         (10, 1, 200), (32, 2, 256)]
+         (10, 1, 200), (32, 2, 256), (4, 2, 200)]
 
 
 @pytest.mark.parametrize("kv_type", TYPES)
 @pytest.mark.parametrize("nh,nkv,hd", HEADS)
 def test_heads(dev, kv_type, nh, nkv, hd):
-    check(dev, kv_type, nh, nkv, hd, 16, [(5, 144)], [1, 37, 16, 0, 60])
-    check(dev, kv_type, nh, nkv, hd, 32, [(20, 320)], own_rows(np.random.default_rng(hd), 20, 90))
+    check(dev, kv_type, nh, nkv, hd, 16, [(5, 144)], [1, 37, 16, 0, 60], form=None)
+    # narrow heads and 16 of a KV head pay for many sequences only, wide ones where few share a KV head
+    n, form = 20 if hd > 8 and nh < 16 * nkv and hd != 200 else 100, int(hd <= 128 or nh <= 2 * nkv)
+    check(dev, kv_type, nh, nkv, hd, 32, [(n, 320)], own_rows(np.random.default_rng(hd), n, 90), form=form)
 
 
 @pytest.mark.parametrize("kv_type", TYPES)
@@ -157,7 +168,7 @@ def test_heads(dev, kv_type, nh, nkv, hd):
 def test_shared_rows(dev, kv_type, page, shared, n):
     """shared rows of any number: the page that they end in is each sequence's own"""
     rng = np.random.default_rng(page + n)
-    check(dev, kv_type, 8, 2, 64, page, [(n, shared)], own_rows(rng, n, 50), copies=shared == 200)
+    check(dev, kv_type, 8, 2, 64, page, [(n, shared)], own_rows(rng, n, 50), copies=shared == 200, form=int(n > 2))
 
 
 @pytest.mark.parametrize("kv_type", TYPES)
@@ -175,14 +186,26 @@ def test_sequences_within_the_shared_rows(dev, kv_type):
     """sequences that end before the shared rows do, the first of the group among them, and empty ones"""
     check(dev, kv_type, 8, 2, 64, 16, [(9, 160)], [-150, 5, -1, 0, -160, -80, 3, 17, -159])
     check(dev, kv_type, 8, 2, 128, 16, [(20, 96), (9, 200)], [-96] * 20 + [-200, -190, -30, -130, -200, -100, -60, -199, -64])
-    check(dev, kv_type, 8, 2, 64, 16, [(4, 64)], [-64] * 4)
+    check(dev, kv_type, 8, 2, 64, 16, [(9, 64)], [-64] * 9)
 
 
 @pytest.mark.parametrize("kv_type", TYPES)
-@pytest.mark.parametrize("window,cap", [(1, 0), (33, 50.0), (100, 0), (400, 2.0), (5000, 0), (0, 30.0)])
-def test_window_cap(dev, kv_type, window, cap):
-    check(dev, kv_type, 8, 4, 128, 16, [(12, 320), (5, 160)], [1, 40, 0, 333, 25, 600, 7, -20, -320, 90, 100, 320] +
-          [200, 5, 40, -100, 33], window=window, cap=cap)
+@pytest.mark.parametrize("window,cap,form", [(1, 0, 0), (33, 50.0, 0), (400, 2.0, 0), (0, 30.0, 1), (5000, 0, 1)])
+def test_window_cap(dev, kv_type, window, cap, form):
+    """short windows leave nothing to share: each sequence reads its own"""
+    rng = np.random.default_rng(window)
+    check(dev, kv_type, 8, 4, 128, 16, [(12, 320), (30, 160)], [1, 40, 0, 333, 25, 600, 7, -20, -320, 90, 100, 320] +
+          [200, 5, 40, -100, 33] + own_rows(rng, 25, 60), window=window, cap=cap, form=form)
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("window,shared,cap", [(2500, 2800, 0), (2500, 2544, 30.0), (4000, 3008, 0)])
+def test_long_windows(dev, kv_type, window, shared, cap):
+    """windows that begin within the shared rows, of some sequences or of all, or behind them"""
+    rng = np.random.default_rng(window + shared)
+    own = own_rows(rng, 60, 300)
+    own[1], own[7], own[30], own[41] = 2400, -shared, 2600, -1000
+    check(dev, kv_type, 8, 4, 128, 32, [(40, shared), (20, shared - 600)], own, window=window, cap=cap)
 
 
 @pytest.mark.parametrize("kv_type,hd", [(t, h) for t in TYPES for h in (64, 128, 256)])
@@ -198,8 +221,8 @@ def test_long(dev, kv_type):
     """long shared rows, cut into many parts; a batch whose longest is far under max_len"""
     rng = np.random.default_rng(4)
     check(dev, kv_type, 8, 2, 64, 64, [(10, 5120)], own_rows(rng, 10, 300))
-    check(dev, kv_type, 7, 1, 128, 32, [(20, 1600)], own_rows(rng, 20, 100), max_len=20000)
-    check(dev, kv_type, 4, 1, 64, 64, [(3, 640), (12, 2560)], own_rows(rng, 15, 900))
+    check(dev, kv_type, 7, 1, 128, 32, [(20, 1600)], own_rows(rng, 20, 100), max_len=20000, form=None)
+    check(dev, kv_type, 4, 1, 64, 64, [(3, 640), (32, 2560)], own_rows(rng, 35, 900))
 
 
 def test_64_groups(dev):
@@ -207,15 +230,28 @@ def test_64_groups(dev):
     check(dev, K.ML_F16, 4, 2, 64, 16, [(3, 16 * (g % 5 + 1)) for g in range(64)], own_rows(rng, 200, 30), alone=(0, 8))
 
 
+def test_bounds_decide(dev):
+    """with the bounds as the lengths are, few rows are each sequence's own and many are shared"""
+    rng = np.random.default_rng(7)
+    for groups, own, form in (([(4, 208)], [90, 3, 17, 40], 0), ([(64, 4096)], own_rows(rng, 64, 100), 1)):
+        b = Batch(dev, rng, K.ML_F16, 8, 2, 128, 16, groups, own).spoil()
+        b.put(max_len=max(b.lens), max_shared=groups[0][1])
+        assert b.form() == form
+        b.run()
+        ok()
+        b.check(b.out())
+
+
 def test_long_shared_of_many_kv_heads(dev):
     """more KV heads than workgroups are wanted: a share holds everything"""
-    check(dev, K.ML_F16, 2100, 2100, 8, 16, [(40, 48)], [v % 5 for v in range(40)])
+    check(dev, K.ML_F16, 2100, 2100, 8, 16, [(100, 48)], [v % 5 for v in range(100)])
 
 
 def test_equals_the_call_without_shares(dev):
     """to rounding; and the call is the other one where nothing is shared"""
     rng = np.random.default_rng(8)
     b = Batch(dev, rng, K.ML_F16, 8, 2, 64, 16, [(30, 640)], own_rows(rng, 30, 100)).put()
+    assert b.form() == 1
     b.run()
     ok()
     o = b.out()
@@ -226,6 +262,7 @@ def test_equals_the_call_without_shares(dev):
     o2 = b.out()
     b.check(o)
     b.check(o2)
+    b.sb = dev.put(i32([0]))
     for ng, ms in ((0, 0), (0, 640), (1, 0)):
         K.hip.krh_paged_attention_shared(b.ob.ptr, b.p.ref, b.p.tab.ptr, b.p.ld, b.lb.ptr, 30, None if ng == 0 else b.gb.ptr,
                                          None if ng == 0 else b.sb.ptr, ng, ms, b.qb.ptr, 8, b.max_len, 0, 0.125, 0.0,
@@ -248,7 +285,7 @@ def test_bad_device_data(dev, what):
     elif what == "order":
         start[1] = 2 ** 30
     elif what == "rows":
-        shared[1], good = b.max_shared + 1, range(30)
+        shared[1], good = b.max_shared + 1, range(30)   # (then the second group shares nothing)
     elif what == "negative":
         shared[0], good = -7, range(30, 60)
     elif what == "len":
@@ -290,8 +327,9 @@ def test_captured(dev):
     rng = np.random.default_rng(11)
     a = Batch(dev, rng, K.ML_F16, 8, 2, 64, 16, [(20, 320), (13, 96)], own_rows(rng, 33, 60))
     b = Batch(dev, rng, K.ML_Q8_0, 8, 2, 128, 16, [(33, 160)], own_rows(rng, 33, 60))
-    a.put(max_len=500, max_shared=400)
-    b.put(max_len=500, max_shared=400)
+    a.put(max_len=2 ** 17, max_shared=2 ** 16)
+    b.put(max_len=2 ** 17, max_shared=2 ** 16)
+    assert a.form() == b.form() == 1
     if b.nb > a.nb:
         a.ws, a.nb = b.ws, b.nb
     else:
