@@ -28,10 +28,11 @@ namespace {
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int SH_R = 32;   // rows a tile
+constexpr int SH_FEW = 8;   // tiles a share up to which a compute unit has one workgroup
 constexpr int SH_WC = 4, SH_CT = 32 * SH_WC;   // waves and columns of a workgroup
 struct ShArgs : PaShared {
     float *spart, *spml;   // [n_kv][column tiles + shares][SH_CT][hd] and [2]: the shared rows' parts
-    int sshares, sleast, slots;
+    int sshares, sfew, sleast, slots;
     int *fault;
 };
 
@@ -91,7 +92,9 @@ __device__ __forceinline__ ShTiles sh_tiles(const PgView &p, const ShArgs &a, in
     r.sum = pg_scan(r.rts * r.cts);
     r.csum = pg_scan(r.cts);
     const int all = __builtin_amdgcn_readlane(r.sum, 63);
-    r.shares = max(1, min(a.sshares, (all + a.sleast - 1) / a.sleast));
+    // as many workgroups as there are compute units, the own rows' among them, where that gives each a few tiles only
+    const int most = all <= SH_FEW * a.sfew ? a.sfew : a.sshares;
+    r.shares = max(1, min(most, (all + a.sleast - 1) / a.sleast));
     return r;
 }
 
@@ -650,7 +653,7 @@ __global__ void __launch_bounds__(SJ_T) k_shared_join(const PgView p, const ShAr
 constexpr int SH_CUS = 256;
 
 struct ShSizes {
-    int shares, sshares, slots;
+    int shares, sshares, sfew, slots;
     size_t part, pml, spart, spml;   // floats
 };
 ShSizes sh_sizes(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_shared) {
@@ -660,6 +663,9 @@ ShSizes sh_sizes(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_s
     // as many workgroups as the chip holds at once, a quarter of them for the sequences' own rows
     const int wgs = SH_CUS * sh_waves(kv->kv_type, kv->head_dim), want = wgs * 3 / 4 / kv->n_kv_heads;
     r.sshares = (int)(want < 1 ? 1 : want < tiles ? want : tiles);
+    // Where a compute unit holds two, one each while there are few tiles (8B shape, halves, in us, 128 / 256 / 384
+    // workgroups for the shared rows: 16 sequences behind 2048 20.9 / 23.7 / -, 64 33.0 / 37.8 / 38.7, behind 4096 42.0 / - / 40.6)
+    r.sfew = wgs > SH_CUS && wgs / 4 / kv->n_kv_heads < r.sshares ? wgs / 4 / kv->n_kv_heads : r.sshares;
     r.slots = (int)(cts + r.sshares);
     r.shares = SH_WC * (wgs / 4 / kv->n_kv_heads > 0 ? wgs / 4 / kv->n_kv_heads : 1);
     const size_t own = (size_t)kv->n_kv_heads * (n_seq + r.shares) * group;
@@ -758,7 +764,7 @@ extern "C" void krh_paged_attention_shared(float *o, const krh_pages *kv, const 
     a.least = 1;
     a.scale = scale, a.cap = softcap;
     a.group = group, a.shared = shared, a.n_groups = n_groups, a.max_shared = max_shared;
-    a.sshares = r.sshares, a.sleast = sh_least(kv), a.slots = r.slots, a.fault = kr_fault_word();
+    a.sshares = r.sshares, a.sfew = r.sfew, a.sleast = sh_least(kv), a.slots = r.slots, a.fault = kr_fault_word();
     const PgView p = pg_view(kv, table, table_ld, n_seq);
     const int hd = kv->head_dim, own = (r.shares + SH_WC - 1) / SH_WC;
     const ShRows f = kv->kv_type == ML_F32 ? sh_rows<PG_F32>(hd) : kv->kv_type == ML_F16 ? sh_rows<PG_F16>(hd) : sh_rows<PG_Q8>(hd);
