@@ -39,10 +39,10 @@
 
 namespace {
 
-template <int KT, int CL, bool FULL>
+template <int KT, int CL, bool FULL, bool FINE>
 __global__ void __launch_bounds__(64, pa_waves(KT, CL)) k_paged_shares(const PgView p, const PaArgs a, int *fault) {
     const int u = blockIdx.x, kvh = blockIdx.y;
-    PaWave<KT, CL, FULL> w(p, a, kvh);
+    PaWave<KT, CL, FULL, PaArgs, FINE> w(p, a, kvh);
     if (a.whole) {
         w.seq = u;
         w.sp = pa_span(a, kr_page_len(a.len[u], a.max_len, w.bad), 0);
@@ -223,11 +223,11 @@ using PaKernel = void (*)(const PgView, const PaArgs, int *);
 // Heads take the next width of 64, 128 and 256 dims; a kernel of its own has them
 // where they fill it (without, halves take 0 to 2% more, 8 bits 0 to 6, floats 1 and of
 // 256 dims 7).
-template <int KT, int CL> PaKernel pa_kernel(int hd) {
-    return hd == CL ? k_paged_shares<KT, CL, true> : k_paged_shares<KT, CL, false>;
+template <int KT, int CL, bool FINE> PaKernel pa_kernel(int hd) {
+    return hd == CL ? k_paged_shares<KT, CL, true, FINE> : k_paged_shares<KT, CL, false, FINE>;
 }
-template <int KT> PaKernel pa_kernel(int hd) {
-    return hd <= 64 ? pa_kernel<KT, 64>(hd) : hd <= 128 ? pa_kernel<KT, 128>(hd) : pa_kernel<KT, 256>(hd);
+template <int KT, bool FINE = false> PaKernel pa_kernel(int hd) {
+    return hd <= 64 ? pa_kernel<KT, 64, FINE>(hd) : hd <= 128 ? pa_kernel<KT, 128, FINE>(hd) : pa_kernel<KT, 256, FINE>(hd);
 }
 
 }  // namespace
@@ -238,9 +238,9 @@ extern "C" size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_h
     return sizeof(float) * (r.part + r.pml + r.z + 4);
 }
 
-extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len,
-                                    int n_seq, const float *q, int n_heads, int max_len, int window, float scale,
-                                    float softcap, float *mass, size_t mass_ld, void *ws) {
+void kr_paged_attention(bool fine, float *o, const krh_pages *kv, const int *table, int table_ld, const int *len, int n_seq,
+                        const float *q, int n_heads, int max_len, int window, float scale, float softcap, float *mass,
+                        size_t mass_ld, void *ws) {
     if (n_seq == 0) return;
     if (pg_refuse(pa_args_ok(kv, n_seq, n_heads, max_len), "paged_attention sizes") ||
         pg_refuse(o && table && table_ld > 0 && len && q && ws && pg_aligned(o) && pg_aligned(q) && pg_aligned(ws),
@@ -270,8 +270,10 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
     a.scale = scale, a.cap = softcap;
     const PgView p = pg_view(kv, table, table_ld, n_seq);
     const int hd = kv->head_dim;
-    const PaKernel f = kv->kv_type == ML_F32 ? pa_kernel<PG_F32>(hd) : kv->kv_type == ML_F16 ? pa_kernel<PG_F16>(hd)
-                                                                                                    : pa_kernel<PG_Q8>(hd);
+    const PaKernel f = kv->kv_type == ML_F16   ? pa_kernel<PG_F16>(hd)
+                       : kv->kv_type == ML_Q8_0 ? pa_kernel<PG_Q8>(hd)
+                       : fine                   ? pa_kernel<PG_F32, true>(hd)
+                                                : pa_kernel<PG_F32>(hd);
     hipLaunchKernelGGL(f, dim3(shares, kv->n_kv_heads), dim3(64), 0, kr_stream(), p, a, kr_fault_word());
     kr_check_launch("paged_attention");
     if ((shares > 1 && !whole) || mass) {
@@ -279,4 +281,10 @@ extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *ta
                            pg_log2(hd / 4), blocks);
         kr_check_launch("paged_attention");
     }
+}
+
+extern "C" void krh_paged_attention(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len,
+                                    int n_seq, const float *q, int n_heads, int max_len, int window, float scale,
+                                    float softcap, float *mass, size_t mass_ld, void *ws) {
+    kr_paged_attention(false, o, kv, table, table_ld, len, n_seq, q, n_heads, max_len, window, scale, softcap, mass, mass_ld, ws);
 }
