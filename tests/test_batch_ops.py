@@ -20,14 +20,14 @@ NORM = dict(xo=PTR, ldxo=64, x=PTR, ldx=64, y=PTR + 4096, ldy=64, post=PTR, gate
 DEQ = dict(x=PTR, ldx=64, q=PTR, ldq=64, d=PTR, ldd=1, n=64, rows=3)
 
 BAD_MATS = [dict(q=None), dict(d=None), dict(q=PTR + 8), dict(ld=48), dict(ld=56), dict(rows=0), dict(rows=-1),
-            dict(rows=2**31 - 1), dict(cols=0), dict(cols=-5), dict(cols=65), dict(cols=1 << 17, ld=1 << 17)]
+            dict(rows=2**31 - 1), dict(ld=2**23 + 16), dict(cols=0), dict(cols=-5), dict(cols=65), dict(cols=1 << 17, ld=1 << 17)]
 
 CASES = [("krh_matmul_i8", I8, kw) for kw in
          [dict(Y=None), dict(xq=None), dict(xd=None), dict(W=None), dict(T=-1), dict(T=70000), dict(ldy=23), dict(ldx=48),
-          dict(ldx=72), dict(xq=PTR + 4)] + [dict(W=mat(**b)) for b in BAD_MATS]]
+          dict(ldx=72), dict(ldx=2**23 + 16), dict(xq=PTR + 4)] + [dict(W=mat(**b)) for b in BAD_MATS]]
 CASES += [("krh_matmul_i8_swiglu", GLU, kw) for kw in
           [dict(H=None), dict(xq=None), dict(xd=None), dict(w1=None), dict(w3=None), dict(T=-1), dict(T=70000), dict(ldh=23),
-           dict(ldx=48), dict(ldx=72), dict(xq=PTR + 8), dict(w3=mat(rows=25)), dict(w1=mat(cols=49))] +
+           dict(ldx=48), dict(ldx=72), dict(ldx=2**23 + 16), dict(xq=PTR + 8), dict(w3=mat(rows=25)), dict(w1=mat(cols=49))] +
           [dict(w1=mat(**b)) for b in BAD_MATS] + [dict(w3=mat(**b)) for b in BAD_MATS]]
 CASES += [("krh_block_norm", NORM, kw) for kw in
           [dict(x=None), dict(xo=None, z=None, q=None, d=None), dict(pre=None), dict(y=None), dict(q=None), dict(d=None),
@@ -112,3 +112,22 @@ def test_shared_attention_workspaces():
     for bad in ((kv, 0, 4, 64, 2, 48), (kv, 20, 5, 64, 2, 48), (kv, 20, 4, 64, 65, 48), (kv, 20, 4, 64, 2, 65),
                 (None, 20, 4, 64, 2, 48)):
         assert ws(*bad) == 0
+
+
+def test_forms():
+    """which tiles or passes a call takes, and that sizes without one have none"""
+    i8 = K.hip.krh_matmul_i8_form
+    for size in ((0, 64, 1), (64, 0, 1), (64, 1 << 17, 1), (64, 64, 0), (-1, 64, 1)):
+        assert i8(*size, 0) == i8(*size, 1) == -1
+    seen = {(glu, i8(rows, cols, T, glu)) for glu in (0, 1) for rows in (16, 300, 4096, 14336) for cols in (64, 4096, 14336)
+            for T in (1, 8, 9, 40, 64, 128, 300, 2047, 8192)}
+    assert {f for _, f in seen} <= set(range(8)) and len(seen) >= 8
+    form = K.hip.krh_paged_attention_shared_form
+    kv = C.byref(pages(head_dim=128, n_kv_heads=8))
+    for bad in ((kv, 0, 32, 4096, 1, 48, 0), (kv, 20, 31, 4096, 1, 48, 0), (kv, 20, 32, 4096, 65, 48, 0),
+                (kv, 20, 32, 4096, 1, 4097, 0), (None, 20, 32, 4096, 1, 48, 0)):
+        assert form(*bad) == -1
+    assert form(kv, 64, 32, 40000, 1, 32000, 0) == 1
+    # nothing shared, few rows, or a window that ends behind them
+    for few in ((kv, 64, 32, 40000, 0, 0, 0), (kv, 64, 32, 40000, 1, 0, 0), (kv, 1, 32, 64, 1, 16, 0), (kv, 64, 32, 40000, 1, 32000, 16)):
+        assert form(*few) == 0
