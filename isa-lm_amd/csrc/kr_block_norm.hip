@@ -7,12 +7,20 @@
 // one write: x' = x + alpha (gate (y / rms(y)) post), z = (x' / rms(x')) pre,
 // q = z's 8-bit row. Three sums over the row at most (two of squares, in 64
 // bits, and the largest |z|) are all that its threads wait for each other for.
+//
+// Bound by HBM with many rows, 16 bytes a value (13 with 8-bit rows): 2047 rows of
+// 4096 29.0 us (4.6 TB/s), 8000 97 (5.4), 2047 of 2048 12.6 (5.3); the sums' 64-bit
+// products, two a value, hide behind it. By the launch and three waits of a row with
+// few: 16 rows of 4096 4.6 us, as long as any small launch takes here. One pass in place of
+// the five calls that do the same in turn, whose values pass through memory each time.
 #include "kr_internal.h"
 #include "kr_numerics.h"
 
 namespace {
 
-constexpr int BN_K = 4, BN_V = 4 * BN_K;   // values a thread
+// values a thread. With 8, twice the threads: 16 rows of 4096 as long, 8000 94.8 us instead of 97.4, 2047 of 8192 55.6
+// instead of 53.8, and rows of 16,384 have no workgroup; with 4, 8000 rows 110.3
+constexpr int BN_K = 4, BN_V = 4 * BN_K;
 constexpr int BN_MAX = 1024 * BN_V;
 
 struct BnArgs {
@@ -161,6 +169,7 @@ template <int T, bool VEC> __global__ void __launch_bounds__(T) k_block_norm(con
     }
 }
 
+// By HBM, 5 bytes a value: 2047 rows of 4096 10 us (4.2 TB/s)
 constexpr int DQ_T = 256;
 template <bool VEC>
 __global__ void __launch_bounds__(DQ_T) k_dequantize_row(float *x, size_t ldx, const int8_t *q, size_t ldq, const float *d,
@@ -218,10 +227,16 @@ extern "C" void krh_block_norm(float *xo, size_t ldxo, const float *x, size_t ld
         hipLaunchKernelGGL(f, dim3(rows), dim3(threads), 0, kr_stream(), a);
         kr_check_launch("block_norm");
     };
+    // the fewest threads whose registers hold a row: 2047 rows of 2048 by 128 threads 12.6 us, by 256 14.4; of 8192 by
+    // 512 53.8, by 1024 64.1
     if (n <= 64 * BN_V) {
         launch(vec ? k_block_norm<64, true> : k_block_norm<64, false>, 64);
+    } else if (n <= 128 * BN_V) {
+        launch(vec ? k_block_norm<128, true> : k_block_norm<128, false>, 128);
     } else if (n <= 256 * BN_V) {
         launch(vec ? k_block_norm<256, true> : k_block_norm<256, false>, 256);
+    } else if (n <= 512 * BN_V) {
+        launch(vec ? k_block_norm<512, true> : k_block_norm<512, false>, 512);
     } else {
         launch(vec ? k_block_norm<1024, true> : k_block_norm<1024, false>, 1024);
     }
