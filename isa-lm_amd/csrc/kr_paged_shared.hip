@@ -601,8 +601,9 @@ __global__ void __launch_bounds__(64 * SH_WC, sh_waves(KT, CL)) k_shared_rows(co
 
 // A head of a sequence a workgroup: its own rows' parts, then the shared ones'
 // (2^dl lanes hold its dims four at a time, the workgroup's other factor the parts
-// side by side)
-constexpr int SJ_T = 256;
+// side by side). By latency, so the parts are asked for before their weights are known: 512
+// heads of 17 parts of 128 dims 6.3 us (7.5 one after the other), 2048 of 26 12.2 (13.6).
+constexpr int SJ_T = 256, SJ_N = 4;   // threads; parts a thread asks for at once
 __global__ void __launch_bounds__(SJ_T) k_shared_join(const PgView p, const ShArgs a, int dl) {
     __shared__ float4v s_o[SJ_T];
     const int s = blockIdx.y, x = blockIdx.x, tid = threadIdx.x, group = a.nh / p.n_kv, kvh = x / group, col = x % group;
@@ -633,26 +634,43 @@ __global__ void __launch_bounds__(SJ_T) k_shared_join(const PgView p, const ShAr
         return *(const float2v *)(i < r.n ? ml0 + (size_t)i * group * 2 : ml1 + (size_t)(i - r.n) * SH_CT * 2);
     };
     const auto at = [&](int i) { return i < r.n ? part0 + (size_t)i * group * p.hd : part1 + (size_t)(i - r.n) * SH_CT * p.hd; };
-    const int lane = tid & 63;
-    float m = -INFINITY, l = 0.0f;
-    for (int i = lane; i < n; i += 64) m = fmaxf(m, get(i).x);
+    // the first parts are on their way while the weights are found
+    const int lane = tid & 63, first = tid >> dl, lanes = SJ_T >> dl, q = tid & ((1 << dl) - 1), d = 4 * q < p.hd ? 4 * q : 0;
+    float4v v[SJ_N];
+    const auto fetch = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < SJ_N; k++) v[k] = *(const float4v *)(at(min(i + k * lanes, n - 1)) + d);
+    };
+    const float2v mine = lane < n ? get(lane) : float2v{ -INFINITY, 0.0f };
+    fetch(first);
+    float m = mine.x;
+    for (int i = lane + 64; i < n; i += 64) m = fmaxf(m, get(i).x);
     for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     const auto weight = [&](float v) { return v == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v - m); };
-    for (int i = lane; i < n; i += 64) {
+    const float w = weight(mine.x);
+    float l = mine.y * w;
+    for (int i = lane + 64; i < n; i += 64) {
         const float2v v = get(i);
         l += v.y * weight(v.x);
     }
     for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
     const float inv = sp.len == 0 ? 0.0f : 1.0f / l;
-    const int q = tid & ((1 << dl) - 1), lanes = SJ_T >> dl, d = 4 * q < p.hd ? 4 * q : 0;
     float4v acc = { 0, 0, 0, 0 };
-    for (int i = tid >> dl; i < n; i += lanes) acc += *(const float4v *)(at(i) + d) * weight(get(i).x);
+    for (int i0 = 0; i0 < n; i0 += SJ_N * lanes) {
+        if (i0 > 0) fetch(i0 + first);
+#pragma unroll
+        for (int k = 0; k < SJ_N; k++) {
+            const int i = i0 + first + k * lanes;
+            const float x = __shfl(w, i & 63);
+            if (i < n) acc += v[k] * (i < 64 ? x : weight(get(i).x));
+        }
+    }
     s_o[tid] = acc;
     for (int k = lanes >> 1; k >= 1; k >>= 1) {
         __syncthreads();
-        if ((tid >> dl) < k) s_o[tid] = acc = acc + s_o[tid + (k << dl)];
+        if (first < k) s_o[tid] = acc = acc + s_o[tid + (k << dl)];
     }
-    if (tid >> dl == 0 && 4 * q < p.hd) *(float4v *)(a.o + ((size_t)s * a.nh + x) * p.hd + d) = acc * inv;
+    if (first == 0 && 4 * q < p.hd) *(float4v *)(a.o + ((size_t)s * a.nh + x) * p.hd + d) = acc * inv;
 }
 
 // ---- the host's side ----
