@@ -499,7 +499,7 @@ void krh_matmul_i8(float *Y, size_t ldy, const krh_mat8 *W, const int8_t *xq, si
 void krh_matmul_i8_swiglu(float *H, size_t ldh, const krh_mat8 *w1, const krh_mat8 *w3, const int8_t *xq, size_t ldx,
                           const float *xd, int T);
 /* The tiles that krh_matmul_i8 takes for these sizes, or krh_matmul_i8_swiglu for a
- * pair of matrices: 0 to 7 (kr_matmul_i8.hip's forms), -1 for no size. The results
+ * pair of matrices: 0 to 8 (kr_matmul_i8.hip's forms), -1 for no size. The results
  * are the same bits whatever they are. */
 int krh_matmul_i8_form(int rows, int cols, int ntok, int swiglu);
 

@@ -6,6 +6,7 @@
 // float conversion and two products an output.
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 #include "kr_internal.h"
 #include "kr_numerics.h"
 
@@ -52,69 +53,6 @@ __device__ __forceinline__ float i8_silu_mul(float g, float u) {
     return kr_fmul(kr_fmul(g, s), u);
 }
 
-// Up to 16 tokens: a workgroup has 16 rows, its waves parts of
-// the reduction: lines of 128 values in turn, read straight into operand
-// registers, FEW_D steps of 64 values ahead. The parts' sums meet in LDS. Bound by
-// HBM: one token, 4096 rows of 14,336 12.0 us (4.9 TB/s), of 4096 5.7. A lane's 16
-// bytes are a row's of its own, which a CU reads at about 16 bytes a clock, so
-// with more tokens their reads take longer than W's (16: 17.0 us).
-constexpr int FEW_W = 8, FEW_T = 64 * FEW_W, FEW_D = 8;
-__global__ void __launch_bounds__(FEW_T) k_i8_few(const I8Args a) {
-    static_assert(FEW_D % 2 == 0, "whole lines");
-    __shared__ v4i s_sum[FEW_W][64];
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int r0 = blockIdx.x * 16;
-    const int8_t *xb = a.x, *wb = a.w[0] + (size_t)r0 * a.ldw[0];
-    const unsigned wo = (unsigned)min(n, a.rows - 1 - r0) * (unsigned)a.ldw[0];
-    const unsigned xo = (unsigned)min(n, a.ntok - 1) * (unsigned)a.ldx;
-    const int last = (a.cols - 1) & ~15;   // the last 16 bytes with a value, which are read for those past them
-    // this wave's step u is half of its line u / 2
-    auto at = [&](int u) { return ((u >> 1) * FEW_W + wave) * 128 + (u & 1) * 64 + 16 * g; };
-    v4i w[FEW_D], x[FEW_D], acc = {};
-    auto load = [&](int u, v4i &w, v4i &x) {
-        const unsigned k = min(at(u), last);
-        w = *(const v4i *)(wb + (wo + k));
-        x = *(const v4i *)(xb + (xo + k));
-    };
-    const int lines = (a.cols + 127) / 128, steps = wave < lines ? 2 * ((lines - wave + FEW_W - 1) / FEW_W) : 0;
-    if (steps > 0) {
-#pragma unroll
-        for (int i = 0; i < FEW_D; i++) load(i, w[i], x[i]);
-        int u = 0;
-        for (; u + FEW_D < steps; u += FEW_D) {
-#pragma unroll
-            for (int i = 0; i < FEW_D; i++) {
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], x[i], acc, 0, 0, 0);
-                load(u + FEW_D + i, w[i], x[i]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        // the last steps, of which some end within the row or lie past it
-#pragma unroll
-        for (int i = 0; i < FEW_D; i++)
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(i8_cut(w[i], a.cols - at(u + i)), x[i], acc, 0, 0, 0);
-    }
-    s_sum[wave][lane] = acc;
-    __syncthreads();
-    // one wave has four rows of a token a lane
-    if (wave > 0) return;
-    v4i sum = {};
-#pragma unroll
-    for (int v = 0; v < FEW_W; v++) sum += s_sum[v][lane];
-    const int r = r0 + 4 * g;
-    if (n >= a.ntok) return;
-    const float xd = a.xd[n];
-    float *y = a.y + (size_t)n * a.ldy + r;
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-        if (r + c >= a.rows) break;
-        float v = i8_scaled(sum[c], xd, a.wd[0][r + c]);
-        if (a.bias) v = kr_fadd(v, a.bias[r + c]);
-        y[c] = a.add ? kr_fadd(y[c], v) : v;
-    }
-}
-
 // Tiles of BT tokens and BR rows (GLU: 32 rows of each matrix in turn), WT x WR
 // waves with an even part each, or WK times as many, each with a part of the
 // reduction. That goes in stages of BK values, which pass from memory to LDS
@@ -130,8 +68,11 @@ __global__ void __launch_bounds__(FEW_T) k_i8_few(const I8Args a) {
 // tokens of the 8B shape's w1 and w3 take 252 us (1.9 POP/s; 267 with waves of 128 x 128,
 // one a SIMD; 333 in tiles of 128 x 128). Small tiles: the way of a stage's operands from
 // LDS, with a wave a SIMD 0.4 us a stage, which the split of the reduction over 8 waves
-// shares out: 64 tokens, 4096 rows of 4096, 7.6 us (18.4 in tiles of 64 x 64 without it,
-// 12.5 with operands from memory).
+// shares out: 64 tokens, 4096 rows of 4096, 7.3 us (18.4 in tiles of 64 x 64 without it,
+// 12.5 with operands from memory). Few tokens: HBM, where all compute units have a
+// tile, for which tiles have 16 rows: one token, 4096 rows of 14,336 12.1 us (4.9 TB/s), 16
+// 13.5 (19.8 in tiles of 32 rows, on half of the units; 20.9 with operands from memory,
+// of which a unit reads about 16 bytes a clock).
 typedef int v16i __attribute__((ext_vector_type(16)));
 
 // 16 bytes a lane from base + off to LDS at `to` (one address a wave) + 16 lane.
@@ -149,10 +90,12 @@ template <int KC> __device__ __forceinline__ int i8_chunk(int row, int c) { retu
 
 template <int BT_, int BR_, int WT_, int WR_, int BK_, int NB_, int WK_ = 1> struct I8Tile {
     static constexpr int BT = BT_, BR = BR_, WT = WT_, WR = WR_, BK = BK_, NB = NB_, WK = WK_;
-    static constexpr int WAVES = WT * WR * WK, T = 64 * WAVES, KC = BK / 16, MT = BT / WT / 32, NT = BR / WR / 32;
+    static constexpr int MB = BR / WR < 32 ? 16 : 32;              // tokens and rows of a product, of G 16-byte chunks each
+    static constexpr int G = 64 / MB, Q = MB * MB / 256;           // a product's values of a lane: Q times four
+    static constexpr int WAVES = WT * WR * WK, T = 64 * WAVES, KC = BK / 16, MT = BT / WT / MB, NT = BR / WR / MB;
     static constexpr int PER = 64 / KC;                            // rows a wave's load covers
     static constexpr int LX = BT / PER / WAVES, LW = BR / PER / WAVES;   // loads a wave and stage
-    static_assert(LX * PER * WAVES == BT && LW * PER * WAVES == BR && 32 % PER == 0 && BK % 64 == 0, "whole loads");
+    static_assert(LX * PER * WAVES == BT && LW * PER * WAVES == BR && MB % PER == 0 && BK % (16 * G * WK) == 0, "whole loads");
 };
 
 // the schedule of P products with R reads spread evenly behind them
@@ -169,7 +112,9 @@ template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(c
     constexpr int XB = S::BT * BK, WB = S::BR * BK;
     __shared__ alignas(16) int8_t s_ring[NB * (XB + WB)];
     int8_t *const s_x = s_ring, *const s_w = s_ring + NB * XB;
-    const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    constexpr int MB = S::MB;
+    static_assert(MB == 32 || !GLU, "32 rows of each matrix");
+    const int lane = threadIdx.x & 63, h = lane / MB, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     // Consecutive workgroups go to the dies in turn: each die has consecutive tiles,
     // 8 token tiles of a row tile after one another, which share what its L2 holds
     const int all = nt * nr, q = all / 8, rem = all % 8, die = blockIdx.x % 8;
@@ -235,29 +180,33 @@ template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(c
         }
         __syncthreads();
     };
-    v16i acc[S::MT][S::NT] = {};
-    const int wk = wave / (S::WT * S::WR), wg = wave % (S::WT * S::WR), wt = wg / S::WR, wr = wg % S::WR, n = lane & 31;
-    constexpr int KS = BK / 32 / S::WK;   // steps of a stage, of which the wave's are wk * KS ..
+    typedef std::conditional_t<MB == 32, v16i, v4i> Sum;
+    Sum acc[S::MT][S::NT] = {};
+    const int wk = wave / (S::WT * S::WR), wg = wave % (S::WT * S::WR), wt = wg / S::WR, wr = wg % S::WR, n = lane % MB;
+    constexpr int KS = BK / (16 * S::G) / S::WK;   // steps of a stage, of which the wave's are wk * KS ..
     // Small tiles ask for a stage's operands at once, whose way from LDS would else
     // be most of a step; larger ones for the next step's among a step's products
     constexpr bool ALL = S::MT * S::NT <= 2 || S::WK > 1;
     constexpr int D = ALL ? KS : 2;
     v4i xv[D][S::MT], wv[D][S::NT];
-    // the operands of 32 values, step k of a stage
+    // a product's operands, step k of a stage
     auto read = [&](int st, int k, v4i (&x)[S::MT], v4i (&w)[S::NT]) {
-        const int c = i8_chunk<KC>(n, 2 * (wk * KS + k) + h) * 16;
-        const int8_t *sx = s_x + st % NB * XB + (wt * S::MT * 32 + n) * BK + c;
-        const int8_t *sw = s_w + st % NB * WB + (wr * S::NT * 32 + n) * BK + c;
+        const int c = i8_chunk<KC>(n, S::G * (wk * KS + k) + h) * 16;
+        const int8_t *sx = s_x + st % NB * XB + (wt * S::MT * MB + n) * BK + c;
+        const int8_t *sw = s_w + st % NB * WB + (wr * S::NT * MB + n) * BK + c;
 #pragma unroll
-        for (int m = 0; m < S::MT; m++) x[m] = *(const v4i *)(sx + m * 32 * BK);
+        for (int m = 0; m < S::MT; m++) x[m] = *(const v4i *)(sx + m * MB * BK);
 #pragma unroll
-        for (int m = 0; m < S::NT; m++) w[m] = *(const v4i *)(sw + m * 32 * BK);
+        for (int m = 0; m < S::NT; m++) w[m] = *(const v4i *)(sw + m * MB * BK);
     };
     auto products = [&](const v4i (&x)[S::MT], const v4i (&w)[S::NT]) {
 #pragma unroll
         for (int m = 0; m < S::MT; m++)
 #pragma unroll
-            for (int c = 0; c < S::NT; c++) acc[m][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[m], w[c], acc[m][c], 0, 0, 0);
+            for (int c = 0; c < S::NT; c++) {
+                if constexpr (MB == 32) acc[m][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[m], w[c], acc[m][c], 0, 0, 0);
+                else acc[m][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[m], w[c], acc[m][c], 0, 0, 0);
+            }
     };
 #pragma unroll
     for (int st = 0; st < NB - 1; st++)
@@ -321,14 +270,14 @@ template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(c
     float wd[S::NT / M][M], bias[S::NT / M];
 #pragma unroll
     for (int c = 0; c < S::NT / M; c++) {
-        r[c] = r0 + (wr * S::NT / M + c) * 32 + n;
+        r[c] = r0 + (wr * S::NT / M + c) * MB + n;
         const int at = min(r[c], a.rows - 1);
         wd[c][0] = a.wd[0][at];
         if constexpr (GLU) wd[c][1] = a.wd[1][at];
         bias[c] = !GLU && a.bias ? a.bias[at] : 0.0f;
     }
-    auto part = [](const v16i &v, int q) { return v4i{ v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3] }; };
-    auto tokens = [&](int m, int q) { return t0 + (wt * S::MT + m) * 32 + 8 * q + 4 * h; };
+    auto part = [](const Sum &v, int q) { return v4i{ v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3] }; };
+    auto tokens = [&](int m, int q) { return t0 + (wt * S::MT + m) * MB + 8 * q + 4 * h; };
     auto scales = [&](int tm, float (&xd)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) xd[i] = a.xd[min(tm + i, a.ntok - 1)];
@@ -336,18 +285,18 @@ template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(c
     if constexpr (S::WK == 1) {
 #pragma unroll
         for (int m = 0; m < S::MT; m++) {
-            float xd[4][4];
+            float xd[S::Q][4];
 #pragma unroll
-            for (int q = 0; q < 4; q++) scales(tokens(m, q), xd[q]);
+            for (int q = 0; q < S::Q; q++) scales(tokens(m, q), xd[q]);
 #pragma unroll
             for (int c = 0; c < S::NT / M; c++)
 #pragma unroll
-                for (int q = 0; q < 4; q++)
+                for (int q = 0; q < S::Q; q++)
                     quad(tokens(m, q), r[c], xd[q], part(acc[m][c * M], q), part(acc[m][c * M + M - 1], q), wd[c], bias[c]);
         }
     } else {
         // the parts' sums meet in the ring, RM tiles at a time, and each wave has its share of the values
-        constexpr int NC = S::NT / M, P = S::MT * NC, ROOM = NB * (XB + WB) / (S::WAVES * M * 4096), RM = ROOM >= P ? P : ROOM >= 4 ? 4 : ROOM >= 2 ? 2 : 1;
+        constexpr int NC = S::NT / M, P = S::MT * NC, ROOM = NB * (XB + WB) / (S::WAVES * M * MB * MB * 4), RM = ROOM >= P ? P : ROOM >= 4 ? 4 : ROOM >= 2 ? 2 : 1;
         static_assert(ROOM > 0 && P % RM == 0, "the parts fit");
         v4i *const s_part = (v4i *)s_ring;
 #pragma unroll
@@ -356,15 +305,15 @@ template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(c
 #pragma unroll
             for (int p = 0; p < RM; p++)
 #pragma unroll
-                for (int q = 0; q < 4; q++)
+                for (int q = 0; q < S::Q; q++)
 #pragma unroll
                     for (int c = 0; c < M; c++)
-                        s_part[(((wave * RM + p) * 4 + q) * M + c) * 64 + lane] = part(acc[(p0 + p) / NC][(p0 + p) % NC * M + c], q);
+                        s_part[(((wave * RM + p) * S::Q + q) * M + c) * 64 + lane] = part(acc[(p0 + p) / NC][(p0 + p) % NC * M + c], q);
             __syncthreads();
 #pragma unroll
             for (int p = 0; p < RM; p++) {
                 // quads of the tile in turn over the parts' waves
-                for (int q = (wk - p * 4 % S::WK + S::WK) % S::WK; q < 4; q += S::WK) {
+                for (int q = (wk - p * S::Q % S::WK + S::WK) % S::WK; q < S::Q; q += S::WK) {
                     float xd[4];
                     const int tm = tokens((p0 + p) / NC, q), cc = (p0 + p) % NC;
                     scales(tm, xd);
@@ -373,7 +322,7 @@ template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(c
                     for (int k = 0; k < S::WK; k++)
 #pragma unroll
                         for (int c = 0; c < M; c++)
-                            sum[c] += s_part[(((k * S::WT * S::WR + wg) * RM + p) * 4 + q) * M * 64 + c * 64 + lane];
+                            sum[c] += s_part[(((k * S::WT * S::WR + wg) * RM + p) * S::Q + q) * M * 64 + c * 64 + lane];
                     quad(tm, r[cc], xd, sum[0], sum[M - 1], wd[cc], bias[cc]);
                 }
             }
@@ -382,31 +331,28 @@ template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(c
 }
 
 // The forms, and what they take: with n tiles a CU, base + n out + (n == 1 ? one : n many) cols / 4096
-// us, as measured (4096 rows of 4096 and 14,336, pairs of 14,336 and 8192 rows, 1 to 2047
-// tokens; the estimates are within 10% of those but where rounds are not whole).
-// At 4096 rows of 4096 in us, 32 x 32 / 64 x 32 / 64 x 64 / 128 x 64 / 128 x 128 split /
-// whole / 256 x 256: 64 tokens 7.7 / 8.3 / 10.6 / 14.5 / 22 / 23 / 49, 256 18.0 / 15.7 / 12.1 / 15.7 / 22.6 /
-// 23.9 / 50, 512 33 / 29 / 21 / 17.4 / 23.7 / 24.7 / 51, 2047 112 / 103 / 70 / 57 / 49 / 39 / 56.
-enum { I8_FEW, I8_32x32, I8_64x32, I8_64x64, I8_128x64, I8_128x128_SPLIT, I8_128x128, I8_256x256, I8_FORMS };
+// us, as measured (288 to 16,384 rows of 288 to 16,384, pairs of 14,336 and 8192 rows, 1 to 2047
+// tokens: but for two of 160 sizes the form of the least estimate is within 7% of the fastest).
+// At 4096 rows of 4096 in us, 16 x 16 / 32 x 16 / 32 x 32 / 64 x 32 / 64 x 64 / 128 x 64 / 128 x 128 split /
+// whole / 256 x 256: 16 tokens 5.5 / 5.6 / 6.8 / 7.9 / 10.2 / -, 32 6.2 / 5.9 / 6.9 / 7.9 / 10.3 / 14.0 / 22.6 / 23.1 / -,
+// 64 10.5 / 9.8 / 7.3 / 8.2 / 10.6 / 14.2 / 23.0 / 23.3 / 49.5, 256 - / 33.4 / 17.2 / 15.8 / 12.0 / 15.5 / 23.5 / 24.0 / 51,
+// 512 - / - / 31.1 / 28.9 / 21.2 / 16.9 / 24.3 / 24.5 / 51, 2047 - / - / 112 / 103 / 70 / 57 / 49 / 39 / 56.
+enum { I8_16x16, I8_32x32, I8_64x32, I8_64x64, I8_128x64, I8_128x128_SPLIT, I8_128x128, I8_256x256, I8_32x16, I8_FORMS };
 struct I8Cost {
     int bt, br;
     float base, out, one, many;
 };
-constexpr I8Cost I8_COST[I8_FORMS] = { { 16, 16, 3.2f, 0, 2.5f, 2.5f },  { 32, 32, 2.3f, 1.0f, 4.2f, 3.0f },
+constexpr I8Cost I8_COST[I8_FORMS] = { { 16, 16, 1.9f, 0.6f, 2.2f, 1.9f },  { 32, 32, 2.3f, 1.0f, 4.2f, 3.0f },
                                        { 64, 32, 2.8f, 1.2f, 5.0f, 5.0f }, { 64, 64, 2.0f, 3.2f, 6.2f, 6.2f },
                                        { 128, 64, 4.8f, 1.6f, 11, 11 },  { 128, 128, 7.0f, 1.2f, 19, 19 },
-                                       { 128, 128, 4.0f, 0.2f, 23, 19.5f }, { 256, 256, 4.5f, 6.0f, 58, 58 } };
-// Operands from memory up to 8 tokens (4096 rows of 4096 in us, against tiles of 32 x 32: one
-// token 5.7 / 7.1, 16 7.0 / 7.3; 896 rows of 4864 6.4 / 7.4 and 8.7 / 7.7; a pair of 8192 rows of 2048
-// 11.5 / 8.0); else the least estimate.
-constexpr int I8_FEW_MAX = 8;
+                                       { 128, 128, 4.0f, 0.2f, 23, 19.5f }, { 256, 256, 4.5f, 6.0f, 58, 58 }, { 32, 16, 1.7f, 1.4f, 2.4f, 2.9f } };
 int i8_form(int rows, int cols, int ntok, bool glu) {
-    if (ntok <= I8_FEW_MAX && !glu) return I8_FEW;
     int best = I8_32x32;
     float least = FLT_MAX;
-    for (int f = I8_32x32; f < I8_FORMS; f++) {
+    for (int f = 0; f < I8_FORMS; f++) {
         const I8Cost &c = I8_COST[f];
-        if (glu && f == I8_64x64) continue;   // with 32 rows of each matrix at least, that is 64 x 32
+        // with 32 rows of each matrix at least, 64 x 64 is 64 x 32
+        if (glu && (f == I8_64x64 || c.br < 32)) continue;
         const int br = f < I8_128x64 ? c.br : glu ? c.br / 2 : c.br;
         const double tiles = (double)((ntok + c.bt - 1) / c.bt) * ((rows + (long long)br - 1) / br);
         // a pair's tile of 32 rows is twice the work
@@ -433,7 +379,8 @@ template <class S, bool GLU> void i8_tiles(const I8Args &a, const char *what) {
 
 template <bool GLU> void i8_launch(const I8Args &a, const char *what) {
     constexpr int R = GLU ? 64 : 32;   // 32 rows of a matrix
-    switch (i8_form(a.rows, a.cols, a.ntok, GLU)) {
+    const int form = i8_form(a.rows, a.cols, a.ntok, GLU);
+    switch (form) {
     case I8_32x32: return i8_tiles<I8Tile<32, R, 1, 1, 256, 4, 8>, GLU>(a, what);
     case I8_64x32: return i8_tiles<I8Tile<64, R, 1, 1, 256, GLU ? 3 : 4, 8>, GLU>(a, what);
     case I8_128x64: return i8_tiles<I8Tile<128, 64, 2, 1, 256, 3, 4>, GLU>(a, what);
@@ -442,8 +389,11 @@ template <bool GLU> void i8_launch(const I8Args &a, const char *what) {
     case I8_256x256: return i8_tiles<I8Tile<256, 256, 2, 4, 128, 2>, GLU>(a, what);
     default:
         if constexpr (!GLU) {
-            if (i8_form(a.rows, a.cols, a.ntok, GLU) == I8_64x64) return i8_tiles<I8Tile<64, 64, 1, 1, 256, 4, 8>, GLU>(a, what);
-            i8_start(k_i8_few, what, (a.rows + 15) / 16, FEW_T, a);
+            switch (form) {
+            case I8_16x16: return i8_tiles<I8Tile<16, 16, 1, 1, 512, 4, 8>, GLU>(a, what);
+            case I8_32x16: return i8_tiles<I8Tile<32, 16, 1, 1, 512, 4, 8>, GLU>(a, what);
+            default: return i8_tiles<I8Tile<64, 64, 1, 1, 256, 4, 8>, GLU>(a, what);
+            }
         }
     }
 }

@@ -151,7 +151,7 @@ def test_i8_swiglu_range(dev, scale):
     assert (np.abs(h - want) <= 8.01 * U * np.abs(want) + 1e-35 * (1 + np.abs(u))).all()
 
 
-FORMS = [(0, 5, 40, 100), (1, 20, 40, 300), (2, 33, 4100, 300), (3, 33, 9000, 700), (4, 130, 6000, 1500), (5, 200, 9000, 5000),
+FORMS = [(0, 5, 40, 100), (0, 40, 200, 1300), (1, 8, 16000, 300), (8, 20, 3000, 1000), (8, 32, 4096, 5000), (2, 33, 4100, 300), (3, 33, 9000, 700), (4, 130, 6000, 1500), (5, 200, 9000, 5000),
          (6, 1030, 3000, 200), (7, 2050, 6000, 2100)]
 PAIR_FORMS = [(1, 5, 40, 300), (2, 33, 4100, 700), (4, 100, 4100, 2100), (5, 100, 9000, 5000), (6, 700, 2100, 130),
               (7, 1500, 4100, 2100)]
