@@ -53,7 +53,7 @@ __device__ __forceinline__ float i8_silu_mul(float g, float u) {
     return kr_fmul(kr_fmul(g, s), u);
 }
 
-// Tiles of BT tokens and BR rows (GLU: 32 rows of each matrix in turn), WT x WR
+// Tiles of BT tokens and BR rows (GLU: MB rows of each matrix in turn), WT x WR
 // waves with an even part each, or WK times as many, each with a part of the
 // reduction. That goes in stages of BK values, which pass from memory to LDS
 // without registers, NB stages in a ring: one barrier a stage, and a stage's loads
@@ -72,7 +72,8 @@ __device__ __forceinline__ float i8_silu_mul(float g, float u) {
 // 12.5 with operands from memory). Few tokens: HBM, where all compute units have a
 // tile, for which tiles have 16 rows: one token, 4096 rows of 14,336 12.1 us (4.9 TB/s), 16
 // 13.5 (19.8 in tiles of 32 rows, on half of the units; 20.9 with operands from memory,
-// of which a unit reads about 16 bytes a clock).
+// of which a unit reads about 16 bytes a clock); of a pair of 14,336 rows of 4096 25.7 and 26.4 (28.4 in
+// tiles of 32 rows of each).
 typedef int v16i __attribute__((ext_vector_type(16)));
 
 // 16 bytes a lane from base + off to LDS at `to` (one address a wave) + 16 lane.
@@ -88,9 +89,9 @@ template <int N> __device__ __forceinline__ void i8_stage_wait() {
 }
 template <int KC> __device__ __forceinline__ int i8_chunk(int row, int c) { return c ^ (KC == 8 ? (row >> 1) & 7 : row & 15); }
 
-template <int BT_, int BR_, int WT_, int WR_, int BK_, int NB_, int WK_ = 1> struct I8Tile {
+template <int BT_, int BR_, int WT_, int WR_, int BK_, int NB_, int WK_ = 1, int MB_ = 32> struct I8Tile {
     static constexpr int BT = BT_, BR = BR_, WT = WT_, WR = WR_, BK = BK_, NB = NB_, WK = WK_;
-    static constexpr int MB = BR / WR < 32 ? 16 : 32;              // tokens and rows of a product, of G 16-byte chunks each
+    static constexpr int MB = MB_;                                 // tokens and rows of a product, of G 16-byte chunks each
     static constexpr int G = 64 / MB, Q = MB * MB / 256;           // a product's values of a lane: Q times four
     static constexpr int WAVES = WT * WR * WK, T = 64 * WAVES, KC = BK / 16, MT = BT / WT / MB, NT = BR / WR / MB;
     static constexpr int PER = 64 / KC;                            // rows a wave's load covers
@@ -113,7 +114,6 @@ template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(c
     __shared__ alignas(16) int8_t s_ring[NB * (XB + WB)];
     int8_t *const s_x = s_ring, *const s_w = s_ring + NB * XB;
     constexpr int MB = S::MB;
-    static_assert(MB == 32 || !GLU, "32 rows of each matrix");
     const int lane = threadIdx.x & 63, h = lane / MB, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     // Consecutive workgroups go to the dies in turn: each die has consecutive tiles,
     // 8 token tiles of a row tile after one another, which share what its L2 holds
@@ -131,9 +131,9 @@ template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(c
         const int row = (j * S::WAVES + wave) * S::PER + sub;
         xo[j] = (unsigned)min(row, a.ntok - 1 - t0) * (unsigned)a.ldx + i8_chunk<KC>(row, slot) * 16;
     }
-    auto second = [&](int j) { return GLU && ((j * S::WAVES + wave) * S::PER >> 5 & 1); };
+    auto second = [&](int j) { return GLU && ((j * S::WAVES + wave) * S::PER / MB & 1); };
     auto ldw = [&](int j) { return (unsigned)(second(j) ? a.ldw[1] : a.ldw[0]); };
-    auto mrow = [&](int row) { return min(GLU ? ((row >> 6) << 5) + (row & 31) : row, a.rows - 1 - r0); };
+    auto mrow = [&](int row) { return min(GLU ? row / (2 * MB) * MB + row % MB : row, a.rows - 1 - r0); };
 #pragma unroll
     for (int j = 0; j < S::LW; j++) {
         const int row = (j * S::WAVES + wave) * S::PER + sub;
@@ -331,8 +331,8 @@ template <class S, bool GLU> __global__ void __launch_bounds__(S::T) k_i8_tile(c
 }
 
 // The forms, and what they take: with n tiles a CU, base + n out + (n == 1 ? one : n many) cols / 4096
-// us, as measured (288 to 16,384 rows of 288 to 16,384, pairs of 14,336 and 8192 rows, 1 to 2047
-// tokens: but for two of 160 sizes the form of the least estimate is within 7% of the fastest).
+// us, as measured (288 to 16,384 rows of 288 to 16,384, 1 to 2047 tokens, and pairs of 300 to 20,000 rows of 300 to
+// 8192: but for 2 of 160 sizes and 4 of 135 the form of the least estimate is within 7% of the fastest).
 // At 4096 rows of 4096 in us, 16 x 16 / 32 x 16 / 32 x 32 / 64 x 32 / 64 x 64 / 128 x 64 / 128 x 128 split /
 // whole / 256 x 256: 16 tokens 5.5 / 5.6 / 6.8 / 7.9 / 10.2 / -, 32 6.2 / 5.9 / 6.9 / 7.9 / 10.3 / 14.0 / 22.6 / 23.1 / -,
 // 64 10.5 / 9.8 / 7.3 / 8.2 / 10.6 / 14.2 / 23.0 / 23.3 / 49.5, 256 - / 33.4 / 17.2 / 15.8 / 12.0 / 15.5 / 23.5 / 24.0 / 51,
@@ -342,22 +342,23 @@ struct I8Cost {
     int bt, br;
     float base, out, one, many;
 };
-constexpr I8Cost I8_COST[I8_FORMS] = { { 16, 16, 1.9f, 0.6f, 2.2f, 1.9f },  { 32, 32, 2.3f, 1.0f, 4.2f, 3.0f },
-                                       { 64, 32, 2.8f, 1.2f, 5.0f, 5.0f }, { 64, 64, 2.0f, 3.2f, 6.2f, 6.2f },
-                                       { 128, 64, 4.8f, 1.6f, 11, 11 },  { 128, 128, 7.0f, 1.2f, 19, 19 },
-                                       { 128, 128, 4.0f, 0.2f, 23, 19.5f }, { 256, 256, 4.5f, 6.0f, 58, 58 }, { 32, 16, 1.7f, 1.4f, 2.4f, 2.9f } };
+constexpr I8Cost I8_COST[2][I8_FORMS] = {
+    { { 16, 16, 1.9f, 0.6f, 2.2f, 1.9f }, { 32, 32, 2.3f, 1.0f, 4.2f, 3.0f }, { 64, 32, 2.8f, 1.2f, 5.0f, 5.0f },
+      { 64, 64, 2.0f, 3.2f, 6.2f, 6.2f }, { 128, 64, 4.8f, 1.6f, 11, 11 }, { 128, 128, 7.0f, 1.2f, 19, 19 },
+      { 128, 128, 4.0f, 0.2f, 23, 19.5f }, { 256, 256, 4.5f, 6.0f, 58, 58 }, { 32, 16, 1.7f, 1.4f, 2.4f, 2.9f } },
+    // a pair: br rows of each matrix; no 64 x 64 but 64 x 32, and no 32 x 16
+    { { 16, 16, 3.0f, 0.8f, 2.1f, 2.5f }, { 32, 32, 3.1f, 1.5f, 5.0f, 7.8f }, { 64, 32, 2.4f, 3.1f, 6.4f, 9.6f }, {},
+      { 128, 32, 2.0f, 3.7f, 10.4f, 12.8f }, { 128, 64, 0.6f, 5.4f, 21.1f, 21.1f }, { 128, 64, 3.5f, 0.5f, 25.5f, 23.9f },
+      { 256, 128, 5.0f, 5.6f, 47.9f, 64.5f }, {} }
+};
 int i8_form(int rows, int cols, int ntok, bool glu) {
     int best = I8_32x32;
     float least = FLT_MAX;
     for (int f = 0; f < I8_FORMS; f++) {
-        const I8Cost &c = I8_COST[f];
-        // with 32 rows of each matrix at least, 64 x 64 is 64 x 32
-        if (glu && (f == I8_64x64 || c.br < 32)) continue;
-        const int br = f < I8_128x64 ? c.br : glu ? c.br / 2 : c.br;
-        const double tiles = (double)((ntok + c.bt - 1) / c.bt) * ((rows + (long long)br - 1) / br);
-        // a pair's tile of 32 rows is twice the work
-        const float n = (float)ceil(tiles / 256), k = cols / 4096.0f * (glu && f < I8_128x64 ? 1.5f : 1.0f);
-        const float us = c.base + n * c.out + (n == 1 ? c.one : n * c.many) * k;
+        const I8Cost &c = I8_COST[glu][f];
+        if (c.bt == 0) continue;
+        const double tiles = (double)((ntok + c.bt - 1) / c.bt) * ((rows + (long long)c.br - 1) / c.br);
+        const float n = (float)ceil(tiles / 256), us = c.base + n * c.out + (n == 1 ? c.one : n * c.many) * (cols / 4096.0f);
         if (us < least) least = us, best = f;
     }
     return best;
@@ -381,6 +382,8 @@ template <bool GLU> void i8_launch(const I8Args &a, const char *what) {
     constexpr int R = GLU ? 64 : 32;   // 32 rows of a matrix
     const int form = i8_form(a.rows, a.cols, a.ntok, GLU);
     switch (form) {
+    // a pair's ring of three has two workgroups a CU: 8 tokens of 14,336 rows of 4096 25.7 us, of four 30.4
+    case I8_16x16: return i8_tiles<I8Tile<16, GLU ? 32 : 16, 1, 1, 512, GLU ? 3 : 4, 8, 16>, GLU>(a, what);
     case I8_32x32: return i8_tiles<I8Tile<32, R, 1, 1, 256, 4, 8>, GLU>(a, what);
     case I8_64x32: return i8_tiles<I8Tile<64, R, 1, 1, 256, GLU ? 3 : 4, 8>, GLU>(a, what);
     case I8_128x64: return i8_tiles<I8Tile<128, 64, 2, 1, 256, 3, 4>, GLU>(a, what);
@@ -389,11 +392,8 @@ template <bool GLU> void i8_launch(const I8Args &a, const char *what) {
     case I8_256x256: return i8_tiles<I8Tile<256, 256, 2, 4, 128, 2>, GLU>(a, what);
     default:
         if constexpr (!GLU) {
-            switch (form) {
-            case I8_16x16: return i8_tiles<I8Tile<16, 16, 1, 1, 512, 4, 8>, GLU>(a, what);
-            case I8_32x16: return i8_tiles<I8Tile<32, 16, 1, 1, 512, 4, 8>, GLU>(a, what);
-            default: return i8_tiles<I8Tile<64, 64, 1, 1, 256, 4, 8>, GLU>(a, what);
-            }
+            if (form == I8_32x16) return i8_tiles<I8Tile<32, 16, 1, 1, 512, 4, 8, 16>, GLU>(a, what);
+            return i8_tiles<I8Tile<64, 64, 1, 1, 256, 4, 8>, GLU>(a, what);
         }
     }
 }

@@ -153,7 +153,7 @@ def test_i8_swiglu_range(dev, scale):
 
 FORMS = [(0, 5, 40, 100), (0, 40, 200, 1300), (1, 8, 16000, 300), (8, 20, 3000, 1000), (8, 32, 4096, 5000), (2, 33, 4100, 300), (3, 33, 9000, 700), (4, 130, 6000, 1500), (5, 200, 9000, 5000),
          (6, 1030, 3000, 200), (7, 2050, 6000, 2100)]
-PAIR_FORMS = [(1, 5, 40, 300), (2, 33, 4100, 700), (4, 100, 4100, 2100), (5, 100, 9000, 5000), (6, 700, 2100, 130),
+PAIR_FORMS = [(0, 5, 40, 300), (0, 16, 3000, 130), (6, 16, 9000, 130), (0, 50, 300, 1100), (1, 20, 5000, 600), (2, 33, 4100, 700), (4, 100, 4100, 2100), (5, 100, 9000, 5000), (6, 700, 2100, 130),
               (7, 1500, 4100, 2100)]
 
 
