@@ -621,10 +621,10 @@ __global__ void __launch_bounds__(64 * SH_WC, sh_waves(KT, CL)) k_shared_rows(co
 // A head of a sequence a workgroup: its own rows' parts, then the shared ones'
 // (2^dl lanes hold its dims four at a time, the workgroup's other factor the parts
 // side by side). By latency, so the parts are asked for before their weights are known: 512
-// heads of 17 parts of 128 dims 6.3 us (7.5 one after the other), 2048 of 26 12.2 (13.6).
-constexpr int SJ_T = 256, SJ_N = 4;   // threads; parts a thread asks for at once
-__global__ void __launch_bounds__(SJ_T) k_shared_join(const PgView p, const ShArgs a, int dl) {
-    __shared__ float4v s_o[SJ_T];
+// heads of 17 parts of 128 dims 5.8 us (7.5 one after the other).
+constexpr int SJ_N = 4;   // parts a thread asks for at once
+template <int T> __global__ void __launch_bounds__(T) k_shared_join(const PgView p, const ShArgs a, int dl) {
+    __shared__ float4v s_o[T];
     const int s = blockIdx.y, x = blockIdx.x, tid = threadIdx.x, group = a.nh / p.n_kv, kvh = x / group, col = x % group;
     int bad = 0;   // reported by the other launches
     PaSpan sp;
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(SJ_T) k_shared_join(const PgView p, const ShAr
     };
     const auto at = [&](int i) { return i < r.n ? part0 + (size_t)i * group * p.hd : part1 + (size_t)(i - r.n) * SH_CT * p.hd; };
     // the first parts are on their way while the weights are found
-    const int lane = tid & 63, first = tid >> dl, lanes = SJ_T >> dl, q = tid & ((1 << dl) - 1), d = 4 * q < p.hd ? 4 * q : 0;
+    const int lane = tid & 63, first = tid >> dl, lanes = T >> dl, q = tid & ((1 << dl) - 1), d = 4 * q < p.hd ? 4 * q : 0;
     float4v v[SJ_N];
     const auto fetch = [&](int i) {
 #pragma unroll
@@ -814,6 +814,12 @@ extern "C" void krh_paged_attention_shared(float *o, const krh_pages *kv, const 
     const ShRows f = kv->kv_type == ML_F32 ? sh_rows<PG_F32>(hd) : kv->kv_type == ML_F16 ? sh_rows<PG_F16>(hd) : sh_rows<PG_Q8>(hd);
     hipLaunchKernelGGL(f, dim3((own + r.sshares) * kv->n_kv_heads), dim3(64 * SH_WC), 0, kr_stream(), p, a, own);
     kr_check_launch("paged_attention_shared");
-    hipLaunchKernelGGL(k_shared_join, dim3(n_heads, n_seq), dim3(SJ_T), 0, kr_stream(), p, a, pg_log2(hd / 4));
+    // Threads a head: with few heads the parts are asked for side by side, with many each wave's search for its parts
+    // is what takes the time (a call of 512 heads of 128 dims by 256 / 128 / 64 20.1 / 20.5 / 21.1 us, 1024 of 64 36.2 / 35.2 /
+    // 35.8, 1536 of 64 30.0 / 28.1 / 27.3, 2048 of 64 46.2 / 43.0 / 43.0)
+    const long long heads = (long long)n_heads * n_seq;
+    const int threads = heads <= 512 ? 256 : heads <= 1024 ? 128 : 64;
+    hipLaunchKernelGGL(threads == 256 ? k_shared_join<256> : threads == 128 ? k_shared_join<128> : k_shared_join<64>,
+                       dim3(n_heads, n_seq), dim3(threads), 0, kr_stream(), p, a, pg_log2(hd / 4));
     kr_check_launch("paged_attention_shared");
 }

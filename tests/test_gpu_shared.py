@@ -216,6 +216,14 @@ def test_many_sequences(dev, kv_type, hd):
     check(dev, kv_type, 2, 1, hd, 16, [(70, 64), (70, 160)], own_rows(rng, 170, 20), alone=(30, 0))
 
 
+@pytest.mark.parametrize("hd", [40, 128, 256])
+@pytest.mark.parametrize("n", [31, 60, 70])
+def test_heads_of_a_call(dev, n, hd):
+    """480 heads, 944 and 1104: joined by fewer threads a head the more there are"""
+    rng = np.random.default_rng(hd + n)
+    check(dev, K.ML_F16, 16, 2, hd, 16, [(n - 3, 192)], own_rows(rng, n - 1, 50), alone=(1, 1))
+
+
 @pytest.mark.parametrize("kv_type", TYPES)
 def test_long(dev, kv_type):
     """long shared rows, cut into many parts; a batch whose longest is far under max_len"""
