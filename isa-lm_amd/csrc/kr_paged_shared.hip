@@ -20,10 +20,10 @@
 // workgroup and KV head, by the lengths that the device has; a share's sums of a
 // column tile are a part.
 //
-// What bounds it (8B shape, halves): 64 sequences behind 32,000 rows 102 to 117 us by
-// the card, of which the join's reads of the parts 12; the matrix cores and the
+// What bounds it (8B shape, halves): 64 sequences behind 32,000 rows 99 to 113 us by
+// the card, of which the join's reads of the parts 9; the matrix cores and the
 // softmax's instructions beside each other, at the 1.6 GHz that power leaves (67 GFLOP
-// with both halves, 54 us of a large product's rate). 16 behind 2048 19.6 us: four tiles
+// with both halves, 54 us of a large product's rate). 16 behind 2048 19.7 us: four tiles
 // a workgroup, 1.8 us each on their way, and the join's latency, 5.8. Each sequence
 // reading its own (krh_paged_attention) takes 1069 us and 26.8 there.
 #include <cfloat>
