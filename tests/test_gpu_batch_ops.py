@@ -102,6 +102,28 @@ def test_i8_largest_sums(dev, T, rows):
     assert (yb.get(np.float32, T * rows) == np.float32(cols * 2.0 ** 14)).all()
 
 
+@pytest.mark.parametrize("T", [2, 20, 70, 300])
+def test_i8_offsets_past_32_bits(dev, T):
+    """a matrix of more than 2^32 bytes, into rows more than 2^32 bytes apart; what the other rows hold does not matter"""
+    rng = np.random.default_rng(T)
+    rows, cols, ld, some = 530000, 8100, 8192, 300
+    ldy = max(rows, 2 ** 31 // T)
+    w, d, y = K.DevBuf(rows * ld), K.DevBuf(4 * rows), K.DevBuf(4 * (ldy * (T - 1) + rows))
+    dev.bufs += [w, d, y]
+    q, s = rng.integers(-128, 128, (some, ld)).astype(np.int8), f32(0.01 * rng.random(some))
+    K.check(K.hip.krh_copy_h2d(w.ptr + (rows - some) * ld, q.ctypes.data, q.nbytes))
+    K.check(K.hip.krh_copy_h2d(d.ptr + 4 * (rows - some), s.ctypes.data, s.nbytes))
+    x = Mat(dev, rng, T, cols, 32)
+    m = K.KrhMat8(w.ptr, d.ptr, ld, rows, cols)
+    K.hip.krh_matmul_i8(y.ptr, ldy, C.byref(m), x.qb.ptr, x.ld, x.sb.ptr, None, T, 0)
+    ok()
+    want = ((x.v.astype(np.float64) @ q[:, :cols].astype(np.float64).T).astype(np.float32) * x.s[:, None]) * s[None, :]
+    for t in range(T):
+        got = np.empty(some, np.float32)
+        K.check(K.hip.krh_copy_d2h(got.ctypes.data, y.ptr + 4 * (t * ldy + rows - some), got.nbytes))
+        assert np.array_equal(bits(got), bits(want[t])), t
+
+
 @pytest.mark.parametrize("T", TOKENS)
 @pytest.mark.parametrize("rows,cols", [(1, 3), (16, 64), (37, 130), (130, 1000), (300, 272)])
 def test_i8_swiglu(dev, T, rows, cols):

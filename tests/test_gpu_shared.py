@@ -233,6 +233,41 @@ def test_long(dev, kv_type):
     check(dev, kv_type, 4, 1, 64, 64, [(3, 640), (32, 2560)], own_rows(rng, 35, 900))
 
 
+def test_offsets_past_32_bits(dev):
+    """shared and own rows in pages beyond 2^31 values"""
+    n, nkv, hd, page, S, shared = 270000, 2, 256, 16, 40, 96
+    k, v = (K.DevBuf(4 * n * nkv * hd * page) for _ in range(2))
+    dev.bufs += [k, v]
+    kv = K.KrhPages(k.ptr, v.ptr, None, None, K.ML_F32, n, page, nkv, hd)
+    ref, rng = C.byref(kv), np.random.default_rng(12)
+    table = np.full((S, 7), -1, np.int32)
+    table[:, :6] = [n - 1, 7, n - 2, n // 2 + 1, n - 70, 3]
+    table[:, 6] = n - 10 - np.arange(S)
+    lens = i32(shared + rng.integers(0, 16, S))
+    seq = i32([0] * shared + [i for i in range(S) for _ in range(lens[i] - shared)])
+    row = i32(list(range(shared)) + [r for i in range(S) for r in range(shared, lens[i])])
+    T, nh = len(seq), 4
+    kr, vr = (f32(rng.standard_normal((T, nkv * hd))) for _ in range(2))
+    q = f32(rng.standard_normal((S, nh, hd)))
+    tb, ob = dev.put(table), dev.zeros(q.nbytes)
+    K.hip.krh_paged_qkv(None, 0, ref, tb.ptr, 7, S, None, 0, dev.put(kr).ptr, nkv * hd, dev.put(vr).ptr, nkv * hd, T, 0,
+                        dev.put(seq).ptr, dev.put(row).ptr, None, None, None, 0.0, None, None, 0)
+    most = 128
+    while K.hip.krh_paged_attention_shared_form(ref, S, nh, most, 1, most - 1, 0) != 1:
+        most *= 2
+    ws = dev.zeros(K.hip.krh_paged_attention_shared_ws(ref, S, nh, most, 1, most - 1))
+    K.hip.krh_paged_attention_shared(ob.ptr, ref, tb.ptr, 7, dev.put(lens).ptr, S, dev.put(i32([0, S])).ptr,
+                                     dev.put(i32([shared])).ptr, 1, most - 1, dev.put(q).ptr, nh, most, 0, 0.0625, 0.0, ws.ptr)
+    ok()
+    o = ob.get(np.float32, q.size).reshape(q.shape)
+    k64, v64 = (x.reshape(T, nkv, hd).astype(np.float64) for x in (kr, vr))
+    for i in range(S):
+        at = np.concatenate([np.arange(shared), np.flatnonzero((seq == i) & (row >= shared))])
+        for h in range(nh):
+            w, _, bound, _ = attention(q[i, h].astype(np.float64), k64[at, h // 2], v64[at, h // 2], 0.0625, 0, 0)
+            assert (np.abs(o[i, h] - w) <= bound).all(), (i, h)
+
+
 def test_64_groups(dev):
     rng = np.random.default_rng(6)
     check(dev, K.ML_F16, 4, 2, 64, 16, [(3, 16 * (g % 5 + 1)) for g in range(64)], own_rows(rng, 200, 30), alone=(0, 8))
