@@ -407,8 +407,8 @@ size_t krh_paged_attention_ws(const krh_pages *kv, int n_seq, int n_heads, int m
 void krh_paged_attention(float *o, const krh_pages *kv, const int *table, int table_ld, const int *len, int n_seq,
                          const float *q, int n_heads, int max_len, int window, float scale, float softcap,
                          float *mass, size_t mass_ld, void *ws);
-/* Bytes of workspace that krh_paged_attention_shared takes for these sizes and
- * any window (0 for sizes that it refuses) */
+/* Bytes of workspace that krh_paged_attention_shared takes for these sizes, any that
+ * are not larger, and any window (0 for sizes that it refuses) */
 size_t krh_paged_attention_shared_ws(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_groups,
                                      int max_shared);
 /* krh_paged_attention of sequences that begin alike (a common prompt's pages),

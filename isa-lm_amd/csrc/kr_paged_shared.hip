@@ -744,10 +744,8 @@ bool sh_pays(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_share
     const double tiles = ceil(cts * ceil(rows / SH_R) * kv->n_kv_heads / (SH_CUS * sh_waves(kv->kv_type, kv->head_dim) * 3 / 4));
     return n_seq > n_groups && 11.5 + n_seq * rows * row / rate[t] > 13.0 + 0.1 * n_seq + tiles * tile[t][c];
 }
-// a workspace is sized without a window, so what it takes has to hold for that too
 bool sh_shared(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_shared, int window) {
-    return n_groups > 0 && max_shared > 0 && sh_pays(kv, n_seq, nh, n_groups, max_shared, 0) &&
-           (window == 0 || sh_pays(kv, n_seq, nh, n_groups, max_shared, window));
+    return n_groups > 0 && max_shared > 0 && sh_pays(kv, n_seq, nh, n_groups, max_shared, window);
 }
 
 bool sh_args_ok(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_groups, int max_shared) {
@@ -776,7 +774,8 @@ extern "C" size_t krh_paged_attention_shared_ws(const krh_pages *kv, int n_seq, 
                                                 int max_shared) {
     if (!sh_args_ok(kv, n_seq, n_heads, max_len, n_groups, max_shared)) return 0;
     const size_t base = krh_paged_attention_ws(kv, n_seq, n_heads, max_len, 0);
-    if (!sh_shared(kv, n_seq, n_heads, n_groups, max_shared, 0)) return base;
+    if (n_groups == 0 || max_shared == 0) return base;
+    // for both ways, whichever pays: fewer sequences may pay where more do not, and a window where none does
     const ShSizes r = sh_sizes(kv, n_seq, n_heads, n_groups, max_shared);
     const size_t b = sizeof(float) * (r.part + r.pml + r.spart + r.spml + 4);
     return b > base ? b : base;

@@ -114,6 +114,22 @@ def test_shared_attention_workspaces():
         assert ws(*bad) == 0
 
 
+@pytest.mark.parametrize("kw,nh", [(dict(), 4), (dict(head_dim=128, n_kv_heads=8), 32), (dict(kv_type=K.ML_F32, head_dim=256), 4),
+                                   (dict(kv_type=K.ML_Q8_0, kd=PTR, vd=PTR, n_kv_heads=1), 7)])
+def test_shared_attention_workspaces_grow(kw, nh):
+    """a workspace for larger sizes serves smaller ones, whichever of them pass over shared rows once"""
+    kv = C.byref(pages(**kw))
+    sizes = [(n, most, g, shared) for n in (1, 2, 7, 16, 31, 32, 33, 64, 65, 200) for most in (64, 4096, 40000) for g in (1, 3, 64)
+             for shared in (1, 48, 64, 1000, 4000, 39000) if shared <= most]
+    ws = {s: K.hip.krh_paged_attention_shared_ws(kv, s[0], nh, *s[1:]) for s in sizes}
+    assert len({K.hip.krh_paged_attention_shared_form(kv, s[0], nh, *s[1:], 0) for s in sizes}) == 2
+    for a in sizes:
+        assert ws[a] > 0
+        for b in sizes:
+            if all(x <= y for x, y in zip(a, b)):
+                assert ws[a] <= ws[b], (a, b)
+
+
 def test_forms():
     """which tiles or passes a call takes, and that sizes without one have none"""
     i8 = K.hip.krh_matmul_i8_form
