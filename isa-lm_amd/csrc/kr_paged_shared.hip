@@ -728,21 +728,22 @@ ShSizes sh_sizes(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_s
 int sh_least(const krh_pages *kv) { return kv->kv_type == ML_F32 || kv->head_dim > 128 ? 1 : 2; }
 
 // Whether the shared rows are better passed over once, by estimated times in us. Each
-// sequence by itself (krh_paged_attention): 11.5, and all sequences' rows at the rate at which
-// dies read what others read too (TB/s: halves 14, floats 11, 8 bits 7). Once for
-// all: 13, 0.1 a sequence, and a workgroup's tiles, `tile` each. Measured, each / once,
-// sequences of up to 200 rows behind 256 / 1024 / 4096 / 16,384: 8B shape, halves, 8 13.0 / 15.2, 15.7 /
-// 16.1, 23.6 / 22.5, 49.9 / 32.5, 64 17.1 / 23.8, 37.8 / 30.9, 93 / 38.6, 307 / 67; 1B shape, 8 bits, 16 14.2 / 14.4,
-// 15.5 / 15.3, 22.9 / 21.5, 49.6 / 33.7; floats of 256 dims, 32 23.3 / 37.2, 43.6 / 50.7, 121 / 85.5, 408 / 248.
+// sequence by itself (krh_paged_attention): 11.5, 0.04 a sequence, and all sequences' rows at the rate at which
+// dies read what others read too (TB/s: halves 15, floats 11, 8 bits 6.3). Once for
+// all: 12.1, 0.08 a sequence, and a workgroup's tiles, `tile` each. Measured, each / once,
+// sequences of 150 rows on average behind 256 / 1024 / 4096 / 8192: 8B shape, halves, 8 12.2 / 14.0, 15.1 /
+// 15.1, 23.3 / 21.8, 31.8 / 24.1, 64 15.0 / 18.2, 37.4 / 22.6, 90.5 / 35.0, 161 / 43.3; 1B shape, 8 bits, 16 12.5 / 13.5,
+// 15.2 / 14.4, 22.1 / 21.7, 31.5 / 23.2; floats of 256 dims, 32 22.5 / 33.5, 41.8 / 47.5, 114 / 86.7, 209 / 140. Of 216 such
+// sizes eight take the slower way by more than 5%, the worst by 18.
 bool sh_pays(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_shared, int window) {
-    static const float rate[3] = { 11e6f, 14e6f, 7e6f };                                     // bytes a us: F32, F16, Q8
-    static const float tile[3][3] = { { 1.8f, 4.2f, 20 }, { 1.4f, 1.8f, 6 }, { 1.6f, 2.3f, 8 } };
+    static const float rate[3] = { 11e6f, 15e6f, 6.3e6f };                                   // bytes a us: F32, F16, Q8
+    static const float tile[3][3] = { { 2.9f, 4.2f, 20 }, { 1.6f, 1.75f, 6 }, { 1.6f, 3.5f, 8 } };
     const int t = kv->kv_type == ML_F32 ? 0 : kv->kv_type == ML_F16 ? 1 : 2, c = kv->head_dim <= 64 ? 0 : kv->head_dim <= 128 ? 1 : 2;
     const double rows = window > 0 && window < max_shared ? window : max_shared;
     const double row = (double)kv->n_kv_heads * kv->head_dim * (t == 0 ? 8 : t == 1 ? 4 : 2) + (t == 2 ? 8 * kv->n_kv_heads : 0);
     const double cts = ceil((double)n_seq * (nh / kv->n_kv_heads) / SH_CT);
     const double tiles = ceil(cts * ceil(rows / SH_R) * kv->n_kv_heads / (SH_CUS * sh_waves(kv->kv_type, kv->head_dim) * 3 / 4));
-    return n_seq > n_groups && 11.5 + n_seq * rows * row / rate[t] > 13.0 + 0.1 * n_seq + tiles * tile[t][c];
+    return n_seq > n_groups && 11.5 + n_seq * (0.04 + rows * row / rate[t]) > 12.1 + 0.08 * n_seq + tiles * tile[t][c];
 }
 bool sh_shared(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_shared, int window) {
     return n_groups > 0 && max_shared > 0 && sh_pays(kv, n_seq, nh, n_groups, max_shared, window);

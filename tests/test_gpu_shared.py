@@ -221,7 +221,7 @@ def test_many_sequences(dev, kv_type, hd):
 def test_heads_of_a_call(dev, n, hd):
     """480 heads, 944 and 1104: joined by fewer threads a head the more there are"""
     rng = np.random.default_rng(hd + n)
-    check(dev, K.ML_F16, 16, 2, hd, 16, [(n - 3, 192)], own_rows(rng, n - 1, 50), alone=(1, 1))
+    check(dev, K.ML_F16, 16, 4, hd, 16, [(n - 3, 192)], own_rows(rng, n - 1, 50), alone=(1, 1))
 
 
 @pytest.mark.parametrize("kv_type", TYPES)
