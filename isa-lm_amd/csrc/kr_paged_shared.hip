@@ -110,12 +110,13 @@ __device__ __forceinline__ float sh_other(float v) {   // the same column's valu
     return __uint_as_float(threadIdx.x & 32 ? s[0] : s[1]);
 }
 
-template <int KT, int CL> struct ShLds {
+template <int KT, int CL, bool WIN> struct ShLds {
     static constexpr int EB = KT == PG_F32 ? 4 : 2;
     alignas(16) char k[2][SH_R * CL * EB];
     alignas(16) char v[2][SH_R * CL * EB];
     alignas(16) float kd[2][KT == PG_Q8 ? SH_R : 4], vd[2][KT == PG_Q8 ? SH_R : 4];
-    int range[2];
+    std::conditional_t<WIN, unsigned long long, int> range[2];
+    int2 col[WIN ? SH_CT : 1];   // the rows that each column attends
 };
 
 // where 16 bytes of a K row lie (F32: of a V row too): 16 rows of one chunk in all banks
@@ -127,7 +128,10 @@ __device__ __forceinline__ int sh_vt(int dim, int chunk) { return dim * 64 + ((c
 
 constexpr int sh_waves(int kt, int cl) { return cl > 128 || (kt == PG_F32 && cl > 64) ? 1 : 2; }   // a SIMD
 
-template <int KT, int CL> struct ShWork {
+// WIN: there is a window, and rows that no column attends may lie between those that some do. A kernel of its own has
+// such calls, so that the others' registers hold what they work on (one kernel for both: 32 sequences behind 4096 rows of
+// 256 floats 88 us instead of 84, 64 behind the 8B shape's 38.6 instead of 38.0).
+template <int KT, int CL, bool WIN> struct ShWork {
     static constexpr bool HALF = KT != PG_F32;
     static constexpr int NTH = 64 * SH_WC, CT = SH_CT;
     static constexpr int KC = HALF ? CL / 8 : CL / 4;          // LDS chunks of 16 bytes a row
@@ -146,14 +150,15 @@ template <int KT, int CL> struct ShWork {
 
     const PgView &p;
     const ShArgs &a;
-    ShLds<KT, CL> &lds;
+    ShLds<KT, CL, WIN> &lds;
     const int lane, h, wave, kvh, hd, group;
     int bad;
-    // the piece: rows [row0, row1) in tiles, of which [vf, vl) are attended by a column here
+    // the piece: rows [row0, row1) in tiles; columns here attend rows of [vf, vl)
     int lead, vf, vl;
     bool live, busy;   // the lane's column, or any of the wave's, is a query head's
     int first, last, wf, wl;   // the column's rows; all columns of the wave have [wf, wl)
     int ids, ids_at;
+    unsigned in;   // WIN: which rows of its half tile any column attends
     unsigned kr[KN][KW], vr[VN][VW];
     unsigned ko[KN], vo[VN];   // this thread's pieces of a tile, bytes from the row that its half of the tile starts at
     float sr, minus;   // minus: -1, which the compiler does not see, so that a lo is one instruction
@@ -162,7 +167,7 @@ template <int KT, int CL> struct ShWork {
     int ev;
     float16v o[DT];
 
-    __device__ __forceinline__ ShWork(const PgView &p_, const ShArgs &a_, ShLds<KT, CL> &l, int kvh_)
+    __device__ __forceinline__ ShWork(const PgView &p_, const ShArgs &a_, ShLds<KT, CL, WIN> &l, int kvh_)
         : p(p_), a(a_), lds(l), lane(threadIdx.x & 63), h(lane >> 5),
           wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))), kvh(kvh_), hd(p_.hd), group(a_.nh / p_.n_kv), bad(0), sr(0.0f), minus(-1.0f) {
         asm("" : "+v"(minus));
@@ -191,7 +196,14 @@ template <int KT, int CL> struct ShWork {
         last = min(len, rows);
         first = a.window > 0 && len > a.window ? min(len - a.window, rows) : 0;
         const bool some = live && first < last;
-        int f = some ? first : INT_MAX, l = some ? last : 0;
+        // the columns' least first row and largest end; WIN: below it, of those that begin or end there, the most rows
+        using Key = std::conditional_t<WIN, unsigned long long, int>;
+        constexpr int SH = WIN ? 32 : 0;
+        Key f = (Key)(some ? first : INT_MAX) << SH, l = (Key)(some ? last : 0) << SH;
+        if constexpr (WIN) {
+            f |= INT_MAX - (some ? last : 0);
+            l |= INT_MAX - (some ? first : INT_MAX);
+        }
         wf = live ? first : 0;
         wl = live ? last : INT_MAX;
         for (int o = 16; o >= 1; o >>= 1) {
@@ -203,22 +215,41 @@ template <int KT, int CL> struct ShWork {
         wf = __builtin_amdgcn_readfirstlane(wf);
         wl = __builtin_amdgcn_readfirstlane(wl);
         __syncthreads();   // the piece before has been read
-        if (threadIdx.x == 0) lds.range[0] = INT_MAX, lds.range[1] = 0;
+        if (threadIdx.x == 0) lds.range[0] = (Key)INT_MAX << SH, lds.range[1] = 0;
         __syncthreads();
         if (lane == 0) {
             atomicMin(&lds.range[0], f);
             atomicMax(&lds.range[1], l);
         }
+        if (WIN && h == 0) lds.col[wave * 32 + lane] = some ? make_int2(first, last) : make_int2(INT_MAX, 0);
         __syncthreads();
-        vf = __builtin_amdgcn_readfirstlane(lds.range[0]);
-        vl = __builtin_amdgcn_readfirstlane(lds.range[1]);
+        vf = __builtin_amdgcn_readfirstlane((int)(lds.range[0] >> SH));
+        vl = __builtin_amdgcn_readfirstlane((int)(lds.range[1] >> SH));
     }
 
-    // the pages of the 64 half tiles from r0 on
+    // The pages of the 64 half tiles from r0 on. Windows may leave rows within [vf, vl) to no column, between sequences
+    // far apart: those may hold anything, and pages of such rows alone need not be in the table.
     __device__ __forceinline__ void find(int r0) {
         ids_at = r0;
         const int r = r0 + 16 * lane;
-        ids = r + 16 > vf && r < vl ? pg_page(p, lead, r, bad) : -1;
+        if constexpr (WIN) {
+            const auto rows = [&](int f, int l) {   // of the half tile, those of [f, l)
+                const int b = max(f - r, 0), e = min(l - r, 16);
+                return b < e ? (1u << e) - (1u << b) : 0u;
+            };
+            in = rows(vf, vl);
+            // a column has all rows from vf to f, and another all from l to vl
+            const int f = INT_MAX - __builtin_amdgcn_readfirstlane((int)(unsigned)lds.range[0]);
+            const int l = INT_MAX - __builtin_amdgcn_readfirstlane((int)(unsigned)lds.range[1]);
+            if (f < l && r0 < l && r0 + 64 * 16 > f) {
+                in = 0;
+#pragma unroll 1
+                for (int c = 0; c < CT; c++) in |= rows(lds.col[c].x, lds.col[c].y);
+            }
+            ids = in ? pg_page(p, lead, r, bad) : -1;
+        } else {
+            ids = r + 16 > vf && r < vl ? pg_page(p, lead, r, bad) : -1;
+        }
     }
 
     // asks for the rows of the tile at r0
@@ -258,10 +289,15 @@ template <int KT, int CL> struct ShWork {
         }
     }
 
-    // and lays them down; rows that no column attends may hold anything, so of V they are zeros
+    // and lays them down; rows that no column attends may hold anything, so of V (or its scales) they are zeros
     __device__ __forceinline__ void put(int buf, int r0) {
-        const bool whole = r0 >= vf && r0 + SH_R <= vl;
-        auto in = [&](int row) { return r0 + row >= vf && r0 + row < vl; };
+        [[maybe_unused]] unsigned some = 0;   // which of its rows a column attends
+        if constexpr (WIN) {
+            const int at = (r0 - ids_at) >> 4;
+            some = __builtin_amdgcn_readlane(in, at) | __builtin_amdgcn_readlane(in, at + 1) << 16;
+        }
+        const bool whole = WIN ? some == ~0u : r0 >= vf && r0 + SH_R <= vl;
+        auto has = [&](int row) { return WIN ? (some >> row & 1) != 0 : r0 + row >= vf && r0 + row < vl; };
 #pragma unroll
         for (int j = 0; j < KN; j++) {
             const int u = j * NTH + (int)threadIdx.x, row = u / KC, c = u % KC;
@@ -280,8 +316,12 @@ template <int KT, int CL> struct ShWork {
             const int u = j * NTH + (int)threadIdx.x;
             if (VU % NTH != 0 && u >= VU) continue;
             if (!whole && KT != PG_Q8) {
+                [[maybe_unused]] const unsigned mine = some >> vrow(u);   // (each row's own shift would be kept in a register)
 #pragma unroll
-                for (int w = 0; w < VW; w++) vr[j][w] = in(vrow(u) + (HALF ? w / (VW / 4) : 0)) ? vr[j][w] : 0u;
+                for (int w = 0; w < VW; w++) {
+                    const int i = HALF ? w / (VW / 4) : 0;
+                    vr[j][w] = (WIN ? (mine >> i & 1) != 0 : has(vrow(u) + i)) ? vr[j][w] : 0u;
+                }
             }
             if constexpr (HALF) {
                 const int quad = u / VC, d = u % VC * 4;
@@ -316,7 +356,7 @@ template <int KT, int CL> struct ShWork {
         }
         if constexpr (KT == PG_Q8) {
             // 8-bit rows are numbers whatever they hold; their scales may be none
-            if (wave == 0) (lane < 32 ? lds.kd : lds.vd)[buf][lane & 31] = whole || in(lane & 31) ? sr : 0.0f;
+            if (wave == 0) (lane < 32 ? lds.kd : lds.vd)[buf][lane & 31] = whole || has(lane & 31) ? sr : 0.0f;
         }
     }
 
@@ -576,9 +616,9 @@ template <int KT, int CL> struct ShWork {
 // The first workgroups' waves have shares of the sequences' own rows, the others shares of the
 // shared ones: the former wait for HBM, the latter for the matrix cores (and
 // for power: 64 sequences behind 32,000 rows run at 1.6 GHz), so they are one launch.
-template <int KT, int CL>
+template <int KT, int CL, bool WIN>
 __global__ void __launch_bounds__(64 * SH_WC, sh_waves(KT, CL)) k_shared_rows(const PgView p, const ShArgs a, int own) {
-    __shared__ ShLds<KT, CL> lds;
+    __shared__ ShLds<KT, CL, WIN> lds;
     // KV heads in turn, so that a die has few of them (of eight one), whose rows its L2 holds for all columns
     const int kvh = (int)blockIdx.x % p.n_kv, block = (int)blockIdx.x / p.n_kv;
     if (block < own) {
@@ -598,7 +638,7 @@ __global__ void __launch_bounds__(64 * SH_WC, sh_waves(KT, CL)) k_shared_rows(co
         return;
     }
     const int u = block - own;
-    ShWork<KT, CL> w(p, a, lds, kvh);
+    ShWork<KT, CL, WIN> w(p, a, lds, kvh);
     const ShTiles all = sh_tiles(p, a, w.bad);
     const int tiles = __builtin_amdgcn_readlane(all.sum, 63);
     if (u < all.shares && tiles > 0) {
@@ -759,9 +799,10 @@ bool sh_args_ok(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_
 }
 
 using ShRows = void (*)(const PgView, const ShArgs, int);
-template <int KT> ShRows sh_rows(int hd) {
-    return hd <= 64 ? k_shared_rows<KT, 64> : hd <= 128 ? k_shared_rows<KT, 128> : k_shared_rows<KT, 256>;
+template <int KT, bool WIN> ShRows sh_rows(int hd) {
+    return hd <= 64 ? k_shared_rows<KT, 64, WIN> : hd <= 128 ? k_shared_rows<KT, 128, WIN> : k_shared_rows<KT, 256, WIN>;
 }
+template <int KT> ShRows sh_rows(int hd, bool win) { return win ? sh_rows<KT, true>(hd) : sh_rows<KT, false>(hd); }
 
 }  // namespace
 
@@ -811,7 +852,10 @@ extern "C" void krh_paged_attention_shared(float *o, const krh_pages *kv, const 
     a.sshares = r.sshares, a.sfew = r.sfew, a.sleast = sh_least(kv), a.slots = r.slots, a.fault = kr_fault_word();
     const PgView p = pg_view(kv, table, table_ld, n_seq);
     const int hd = kv->head_dim, own = (r.shares + SH_WC - 1) / SH_WC;
-    const ShRows f = kv->kv_type == ML_F32 ? sh_rows<PG_F32>(hd) : kv->kv_type == ML_F16 ? sh_rows<PG_F16>(hd) : sh_rows<PG_Q8>(hd);
+    const bool win = window > 0;
+    const ShRows f = kv->kv_type == ML_F32   ? sh_rows<PG_F32>(hd, win)
+                     : kv->kv_type == ML_F16 ? sh_rows<PG_F16>(hd, win)
+                                             : sh_rows<PG_Q8>(hd, win);
     hipLaunchKernelGGL(f, dim3((own + r.sshares) * kv->n_kv_heads), dim3(64 * SH_WC), 0, kr_stream(), p, a, own);
     kr_check_launch("paged_attention_shared");
     // Threads a head: with few heads the parts are asked for side by side, with many each wave's search for its parts

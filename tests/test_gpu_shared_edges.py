@@ -1,0 +1,126 @@
+"""Attention over shared rows at the edges of what the call accepts: windows that
+leave a gap between a group's sequences, soft-caps and queries near the ends of the
+floats, empty places beside values that are not finite, bad group starts, pools past
+32 bits. Needs a gfx950 device."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import krafla as K
+from test_gpu_kernels import bits, f32, ok
+from test_gpu_paged import TYPES, U, attention, i32
+from test_gpu_shared import Batch, dev, device, own_rows  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def gap(b, window):
+    """rows of a group's shared ones that no sequence of it attends: True [groups][shared rows]"""
+    out = []
+    for g, rows in enumerate(b.shared):
+        free = np.ones(rows, bool)
+        for n in b.lens[b.start[g]:b.start[g + 1]]:
+            free[max(0, n - window):n] = False
+        out.append(free)
+    return out
+
+
+GAPS = [
+    # one gap, in the first column tile (narrow groups) or in each of several
+    (8, 4, 128, 32, 2500, [(60, 2800)], {0: -2670, 7: -2795, 30: -2700}),
+    # the short ones at the end: the tile of the others has no gap
+    (8, 2, 64, 64, 2500, [(60, 3000)], {57: -2990, 58: -2900, 59: -2680}),
+    # three runs of rows with gaps between them, which begin and end within tiles and pages, and a group without one
+    (16, 8, 128, 16, 600, [(70, 3100), (30, 480)], {0: -3000, 1: -1717, 2: -1700, 40: -3093, 41: -1690}),
+    (8, 4, 256, 16, 1800, [(40, 4000)], {0: -3900, 11: -1990, 12: -2000}),
+]
+
+
+@pytest.fixture(autouse=True)
+def no_error():
+    yield
+    K.hip.krh_clear_error()
+
+
+@pytest.mark.parametrize("paged", [True, False])
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd,page,window,groups,short", GAPS)
+def test_gaps_between_windows(dev, kv_type, nh, nkv, hd, page, window, groups, short, paged):  # noqa: F811
+    """rows that no sequence's window reaches may hold anything, and pages of such rows alone need not be in a table"""
+    rng = np.random.default_rng(hd + page)
+    n = sum(g[0] for g in groups)
+    own = [100 + v for v in own_rows(rng, n, 90)]
+    for i, v in short.items():
+        own[i] = v
+    b = Batch(dev, rng, kv_type, nh, nkv, hd, page, groups, own)
+    p = b.p
+    whole = {name: x.copy() for name, x in p.a.items()}
+    free = gap(b, window)
+    assert free[0].sum() > 60
+    table = p.table.copy()
+    for g, rows in enumerate(free):
+        a, e = b.start[g], b.start[g + 1]
+        for r in np.flatnonzero(rows):
+            for name in "kv":
+                x = p.a[name + "d"] if kv_type == K.ML_Q8_0 else p.a[name]
+                x[p.table[a, r // page], :, r % page] = np.nan if name == "v" or r % 2 else np.inf
+        for j in range(len(rows) // page):
+            if rows[j * page:(j + 1) * page].all():
+                table[a:e, j] = -1
+    b.put(window=window)
+    assert b.form(window) == 1
+    if not paged:
+        p.tab = dev.put(table)
+    p.a = whole   # (the 64-bit form reads all rows before it leaves out those behind the window)
+    b.run(window)
+    ok()
+    b.check(b.out(), window)
+
+
+def run(b, scale, cap=0.0, window=0):
+    """b's call with a scale of its own"""
+    K.hip.krh_paged_attention_shared(b.ob.ptr, b.p.ref, b.p.tab.ptr, b.p.ld, b.lb.ptr, len(b.lens), b.gb.ptr, b.sb.ptr,
+                                     len(b.shared), b.max_shared, b.qb.ptr, b.nh, b.max_len, window, scale, cap, b.ws.ptr)
+    ok()
+    return b.out()
+
+
+def compare(b, o, scale, score=0.0):
+    """against the softmax in 64 bits of scores that no cap changes; `score`: how far a score may be off beside that"""
+    for i, n in enumerate(b.lens):
+        k, v = b.p.rows("k", i, n), b.p.rows("v", i, n)
+        for h in range(b.nh):
+            g = h * b.nkv // b.nh
+            w, _, bound, _ = attention(b.q[i, h].astype(np.float64), k[:, g], v[:, g], scale, 0, 0)
+            # a score off by e makes the weights wrong by a factor of e^2e at most
+            assert (np.abs(o[i, h] - w) <= bound + 2 * score * np.abs(v[:, g]).max()).all(), (i, h)
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("hd,peak,cap", [(64, 0.1, 1e36), (64, 0.01, 1e37), (128, 1.0, 2.0 ** 126), (128, 0.005, 2.0 ** 126),
+                                         (48, 0.005, 2.0 ** 126), (256, 0.01, 1e35), (80, 1.0, 2.0 ** 100)])
+def test_large_soft_caps(dev, kv_type, hd, peak, cap):  # noqa: F811
+    """caps far above the scores leave them, however small the queries are: tanh(x) is x, and what is left is the division's
+    rounding, a step of 2^-149 where the quotient is that small, and two roundings of the float"""
+    rng = np.random.default_rng(hd)
+    b = Batch(dev, rng, kv_type, 4, 2, hd, 16, [(9, 200), (20, 330)], own_rows(rng, 29, 60))
+    b.q = f32(b.q * (peak / np.abs(b.q).max()))
+    # keys that make the scores differ by a few whatever the queries are
+    name = "kd" if kv_type == K.ML_Q8_0 else "k"
+    b.p.a[name] = (b.p.a[name] * min(1 / peak, 100)).astype(b.p.a[name].dtype)
+    b.put()
+    assert b.form() == 1
+    o = run(b, hd ** -0.5, cap)
+    compare(b, o, hd ** -0.5, 2 * 2.0 ** -149 * cap)
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_small_soft_caps(dev, kv_type):  # noqa: F811
+    """a cap far below the scores gives every row the same weight"""
+    rng = np.random.default_rng(5)
+    b = Batch(dev, rng, kv_type, 4, 2, 128, 16, [(9, 200), (20, 330)], own_rows(rng, 29, 60)).put()
+    assert b.form() == 1
+    o = run(b, 128 ** -0.5, 2.0 ** -126)
+    b.q = np.zeros_like(b.q)
+    compare(b, o, 1.0, 8 * U)
