@@ -462,9 +462,10 @@ template <int KT, int CL, bool WIN> struct ShWork {
         }
         float ce = cs;   // a score's power of two is s ce
         if (a.cap > 0.0f) {
-            const float inv_cap = cs / a.cap;
+            // one after the other: the product of both factors may lie below the normal floats
+            const float inv_cap = 1.0f / a.cap;
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = pa_tanh(s[i] * inv_cap);
+            for (int i = 0; i < 16; i++) s[i] = pa_tanh(s[i] * cs * inv_cap);
             ce = a.cap * 1.4426950408889634f;
         }
         if (r0 < wf || r0 + SH_R > wl) {
