@@ -382,7 +382,7 @@ template <int KT, int CL, bool WIN> struct ShWork {
                 }
             }
             m = fmaxf(m, sh_other(m));
-            if (m > 0.0f && m < INFINITY) e = 13 - ilogbf(m);
+            e = pa_power(m, a.scale);
 #pragma unroll
             for (int j = 0; j < KS; j++) {
                 half8 hi, lo;
@@ -452,20 +452,22 @@ template <int KT, int CL, bool WIN> struct ShWork {
             __builtin_amdgcn_sched_barrier(0);
         }
         // value i is row (i & 3) + 8 (i >> 2) + 4 h
+        float ce = cs;   // a score's power of two is s ce, ce > 0: what is cut off stays -inf
         if constexpr (KT == PG_Q8) {
+            // both factors first: either one alone may take the products out of the floats
+            ce = 1.0f;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const float4v d = *(const float4v *)(lds.kd[buf] + 2 * i + 4 * h);
 #pragma unroll
-                for (int c = 0; c < 4; c++) s[i + c] *= d[c];
+                for (int c = 0; c < 4; c++) s[i + c] *= cs * d[c];
             }
         }
-        float ce = cs;   // a score's power of two is s ce
         if (a.cap > 0.0f) {
             // one after the other: the product of both factors may lie below the normal floats
             const float inv_cap = 1.0f / a.cap;
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = pa_tanh(s[i] * cs * inv_cap);
+            for (int i = 0; i < 16; i++) s[i] = pa_tanh(s[i] * ce * inv_cap);
             ce = a.cap * 1.4426950408889634f;
         }
         if (r0 < wf || r0 + SH_R > wl) {

@@ -152,6 +152,15 @@ __device__ __forceinline__ float pa_sum_g(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// The power of two by which a head's queries are scaled to become halves, the largest of them m: to 2^13 or more, but that
+// the scores' factor, scale times the other power, stays a normal float
+__device__ __forceinline__ int pa_power(float m, float scale) {
+    if (!(m > 0.0f && m < INFINITY)) return 0;
+    // |scale| 2^-e >= 2^(s - 127) 2^-e
+    const int s = (int)(__float_as_uint(scale) >> 23 & 255);
+    return min(13 - ilogbf(m), s - 1);
+}
+
 __device__ __forceinline__ float4v pa_weigh(half8 v, half8 p, float4v o) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, o, 0, 0, 0);
 }
@@ -273,7 +282,7 @@ template <int KT, int CL, bool FULL, class A = PaArgs, bool FINE = false> struct
                 }
             }
             m = pa_max_g(m);
-            if (m > 0.0f && m < INFINITY) e = 13 - ilogbf(m);
+            e = pa_power(m, a.scale);
 #pragma unroll
             for (int j = 0; j < KS; j++) {
                 half8 h, l;

@@ -89,6 +89,9 @@ def run(b, scale, cap=0.0, window=0):
 def compare(b, o, scale, score=0.0):
     """against the softmax in 64 bits of scores that no cap changes; `score`: how far a score may be off beside that"""
     for i, n in enumerate(b.lens):
+        if n == 0:
+            assert (o[i] == 0).all(), i
+            continue
         k, v = b.p.rows("k", i, n), b.p.rows("v", i, n)
         for h in range(b.nh):
             g = h * b.nkv // b.nh
@@ -124,3 +127,55 @@ def test_small_soft_caps(dev, kv_type):  # noqa: F811
     o = run(b, 128 ** -0.5, 2.0 ** -126)
     b.q = np.zeros_like(b.q)
     compare(b, o, 1.0, 8 * U)
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("hd,power,scale", [(128, -140, None), (64, -148, None), (48, -133, None), (64, -10, 2.0 ** -140),
+                                            (128, 0, 2.0 ** -149), (256, -100, 1e-20), (64, -126, -2.0 ** -60)])
+def test_scores_near_nothing(dev, kv_type, hd, power, scale):  # noqa: F811
+    """queries or a scale so small that their product is under the floats: every row has the same weight, and those that
+    are cut off none"""
+    rng = np.random.default_rng(hd)
+    own = own_rows(rng, 40, 60)
+    own[2], own[9], own[39] = -190, -5, -330
+    b = Batch(dev, rng, kv_type, 4, 2, hd, 16, [(19, 200), (21, 330)], own)
+    b.spoil()
+    b.q = f32(b.q * 2.0 ** power)
+    b.put()
+    assert b.form() == 1
+    s = hd ** -0.5 if scale is None else scale
+    for cap in (0.0, 2.0):
+        o = run(b, s, cap)
+        assert np.isfinite(o).all()
+        compare(b, o, s, 2.0 ** -80)   # no score is larger (2^-100, at most 256 dims, and products below 2^6)
+
+
+@pytest.mark.parametrize("power,keys", [(0, 95), (-100, 100), (-132, 119), (-140, 124), (124, -119), (110, -112)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_8_bit_scales_against_the_queries(dev, hd, power, keys):  # noqa: F811
+    """queries and keys' scales at opposite ends of the floats, whose scores are ordinary numbers (or, in the first case,
+    large ones: the largest has all the weight)"""
+    rng = np.random.default_rng(hd + abs(keys))
+    b = Batch(dev, rng, K.ML_Q8_0, 4, 2, hd, 16, [(19, 200), (21, 330)], own_rows(rng, 40, 60))
+    b.q = f32(b.q * 2.0 ** power)
+    b.p.a["kd"] = f32(b.p.a["kd"] * 2.0 ** keys)
+    b.put()
+    assert b.form() == 1 and np.abs(b.q).max() > 0
+    scale = 2.0 ** -(power + keys) * hd ** -0.5 if power else hd ** -0.5
+    o = run(b, scale)
+    assert np.isfinite(o).all()
+    if power:
+        compare(b, o, scale)
+        # each sequence reading its own rows as well
+        ws = dev.zeros(K.hip.krh_paged_attention_ws(b.p.ref, len(b.lens), 4, b.max_len, 0))
+        K.hip.krh_paged_attention(b.ob.ptr, b.p.ref, b.p.tab.ptr, b.p.ld, b.lb.ptr, len(b.lens), b.qb.ptr, 4, b.max_len, 0, scale,
+                                  0.0, None, 0, ws.ptr)
+        ok()
+        compare(b, b.out(), scale)
+        return
+    for i, n in enumerate(b.lens):
+        k, v = b.p.rows("k", i, n), b.p.rows("v", i, n)
+        for h in range(4):
+            z = k[:, h // 2] @ b.q[i, h].astype(np.float64)
+            if np.diff(np.sort(z)[-2:])[0] > 2.0 ** -18 * (np.abs(k[:, h // 2]) @ np.abs(b.q[i, h])).max():
+                assert (np.abs(o[i, h] - v[z.argmax(), h // 2]) <= 8 * U * np.abs(v[:, h // 2]).max()).all(), (i, h)
