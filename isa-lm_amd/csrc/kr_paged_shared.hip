@@ -716,7 +716,7 @@ template <int T> __global__ void __launch_bounds__(T) k_shared_join(const PgView
         l += v.y * weight(v.x);
     }
     for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
-    const float inv = sp.len == 0 ? 0.0f : 1.0f / l;
+    const float inv = 1.0f / l;
     float4v acc = { 0, 0, 0, 0 };
     for (int i0 = 0; i0 < n; i0 += SJ_N * lanes) {
         if (i0 > 0) fetch(i0 + first);
@@ -732,7 +732,8 @@ template <int T> __global__ void __launch_bounds__(T) k_shared_join(const PgView
         __syncthreads();
         if (first < k) s_o[tid] = acc = acc + s_o[tid + (k << dl)];
     }
-    if (first == 0 && 4 * q < p.hd) *(float4v *)(a.o + ((size_t)s * a.nh + x) * p.hd + d) = acc * inv;
+    // (zeros for no rows: the shared ones' parts hold what their NaNs times 0 are)
+    if (first == 0 && 4 * q < p.hd) *(float4v *)(a.o + ((size_t)s * a.nh + x) * p.hd + d) = sp.len == 0 ? float4v{} : acc * inv;
 }
 
 // ---- the host's side ----

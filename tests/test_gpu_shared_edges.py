@@ -179,3 +179,22 @@ def test_8_bit_scales_against_the_queries(dev, hd, power, keys):  # noqa: F811
             z = k[:, h // 2] @ b.q[i, h].astype(np.float64)
             if np.diff(np.sort(z)[-2:])[0] > 2.0 ** -18 * (np.abs(k[:, h // 2]) @ np.abs(b.q[i, h])).max():
                 assert (np.abs(o[i, h] - v[z.argmax(), h // 2]) <= 8 * U * np.abs(v[:, h // 2]).max()).all(), (i, h)
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+def test_empty_places_beside_values_not_finite(dev, kv_type):  # noqa: F811
+    """a place without a sequence gets zeros, whatever the rows hold that its group shares"""
+    rng = np.random.default_rng(3)
+    own = own_rows(rng, 30, 60)
+    own[0], own[7], own[29] = -320, -320, -320
+    b = Batch(dev, rng, kv_type, 8, 2, 64, 16, [(30, 320)], own)
+    name = "vd" if kv_type == K.ML_Q8_0 else "v"
+    b.p.a[name][b.p.table[0, 3], :, 5] = np.nan
+    b.p.a[name][b.p.table[0, 4], 0, 6] = np.inf
+    b.put()
+    assert b.form() == 1
+    b.run()
+    ok()
+    o = b.out()
+    for i, n in enumerate(b.lens):
+        assert (o[i] == 0).all() if n == 0 else np.isnan(o[i]).all(), i
