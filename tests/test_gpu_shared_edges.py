@@ -198,3 +198,59 @@ def test_empty_places_beside_values_not_finite(dev, kv_type):  # noqa: F811
     o = b.out()
     for i, n in enumerate(b.lens):
         assert (o[i] == 0).all() if n == 0 else np.isnan(o[i]).all(), i
+
+
+@pytest.mark.parametrize("what,at,value", [("start", 0, -5), ("end", 2, 61), ("order", 1, 2 ** 30), ("order", 0, 31)])
+def test_bad_group_starts(dev, what, at, value):  # noqa: F811
+    """are reported, and leave no group: each sequence reads all of its own rows"""
+    rng = np.random.default_rng(9)
+    b = Batch(dev, rng, K.ML_F16, 8, 2, 64, 16, [(30, 320), (30, 160)], own_rows(rng, 60, 40)).put()
+    assert b.form() == 1
+    start = i32(b.start)
+    start[at] = value
+    b.gb = dev.put(start)
+    b.run()
+    assert K.hip.krh_sync() == K.ML_E_SHAPE
+    K.hip.krh_clear_error()
+    b.check(b.out())
+
+
+@pytest.mark.parametrize("kv_type,n", [(K.ML_F16, 270000), (K.ML_Q8_0, 530000)])
+def test_offsets_past_32_bits(dev, kv_type, n):  # noqa: F811
+    """shared and own rows of halves and 8 bits in pages beyond 2^32 bytes"""
+    nkv, hd, page, S, shared = 2, 256, 16, 40, 96
+    size = 2 if kv_type == K.ML_F16 else 1
+    assert n * nkv * hd * page * size > 2 ** 32
+    pool = [K.DevBuf(size * n * nkv * hd * page) for _ in range(2)]
+    scales = [K.DevBuf(4 * n * nkv * page) for _ in range(2)] if size == 1 else []
+    dev.bufs += pool + scales
+    kv = K.KrhPages(*[x.ptr for x in pool], *([x.ptr for x in scales] or [None, None]), kv_type, n, page, nkv, hd)
+    ref, rng = C.byref(kv), np.random.default_rng(12)
+    table = np.full((S, 7), -1, np.int32)
+    table[:, :6] = [n - 1, 7, n - 2, n // 2 + 1, n - 70, 3]
+    table[:, 6] = n - 10 - np.arange(S)
+    lens = i32(shared + rng.integers(0, 16, S))
+    seq = i32([0] * shared + [i for i in range(S) for _ in range(lens[i] - shared)])
+    row = i32(list(range(shared)) + [r for i in range(S) for r in range(shared, lens[i])])
+    T, nh = len(seq), 4
+    q = f32(rng.standard_normal((S, nh, hd)))
+    kr, vr = (dev.put(f32(rng.standard_normal((T, nkv * hd)))) for _ in range(2))
+    tb, ob, sb, rb = dev.put(table), dev.zeros(q.nbytes), dev.put(seq), dev.put(row)
+    K.hip.krh_paged_qkv(None, 0, ref, tb.ptr, 7, S, None, 0, kr.ptr, nkv * hd, vr.ptr, nkv * hd, T, 0, sb.ptr, rb.ptr, None, None,
+                        None, 0.0, None, None, 0)
+    K.hip.krh_paged_load(kr.ptr, nkv * hd, vr.ptr, nkv * hd, ref, tb.ptr, 7, S, T, sb.ptr, rb.ptr)   # what the pages hold
+    most = 128
+    while K.hip.krh_paged_attention_shared_form(ref, S, nh, most, 1, most - 1, 0) != 1:
+        most *= 2
+    ws = dev.zeros(K.hip.krh_paged_attention_shared_ws(ref, S, nh, most, 1, most - 1))
+    K.hip.krh_paged_attention_shared(ob.ptr, ref, tb.ptr, 7, dev.put(lens).ptr, S, dev.put(i32([0, S])).ptr,
+                                     dev.put(i32([shared])).ptr, 1, most - 1, dev.put(q).ptr, nh, most, 0, 0.0625, 0.0, ws.ptr)
+    ok()
+    o = ob.get(np.float32, q.size).reshape(q.shape)
+    k64, v64 = (x.get(np.float32, T * nkv * hd).reshape(T, nkv, hd).astype(np.float64) for x in (kr, vr))
+    assert np.abs(k64).max() > 2
+    for i in range(S):
+        at = np.concatenate([np.arange(shared), np.flatnonzero((seq == i) & (row >= shared))])
+        for h in range(nh):
+            w, _, bound, _ = attention(q[i, h].astype(np.float64), k64[at, h // 2], v64[at, h // 2], 0.0625, 0, 0)
+            assert (np.abs(o[i, h] - w) <= bound).all(), (i, h)
