@@ -406,10 +406,11 @@ bool i8_not_ready(const char *what) {
     if (!kr_stream()) kr_fail(ML_E_ISA, what, hipSuccess);
     return !kr_stream();
 }
+bool i8_size_ok(int rows, int cols) { return rows > 0 && rows <= INT32_MAX - 1024 && cols > 0 && cols <= I8_COLS; }
 bool i8_aligned(const void *p) { return !((uintptr_t)p & 15); }
 bool i8_mat_ok(const krh_mat8 *w) {
-    return w && w->q && w->d && i8_aligned(w->q) && w->rows > 0 && w->rows <= INT32_MAX - 1024 && w->cols > 0 &&
-           w->cols <= I8_COLS && w->ld % 16 == 0 && w->ld >= (size_t)w->cols && w->ld <= I8_LD;
+    return w && w->q && w->d && i8_aligned(w->q) && i8_size_ok(w->rows, w->cols) && w->ld % 16 == 0 &&
+           w->ld >= (size_t)w->cols && w->ld <= I8_LD;
 }
 bool i8_args_ok(const krh_mat8 *w, const float *y, size_t ldy, const int8_t *xq, size_t ldx, const float *xd) {
     return y && xq && xd && i8_aligned(xq) && ldy >= (size_t)w->rows && ldx % 16 == 0 && ldx >= (size_t)w->cols && ldx <= I8_LD;
@@ -418,7 +419,7 @@ bool i8_args_ok(const krh_mat8 *w, const float *y, size_t ldy, const int8_t *xq,
 }  // namespace
 
 extern "C" int krh_matmul_i8_form(int rows, int cols, int ntok, int swiglu) {
-    return rows > 0 && cols > 0 && cols <= I8_COLS && ntok > 0 ? i8_form(rows, cols, ntok, swiglu != 0) : -1;
+    return i8_size_ok(rows, cols) && ntok > 0 && ntok <= KRH_ROWS_MAX ? i8_form(rows, cols, ntok, swiglu != 0) : -1;
 }
 
 extern "C" void krh_matmul_i8(float *Y, size_t ldy, const krh_mat8 *W, const int8_t *xq, size_t ldx, const float *xd,
