@@ -495,7 +495,7 @@ void krh_matmul_i8(float *Y, size_t ldy, const krh_mat8 *W, const int8_t *xq, si
                    const float *bias, int T, int accumulate);
 /* H[t * ldh + r] = silu(g) u of the two products g (w1) and u (w3) of the same
  * sizes, each as krh_matmul_i8 leaves it, silu(g) = g / (1 + e^-g) and its product
- * within 8 half steps of a float (1e-35 where e^-g leaves the floats) */
+ * within 8 half steps of a float, and 1e-35 (1 + |u|) where e^-g or a product leaves the normal floats */
 void krh_matmul_i8_swiglu(float *H, size_t ldh, const krh_mat8 *w1, const krh_mat8 *w3, const int8_t *xq, size_t ldx,
                           const float *xd, int T);
 /* The tiles that krh_matmul_i8 takes for these sizes, or krh_matmul_i8_swiglu for a

@@ -79,7 +79,8 @@ typedef int v16i __attribute__((ext_vector_type(16)));
 // 16 bytes a lane from base + off to LDS at `to` (one address a wave) + 16 lane.
 // No register waits for it: a wait on the vector memory counter ends it. (The
 // compiler does not see into it, so it holds the 5 clocks that a load waits for an
-// address register which a vector instruction has written.)
+// address register which a vector instruction has written. m0 is
+// reserved, which a clobber would not change, and no other instruction here takes it.)
 __device__ __forceinline__ void i8_to_lds(unsigned to, const int8_t *base, unsigned off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
 }
