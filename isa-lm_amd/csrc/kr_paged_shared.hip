@@ -812,7 +812,7 @@ template <int KT> ShRows sh_rows(int hd, bool win) { return win ? sh_rows<KT, tr
 
 extern "C" int krh_paged_attention_shared_form(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_groups,
                                                int max_shared, int window) {
-    if (!sh_args_ok(kv, n_seq, n_heads, max_len, n_groups, max_shared)) return -1;
+    if (!sh_args_ok(kv, n_seq, n_heads, max_len, n_groups, max_shared) || window < 0) return -1;
     return sh_shared(kv, n_seq, n_heads, n_groups, max_shared, window);
 }
 
