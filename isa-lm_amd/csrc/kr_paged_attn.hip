@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(64, pa_waves(KT, CL)) k_paged_shares(const PgV
         kr_report(fault, w.bad);
         return;
     }
-    PaAll all = pa_all(p, a, w.bad);
+    PaAll all = pa_all(p, a, w.bad, a.shares);
     if (u < all.shares) {
         int left = pa_bound(all, u + 1) - pa_bound(all, u), t = pa_bound(all, u);
         for (w.seq = pa_find(p, a, all, t, w.bad); left > 0; w.seq++, t = 0) {
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
     PaSpan sp;
     if (x < a.nh) {
         const int kvh = x / group, col = x % group;
-        const PaParts r = pa_parts(p, a, s, kvh, sp);
+        const PaParts r = pa_parts(p, a, s, kvh, sp, a.shares);
         if (r.n <= 1) return;
         const float *ml = a.pml + (r.slot * group + col) * 2, *part = a.part + (r.slot * group + col) * p.hd;
         const int l = tid & ((1 << dl) - 1), lanes = PJ_T >> dl, d = 4 * l < p.hd ? 4 * l : 0, i0 = tid >> dl;
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(PJ_T) k_paged_join(const PgView p, const PaArg
         return;
     }
     const int kvh = (x - a.nh) / blocks, block = (x - a.nh) % blocks;
-    const PaParts r = pa_parts(p, a, s, kvh, sp);
+    const PaParts r = pa_parts(p, a, s, kvh, sp, a.shares);
     const int r0 = sp.first + block * PJ_ROWS;
     if (r0 >= sp.len) return;
     const float *z = a.z + ((size_t)s * a.nh + kvh * group) * a.z_ld;

@@ -39,7 +39,9 @@ constexpr int SH_FEW = 8;   // tiles a share up to which a compute unit has one 
 constexpr int SH_WC = 4, SH_CT = 32 * SH_WC;   // waves and columns of a workgroup
 struct ShArgs : PaShared {
     float *spart, *spml;   // [n_kv][column tiles + shares][SH_CT][hd] and [2]: the shared rows' parts
-    int sshares, sfew, sleast, slots;
+    int wgs, own;    // workgroups of a KV head, and of these for the sequences' own rows at least
+    float weigh;     // a wave's work on a tile of those, in a workgroup's on one of the shared rows, a wave
+    int sfew, sleast, slots;
     int *fault;
 };
 
@@ -68,17 +70,20 @@ __device__ __forceinline__ int pa_skip(const PgView &p, const PaShared &a, int i
     return skip;
 }
 
+__device__ __forceinline__ int sh_rts(int rows, int begin) { return (rows - begin + SH_R - 1) / SH_R; }
+__device__ __forceinline__ int sh_cts(int seqs, int group) { return (seqs * group + SH_CT - 1) / SH_CT; }
 // The tiles of the groups, one group a lane: `cts` column tiles of the rows from
 // `begin` on in `rts` row tiles; `sum`, `csum`: inclusive sums of all tiles and of
 // the column tiles
 struct ShTiles {
     ShGroups g;
-    int begin, rts, cts, sum, csum, shares;
+    int begin, rts, cts, sum, csum;
+    int tiles, own;   // of all groups, and workgroups of a KV head that have the sequences' own rows
 };
 __device__ __forceinline__ ShTiles sh_tiles(const PgView &p, const ShArgs &a, int &bad) {
     ShTiles r;
-    r.g = sh_groups(p, a, bad);
     const int lane = (int)(threadIdx.x & 63), group = a.nh / p.n_kv;
+    r.g = sh_groups(p, a, bad);
     r.begin = 0;
     if (a.window > 0) {
         // of a window the first row that any sequence of the group attends
@@ -94,15 +99,31 @@ __device__ __forceinline__ ShTiles sh_tiles(const PgView &p, const ShArgs &a, in
             if (lane == g) r.begin = min(least, r.g.rows) & -SH_R;
         }
     }
-    r.rts = (r.g.rows - r.begin + SH_R - 1) / SH_R;
-    r.cts = r.g.rows > 0 ? ((r.g.s1 - r.g.s0) * group + SH_CT - 1) / SH_CT : 0;
+    r.rts = sh_rts(r.g.rows, r.begin);
+    r.cts = r.g.rows > 0 ? sh_cts(r.g.s1 - r.g.s0, group) : 0;
     r.sum = pg_scan(r.rts * r.cts);
     r.csum = pg_scan(r.cts);
-    const int all = __builtin_amdgcn_readlane(r.sum, 63);
-    // as many workgroups as there are compute units, the own rows' among them, where that gives each a few tiles only
-    const int most = all <= SH_FEW * a.sfew ? a.sfew : a.sshares;
-    r.shares = max(1, min(most, (all + a.sleast - 1) / a.sleast));
+    r.tiles = __builtin_amdgcn_readlane(r.sum, 63);
+    r.own = a.own;
+    if (a.weigh > 0.0f) {
+        // what is attended but for the shared rows, in tiles of SH_R
+        int own = -(r.cts > 0 ? r.g.s1 - r.g.s0 : 0) * r.rts;
+        for (int i = lane; i < p.n_seq; i += 64) {
+            const int len = kr_page_len(a.len[i], a.max_len, bad);
+            own += ((a.window > 0 ? min(len, a.window) : len) + SH_R - 1) / SH_R;
+        }
+        // (sequences shorter than their group's shared rows may leave less than nothing)
+        const float w = a.weigh * (float)max(__builtin_amdgcn_readlane(pg_scan(own), 63), 0);
+        const int part = __builtin_amdgcn_readfirstlane((int)((float)a.wgs * (w / (w + (float)max(r.tiles, 1)))));
+        r.own = r.tiles == 0 ? a.wgs : min(max(a.own, part), a.wgs - 1);
+    }
     return r;
+}
+// how many shares they make: as many as there are compute units, the own rows' workgroups among them, where that gives
+// each a few tiles only
+__device__ __forceinline__ int sh_shares(const ShArgs &a, const ShTiles &r) {
+    const int most = min(r.tiles <= SH_FEW * a.sfew ? a.sfew : a.wgs, a.wgs - r.own);
+    return max(1, min(most, (r.tiles + a.sleast - 1) / a.sleast));
 }
 
 __device__ __forceinline__ float sh_other(float v) {   // the same column's value in the other half of the wave
@@ -117,6 +138,8 @@ template <int KT, int CL, bool WIN> struct ShLds {
     alignas(16) float kd[2][KT == PG_Q8 ? SH_R : 4], vd[2][KT == PG_Q8 ? SH_R : 4];
     std::conditional_t<WIN, unsigned long long, int> range[2];
     int2 col[WIN ? SH_CT : 1];   // the rows that each column attends
+    int4 group[64];              // the groups: sequences, rows, and the first row of their tiles
+    int2 sums[64];               // sum, csum
 };
 
 // where 16 bytes of a K row lie (F32: of a V row too): 16 rows of one chunk in all banks
@@ -620,18 +643,21 @@ template <int KT, int CL, bool WIN> struct ShWork {
 // shared ones: the former wait for HBM, the latter for the matrix cores (and
 // for power: 64 sequences behind 32,000 rows run at 1.6 GHz), so they are one launch.
 template <int KT, int CL, bool WIN>
-__global__ void __launch_bounds__(64 * SH_WC, sh_waves(KT, CL)) k_shared_rows(const PgView p, const ShArgs a, int own) {
+__global__ void __launch_bounds__(64 * SH_WC, sh_waves(KT, CL)) k_shared_rows(const PgView p, const ShArgs a) {
     __shared__ ShLds<KT, CL, WIN> lds;
     // KV heads in turn, so that a die has few of them (of eight one), whose rows its L2 holds for all columns
     const int kvh = (int)blockIdx.x % p.n_kv, block = (int)blockIdx.x / p.n_kv;
-    if (block < own) {
+    int bad = 0;
+    const ShTiles all = sh_tiles(p, a, bad);
+    if (block < all.own) {
         const int u = block * SH_WC + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
         PaWave<KT, CL, false, ShArgs, true> w(p, a, kvh);
-        PaAll all = pa_all(p, a, w.bad);
-        if (u < all.shares) {
-            int left = pa_bound(all, u + 1) - pa_bound(all, u), t = pa_bound(all, u);
-            for (w.seq = pa_find(p, a, all, t, w.bad); left > 0; w.seq++, t = 0) {
-                w.sp = pa_of(p, a, all, w.seq, w.bad);
+        w.bad = bad;
+        PaAll pa = pa_all(p, a, w.bad, SH_WC * all.own);
+        if (u < pa.shares) {
+            int left = pa_bound(pa, u + 1) - pa_bound(pa, u), t = pa_bound(pa, u);
+            for (w.seq = pa_find(p, a, pa, t, w.bad); left > 0; w.seq++, t = 0) {
+                w.sp = pa_of(p, a, pa, w.seq, w.bad);
                 const int end = min(w.sp.tiles, t + left);
                 w.part(t, end, (size_t)kvh * (p.n_seq + a.shares) + w.seq + u);
                 left -= end - t;
@@ -640,22 +666,32 @@ __global__ void __launch_bounds__(64 * SH_WC, sh_waves(KT, CL)) k_shared_rows(co
         kr_report(a.fault, w.bad);
         return;
     }
-    const int u = block - own;
+    const int u = block - all.own, tiles = all.tiles, shares = sh_shares(a, all);
     ShWork<KT, CL, WIN> w(p, a, lds, kvh);
-    const ShTiles all = sh_tiles(p, a, w.bad);
-    const int tiles = __builtin_amdgcn_readlane(all.sum, 63);
-    if (u < all.shares && tiles > 0) {
-        const int end = (int)((long long)tiles * (u + 1) / all.shares);
-        for (int t = (int)((long long)tiles * u / all.shares); t < end;) {
-            const int g = __popcll(__ballot(all.sum <= t));
-            const int rts = __builtin_amdgcn_readlane(all.rts, g), cts = __builtin_amdgcn_readlane(all.cts, g);
-            const int at = t - (__builtin_amdgcn_readlane(all.sum, g) - rts * cts), ct = at / rts, r = at % rts;
-            const int n = min(rts - r, end - t), begin = __builtin_amdgcn_readlane(all.begin, g);
-            const int rows = __builtin_amdgcn_readlane(all.g.rows, g);
-            const size_t slot = (size_t)kvh * a.slots + __builtin_amdgcn_readlane(all.csum, g) - cts + ct + u;
-            w.part(__builtin_amdgcn_readlane(all.g.s0, g), __builtin_amdgcn_readlane(all.g.s1, g), rows, ct, begin + r * SH_R,
-                   min(rows, begin + (r + n) * SH_R), slot);
-            t += n;
+    w.bad = bad;
+    if (u < shares && tiles > 0) {
+        // what the later pieces are found by lies in LDS, as registers are short in between
+        const int lane = (int)(threadIdx.x & 63);
+        if (threadIdx.x < 64) {
+            lds.group[lane] = make_int4(all.g.s0, all.g.s1, all.g.rows, all.begin);
+            lds.sums[lane] = make_int2(all.sum, all.csum);
+        }
+        const auto at = [](int v, int g) { return __builtin_amdgcn_readlane(v, g); };
+        const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+        const int end = (int)((long long)tiles * (u + 1) / shares);
+        int t = (int)((long long)tiles * u / shares), g = __popcll(__ballot(all.sum <= t));
+        int s0 = at(all.g.s0, g), s1 = at(all.g.s1, g), rows = at(all.g.rows, g), begin = at(all.begin, g);
+        int sum = at(all.sum, g), csum = at(all.csum, g);
+        for (;;) {
+            const int rts = sh_rts(rows, begin), cts = sh_cts(s1 - s0, w.group);
+            const int i = t - (sum - rts * cts), ct = i / rts, r = i % rts, n = min(rts - r, end - t);
+            w.part(s0, s1, rows, ct, begin + r * SH_R, min(rows, begin + (r + n) * SH_R),
+                   (size_t)kvh * a.slots + csum - cts + ct + u);
+            if ((t += n) >= end) break;
+            g = __popcll(__ballot(lds.sums[lane].x <= t));
+            const int4 of = lds.group[g];
+            const int2 sums = lds.sums[g];
+            s0 = one(of.x), s1 = one(of.y), rows = one(of.z), begin = one(of.w), sum = one(sums.x), csum = one(sums.y);
         }
     }
     kr_report(a.fault, w.bad);
@@ -671,19 +707,19 @@ template <int T> __global__ void __launch_bounds__(T) k_shared_join(const PgView
     const int s = blockIdx.y, x = blockIdx.x, tid = threadIdx.x, group = a.nh / p.n_kv, kvh = x / group, col = x % group;
     int bad = 0;   // reported by the other launches
     PaSpan sp;
-    const PaParts r = pa_parts(p, a, s, kvh, sp);
+    const ShTiles all = sh_tiles(p, a, bad);
+    const PaParts r = pa_parts(p, a, s, kvh, sp, SH_WC * all.own);
     const float *ml0 = a.pml + (r.slot * group + col) * 2, *part0 = a.part + (r.slot * group + col) * p.hd;
     const float *ml1 = nullptr, *part1 = nullptr;
     int n1 = 0;
-    const ShTiles all = sh_tiles(p, a, bad);
     const unsigned long long in = __ballot(all.g.rows > 0 && s >= all.g.s0 && s < all.g.s1);
     if (in) {
         const int g = __builtin_ctzll(in), rts = __builtin_amdgcn_readlane(all.rts, g), cts = __builtin_amdgcn_readlane(all.cts, g);
         const int c = (s - __builtin_amdgcn_readlane(all.g.s0, g)) * group + col, ct = c / SH_CT;
         if (rts > 0) {
-            const int tiles = __builtin_amdgcn_readlane(all.sum, 63);
+            const int tiles = all.tiles, shares = sh_shares(a, all);
             const int t0 = __builtin_amdgcn_readlane(all.sum, g) - rts * cts + ct * rts;
-            const auto share = [&](int t) { return (int)((((long long)t + 1) * all.shares - 1) / tiles); };
+            const auto share = [&](int t) { return (int)((((long long)t + 1) * shares - 1) / tiles); };
             const int u0 = share(t0);
             n1 = share(t0 + rts - 1) - u0 + 1;
             const size_t slot = (size_t)kvh * a.slots + __builtin_amdgcn_readlane(all.csum, g) - cts + ct + u0;
@@ -741,22 +777,23 @@ template <int T> __global__ void __launch_bounds__(T) k_shared_join(const PgView
 constexpr int SH_CUS = 256;
 
 struct ShSizes {
-    int shares, sshares, sfew, slots;
+    int wgs, own, sfew, slots;
     size_t part, pml, spart, spml;   // floats
 };
 ShSizes sh_sizes(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_shared) {
     ShSizes r;
     const int group = nh / kv->n_kv_heads;
     const long long cts = (long long)n_seq * group / SH_CT + n_groups, tiles = cts * ((max_shared + SH_R - 1) / SH_R);
-    // as many workgroups as the chip holds at once, a quarter of them for the sequences' own rows
-    const int wgs = SH_CUS * sh_waves(kv->kv_type, kv->head_dim), want = wgs * 3 / 4 / kv->n_kv_heads;
-    r.sshares = (int)(want < 1 ? 1 : want < tiles ? want : tiles);
+    // as many workgroups as the chip holds at once
+    const int most = SH_CUS * sh_waves(kv->kv_type, kv->head_dim) / kv->n_kv_heads;
+    r.wgs = most < 2 ? 2 : most;
+    r.own = r.wgs / 4 > 0 ? r.wgs / 4 : 1;
+    const int shared = (int)(r.wgs - r.own < tiles ? r.wgs - r.own : tiles);
     // Where a compute unit holds two, one each while there are few tiles (8B shape, halves, in us, 128 / 256 / 384
     // workgroups for the shared rows: 16 sequences behind 2048 20.9 / 23.7 / -, 64 33.0 / 37.8 / 38.7, behind 4096 42.0 / - / 40.6)
-    r.sfew = wgs > SH_CUS && wgs / 4 / kv->n_kv_heads < r.sshares ? wgs / 4 / kv->n_kv_heads : r.sshares;
-    r.slots = (int)(cts + r.sshares);
-    r.shares = SH_WC * (wgs / 4 / kv->n_kv_heads > 0 ? wgs / 4 / kv->n_kv_heads : 1);
-    const size_t own = (size_t)kv->n_kv_heads * (n_seq + r.shares) * group;
+    r.sfew = sh_waves(kv->kv_type, kv->head_dim) > 1 && r.own < shared ? r.own : shared;
+    r.slots = (int)(cts + shared);
+    const size_t own = (size_t)kv->n_kv_heads * (n_seq + SH_WC * r.wgs) * group;
     const size_t both = (size_t)kv->n_kv_heads * r.slots * SH_CT;
     r.part = own * kv->head_dim;
     r.pml = (own * 2 + 3) & ~(size_t)3;
@@ -770,6 +807,26 @@ ShSizes sh_sizes(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_s
 // that take long (floats of 256 dims, 32 behind 1024 rows 50.7 / 60 / 83.5, of 128 30.7 / 29.4 / 37.7;
 // halves of 256 dims 27.3 / 27.9 / 35.7).
 int sh_least(const krh_pages *kv) { return kv->kv_type == ML_F32 || kv->head_dim > 128 ? 1 : 2; }
+
+// Column tiles of groups of as many sequences each
+double sh_cols(const krh_pages *kv, int n_seq, int nh, int n_groups) {
+    return n_groups * ceil(ceil((double)n_seq / n_groups) * (nh / kv->n_kv_heads) / SH_CT);
+}
+
+// What a wave does on SH_R own rows, in the work of a workgroup, a wave, on a tile of the shared ones: by it the device
+// has as many workgroups for the own rows as their part of all work is. 0: they have a quarter, which needs no look at all
+// lengths (0.5 to 0.9 us: 16 sequences of up to 1001 rows behind 2048 of the 8B shape 20.4 us instead of 19.6), where they
+// are at most (by max_len) little more than that. Measured, a quarter / by the work / each sequence by itself, 64 sequences of 4000 to
+// 8000 own rows behind 1024: 8B shape, halves 349 / 287 / 282 us, floats 1150 / 535 / 547; 1B shape, 8 bits 178 / 95 / 96;
+// floats of 256 dims 1150 / 544 / 526, 8 bits 471 / 175 / 160. Behind 4096: 364 / 289 / 357, 1133 / 525 / 703, 184 / 102 / 120,
+// 1145 / 560 / 714, 467 / 193 / 227.
+float sh_weigh(const krh_pages *kv, int n_seq, int nh, int max_len, int n_groups, int max_shared, int window) {
+    static const float weigh[3][3] = { { .12f, .19f, .06f }, { .11f, .12f, .08f }, { .12f, .15f, .06f } };   // F32, F16, Q8
+    const float w = weigh[kv->kv_type == ML_F32 ? 0 : kv->kv_type == ML_F16 ? 1 : 2][kv->head_dim <= 64 ? 0 : kv->head_dim <= 128 ? 1 : 2];
+    const double most = max_len - max_shared, own = n_seq * (window > 0 && window < most ? window : most);
+    const double shared = sh_cols(kv, n_seq, nh, n_groups) * (window > 0 && window < max_shared ? window : max_shared);
+    return w * own > (sh_waves(kv->kv_type, kv->head_dim) > 1 ? 1.5 : 0.7) * shared ? w : 0.0f;
+}
 
 // Whether the shared rows are better passed over once, by estimated times in us. Each
 // sequence by itself (krh_paged_attention): 11.5, 0.04 a sequence, and all sequences' rows at the rate at which
@@ -802,7 +859,7 @@ bool sh_args_ok(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_
            ((long long)n_seq * (n_heads / kv->n_kv_heads) / 32 + n_groups) * (max_shared / SH_R + 1) <= INT32_MAX / 2;
 }
 
-using ShRows = void (*)(const PgView, const ShArgs, int);
+using ShRows = void (*)(const PgView, const ShArgs);
 template <int KT, bool WIN> ShRows sh_rows(int hd) {
     return hd <= 64 ? k_shared_rows<KT, 64, WIN> : hd <= 128 ? k_shared_rows<KT, 128, WIN> : k_shared_rows<KT, 256, WIN>;
 }
@@ -849,18 +906,18 @@ extern "C" void krh_paged_attention_shared(float *o, const krh_pages *kv, const 
     ShArgs a = {};
     a.o = o, a.q = q, a.len = len;
     a.part = w, a.pml = w + r.part, a.spart = a.pml + r.pml, a.spml = a.spart + r.spart;
-    a.nh = n_heads, a.max_len = max_len, a.window = window, a.shares = r.shares, a.tl = pg_log2(pa_tile(kv->head_dim));
+    a.nh = n_heads, a.max_len = max_len, a.window = window, a.shares = SH_WC * r.wgs, a.tl = pg_log2(pa_tile(kv->head_dim));
     a.least = 1;
     a.scale = scale, a.cap = softcap;
     a.group = group, a.shared = shared, a.n_groups = n_groups, a.max_shared = max_shared;
-    a.sshares = r.sshares, a.sfew = r.sfew, a.sleast = sh_least(kv), a.slots = r.slots, a.fault = kr_fault_word();
+    a.wgs = r.wgs, a.own = r.own, a.weigh = sh_weigh(kv, n_seq, n_heads, max_len, n_groups, max_shared, window), a.sfew = r.sfew, a.sleast = sh_least(kv), a.slots = r.slots, a.fault = kr_fault_word();
     const PgView p = pg_view(kv, table, table_ld, n_seq);
-    const int hd = kv->head_dim, own = (r.shares + SH_WC - 1) / SH_WC;
+    const int hd = kv->head_dim;
     const bool win = window > 0;
     const ShRows f = kv->kv_type == ML_F32   ? sh_rows<PG_F32>(hd, win)
                      : kv->kv_type == ML_F16 ? sh_rows<PG_F16>(hd, win)
                                              : sh_rows<PG_Q8>(hd, win);
-    hipLaunchKernelGGL(f, dim3((own + r.sshares) * kv->n_kv_heads), dim3(64 * SH_WC), 0, kr_stream(), p, a, own);
+    hipLaunchKernelGGL(f, dim3(r.wgs * kv->n_kv_heads), dim3(64 * SH_WC), 0, kr_stream(), p, a);
     kr_check_launch("paged_attention_shared");
     // Threads a head: with few heads the parts are asked for side by side, with many each wave's search for its parts
     // is what takes the time (a call of 512 heads of 128 dims by 256 / 128 / 64 20.1 / 20.5 / 21.1 us, 1024 of 64 36.2 / 35.2 /

@@ -84,7 +84,8 @@ template <class A> __device__ __forceinline__ void pa_fetch(const PgView &p, con
     r.skip = pa_skip(p, a, i, bad);
     r.sum = pg_scan(i < p.n_seq ? pa_span(a, r.len, r.skip).tiles : 0);
 }
-template <class A> __device__ __forceinline__ PaAll pa_all(const PgView &p, const A &a, int &bad) {
+// most: the shares that there are at most
+template <class A> __device__ __forceinline__ PaAll pa_all(const PgView &p, const A &a, int &bad, int most) {
     PaAll r;
     int t = 0;
     for (int i0 = 0; i0 < p.n_seq; i0 += 64) {
@@ -93,7 +94,7 @@ template <class A> __device__ __forceinline__ PaAll pa_all(const PgView &p, cons
         t += __builtin_amdgcn_readlane(r.sum, 63);
     }
     r.tiles = t;
-    r.shares = max(1, min(a.shares, (t + a.least - 1) / a.least));
+    r.shares = max(1, min(most, (t + a.least - 1) / a.least));
     return r;
 }
 template <class A> __device__ __forceinline__ PaSpan pa_of(const PgView &p, const A &a, PaAll &r, int s, int &bad) {
@@ -619,9 +620,10 @@ struct PaParts {
     size_t slot;
     int n;
 };
-template <class A> __device__ __forceinline__ PaParts pa_parts(const PgView &p, const A &a, int s, int kvh, PaSpan &sp) {
+template <class A>
+__device__ __forceinline__ PaParts pa_parts(const PgView &p, const A &a, int s, int kvh, PaSpan &sp, int most) {
     int bad = 0;   // reported by the shares
-    PaAll all = pa_all(p, a, bad);
+    PaAll all = pa_all(p, a, bad, most);
     int before = 0;
     for (int i = threadIdx.x & 63; i < (s & ~63); i += 64)
         before += pa_span(a, kr_page_len(a.len[i], a.max_len, bad), pa_skip(p, a, i, bad)).tiles;

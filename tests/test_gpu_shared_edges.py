@@ -254,3 +254,27 @@ def test_offsets_past_32_bits(dev, kv_type, n):  # noqa: F811
         for h in range(nh):
             w, _, bound, _ = attention(q[i, h].astype(np.float64), k64[at, h // 2], v64[at, h // 2], 0.0625, 0, 0)
             assert (np.abs(o[i, h] - w) <= bound).all(), (i, h)
+
+
+@pytest.mark.parametrize("kv_type", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd,window", [(14, 2, 64, 0), (8, 8, 128, 0), (8, 4, 256, 0), (8, 8, 128, 2500)])
+def test_own_rows_as_their_part_is(dev, kv_type, nh, nkv, hd, window):  # noqa: F811
+    """lengths from nothing to far more own rows than shared ones, under bounds that allow own rows to be most of the work"""
+    rng = np.random.default_rng(hd + window)
+    for n, shared, own in ((70, 2000, own_rows(rng, 70, 40)), (70, 320, own_rows(rng, 70, 3000)), (70, 96, [2500] * 3 + [0] * 67)):
+        own[4], own[69] = -shared, -shared // 2
+        b = Batch(dev, rng, kv_type, nh, nkv, hd, 32, [(n - 20, shared), (20, shared // 2)], own).spoil()
+        b.put(max_len=50000, max_shared=4000)
+        assert b.form(window) == 1
+        b.run(window)
+        ok()
+        o = b.out()
+        b.check(o, window)
+        b.run(window)
+        ok()
+        assert np.array_equal(bits(b.out()), bits(o))
+        # no groups at all: every row is a sequence's own
+        b.gb = dev.put(i32([n, n, n]))
+        b.run(window)
+        ok()
+        b.check(b.out(), window)
