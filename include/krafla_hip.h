@@ -418,8 +418,8 @@ size_t krh_paged_attention_shared_ws(const krh_pages *kv, int n_seq, int n_heads
  * are read, as far as any of the group attends; len counts them. group ascends
  * within [0, n_seq]; sequences before group[0] and from group[n_groups] on share
  * nothing. group and shared are device data, checked as lengths and sequences are;
- * max_shared sizes the launch and, with n_seq, decides whether sharing pays. A
- * sequence may be shorter than its group's shared rows, or have none.
+ * max_shared sizes the launch and, with n_seq and n_groups, decides whether sharing
+ * pays. A sequence may be shorter than its group's shared rows, or have none.
  *
  * The results are krh_paged_attention's to rounding, the same from call to call;
  * what that call states of arguments, precision and not finite values holds here
@@ -430,8 +430,8 @@ void krh_paged_attention_shared(float *o, const krh_pages *kv, const int *table,
                                 const float *q, int n_heads, int max_len, int window, float scale, float softcap,
                                 void *ws);
 /* Whether these sizes pass over shared rows once for all (1), or let each sequence
- * read its own as krh_paged_attention does, which is faster for few sequences or few
- * shared rows (0); -1 for sizes that the call refuses. */
+ * read its own as krh_paged_attention does, which is faster for few sequences, few
+ * shared rows, or many small groups (0); -1 for sizes that the call refuses. */
 int krh_paged_attention_shared_form(const krh_pages *kv, int n_seq, int n_heads, int max_len, int n_groups,
                                     int max_shared, int window);
 /* Bytes of workspace that krh_paged_evict takes (0 for sizes that it refuses) */

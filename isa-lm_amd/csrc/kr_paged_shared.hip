@@ -829,22 +829,29 @@ float sh_weigh(const krh_pages *kv, int n_seq, int nh, int max_len, int n_groups
 }
 
 // Whether the shared rows are better passed over once, by estimated times in us. Each
-// sequence by itself (krh_paged_attention): 11.5, 0.04 a sequence, and all sequences' rows at the rate at which
-// dies read what others read too (TB/s: halves 15, floats 11, 8 bits 6.3). Once for
-// all: 12.1, 0.08 a sequence, and a workgroup's tiles, `tile` each. Measured, each / once,
-// sequences of 150 rows on average behind 256 / 1024 / 4096 / 8192: 8B shape, halves, 8 12.2 / 14.0, 15.1 /
-// 15.1, 23.3 / 21.8, 31.8 / 24.1, 64 15.0 / 18.2, 37.4 / 22.6, 90.5 / 35.0, 161 / 43.3; 1B shape, 8 bits, 16 12.5 / 13.5,
-// 15.2 / 14.4, 22.1 / 21.7, 31.5 / 23.2; floats of 256 dims, 32 22.5 / 33.5, 41.8 / 47.5, 114 / 86.7, 209 / 140. Of 216 such
-// sizes eight take the slower way by more than 5%, the worst by 18.
+// sequence by itself (krh_paged_attention): 11.5, a group's shared rows at the rate of HBM, and at the rate at which dies
+// read what others read too for its other sequences (TB/s: halves 4 and 10.5, floats 6.6, 8 bits 5). Once for
+// all: 15, 2.5 for 1024 heads of 128 dims to join (by dims squared), a workgroup's tiles, `tile` each, and with a window
+// 2.5 a group, whose first rows are looked for one after another. As many groups as do not leave a sequence alone; own
+// rows are as long either way. Measured, each / once, 64 sequences of 75 to 150 own rows in 1 / 8 / 16 / 32 / 63 groups:
+// 8B shape, halves, behind 1024 rows 39 / 24, 53 / 29, 54 / 35, 54 / 55, 65 / 87, behind 4096 90 / 36, 161 / 51, 160 / 81,
+// 197 / 140, 196 / 243, floats behind 1024 76 / 40, 95 / 68, 95 / 122, 107 / 227, 117 / 238; 1B shape, 8 bits, behind 2048 36 / 24,
+// 37 / 29, 37 / 41, 38 / 71, 39 / 77; floats of 256 dims behind 2048 124 / 79, 162 / 233, 166 / 422, 168 / 798, 197 / 428. Of 4242
+// sizes (2 to 128 sequences, 1 to 64 groups of 128 to 8192 rows, 30 to 8000 own rows, windows) 4% take the slower way by more
+// than 5%, 1% by more than 15, the worst by 48.
 bool sh_pays(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_shared, int window) {
-    static const float rate[3] = { 11e6f, 15e6f, 6.3e6f };                                   // bytes a us: F32, F16, Q8
-    static const float tile[3][3] = { { 2.9f, 4.2f, 20 }, { 1.6f, 1.75f, 6 }, { 1.6f, 3.5f, 8 } };
+    static const double first[3] = { 6.6e6, 4e6, 5e6 }, again[3] = { 6.6e6, 10.5e6, 5e6 };   // bytes a us: F32, F16, Q8
+    static const double tile[3][3] = { { 2.5, 3.8, 25 }, { 1.1, 1.85, 6 }, { 1.45, 2.7, 10 } };
+    if (n_seq <= n_groups) return false;
     const int t = kv->kv_type == ML_F32 ? 0 : kv->kv_type == ML_F16 ? 1 : 2, c = kv->head_dim <= 64 ? 0 : kv->head_dim <= 128 ? 1 : 2;
+    const int groups = n_groups < n_seq - n_groups ? n_groups : n_seq - n_groups, seqs = n_seq - (n_groups - groups);
     const double rows = window > 0 && window < max_shared ? window : max_shared;
     const double row = (double)kv->n_kv_heads * kv->head_dim * (t == 0 ? 8 : t == 1 ? 4 : 2) + (t == 2 ? 8 * kv->n_kv_heads : 0);
-    const double cts = ceil((double)n_seq * (nh / kv->n_kv_heads) / SH_CT);
-    const double tiles = ceil(cts * ceil(rows / SH_R) * kv->n_kv_heads / (SH_CUS * sh_waves(kv->kv_type, kv->head_dim) * 3 / 4));
-    return n_seq > n_groups && 11.5 + n_seq * (0.04 + rows * row / rate[t]) > 12.1 + 0.08 * n_seq + tiles * tile[t][c];
+    const double tiles = ceil(sh_cols(kv, seqs, nh, groups) * ceil(rows / SH_R) * kv->n_kv_heads /
+                              (SH_CUS * sh_waves(kv->kv_type, kv->head_dim) * 3 / 4));
+    const double heads = (double)n_seq * nh / 1024, dims = kv->head_dim / 128.0;
+    return 11.5 + rows * row * (groups / first[t] + (seqs - groups) / again[t]) >
+           15 + 2.5 * heads * dims * dims + tiles * tile[t][c] + (window > 0 ? 2.5 * n_groups : 0);
 }
 bool sh_shared(const krh_pages *kv, int n_seq, int nh, int n_groups, int max_shared, int window) {
     return n_groups > 0 && max_shared > 0 && sh_pays(kv, n_seq, nh, n_groups, max_shared, window);

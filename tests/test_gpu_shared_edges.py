@@ -30,10 +30,10 @@ GAPS = [
     # one gap, in the first column tile (narrow groups) or in each of several
     (8, 4, 128, 32, 2500, [(60, 2800)], {0: -2670, 7: -2795, 30: -2700}),
     # the short ones at the end: the tile of the others has no gap
-    (8, 2, 64, 64, 2500, [(60, 3000)], {57: -2990, 58: -2900, 59: -2680}),
+    (16, 4, 64, 64, 2500, [(80, 3000)], {77: -2990, 78: -2900, 79: -2680}),
     # three runs of rows with gaps between them, which begin and end within tiles and pages, and a group without one
     (16, 8, 128, 16, 600, [(70, 3100), (30, 480)], {0: -3000, 1: -1717, 2: -1700, 40: -3093, 41: -1690}),
-    (8, 4, 256, 16, 1800, [(40, 4000)], {0: -3900, 11: -1990, 12: -2000}),
+    (8, 4, 256, 16, 1800, [(60, 4000)], {0: -3900, 11: -1990, 12: -2000}),
 ]
 
 
@@ -107,7 +107,7 @@ def test_large_soft_caps(dev, kv_type, hd, peak, cap):  # noqa: F811
     """caps far above the scores leave them, however small the queries are: tanh(x) is x, and what is left is the division's
     rounding, a step of 2^-149 where the quotient is that small, and two roundings of the float"""
     rng = np.random.default_rng(hd)
-    b = Batch(dev, rng, kv_type, 4, 2, hd, 16, [(9, 200), (20, 330)], own_rows(rng, 29, 60))
+    b = Batch(dev, rng, kv_type, 4, 2, hd, 16, [(19, 200), (40, 330)], own_rows(rng, 59, 60))
     b.q = f32(b.q * (peak / np.abs(b.q).max()))
     # keys that make the scores differ by a few whatever the queries are
     name = "kd" if kv_type == K.ML_Q8_0 else "k"
