@@ -20,12 +20,14 @@
 // workgroup and KV head, by the lengths that the device has; a share's sums of a
 // column tile are a part.
 //
-// What bounds it (8B shape, halves): 64 sequences behind 32,000 rows 99 to 113 us by
+// What bounds it (8B shape, halves): 64 sequences behind 32,000 rows 98 to 113 us by
 // the card, of which the join's reads of the parts 9; the matrix cores and the
-// softmax's instructions beside each other, at the 1.6 GHz that power leaves (67 GFLOP
-// with both halves, 54 us of a large product's rate). 16 behind 2048 19.7 us: four tiles
-// a workgroup, 1.8 us each on their way, and the join's latency, 5.8. Each sequence
-// reading its own (krh_paged_attention) takes 1069 us and 26.8 there.
+// softmax's instructions beside each other (busy 37 and 38% of the cycles), at the 1.6 to
+// 2.0 GHz of 2.4 that power leaves (67 GFLOP with both halves, 54 us of a large
+// product's rate). 16 behind 2048 19.9 us: four tiles a workgroup, 1.8 us each on
+// their way (the matrix cores are busy 5% of the cycles), and the join's latency, 5.8. Each sequence
+// reading its own (krh_paged_attention) takes 1069 us and 26.8 there. Floats of 256
+// dims, 32 behind 8192 134 us: one wave a SIMD, the matrix cores busy 17%.
 #include <cfloat>
 #include <cmath>
 #include "kr_paged_wave.h"
@@ -641,7 +643,7 @@ template <int KT, int CL, bool WIN> struct ShWork {
 
 // The first workgroups' waves have shares of the sequences' own rows, the others shares of the
 // shared ones: the former wait for HBM, the latter for the matrix cores (and
-// for power: 64 sequences behind 32,000 rows run at 1.6 GHz), so they are one launch.
+// for power: 64 sequences behind 32,000 rows run at 1.6 to 2.0 GHz), so they are one launch.
 template <int KT, int CL, bool WIN>
 __global__ void __launch_bounds__(64 * SH_WC, sh_waves(KT, CL)) k_shared_rows(const PgView p, const ShArgs a) {
     __shared__ ShLds<KT, CL, WIN> lds;
