@@ -415,7 +415,7 @@ size_t krh_paged_attention_shared_ws(const krh_pages *kv, int n_seq, int n_heads
  * the common rows read once for all of them. Sequences group[g] .. group[g + 1] - 1,
  * g < n_groups <= 64, share their first shared[g] <= max_shared rows: their tables
  * name the same pages for these, or pages of the same rows, and the first one's
- * are read, as far as any of the group attends; len counts them. group ascends
+ * are read, where any of the group attends; len counts them. group ascends
  * within [0, n_seq]; sequences before group[0] and from group[n_groups] on share
  * nothing. group and shared are device data, checked as lengths and sequences are;
  * max_shared sizes the launch and, with n_seq and n_groups, decides whether sharing
