@@ -817,11 +817,12 @@ double sh_cols(const krh_pages *kv, int n_seq, int nh, int n_groups) {
 
 // What a wave does on SH_R own rows, in the work of a workgroup, a wave, on a tile of the shared ones: by it the device
 // has as many workgroups for the own rows as their part of all work is. 0: they have a quarter, which needs no look at all
-// lengths (0.5 to 0.9 us: 16 sequences of up to 1001 rows behind 2048 of the 8B shape 20.4 us instead of 19.6), where they
-// are at most (by max_len) little more than that. Measured, a quarter / by the work / each sequence by itself, 64 sequences of 4000 to
-// 8000 own rows behind 1024: 8B shape, halves 349 / 287 / 282 us, floats 1150 / 535 / 547; 1B shape, 8 bits 178 / 95 / 96;
-// floats of 256 dims 1150 / 544 / 526, 8 bits 471 / 175 / 160. Behind 4096: 364 / 289 / 357, 1133 / 525 / 703, 184 / 102 / 120,
-// 1145 / 560 / 714, 467 / 193 / 227.
+// lengths (0.5 to 0.9 us: 16 sequences of up to 1001 rows behind 2048 of the 8B shape 20.4 us instead of 19.6): where they
+// are at most, by max_len, three fifths of the work, or two fifths of kernels that have one workgroup a compute unit, whose
+// quarter is few waves. Measured, a quarter / by the work / each sequence by itself, 64 sequences of 4000 to 8000 own rows
+// behind 1024: 8B shape, halves 349 / 287 / 282 us, floats 1150 / 535 / 547; 1B shape, 8 bits 178 / 95 / 96; floats of 256
+// dims 1150 / 544 / 526, 8 bits 471 / 175 / 160. Behind 4096: 364 / 289 / 357, 1133 / 525 / 703, 184 / 102 / 120, 1145 / 560 /
+// 714, 467 / 193 / 227.
 float sh_weigh(const krh_pages *kv, int n_seq, int nh, int max_len, int n_groups, int max_shared, int window) {
     static const float weigh[3][3] = { { .12f, .19f, .06f }, { .11f, .12f, .08f }, { .12f, .15f, .06f } };   // F32, F16, Q8
     const float w = weigh[kv->kv_type == ML_F32 ? 0 : kv->kv_type == ML_F16 ? 1 : 2][kv->head_dim <= 64 ? 0 : kv->head_dim <= 128 ? 1 : 2];
@@ -919,7 +920,8 @@ extern "C" void krh_paged_attention_shared(float *o, const krh_pages *kv, const 
     a.least = 1;
     a.scale = scale, a.cap = softcap;
     a.group = group, a.shared = shared, a.n_groups = n_groups, a.max_shared = max_shared;
-    a.wgs = r.wgs, a.own = r.own, a.weigh = sh_weigh(kv, n_seq, n_heads, max_len, n_groups, max_shared, window), a.sfew = r.sfew, a.sleast = sh_least(kv), a.slots = r.slots, a.fault = kr_fault_word();
+    a.wgs = r.wgs, a.own = r.own, a.weigh = sh_weigh(kv, n_seq, n_heads, max_len, n_groups, max_shared, window);
+    a.sfew = r.sfew, a.sleast = sh_least(kv), a.slots = r.slots, a.fault = kr_fault_word();
     const PgView p = pg_view(kv, table, table_ld, n_seq);
     const int hd = kv->head_dim;
     const bool win = window > 0;
